@@ -18,12 +18,17 @@ TS_ERR_HIP = -4
 TS_ERR_NOMEM = -5
 TS_ERR_WORKSPACE = -6
 
+TS_DTYPE_F32, TS_DTYPE_F16, TS_DTYPE_BF16 = 0, 1, 2
+TS_ROPE_INTERLEAVED, TS_ROPE_HALF = 0, 1
+
 # Every symbol the header declares, with (restype, argtypes).
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
 _u64p = ctypes.POINTER(ctypes.c_uint64)
 _i32p = ctypes.POINTER(ctypes.c_int32)
 _f = ctypes.c_float
+_i64 = ctypes.c_int64
+_d = ctypes.c_double
 
 
 class KvDesc(ctypes.Structure):
@@ -85,6 +90,11 @@ SIGNATURES = {
     "ts_attn_out_proj_x2": (ctypes.c_int, [_vp, _i32, _i32, _vp, _i32, _vp, _vp, _vp, ctypes.c_uint64,
                                            _vp]),
     "ts_weights_to_f16x2": (ctypes.c_int, [_i32, _vp, ctypes.c_int64, ctypes.c_int64, _vp, _vp]),
+    "ts_rope_create_scaled": (ctypes.c_int, [_i32, _i32, _d, _d, _i32, _d, _d, _d, ctypes.POINTER(_vp)]),
+    "ts_rope_apply": (ctypes.c_int, [_vp, _i32, _i32, _vp, _i64, _vp, _i32, _i32, _i32, _vp, _i64, _vp]),
+    "ts_append_packed": (ctypes.c_int, [_vp, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _vp]),
+    "ts_read_packed": (ctypes.c_int, [_vp, _i32, _vp, _vp, _i32, _vp, _i64, _vp, _i64, _vp]),
+    "ts_kv_increment_packed": (ctypes.c_int, [_vp, _vp, _vp]),
 }
 
 _lib = None

@@ -10,23 +10,11 @@
 #include <mutex>
 #include <new>
 
-#include "ts_internal.h"
+#include "ts_host.h"
+
+using namespace ts;
 
 namespace {
-
-hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s); }
-
-// True when work enqueued on the stream now goes into a graph being captured.
-static bool capturing(void *stream) {
-    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-    return hipStreamIsCapturing(as_stream(stream), &cs) == hipSuccess && cs != hipStreamCaptureStatusNone;
-}
-// A call that changes the device lengths: note when it is being captured.
-static void note_len_change(ts_kv *kv, void *stream) {
-    if (capturing(stream)) kv->len_captured = true;
-}
-
-int hip_status(hipError_t e) { return e == hipSuccess ? TS_OK : TS_ERR_HIP; }
 
 bool desc_valid(const ts_kv_desc *d) {
     return d && d->n_layers > 0 && d->n_seq > 0 && d->n_head_kv > 0 && d->head_dim > 0 &&
@@ -157,17 +145,6 @@ int ts_rope_info(const ts_rope *rope, const float **d_table, int32_t *n_pos, int
 }
 
 // ---- cache -----------------------------------------------------------------------------------
-
-// The kernels move f32 rows in 16-byte pieces.
-static bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
-
-// Largest rotation position (exclusive) the next n_tok tokens of any sequence use: slots past
-// the sinks are rotated at slot + window base.
-static int64_t rot_end(const ts_kv *kv, int32_t n_tok) {
-    int64_t m = 0;
-    for (int s = 0; s < kv->d.n_seq; s++) m = std::max<int64_t>(m, (int64_t)kv->h_len[s] + kv->h_rot[s] + n_tok);
-    return m;
-}
 
 int ts_kv_bytes(const ts_kv_desc *desc, uint64_t *bytes) {
     if (!desc_valid(desc) || !bytes) return TS_ERR_INVALID;
@@ -393,14 +370,6 @@ int ts_kv_export(const ts_kv *kv, int32_t layer, int32_t seq, int32_t pos0, int3
 
 // ---- hot path --------------------------------------------------------------------------------
 
-static int check_rope(const ts_rope *rope, int hd, int64_t max_pos_exclusive) {
-    if (!rope) return TS_ERR_INVALID;
-    if (rope->rope_dim > hd) return TS_ERR_INVALID;
-    if (max_pos_exclusive > rope->n_pos) return TS_ERR_INVALID;
-    return TS_OK;
-}
-
-
 int ts_append_quant(ts_kv *kv, int32_t layer, const float *d_k, const float *d_v, int32_t n_tok,
                     const ts_rope *rope, void *stream) {
     if (!kv || layer < 0 || layer >= kv->d.n_layers || !aligned16(d_k) || !aligned16(d_v) || !d_k ||
@@ -439,12 +408,6 @@ int ts_requant_all(ts_kv *kv, int32_t layer, const float *d_k_cache, const float
                                                seq_len, ld_pos, rope ? rope->d_table : nullptr,
                                                rope ? rope->rope_dim / 2 : 0, blocks,
                                                as_stream(stream)));
-}
-
-// Any GQA group size: the decode takes more than 8 query heads per kv head as several head
-// groups (each reads the kv head's stream).
-static bool heads_ok(const ts_kv *kv, int32_t n_head) {
-    return n_head > 0 && n_head % kv->d.n_head_kv == 0;
 }
 
 int ts_attn_decode_workspace(const ts_kv *kv, int32_t n_head, uint64_t *bytes) {

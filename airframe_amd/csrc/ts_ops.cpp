@@ -1,0 +1,127 @@
+// ts_ops.cpp -- host side of the packed-batch and shared-prefix entry points: argument checks and dispatch.
+#include "ts_packed.h"
+
+#include <math.h>
+
+#include <cmath>
+#include <new>
+
+#include "ts_host.h"
+
+using namespace ts;
+
+// Rows that 16-byte pieces reach: the first address and the distance from row to row.
+static bool rows_ok(const void *p, int64_t stride, int64_t row, int32_t dtype) {
+    return p && aligned16(p) && stride >= row && stride <= INT64_MAX / 16 / (int64_t)INT32_MAX &&
+           stride * dtype_size(dtype) % 16 == 0;
+}
+
+// The largest length of a sequence after its rows of a packed batch, and its last rotation position.
+static void packed_ends(const ts_kv *kv, const int32_t *off, int64_t &len_end, int64_t &rot_last) {
+    len_end = rot_last = 0;
+    for (int s = 0; s < kv->d.n_seq; s++) {
+        const int64_t n = (int64_t)off[s + 1] - off[s];
+        if (n == 0) continue;
+        len_end = std::max(len_end, kv->h_len[s] + n);
+        rot_last = std::max(rot_last, (int64_t)kv->h_len[s] + kv->h_rot[s] + n);
+    }
+}
+
+extern "C" {
+
+int ts_rope_create_scaled(int32_t n_pos, int32_t rope_dim, double base, double factor, int32_t l_train, double alpha,
+                          double beta, double mult, ts_rope **out) {
+    if (!out) return TS_ERR_INVALID;
+    *out = nullptr;
+    if (n_pos <= 0 || rope_dim <= 0 || (rope_dim & 1) || !(base > 0.0) || !std::isfinite(base) || !(factor > 0.0) ||
+        !std::isfinite(factor) || !(mult > 0.0) || !std::isfinite(mult) || !(alpha >= 0.0) || !(beta >= 0.0) ||
+        !std::isfinite(alpha) || !std::isfinite(beta) || (beta > alpha && l_train <= 0))
+        return TS_ERR_INVALID;
+    ts_rope *r = new (std::nothrow) ts_rope();
+    if (!r) return TS_ERR_NOMEM;
+    if (hipMalloc(&r->d_table, (size_t)n_pos * rope_dim * sizeof(float)) != hipSuccess) {
+        delete r;
+        return TS_ERR_NOMEM;
+    }
+    // (the table is whole when this returns, whatever stream reads it then)
+    hipError_t e = launch_rope_table(r->d_table, n_pos, rope_dim, base, factor, l_train, alpha, beta, mult, nullptr);
+    if (e == hipSuccess) e = hipStreamSynchronize(nullptr);
+    if (e != hipSuccess) {
+        (void)hipFree(r->d_table);
+        delete r;
+        return TS_ERR_HIP;
+    }
+    r->n_pos = n_pos;
+    r->rope_dim = rope_dim;
+    *out = r;
+    return TS_OK;
+}
+
+int ts_rope_apply(const ts_rope *rope, int32_t layout, int32_t dtype, const void *d_x, int64_t x_stride,
+                  const int32_t *d_pos, int32_t n_tok, int32_t n_head, int32_t head_dim, void *d_out, int64_t out_stride,
+                  void *stream) {
+    if (!rope || !dtype_ok(dtype) || (layout != TS_ROPE_INTERLEAVED && layout != TS_ROPE_HALF) || n_tok < 0 || n_head <= 0 ||
+        head_dim <= 0 || head_dim % 8 != 0 || head_dim > 65536 || n_head > 65536 || rope->rope_dim > head_dim)
+        return TS_ERR_INVALID;
+    if (n_tok == 0) return TS_OK;
+    const int64_t row = (int64_t)n_head * head_dim;
+    if (!d_pos || ((uintptr_t)d_pos & 3u) != 0 || !rows_ok(d_x, x_stride, row, dtype) || !rows_ok(d_out, out_stride, row, dtype))
+        return TS_ERR_INVALID;
+    // in place, or apart: a thread reads its rows before it writes them, but not before others write
+    const int size = dtype_size(dtype);
+    const uint8_t *x0 = (const uint8_t *)d_x, *o0 = (const uint8_t *)d_out;
+    const uint8_t *x1 = x0 + ((n_tok - 1) * x_stride + row) * size, *o1 = o0 + ((n_tok - 1) * out_stride + row) * size;
+    if (x0 == o0 ? x_stride != out_stride && n_tok > 1 : x0 < o1 && o0 < x1) return TS_ERR_INVALID;
+    return hip_status(launch_rope_apply(dtype, layout, d_x, x_stride, d_pos, n_tok, n_head, head_dim, rope->d_table,
+                                        rope->rope_dim / 2, rope->n_pos, d_out, out_stride, as_stream(stream)));
+}
+
+int ts_append_packed(ts_kv *kv, int32_t layer, int32_t dtype, const void *d_k, int64_t k_stride, const void *d_v,
+                     int64_t v_stride, const int32_t *tok_off, const ts_rope *rope, void *stream) {
+    if (!kv || layer < 0 || layer >= kv->d.n_layers || !dtype_ok(dtype) || !offsets_ok(tok_off, kv->d.n_seq))
+        return TS_ERR_INVALID;
+    if (tok_off[kv->d.n_seq] == tok_off[0]) return TS_OK;
+    const int64_t row = (int64_t)kv->d.n_head_kv * kv->d.head_dim;
+    if (!rows_ok(d_k, k_stride, row, dtype) || !rows_ok(d_v, v_stride, row, dtype)) return TS_ERR_INVALID;
+    int64_t len_end, rot_last;
+    packed_ends(kv, tok_off, len_end, rot_last);
+    if (len_end > kv->d.max_seq) return TS_ERR_OVERFLOW;
+    if (rope) {
+        const int rc = check_rope(rope, kv->d.head_dim, rot_last);
+        if (rc) return rc;
+    }
+    KvLayerView L = kv->layer(layer);
+    if (!rope) L.qn = L.kn = nullptr;  // (K as it is stored: normalized and rotated by the caller)
+    return hip_status(launch_append_packed(L, kv->d_len, dtype, d_k, k_stride, d_v, v_stride, tok_off,
+                                           rope ? rope->d_table : nullptr, rope ? rope->rope_dim / 2 : 0,
+                                           rope ? rope->n_pos : INT32_MAX, as_stream(stream)));
+}
+
+int ts_read_packed(const ts_kv *kv, int32_t layer, const int32_t *pos0, const int32_t *row_off, int32_t dtype, void *d_k,
+                   int64_t k_stride, void *d_v, int64_t v_stride, void *stream) {
+    if (!kv || layer < 0 || layer >= kv->d.n_layers || !dtype_ok(dtype) || !offsets_ok(row_off, kv->d.n_seq))
+        return TS_ERR_INVALID;
+    if (row_off[kv->d.n_seq] == row_off[0]) return TS_OK;
+    const int64_t row = (int64_t)kv->d.n_head_kv * kv->d.head_dim;
+    if (!rows_ok(d_k, k_stride, row, dtype) || !rows_ok(d_v, v_stride, row, dtype)) return TS_ERR_INVALID;
+    for (int s = 0; s < kv->d.n_seq; s++) {
+        const int64_t p = pos0 ? pos0[s] : 0, n = (int64_t)row_off[s + 1] - row_off[s];
+        if (n > 0 && (p < 0 || p + n > kv->d.max_seq)) return TS_ERR_INVALID;
+    }
+    return hip_status(launch_read_packed(kv->layer(layer), pos0, row_off, dtype, d_k, k_stride, d_v, v_stride,
+                                         as_stream(stream)));
+}
+
+int ts_kv_increment_packed(ts_kv *kv, const int32_t *tok_off, void *stream) {
+    if (!kv || !offsets_ok(tok_off, kv->d.n_seq)) return TS_ERR_INVALID;
+    for (int s = 0; s < kv->d.n_seq; s++)
+        if ((int64_t)kv->h_len[s] + tok_off[s + 1] - tok_off[s] > kv->d.max_seq) return TS_ERR_OVERFLOW;
+    if (tok_off[kv->d.n_seq] == tok_off[0]) return TS_OK;
+    note_len_change(kv, stream);
+    const hipError_t e = launch_len_add(kv->d_len, kv->d.n_seq, tok_off, as_stream(stream));
+    if (e != hipSuccess) return TS_ERR_HIP;
+    for (int s = 0; s < kv->d.n_seq; s++) kv->h_len[s] += tok_off[s + 1] - tok_off[s];
+    return TS_OK;
+}
+
+}  // extern "C"

@@ -14,6 +14,7 @@ import torch
 
 from . import _lib
 from ._lib import KvDesc, check, load
+from .prompt import _dtype, _launch, _offsets, _rows
 
 
 def _stream(stream=None) -> ctypes.c_void_p:
@@ -52,6 +53,20 @@ class RopeTable:
                                                             ctypes.byref(h)))
         self._h = h
         self.n_pos, self.rope_dim, self.base, self.scale = n_pos, rope_dim, base, scale
+
+    @classmethod
+    def scaled(cls, n_pos: int, rope_dim: int, base: float, factor: float = 1.0, l_train: int = 0,
+               alpha: float = 0.0, beta: float = 0.0, mult: float = 1.0) -> "RopeTable":
+        """A table stretched for long contexts, its angles in 64 bits (ts_rope_create_scaled): every
+        frequency divided by factor, or, with beta > alpha, only those of pairs that turn fewer than
+        alpha times within l_train, and a mixture up to beta; cos and sin times mult."""
+        h = ctypes.c_void_p()
+        check("ts_rope_create_scaled", load().ts_rope_create_scaled(n_pos, rope_dim, base, factor, l_train, alpha, beta,
+                                                                    mult, ctypes.byref(h)))
+        t = cls.__new__(cls)
+        t._h = h
+        t.n_pos, t.rope_dim, t.base, t.scale = n_pos, rope_dim, base, 1.0 / factor
+        return t
 
     @staticmethod
     def host_table(n_pos: int, rope_dim: int, base: float, scale: float = 1.0,
@@ -222,6 +237,65 @@ class KVCache:
                                     _ptr(v_cache, torch.float32, "v_cache"), seq_len,
                                     k_cache.shape[1], rope.handle if rope else None,
                                     _stream(stream)))
+
+    # ---- packed batches (rows of all sequences one after another; prompt.py) -----------------
+
+    def append_packed(self, layer: int, k: torch.Tensor, v: torch.Tensor, tok_off, rope: RopeTable | None,
+                      stream=None):
+        """append_quant of a packed batch: rows tok_off[s] .. tok_off[s + 1] - 1 of k and v [rows,
+        n_head_kv, head_dim] (f32, f16 or bf16) go to positions len[s] .. of sequence s.  rope None: K
+        is stored as it is (rotated by the caller).  Lengths do not change (increment_packed)."""
+        pk, sk = _rows(k, self.n_head_kv, self.head_dim, None, "k")
+        pv, sv = _rows(v, self.n_head_kv, self.head_dim, k.dtype, "v")
+        off, keep, _ = _offsets(tok_off, self.n_seq, min(k.shape[0], v.shape[0]))
+        self._check_device(k, v)
+        code = _dtype(k.dtype, "k")
+        _launch(self.device, stream, lambda raw: check("ts_append_packed", load().ts_append_packed(
+            self._h, layer, code, pk, sk, pv, sv, off, rope.handle if rope else None, raw)))
+
+    def read_packed(self, layer: int, row_off, pos0=None, dtype: torch.dtype = torch.float32, out: tuple | None = None,
+                    stream=None):
+        """(K, V) of the cache as the values its codes stand for: positions pos0[s] .. (None: 0 ..) of
+        sequence s in rows row_off[s] .. row_off[s + 1] - 1 of [rows, n_head_kv, head_dim], K as
+        stored (rotated).  out: a pair of such tensors to write into."""
+        off, keep, n_seq = _offsets(row_off, self.n_seq, None, "row_off")
+        p0 = None
+        if pos0 is not None:
+            if len(pos0) != self.n_seq:
+                raise ValueError(f"pos0 must hold {self.n_seq} positions")
+            if not (isinstance(pos0, torch.Tensor) and pos0.dtype == torch.int32 and not pos0.is_cuda and pos0.is_contiguous()):
+                pos0 = torch.tensor([int(p) for p in pos0], dtype=torch.int32)
+            p0 = pos0.data_ptr()
+        if out is not None:
+            dtype = out[0].dtype
+            self._check_device(*out)
+        code = _dtype(dtype, "dtype")
+
+        def call(raw):
+            rows = int(row_off[-1])
+            if out is None:
+                k, v = (torch.empty((max(rows, 0), self.n_head_kv, self.head_dim), dtype=dtype, device=self.device)
+                        for _ in range(2))
+            else:
+                k, v = out
+            pk, sk = _rows(k, self.n_head_kv, self.head_dim, dtype, "K")
+            pv, sv = _rows(v, self.n_head_kv, self.head_dim, dtype, "V")
+            if rows > min(k.shape[0], v.shape[0]):
+                raise ValueError(f"row_off ends at row {rows} of {min(k.shape[0], v.shape[0])}")
+            check("ts_read_packed", load().ts_read_packed(self._h, layer, p0, off, code, pk, sk, pv, sv, raw))
+            return k, v
+
+        return _launch(self.device, stream, call)
+
+    def increment_packed(self, tok_off, stream=None):
+        """increment of a packed batch: sequence s grows by tok_off[s + 1] - tok_off[s]."""
+        off, keep, _ = _offsets(tok_off, self.n_seq, None)
+        _launch(self.device, stream, lambda raw: check("ts_kv_increment_packed", load().ts_kv_increment_packed(self._h, off, raw)))
+
+    def _check_device(self, *tensors):
+        for t in tensors:
+            if t is not None and t.device != self.device:
+                raise ValueError(f"tensor on {t.device}, cache on {self.device}")
 
     def workspace(self, n_head: int) -> torch.Tensor:
         if n_head not in self._ws:

@@ -1,0 +1,119 @@
+"""Operators over packed prompts: the rows of all sequences one after another, sequence s owning rows
+tok_off[s] .. tok_off[s + 1] - 1 (include/turboshimmy.h, "packed batches").  The INT4 cache's side of
+them is in kv_cache.KVCache (append_packed, read_packed, increment_packed, attn_shared).
+
+tok_off is read on the host during the call: a list of ints, or a contiguous int32 CPU tensor (which
+is passed as it is).  Tensors are [rows, heads, head_dim] of float32, float16 or bfloat16; the head
+rows of a token are contiguous, the distance between tokens is free, so that a slice of the fused
+projection's rows can be passed as it is.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+
+import torch
+
+from ._lib import (TS_DTYPE_BF16, TS_DTYPE_F16, TS_DTYPE_F32, TS_ROPE_HALF, TS_ROPE_INTERLEAVED, check, load)
+
+_DTYPE = {torch.float32: TS_DTYPE_F32, torch.float16: TS_DTYPE_F16, torch.bfloat16: TS_DTYPE_BF16}
+_LAYOUT = {"interleaved": TS_ROPE_INTERLEAVED, "half": TS_ROPE_HALF}
+
+
+def _dtype(dtype: torch.dtype, what: str) -> int:
+    code = _DTYPE.get(dtype)
+    if code is None:
+        raise ValueError(f"{what} must be float32, float16 or bfloat16, got {dtype}")
+    return code
+
+
+def _rows(t: torch.Tensor, heads: int | None, head_dim: int | None, dtype: torch.dtype | None, what: str):
+    """(address, stride in elements) of [rows, heads, head_dim] with contiguous head rows."""
+    if t.dim() != 3 or (heads is not None and t.shape[1] != heads) or (head_dim is not None and t.shape[2] != head_dim):
+        raise ValueError(f"{what} must be [rows, {heads or 'heads'}, {head_dim or 'head_dim'}], got {tuple(t.shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{what} must be {dtype}, got {t.dtype}")
+    if not t.is_cuda:
+        raise ValueError(f"{what} must be a device tensor")
+    n, h, d = t.shape
+    if (d > 1 and t.stride(2) != 1) or (h > 1 and t.stride(1) != d):
+        raise ValueError(f"{what}: the heads of a token must be contiguous")
+    return ctypes.c_void_p(t.data_ptr()), t.stride(0) if n > 1 else h * d
+
+
+def _offsets(off, n_seq: int | None, n_rows: int | None, what: str = "tok_off"):
+    """(host pointer, what keeps it alive, number of sequences) of row offsets; n_rows: the most
+    rows that they may reach."""
+    if isinstance(off, torch.Tensor):
+        if off.dtype != torch.int32 or off.is_cuda or off.dim() != 1 or not off.is_contiguous():
+            raise ValueError(f"{what} must be a list of ints or a contiguous int32 CPU tensor")
+        n, last, ptr = off.numel(), None, ctypes.c_void_p(off.data_ptr())
+        if n:
+            last = int(off[-1])
+    else:
+        off = (ctypes.c_int32 * len(off))(*off)
+        n, last, ptr = len(off), off[-1] if len(off) else None, ctypes.cast(off, ctypes.c_void_p)
+    if n < 2 or (n_seq is not None and n != n_seq + 1):
+        raise ValueError(f"{what} must hold {'at least one sequence' if n_seq is None else n_seq} + 1 offsets, got {n}")
+    if n_rows is not None and last > n_rows:
+        raise ValueError(f"{what} ends at row {last} of {n_rows}")
+    return ptr, off, n - 1
+
+
+def _same_device(first: torch.Tensor, *others):
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on {first.device} and {t.device}")
+
+
+@contextlib.contextmanager
+def _on(device: torch.device, stream):
+    """The device and stream of a call as the current ones (allocations inside belong to them)."""
+    with torch.cuda.device(device):
+        if stream is None:
+            yield torch.cuda.current_stream(device).cuda_stream
+        else:
+            if stream.device != device:
+                raise ValueError(f"stream of {stream.device} for tensors on {device}")
+            with torch.cuda.stream(stream):
+                yield stream.cuda_stream
+
+
+def _plain(device: torch.device, stream) -> bool:
+    """Whether a call runs where the thread is already (the usual case: no contexts to enter)."""
+    return stream is None and device.index == torch.cuda.current_device()
+
+
+def _launch(device: torch.device, stream, call):
+    """call(stream address) on the device and the stream of the call."""
+    if _plain(device, stream):
+        return call(torch._C._cuda_getCurrentRawStream(device.index))
+    with _on(device, stream) as raw:
+        return call(raw)
+
+
+def rope_apply(x: torch.Tensor, positions: torch.Tensor, rope, layout: str = "interleaved",
+               out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """Rotary positions: the first rope.rope_dim dims of every head of x [rows, heads, head_dim]
+    rotated at the row's position (positions: [rows] int32 on the device), the rest copied.
+    layout: pairs (2i, 2i + 1), "interleaved" as everywhere else in this library, or (i, i +
+    rope_dim / 2), "half".  out may be x (in place).  A position outside the table gives NaN."""
+    if layout not in _LAYOUT:
+        raise ValueError(f"layout must be one of {sorted(_LAYOUT)}, got {layout!r}")
+    code = _dtype(x.dtype, "x")
+    px, sx = _rows(x, None, None, None, "x")
+    n, heads, hd = x.shape
+    if positions.dtype != torch.int32 or positions.shape != (n,) or (n > 1 and positions.stride(0) != 1):
+        raise ValueError("positions must be [rows] int32, contiguous")
+    _same_device(x, positions, out)
+
+    def call(raw):
+        o = torch.empty((n, heads, hd), dtype=x.dtype, device=x.device) if out is None else out
+        po, so = _rows(o, heads, hd, x.dtype, "out")
+        if o.shape[0] != n:
+            raise ValueError(f"out must have x's {n} rows, got {o.shape[0]}")
+        check("ts_rope_apply", load().ts_rope_apply(rope.handle, _LAYOUT[layout], code, px, sx, positions.data_ptr(), n,
+                                                    heads, hd, po, so, raw))
+        return o
+
+    return _launch(x.device, stream, call)

@@ -396,6 +396,60 @@ int ts_attn_out_proj_gguf(const float *d_attn, int32_t n_tok, int32_t attn_dim, 
                           int32_t dim, float *d_act, float *d_stash, void *d_workspace, uint64_t workspace_bytes,
                           void *stream);
 
+/* ---- packed batches ------------------------------------------------------------------------
+ *
+ * A server admits prompts of different lengths together: the rows of all sequences lie one after
+ * another, sequence s owning rows tok_off[s] .. tok_off[s + 1] - 1 (no counterpart in the reference,
+ * whose batch is 1).  tok_off is a HOST array of n_seq + 1 non-decreasing numbers, read
+ * during the call (a captured call keeps its values); a sequence may own no row, and rows before
+ * tok_off[0] or from tok_off[n_seq] on are neither read nor written.  A token's row holds its heads
+ * one after another, [heads][head_dim]; `stride` is the distance in elements from one token's row to
+ * the next, so that a row may be part of a wider one (the fused projection's).  First addresses and
+ * strides are multiples of 16 bytes.  All of it runs on the current device. */
+
+enum { TS_DTYPE_F32 = 0, TS_DTYPE_F16 = 1, TS_DTYPE_BF16 = 2 };
+
+/* Which dims make a pair: 2i and 2i + 1 (every other entry point), or i and i + rope_dim / 2. */
+enum { TS_ROPE_INTERLEAVED = 0, TS_ROPE_HALF = 1 };
+
+/* A rotary table stretched for long contexts, its angles computed in 64 bits (the f32 angles of
+ * ts_rope_create, the reference's, are off by up to 0.008 rad at position 131072):
+ * entry (p, i) = mult (cos, sin)(p theta_i), theta_i = base^(-2i / rope_dim) divided by factor; or,
+ * with beta > alpha, by parts: theta_i ((1 - ramp) / factor + ramp) with ramp = clamp((l_train theta_i
+ * / (2 pi) - alpha) / (beta - alpha), 0, 1), so that the pairs that turn often within the trained
+ * length l_train stay and the slow ones are stretched.  mult scales both parts of the table (a
+ * softmax temperature; 1: none).  The handle serves every entry point that takes a ts_rope.
+ * Allocates and waits: not for capture. */
+int ts_rope_create_scaled(int32_t n_pos, int32_t rope_dim, double base, double factor, int32_t l_train,
+                          double alpha, double beta, double mult, ts_rope **out);
+
+/* Rotary positions: out = x with the first rope_dim dims of every head rotated at the token's
+ * position d_pos[t] (device, int32) and the rest copied; x: n_tok rows of [n_head][head_dim].  A
+ * position outside the table makes the row's rotated dims NaN.  d_out may be d_x with the same stride
+ * (in place); any other overlap is TS_ERR_INVALID.  Products and sums are rounded to f32 one by
+ * one, the result once to dtype.  head_dim a multiple of 8. */
+int ts_rope_apply(const ts_rope *rope, int32_t layout, int32_t dtype, const void *d_x, int64_t x_stride,
+                  const int32_t *d_pos, int32_t n_tok, int32_t n_head, int32_t head_dim, void *d_out,
+                  int64_t out_stride, void *stream);
+
+/* ts_append_quant for a packed batch: row tok_off[s] + t of sequence s goes to position len[s] + t.
+ * Codes and scales are those of the rows widened to f32.  With rope, K is normalized (QK norm, when
+ * set) and rotated first; with NULL it is taken as it is to be stored (ts_rope_apply's output).
+ * TS_ERR_OVERFLOW if a sequence would pass max_seq; lengths do not change
+ * (ts_kv_increment_packed). */
+int ts_append_packed(ts_kv *kv, int32_t layer, int32_t dtype, const void *d_k, int64_t k_stride, const void *d_v,
+                     int64_t v_stride, const int32_t *tok_off, const ts_rope *rope, void *stream);
+
+/* The cache read back into packed rows: positions pos0[s] .. of sequence s (host array; NULL: from
+ * 0) into rows row_off[s] .. row_off[s + 1] - 1 of K and V, each value (code - 8) * scale rounded to
+ * f32 and then to dtype; K as stored, rotated.  A position at or past max_seq is TS_ERR_INVALID;
+ * one that nothing was written to reads as whatever the cache holds there (zeros at first). */
+int ts_read_packed(const ts_kv *kv, int32_t layer, const int32_t *pos0, const int32_t *row_off, int32_t dtype,
+                   void *d_k, int64_t k_stride, void *d_v, int64_t v_stride, void *stream);
+
+/* ts_kv_increment for a packed batch: sequence s grows by tok_off[s + 1] - tok_off[s] positions. */
+int ts_kv_increment_packed(ts_kv *kv, const int32_t *tok_off, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
