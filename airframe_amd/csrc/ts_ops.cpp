@@ -7,6 +7,7 @@
 #include <new>
 
 #include "ts_host.h"
+#include "ts_prompt.h"
 
 using namespace ts;
 
@@ -122,6 +123,59 @@ int ts_kv_increment_packed(ts_kv *kv, const int32_t *tok_off, void *stream) {
     if (e != hipSuccess) return TS_ERR_HIP;
     for (int s = 0; s < kv->d.n_seq; s++) kv->h_len[s] += tok_off[s + 1] - tok_off[s];
     return TS_OK;
+}
+
+int ts_attn_prompt_workspace(int32_t dtype, int32_t n_rows, int32_t n_head_kv, int32_t head_dim, uint64_t *bytes) {
+    if (!bytes || !dtype_ok(dtype) || n_rows < 0 || n_head_kv <= 0 || n_head_kv > 65536 || head_dim <= 0 || head_dim % 8 != 0)
+        return TS_ERR_INVALID;
+    if (head_dim > 256) return TS_ERR_UNSUPPORTED;
+    *bytes = prompt_workspace(dtype, n_rows, n_head_kv, head_dim);
+    return TS_OK;
+}
+
+int ts_attn_prompt(int32_t dtype, const void *d_q, int64_t q_stride, const void *d_k, int64_t k_stride, const void *d_v,
+                   int64_t v_stride, const int32_t *tok_off, int32_t n_seq, int32_t n_head, int32_t n_head_kv,
+                   int32_t head_dim, float softcap, void *d_out, int64_t out_stride, void *d_workspace,
+                   uint64_t workspace_bytes, void *stream) {
+    if (!dtype_ok(dtype) || n_seq < 0 || n_head_kv <= 0 || n_head <= 0 || n_head > 65536 || n_head % n_head_kv != 0 ||
+        head_dim <= 0 || head_dim % 8 != 0 || !(softcap >= 0.0f) || !std::isfinite(softcap) || !offsets_ok(tok_off, n_seq))
+        return TS_ERR_INVALID;
+    if (head_dim > 256) return TS_ERR_UNSUPPORTED;
+    const int64_t rows = (int64_t)tok_off[n_seq] - tok_off[0];
+    if (rows == 0) return TS_OK;
+    const int64_t qrow = (int64_t)n_head * head_dim, krow = (int64_t)n_head_kv * head_dim;
+    if (!rows_ok(d_q, q_stride, qrow, dtype) || !rows_ok(d_k, k_stride, krow, dtype) || !rows_ok(d_v, v_stride, krow, dtype) ||
+        !rows_ok(d_out, out_stride, qrow, dtype))
+        return TS_ERR_INVALID;
+    // a token's rows are read by the workgroups of later tokens: the output is apart from all inputs
+    const int size = dtype_size(dtype);
+    auto span = [&](const void *p, int64_t stride, int64_t row, int end) {
+        return (uintptr_t)p + (uintptr_t)((end ? (tok_off[n_seq] - 1) * stride + row : tok_off[0] * stride) * size);
+    };
+    const uintptr_t o0 = span(d_out, out_stride, qrow, 0), o1 = span(d_out, out_stride, qrow, 1);
+    auto apart = [&](const void *p, int64_t stride, int64_t row) { return span(p, stride, row, 1) <= o0 || o1 <= span(p, stride, row, 0); };
+    if (!apart(d_q, q_stride, qrow) || !apart(d_k, k_stride, krow) || !apart(d_v, v_stride, krow)) return TS_ERR_INVALID;
+    const uint64_t need = prompt_workspace(dtype, rows, n_head_kv, head_dim);
+    if (need > 0 && (!d_workspace || workspace_bytes < need)) return TS_ERR_WORKSPACE;
+    if (need > 0 && !aligned16(d_workspace)) return TS_ERR_INVALID;
+    PromptCall c;
+    c.dtype = dtype;
+    c.q = d_q;
+    c.k = d_k;
+    c.v = d_v;
+    c.out = d_out;
+    c.q_stride = q_stride;
+    c.k_stride = k_stride;
+    c.v_stride = v_stride;
+    c.out_stride = out_stride;
+    c.off = tok_off;
+    c.n_seq = n_seq;
+    c.n_head = n_head;
+    c.n_kv = n_head_kv;
+    c.hd = head_dim;
+    c.softcap = softcap;
+    c.ws = d_workspace;
+    return hip_status(launch_prompt(c, as_stream(stream)));
 }
 
 }  // extern "C"

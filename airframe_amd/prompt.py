@@ -117,3 +117,49 @@ def rope_apply(x: torch.Tensor, positions: torch.Tensor, rope, layout: str = "in
         return o
 
     return _launch(x.device, stream, call)
+
+
+def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tok_off, softcap: float = 0.0,
+                out: torch.Tensor | None = None, workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """Causal attention over a packed batch of prompts: rows tok_off[s] .. tok_off[s + 1] - 1 of q
+    [rows, n_head, head_dim], k and v [rows, n_head_kv, head_dim] (rotated where the model rotates;
+    f32, f16 or bf16) are sequence s.  Rows outside the offsets are left as they are (zeros in an out
+    allocated here).  workspace: uint8 of attn_prompt_workspace bytes (f32 only; None: allocated)."""
+    code = _dtype(q.dtype, "q")
+    pq, sq = _rows(q, None, None, None, "q")
+    n, heads, hd = q.shape
+    pk, sk = _rows(k, None, hd, q.dtype, "k")
+    kv = k.shape[1]
+    pv, sv = _rows(v, kv, hd, q.dtype, "v")
+    off, keep, n_seq = _offsets(tok_off, None, min(n, k.shape[0], v.shape[0]))
+    _same_device(q, k, v, out, workspace)
+
+    def call(raw):
+        first, last = int(tok_off[0]), int(tok_off[-1])
+        o = out
+        if o is None:
+            o = torch.empty((n, heads, hd), dtype=q.dtype, device=q.device)
+            if first > 0:
+                o[:first].zero_()
+            if last < n:
+                o[max(last, 0):].zero_()
+        po, so = _rows(o, heads, hd, q.dtype, "out")
+        if o.shape[0] < last:
+            raise ValueError(f"out has {o.shape[0]} rows, tok_off ends at {last}")
+        ws = workspace
+        if ws is None and q.dtype == torch.float32:
+            ws = torch.empty(attn_prompt_workspace(q.dtype, max(last - first, 0), kv, hd), dtype=torch.uint8, device=q.device)
+        check("ts_attn_prompt", load().ts_attn_prompt(code, pq, sq, pk, sk, pv, sv, off, n_seq, heads, kv, hd, softcap, po, so,
+                                                      ws.data_ptr() if ws is not None else None,
+                                                      ws.numel() if ws is not None else 0, raw))
+        return o
+
+    return _launch(q.device, stream, call)
+
+
+def attn_prompt_workspace(dtype: torch.dtype, n_rows: int, n_head_kv: int, head_dim: int) -> int:
+    """Bytes of scratch that attn_prompt needs for n_rows rows in all."""
+    b = ctypes.c_uint64()
+    check("ts_attn_prompt_workspace",
+          load().ts_attn_prompt_workspace(_dtype(dtype, "dtype"), n_rows, n_head_kv, head_dim, ctypes.byref(b)))
+    return b.value

@@ -450,6 +450,23 @@ int ts_read_packed(const ts_kv *kv, int32_t layer, const int32_t *pos0, const in
 /* ts_kv_increment for a packed batch: sequence s grows by tok_off[s + 1] - tok_off[s] positions. */
 int ts_kv_increment_packed(ts_kv *kv, const int32_t *tok_off, void *stream);
 
+/* Bytes of scratch ts_attn_prompt needs for n_rows rows in all (0 but for f32).  Host only. */
+int ts_attn_prompt_workspace(int32_t dtype, int32_t n_rows, int32_t n_head_kv, int32_t head_dim, uint64_t *bytes);
+
+/* Causal attention over a packed batch of whole prompts: token t of a sequence attends to tokens
+ * 0 .. t of the same one (main_attn_out's formula, sh_layer_v1.wgsl:662-762, over rows that are
+ * already rotated): out_t = softmax(cap(q_t k_j / sqrt(head_dim))) v_j, cap(x) = softcap tanh(x /
+ * softcap) with softcap > 0.  d_q, d_out: rows of [n_head][head_dim], d_k, d_v: of
+ * [n_head_kv][head_dim]; n_head a multiple of n_head_kv; head_dim a multiple of 8 up to 256; d_out
+ * apart from the inputs (else TS_ERR_INVALID).  f16 and bf16 are multiplied as they are, the
+ * probabilities rounded to the same type; f32 at 22 bits of every factor.  Scores, softmax and sums
+ * are f32.  What a token does not attend to has no part in its output, infinities and NaN
+ * included.  d_workspace: ts_attn_prompt_workspace bytes of tok_off[n_seq] - tok_off[0] rows. */
+int ts_attn_prompt(int32_t dtype, const void *d_q, int64_t q_stride, const void *d_k, int64_t k_stride,
+                   const void *d_v, int64_t v_stride, const int32_t *tok_off, int32_t n_seq, int32_t n_head,
+                   int32_t n_head_kv, int32_t head_dim, float softcap, void *d_out, int64_t out_stride,
+                   void *d_workspace, uint64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
