@@ -95,6 +95,9 @@ SIGNATURES = {
     "ts_append_packed": (ctypes.c_int, [_vp, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _vp]),
     "ts_read_packed": (ctypes.c_int, [_vp, _i32, _vp, _vp, _i32, _vp, _i64, _vp, _i64, _vp]),
     "ts_kv_increment_packed": (ctypes.c_int, [_vp, _vp, _vp]),
+    "ts_attn_shared_workspace": (ctypes.c_int, [_vp, _vp, _i32, _i32, _u64p]),
+    "ts_attn_shared": (ctypes.c_int, [_vp, _vp, _i32, _i32, _vp, _vp, _vp, _i32, _i32, _vp, _f, _vp, _vp, ctypes.c_uint64,
+                                      _vp]),
     "ts_attn_prompt_workspace": (ctypes.c_int, [_i32, _i32, _i32, _i32, _u64p]),
     "ts_attn_prompt": (ctypes.c_int, [_i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _f, _vp, _i64,
                                       _vp, ctypes.c_uint64, _vp]),

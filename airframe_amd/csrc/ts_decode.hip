@@ -62,6 +62,10 @@ struct DecodeArgs {
     // Fused append (ts_attn_decode_append): the new token's raw K and V, [S][H][hd], or null.
     const float *k_new, *v_new;
 
+    // The caller joins the partials itself (attention behind a shared prefix): they are written also
+    // without a split, and no combine kernel follows.
+    bool keep;
+
     // ts_attn_decode_append_advance: the lengths to advance by one (the array len points to)
     // and the arrival counter of the kernel that does it, or null.
     int32_t *adv_len;
@@ -706,7 +710,7 @@ __global__ __launch_bounds__(64 * NW, NW > 4 ? 1 : (HD > 128 ? 1 : 2)) void deco
             lsum += e;
         }
         const size_t head = (size_t)s * a.n_head + hb + hh;
-        if (n_split_s == 1) {
+        if (n_split_s == 1 && !a.keep) {
             // hdr is a multiple of 8: a float4 of dims lies wholly inside or outside the row
             if (d < hdr) {
                 const float inv = lsum > 0.0f ? 1.0f / lsum : 0.0f;
@@ -1378,7 +1382,7 @@ windows_done:
             lsum += e;
         }
         const size_t head = (size_t)s * a.n_head + h * G + hh;
-        if (n_split_s == 1) {
+        if (n_split_s == 1 && !a.keep) {
             // hdr is a multiple of 8: a float4 of dims lies wholly inside or outside the row
             const float inv = lsum > 0.0f ? 1.0f / lsum : 0.0f;
             if (d < hdr) {
@@ -1705,8 +1709,9 @@ void launch_integer(const DecodeArgs &a, int n_split, bool pad, int Gt, hipStrea
 hipError_t launch_decode(const KvLayerView &L, int32_t *d_len, const int32_t *h_len, const float *q, int n_head,
                          const float *rope, int rope_pairs, float softcap, float *out,
                          float *ws, const DecodePlan &plan, const float *k_new,
-                         const float *v_new, int32_t *adv, hipStream_t st) {
+                         const float *v_new, int32_t *adv, hipStream_t st, bool keep) {
     DecodeArgs a;
+    a.keep = keep;
     a.L = L;
     a.len = d_len;
     a.hlen = h_len && L.S == 1 ? h_len[0] : -1;
@@ -1744,13 +1749,13 @@ hipError_t launch_decode(const KvLayerView &L, int32_t *d_len, const int32_t *h_
          : (norm ? TS_SPLIT(HDV, false, true) : TS_SPLIT(HDV, false, false)))
     if (L.hd == 256) {
         TS_SPLIT_HD(256);
-        if (plan.n_split > 1) decode_combine_kernel<256><<<dim3(n_head, L.S), 256, 0, st>>>(a);
+        if (plan.n_split > 1 && !keep) decode_combine_kernel<256><<<dim3(n_head, L.S), 256, 0, st>>>(a);
     } else if (L.hd == 128) {
         TS_SPLIT_HD(128);
-        if (plan.n_split > 1) decode_combine_kernel<128><<<dim3(n_head, L.S), 256, 0, st>>>(a);
+        if (plan.n_split > 1 && !keep) decode_combine_kernel<128><<<dim3(n_head, L.S), 256, 0, st>>>(a);
     } else if (L.hd == 64) {
         TS_SPLIT_HD(64);
-        if (plan.n_split > 1) decode_combine_kernel<64><<<dim3(n_head, L.S), 256, 0, st>>>(a);
+        if (plan.n_split > 1 && !keep) decode_combine_kernel<64><<<dim3(n_head, L.S), 256, 0, st>>>(a);
     } else {
         return hipErrorInvalidValue;
     }

@@ -8,6 +8,7 @@
 
 #include "ts_host.h"
 #include "ts_prompt.h"
+#include "ts_shared.h"
 
 using namespace ts;
 
@@ -176,6 +177,96 @@ int ts_attn_prompt(int32_t dtype, const void *d_q, int64_t q_stride, const void 
     c.softcap = softcap;
     c.ws = d_workspace;
     return hip_status(launch_prompt(c, as_stream(stream)));
+}
+
+// Partials of a call: the prefix's pieces (and one of the own keys for a chunk), then the decode
+// kernel's.
+static uint64_t shared_part_floats(const ts_kv *kv, int32_t n_head, int32_t n_tok, int slots) {
+    return (uint64_t)kv->d.n_seq * n_tok * n_head * slots * (kv->hdp + 2);
+}
+
+static bool shared_shape_ok(const ts_kv *kv, const ts_kv *prefix, int32_t n_head, int32_t n_tok) {
+    return kv && prefix && kv != prefix && heads_ok(kv, n_head) && n_head <= 65536 && n_tok >= 0 &&
+           (int64_t)kv->d.n_seq * n_tok * n_head <= INT32_MAX && kv->d.n_head_kv == prefix->d.n_head_kv &&
+           kv->d.head_dim == prefix->d.head_dim && kv->device == prefix->device;
+}
+
+int ts_attn_shared_workspace(const ts_kv *kv, const ts_kv *prefix, int32_t n_head, int32_t n_tok, uint64_t *bytes) {
+    if (!bytes || !shared_shape_ok(kv, prefix, n_head, n_tok)) return TS_ERR_INVALID;
+    *bytes = 0;
+    if (n_tok == 0) return TS_OK;
+    const int cap = shared_parts_cap(kv->d.n_seq * n_tok, n_head / kv->d.n_head_kv, kv->d.n_head_kv, prefix->d.max_seq, kv->hdp,
+                                     kv->n_cu);
+    uint64_t n = shared_part_floats(kv, n_head, n_tok, cap + (n_tok > 1)) * sizeof(float);
+    if (n_tok == 1) {
+        uint64_t own;
+        ts_attn_decode_workspace(kv, n_head, &own);
+        n += own;
+    }
+    *bytes = n;
+    return TS_OK;
+}
+
+int ts_attn_shared(ts_kv *kv, const ts_kv *prefix, int32_t prefix_seq, int32_t layer, const float *d_k, const float *d_v,
+                   const float *d_q, int32_t n_head, int32_t n_tok, const ts_rope *rope, float softcap, float *d_out,
+                   void *d_workspace, uint64_t workspace_bytes, void *stream) {
+    if (!shared_shape_ok(kv, prefix, n_head, n_tok) || layer < 0 || layer >= kv->d.n_layers || layer >= prefix->d.n_layers ||
+        prefix_seq < 0 || prefix_seq >= prefix->d.n_seq || !(softcap >= 0.0f) || !std::isfinite(softcap) ||
+        (d_k == nullptr) != (d_v == nullptr) || (d_k && n_tok != 1) || !aligned16(d_k) || !aligned16(d_v))
+        return TS_ERR_INVALID;
+    if (n_tok == 0) return TS_OK;
+    if (!d_q || !d_out || !aligned16(d_q) || !aligned16(d_out)) return TS_ERR_INVALID;
+    // the own positions continue the prefix's: slot p of a sequence is position window base + p
+    const int P = prefix->h_len[prefix_seq];
+    for (int s = 0; s < kv->d.n_seq; s++) {
+        if (kv->h_rot[s] < P) return TS_ERR_INVALID;
+        if ((int64_t)kv->h_len[s] + n_tok > kv->d.max_seq) return TS_ERR_OVERFLOW;
+    }
+    const int rc = check_rope(rope, kv->d.head_dim, rot_end(kv, n_tok));
+    if (rc) return rc;
+    if (P == 0)
+        return n_tok > 1 ? ts_attn_prefill(kv, layer, d_q, n_head, n_tok, rope, softcap, d_out, stream)
+               : d_k     ? ts_attn_decode_append(kv, layer, d_k, d_v, d_q, n_head, rope, softcap, d_out, d_workspace,
+                                                 workspace_bytes, stream)
+                         : ts_attn_decode(kv, layer, d_q, n_head, rope, softcap, d_out, d_workspace, workspace_bytes, stream);
+    uint64_t need;
+    ts_attn_shared_workspace(kv, prefix, n_head, n_tok, &need);
+    if (!d_workspace || workspace_bytes < need) return TS_ERR_WORKSPACE;
+    if (!aligned16(d_workspace)) return TS_ERR_INVALID;
+
+    SharedCall c;
+    c.own = kv->layer(layer);
+    c.pre = prefix->layer(layer);
+    c.prefix_seq = prefix_seq;
+    c.prefix_len = P;
+    c.d_len = kv->d_len;
+    c.q = d_q;
+    c.n_head = n_head;
+    c.n_tok = n_tok;
+    c.rope = rope->d_table;
+    c.rope_pairs = rope->rope_dim / 2;
+    c.rope_rows = rope->n_pos;
+    c.softcap = softcap;
+    c.out = d_out;
+    const int G = n_head / kv->d.n_head_kv;
+    c.plan = shared_plan(kv->d.n_seq * n_tok, G, kv->d.n_head_kv, P, kv->hdp, kv->n_cu);
+    c.part = static_cast<float *>(d_workspace);
+    c.own_part = nullptr;
+    c.own_plan = DecodePlan{1, 1, false, 4, 1};
+    c.hlen = -1;
+    const hipStream_t st = as_stream(stream);
+    if (n_tok == 1) {
+        float *own = c.part + shared_part_floats(kv, n_head, 1, c.plan.n_part);
+        for (int s = 0; s < kv->d.n_seq; s++) kv->h_ctx[s] = kv->h_len[s] + 1;
+        c.own_plan = decode_plan(kv->h_ctx.data(), kv->d.n_seq, kv->d.n_head_kv, G, kv->n_cu, kv->hdp, d_k != nullptr);
+        c.own_part = own;
+        const int32_t *h_len = capturing(stream) || kv->len_captured ? nullptr : kv->h_len.data();
+        if (h_len && kv->d.n_seq == 1) c.hlen = h_len[0];
+        const hipError_t e = launch_decode(c.own, kv->d_len, h_len, d_q, n_head, c.rope, c.rope_pairs, softcap, d_out, own,
+                                           c.own_plan, d_k, d_v, nullptr, st, true);
+        if (e != hipSuccess) return TS_ERR_HIP;
+    }
+    return hip_status(launch_shared(c, st));
 }
 
 }  // extern "C"

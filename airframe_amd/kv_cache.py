@@ -292,6 +292,54 @@ class KVCache:
         off, keep, _ = _offsets(tok_off, self.n_seq, None)
         _launch(self.device, stream, lambda raw: check("ts_kv_increment_packed", load().ts_kv_increment_packed(self._h, off, raw)))
 
+    # ---- a prefix shared by the batch ----------------------------------------------------------
+
+    def share_prefix(self, prefix: "KVCache", prefix_seq: int = 0, stream=None):
+        """Makes every (empty) sequence continue sequence prefix_seq of `prefix`: its slot p is
+        position P + p from then on (advance_window_base).  attn_shared then attends over both."""
+        n = prefix.get_seq_len(prefix_seq)
+        if any(self.seq_lens()) or any(self.get_window_base(s) for s in range(self.n_seq)):
+            raise ValueError("share_prefix needs empty sequences (reset)")
+        for s in range(self.n_seq):
+            self.advance_window_base(n, s, stream)
+
+    def attn_shared_workspace(self, prefix: "KVCache", n_head: int, n_tok: int = 1) -> int:
+        """Bytes of scratch attn_shared needs for this shape."""
+        b = ctypes.c_uint64()
+        check("ts_attn_shared_workspace",
+              load().ts_attn_shared_workspace(self._h, prefix.handle, n_head, n_tok, ctypes.byref(b)))
+        return b.value
+
+    def attn_shared(self, layer: int, q: torch.Tensor, rope: RopeTable, prefix: "KVCache", prefix_seq: int = 0,
+                    k: torch.Tensor | None = None, v: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                    softcap: float = 0.0, workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+        """Attention of every sequence's new tokens over the shared prefix and their own keys
+        (ts_attn_shared).  q: [n_seq, n_tok, n_head, head_dim] f32, the tokens appended before; or,
+        with n_tok 1, k and v [n_seq, 1, n_head_kv, head_dim] to append in the same launch."""
+        if q.dim() != 4 or q.shape[0] != self.n_seq or q.shape[3] != self.head_dim:
+            raise ValueError("q must be [n_seq, n_tok, n_head, head_dim]")
+        if (k is None) != (v is None):
+            raise ValueError("k and v come together")
+        n_tok, n_head = q.shape[1], q.shape[2]
+        pq = _ptr(q, torch.float32, "q")
+        pk = pv = None
+        if k is not None:
+            self._check_kv(k, v, 1)
+            pk, pv = _ptr(k, torch.float32, "k"), _ptr(v, torch.float32, "v")
+        self._check_device(q, k, v, out, workspace)
+
+        def call(raw):
+            o = self._out_like(q, out)
+            ws = workspace
+            if ws is None:
+                ws = torch.empty(self.attn_shared_workspace(prefix, n_head, n_tok), dtype=torch.uint8, device=self.device)
+            check("ts_attn_shared", load().ts_attn_shared(self._h, prefix.handle, prefix_seq, layer, pk, pv, pq, n_head, n_tok,
+                                                          rope.handle, softcap, _ptr(o, torch.float32, "out"), ws.data_ptr(),
+                                                          ws.numel(), raw))
+            return o
+
+        return _launch(self.device, stream, call)
+
     def _check_device(self, *tensors):
         for t in tensors:
             if t is not None and t.device != self.device:

@@ -467,6 +467,31 @@ int ts_attn_prompt(int32_t dtype, const void *d_q, int64_t q_stride, const void 
                    int32_t n_head_kv, int32_t head_dim, float softcap, void *d_out, int64_t out_stride,
                    void *d_workspace, uint64_t workspace_bytes, void *stream);
 
+/* ---- a prefix shared by a batch ---------------------------------------------------------------
+ *
+ * A long system prompt or document that every sequence of a batch starts with is cached once, as
+ * one sequence of a cache of its own (ts_append_quant, ts_append_packed, ts_kv_increment).  The batch's
+ * cache holds only what follows: slot p of a sequence is position P + p, P the prefix's length, which
+ * ts_kv_advance_window_base(kv, s, P) on an empty sequence sets up; every entry point that appends
+ * then rotates K there.  (A window compacted later keeps working with keep_sink 0: the prefix stays,
+ * the own keys move.) */
+
+/* Bytes of scratch ts_attn_shared needs, for any length of the prefix's cache.  Host only. */
+int ts_attn_shared_workspace(const ts_kv *kv, const ts_kv *prefix, int32_t n_head, int32_t n_tok, uint64_t *bytes);
+
+/* Attention of n_tok new tokens of every sequence over the shared prefix (all positions of sequence
+ * prefix_seq of `prefix`) and over the sequence's own keys, causal: token t sits in slot len[s] + t,
+ * appended before as for ts_attn_prefill / ts_attn_decode.  The prefix is read and multiplied once for
+ * the batch.  d_q, d_out: [n_seq][n_tok][n_head][head_dim]; q is normalized (kv's QK norm) and
+ * rotated at its position like there.  With n_tok 1, d_k and d_v: NULL, or the new token's K and V
+ * [n_seq][n_head_kv][head_dim], appended in the same launch (ts_attn_decode_append).  Both caches have
+ * the same heads, head_dim and device; every window base has to be P or more (TS_ERR_INVALID).  The
+ * prefix's length is taken at the call, also into a graph.  d_workspace: ts_attn_shared_workspace
+ * bytes, 16-byte aligned. */
+int ts_attn_shared(ts_kv *kv, const ts_kv *prefix, int32_t prefix_seq, int32_t layer, const float *d_k,
+                   const float *d_v, const float *d_q, int32_t n_head, int32_t n_tok, const ts_rope *rope,
+                   float softcap, float *d_out, void *d_workspace, uint64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
