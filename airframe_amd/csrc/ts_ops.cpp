@@ -195,9 +195,8 @@ int ts_attn_shared_workspace(const ts_kv *kv, const ts_kv *prefix, int32_t n_hea
     if (!bytes || !shared_shape_ok(kv, prefix, n_head, n_tok)) return TS_ERR_INVALID;
     *bytes = 0;
     if (n_tok == 0) return TS_OK;
-    const int cap = shared_parts_cap(kv->d.n_seq * n_tok, n_head / kv->d.n_head_kv, kv->d.n_head_kv, prefix->d.max_seq, kv->hdp,
-                                     kv->n_cu);
-    uint64_t n = shared_part_floats(kv, n_head, n_tok, cap + (n_tok > 1)) * sizeof(float);
+    const int cap = shared_slots_cap(kv->d.n_seq, n_tok, n_head / kv->d.n_head_kv, kv->d.n_head_kv, prefix->d.max_seq, kv->n_cu);
+    uint64_t n = shared_part_floats(kv, n_head, n_tok, cap) * sizeof(float);
     if (n_tok == 1) {
         uint64_t own;
         ts_attn_decode_workspace(kv, n_head, &own);
@@ -231,8 +230,8 @@ int ts_attn_shared(ts_kv *kv, const ts_kv *prefix, int32_t prefix_seq, int32_t l
                          : ts_attn_decode(kv, layer, d_q, n_head, rope, softcap, d_out, d_workspace, workspace_bytes, stream);
     uint64_t need;
     ts_attn_shared_workspace(kv, prefix, n_head, n_tok, &need);
-    if (!d_workspace || workspace_bytes < need) return TS_ERR_WORKSPACE;
-    if (!aligned16(d_workspace)) return TS_ERR_INVALID;
+    if (need > 0 && (!d_workspace || workspace_bytes < need)) return TS_ERR_WORKSPACE;
+    if (need > 0 && !aligned16(d_workspace)) return TS_ERR_INVALID;
 
     SharedCall c;
     c.own = kv->layer(layer);
@@ -249,7 +248,7 @@ int ts_attn_shared(ts_kv *kv, const ts_kv *prefix, int32_t prefix_seq, int32_t l
     c.softcap = softcap;
     c.out = d_out;
     const int G = n_head / kv->d.n_head_kv;
-    c.plan = shared_plan(kv->d.n_seq * n_tok, G, kv->d.n_head_kv, P, kv->hdp, kv->n_cu);
+    c.plan = shared_plan(kv->d.n_seq, n_tok, G, kv->d.n_head_kv, P, kv->hdp, kv->n_cu);
     c.part = static_cast<float *>(d_workspace);
     c.own_part = nullptr;
     c.own_plan = DecodePlan{1, 1, false, 4, 1};

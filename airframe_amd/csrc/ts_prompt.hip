@@ -16,6 +16,8 @@
 // Scores, maxima, sums and outputs are f32 until the output is rounded once.
 #include "ts_prompt.h"
 
+#include <type_traits>
+
 #include "ts_mfma.h"
 
 namespace ts {
@@ -68,16 +70,12 @@ __device__ inline int kslot(int r, int c) { return c ^ (r & (CPR < 16 ? CPR - 1 
 template <int CPR>
 __device__ inline int vslot(int r, int c) { return c ^ (CPR < 16 ? (r & 1) << 2 : (r & 3) << 2); }
 
-// The 8 keys of one lane of a 16-key step, of one dim (lane % 32 of tile db): rows 4h .. and 8 + 4h ..
-// of the step.  Each group of 16 lanes reads 4 rows x 16 dims and gets them transposed.
-template <class T, int CPR>
-__device__ inline typename Vec8<T>::type v_operand(const u32x4 *tile, int row0, int chunk0, int lane) {
-    const int i = lane & 15, r = row0 + 4 * (lane >> 5) + (i >> 2), c = chunk0 + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+// The 8 keys of one lane of a 16-key step, of one dim: 4 rows at p and 4 rows 8 further on.  Each group
+// of 16 lanes points at 4 rows x 16 dims and gets them transposed.
+template <class T, int ROWB>
+__device__ inline typename Vec8<T>::type v_operand(const unsigned char *p) {
     typedef __attribute__((address_space(3))) short4v *lds4;
-    auto at = [&](int row) {
-        return (lds4)(reinterpret_cast<const short4v *>(tile + row * CPR + vslot<CPR>(row, c)) + (i & 1));
-    };
-    const short4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(r)), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(r + 8));
+    const short4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 8 * ROWB));
     const short8v s = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     return __builtin_bit_cast(typename Vec8<T>::type, s);
 }
@@ -104,24 +102,44 @@ __device__ inline typename Vec8<T>::type bad_part(typename Vec8<T>::type v, int 
     return v;
 }
 
+// One tile of 64 lanes x 16 bytes from memory straight into LDS: lane l's 16 bytes at byte voff of the
+// buffer (0s past its end) go to lds + 16 l.  In asm because the compiler would make every LDS read
+// wait for all such loads; it has no outputs, and tile_barrier() waits for it.
+__device__ inline void load_lds(const u32x4 &rsrc, uint32_t voff, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "s"(lds)
+                 : "memory");
+}
+// All loads into LDS of this wave have landed, and every wave of the workgroup got here.
+__device__ inline void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// A buffer of `bytes` from p on; reads past it give 0.
+__device__ inline u32x4 buffer_of(const void *p, int64_t bytes) {
+    const uint64_t a = (uint64_t)p;
+    u32x4 r = {(uint32_t)a, (uint32_t)(a >> 32) & 0xFFFFu, (uint32_t)min(bytes, (int64_t)0xFFFFFFFF), 0x00027000u};
+#pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = __builtin_amdgcn_readfirstlane(r[i]);
+    return r;
+}
+
 // T: the matrix cores' type; O: the rows' type (float with two planes); HD: head dims, padded; NP:
 // planes; KT: keys per tile.
 template <class T, class O, int HD, int NP, int KT, bool SOFTCAP>
 __global__ __launch_bounds__(64 * kPromptNW, HD * NP > 128 ? 1 : 2) void prompt_kernel(PromptArgs a) {
     using V8 = typename Vec8<T>::type;
     constexpr int CPR = NP * HD / 8;  // 16-byte chunks of a tile's row
+    constexpr int ROWB = 16 * CPR, TILEB = KT * ROWB;
     constexpr int NKS = HD / 16, NDB = HD / 32, NKB = KT / 32;
-    constexpr int NT = 64 * kPromptNW, NPC = KT * CPR / NT;  // pieces of a tile per thread
-    constexpr bool F16 = sizeof(T) == 2 && __is_same(T, _Float16);
-    static_assert(KT * CPR % NT == 0 && NPC > 0, "a tile's pieces spread evenly");
-    extern __shared__ __align__(16) unsigned char pr_smem[];
-    u32x4 *const kt = reinterpret_cast<u32x4 *>(pr_smem);  // [2][KT][CPR]
-    u32x4 *const vt = kt + 2 * KT * CPR;
-    float *const se = reinterpret_cast<float *>(vt + 2 * KT * CPR);  // two planes: [2][2][KT] K and V exponents
+    constexpr int NW = kPromptNW, NLD = TILEB / 1024 / NW;  // loads of 1 KB of a tile per wave
+    constexpr bool F16 = __is_same(T, _Float16);
+    constexpr bool RAW = NP == 1 && !SOFTCAP;  // scores stay unscaled until the exponent's FMA
+    static_assert(TILEB % (1024 * NW) == 0, "a tile's loads spread evenly");
+    // [2 buffers] K tile, V tile; then, of two planes, [2][2][KT] K scales and V exponents
+    extern __shared__ __align__(1024) unsigned char pr_smem[];
+    float *const se = reinterpret_cast<float *>(pr_smem + 4 * TILEB);
 
     const int item = blockIdx.x / a.H, h = blockIdx.x - item * a.H;
     const int i = pack_find(a.t, item);
-    const int row0 = a.t.tok[i], n = a.t.tok[i + 1] - row0;
+    const int row0 = a.t.tok[i], n = a.t.pos0[i];  // (rows of the i-th sequence: pos0)
     const int G = a.G, n_cols = n * G;
     const int cblk = a.t.item[i + 1] - 1 - item;  // later tokens, the longer walks, first
     const int tid = threadIdx.x, lane = tid & 63;
@@ -136,42 +154,52 @@ __global__ __launch_bounds__(64 * kPromptNW, HD * NP > 128 ? 1 : 2) void prompt_
     const int hd = a.hd;
     const int n_chunk = hd / 8;
 
-    // Tiles through registers into LDS.
-    u32x4 pk[NPC], pv[NPC];
-    float pe = 0.0f;
-    auto fetch = [&](int base) __attribute__((always_inline)) {
+    // Loads of a tile: wave w's p-th takes 1 KB of it, 1024 / ROWB rows; the lane's slot in its row holds
+    // the chunk that kslot / vslot put there.
+    const uint8_t *kbase, *vbase;
+    int64_t kstride, vstride;  // bytes from key to key
+    if constexpr (NP == 1) {
+        kbase = reinterpret_cast<const uint8_t *>(static_cast<const T *>(a.k) + (int64_t)row0 * a.ks + (int64_t)h * hd);
+        vbase = reinterpret_cast<const uint8_t *>(static_cast<const T *>(a.v) + (int64_t)row0 * a.vs + (int64_t)h * hd);
+        kstride = 2 * a.ks;
+        vstride = 2 * a.vs;
+    } else {
+        const int64_t at = ((row0 - a.row0) * a.H + h) * (int64_t)(NP * HD);
+        kbase = reinterpret_cast<const uint8_t *>(a.kp + at);
+        vbase = reinterpret_cast<const uint8_t *>(a.vp + at);
+        kstride = vstride = (int64_t)a.H * ROWB;
+    }
+    uint32_t ko[NLD], vo[NLD];
 #pragma unroll
-        for (int p = 0; p < NPC; p++) {
-            const int idx = tid + NT * p, r = idx / CPR, ch = idx % CPR;
-            const int64_t row = row0 + min(base + r, n - 1);  // (keys past the end are masked)
-            if constexpr (NP == 1) {
-                // (chunks past the row repeat its last: q is 0 there, and those outputs are dropped)
-                const int cl = min(ch, n_chunk - 1);
-                pk[p] = *reinterpret_cast<const u32x4 *>(static_cast<const T *>(a.k) + row * a.ks + (int64_t)h * hd + 8 * cl);
-                pv[p] = *reinterpret_cast<const u32x4 *>(static_cast<const T *>(a.v) + row * a.vs + (int64_t)h * hd + 8 * cl);
-            } else {
-                const int64_t at = ((row - a.row0) * a.H + h) * (NP * HD) + 8 * ch;
-                pk[p] = *reinterpret_cast<const u32x4 *>(a.kp + at);
-                pv[p] = *reinterpret_cast<const u32x4 *>(a.vp + at);
-            }
-        }
+    for (int p = 0; p < NLD; p++) {
+        const int at = 64 * (wave + NW * p) + lane, r = at / CPR, s = at % CPR;
+        const int kc = kslot<CPR>(r, s), vc = vslot<CPR>(r, s);  // (an XOR: its own inverse)
+        // chunks past the row are read past the buffer's end: zeros
+        ko[p] = NP == 2 || kc < n_chunk ? (uint32_t)(r * kstride) + 16 * kc : 0xFFFFFFF0u;
+        vo[p] = NP == 2 || vc < n_chunk ? (uint32_t)(r * vstride) + 16 * vc : 0xFFFFFFF0u;
+    }
+    const int row_bytes = NP == 2 ? ROWB : 2 * hd;
+    float pe = 0.0f;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)pr_smem;
+    auto fetch = [&](int w, int buf) __attribute__((always_inline)) {
+        // (keys past the sequence's end read as zeros; they are masked)
+        const int left = n - w * KT;
+        const u32x4 kr = buffer_of(kbase + w * KT * kstride, (left - 1) * kstride + row_bytes);
+        const u32x4 vr = buffer_of(vbase + w * KT * vstride, (left - 1) * vstride + row_bytes);
+        const uint32_t to = lds0 + buf * 2 * TILEB + 1024 * wave;
+#pragma unroll
+        for (int p = 0; p < NLD; p++) load_lds(kr, ko[p], to + 1024 * NW * p);
+#pragma unroll
+        for (int p = 0; p < NLD; p++) load_lds(vr, vo[p], to + TILEB + 1024 * NW * p);
         if constexpr (NP == 2)
             if (tid < 2 * KT) {
-                const int64_t at = (row0 - a.row0 + min(base + tid % KT, n - 1)) * a.H + h;
+                const int64_t at = (row0 - a.row0 + min(w * KT + tid % KT, n - 1)) * a.H + h;
                 pe = tid < KT ? a.ke[at] : a.ve[at];
             }
     };
-    auto stage = [&](int buf) __attribute__((always_inline)) {
-#pragma unroll
-        for (int p = 0; p < NPC; p++) {
-            const int idx = tid + NT * p, r = idx / CPR, ch = idx % CPR;
-            kt[(buf * KT + r) * CPR + kslot<CPR>(r, ch)] = pk[p];
-            vt[(buf * KT + r) * CPR + vslot<CPR>(r, ch)] = pv[p];
-        }
-        if constexpr (NP == 2)
-            if (tid < 2 * KT) se[buf * 2 * KT + tid] = pe;
-    };
-    fetch(0);
+    fetch(0, 0);
+    if constexpr (NP == 2)
+        if (tid < 2 * KT) se[tid] = pe;
 
     // q of this lane's column: k-step t holds dims 16 t + 8 hf ..
     V8 qh[NKS], ql[NP == 2 ? NKS : 1];
@@ -218,6 +246,22 @@ __global__ __launch_bounds__(64 * kPromptNW, HD * NP > 128 ? 1 : 2) void prompt_
     const int n_key = (min(c_blk + kPromptCols, n_cols) - 1) / G + 1;
     const int n_tile = (n_key + KT - 1) / KT;
 
+    // This lane's operand addresses in a tile: K chunk 2 t + hf of row j (rows 32 and more further on),
+    // V rows 4 hf + i / 4 (transposed in groups of 16 lanes), dims of tile db.
+    // The XORs reach 16 chunks: what lies further on is 256 bytes and more away from one of the first.
+    constexpr int NKA = NKS < 8 ? NKS : 8, NVA = NDB < 4 ? NDB : 4;
+    uint32_t ka[NKA], va_[NVA];
+#pragma unroll
+    for (int t = 0; t < NKA; t++) ka[t] = j * ROWB + 16 * kslot<CPR>(j, 2 * t + hf);
+#pragma unroll
+    for (int db = 0; db < NVA; db++) {
+        const int l = lane & 15, r = 4 * hf + (l >> 2), ch = 4 * db + 2 * ((lane >> 4) & 1) + ((l & 3) >> 1);
+        va_[db] = r * ROWB + 16 * vslot<CPR>(r, ch) + 8 * (l & 1);
+    }
+    // (64 dims in two planes are one row of 16 chunks: t and db of the low plane start in its middle)
+    auto k_at = [&](int t) { return HD == 64 && t >= NKS ? ka[t - NKS] ^ 128 : ka[t & (NKA - 1)] + t / NKA * 256; };
+    auto v_at = [&](int db) { return HD == 64 && db >= NDB ? va_[db - NDB] ^ 128 : va_[db & (NVA - 1)] + db / NVA * 256; };
+
     floatx16 o[NDB];
 #pragma unroll
     for (int db = 0; db < NDB; db++) o[db] = (floatx16)0.0f;
@@ -226,142 +270,172 @@ __global__ __launch_bounds__(64 * kPromptNW, HD * NP > 128 ? 1 : 2) void prompt_
     // 2^-30 of the largest before they are lost; bf16 has f32's range.
     constexpr float kTop = F16 ? 6.0f : 0.0f;
 
-    stage(0);
-    if (n_tile > 1) fetch(KT);
-    __syncthreads();
-    for (int w = 0; w < n_tile; w++) {
-        const int buf = w & 1, base = w * KT;
-        const u32x4 *kb = kt + buf * KT * CPR, *vb = vt + buf * KT * CPR;
-        if (w + 1 < n_tile) stage(buf ^ 1);
-        if (w + 2 < n_tile) fetch(base + 2 * KT);
-        if (base <= qmax_w) {
-            floatx16 sc[NKB];
+    auto tile = [&](auto MASKED, int w) __attribute__((always_inline)) {
+        constexpr bool MASK = decltype(MASKED)::value;
+        const int base = w * KT;
+        const unsigned char *kb = pr_smem + (w & 1) * 2 * TILEB, *vb = kb + TILEB;
+        floatx16 sc[NKB];
 #pragma unroll
-            for (int b = 0; b < NKB; b++) sc[b] = (floatx16)0.0f;
-#pragma unroll
-            for (int t = 0; t < NKS; t++)
-#pragma unroll
-                for (int b = 0; b < NKB; b++) {
-                    const int r = 32 * b + j;
-                    const V8 kh = __builtin_bit_cast(V8, kb[r * CPR + kslot<CPR>(r, 2 * t + hf)]);
-                    sc[b] = mfma(kh, qh[t], sc[b]);
-                    if constexpr (NP == 2) {
-                        const V8 kl = __builtin_bit_cast(V8, kb[r * CPR + kslot<CPR>(r, HD / 8 + 2 * t + hf)]);
-                        sc[b] = mfma(kh, ql[t], sc[b]);
-                        sc[b] = mfma(kl, qh[t], sc[b]);
-                    }
-                }
-            // scores in the exp2 domain: x = s scale (K's row scale folded in)
-            const bool mask = base + KT - 1 > qmin_w;
-            const float *ke = se + buf * 2 * KT, *ve = ke + KT;
-            float mloc = -INFINITY;
-            bool odd_rows = false;  // two planes: a value row of the tile is not finite (its K scale is negative)
+        for (int b = 0; b < NKB; b++) sc[b] = (floatx16)0.0f;
+        // (the next k-step's operands are read beside this one's products, and no further ahead: left to
+        // itself the compiler reads the whole tile first and spills)
+        V8 kf[2][NKB][NP];
+        auto read_k = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
             for (int b = 0; b < NKB; b++)
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    floatx4 k4 = (floatx4)qscale, v4 = (floatx4)0.0f;
-                    if constexpr (NP == 2) {
-                        const floatx4 s4 = *reinterpret_cast<const floatx4 *>(ke + 32 * b + 8 * q + 4 * hf);
+                for (int pl = 0; pl < NP; pl++)
+                    kf[t & 1][b][pl] = *reinterpret_cast<const V8 *>(kb + k_at(pl * NKS + t) + 32 * b * ROWB);
+        };
+        read_k(0);
 #pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            odd_rows |= s4[r] < 0.0f;
-                            k4[r] = qscale * fabsf(s4[r]);
-                        }
-                        v4 = *reinterpret_cast<const floatx4 *>(ve + 32 * b + 8 * q + 4 * hf);
-                    }
+        for (int t = 0; t < NKS; t++) {
+            if (t + 1 < NKS) read_k(t + 1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        float x = sc[b][4 * q + r] * k4[r];
-                        if constexpr (SOFTCAP) {
-                            x = tanhf(x / a.softcap) * (a.softcap * kLog2e);
-                        }
-                        // (two planes: the weight that P has to carry is p 2^ve)
-                        if constexpr (NP == 2) x += v4[r];
-                        if (mask && base + 32 * b + 8 * q + 4 * hf + r > qpos) x = -INFINITY;
-                        sc[b][4 * q + r] = x;
-                        mloc = fmaxf(mloc, x);
-                    }
-                }
-            mloc = both_max(mloc);
-            if (__builtin_amdgcn_ballot_w64(mloc - m_run > 8.0f) != 0) {
-                const float m_new = mloc - m_run > 8.0f ? mloc : m_run;
-                const float alpha = exp2f(m_run - m_new);
-                m_run = m_new;
-                l_run *= alpha;
+            for (int b = 0; b < NKB; b++) sc[b] = mfma(kf[t & 1][b][0], qh[t], sc[b]);
+            if constexpr (NP == 2) {
 #pragma unroll
-                for (int db = 0; db < NDB; db++) o[db] *= alpha;
+                for (int b = 0; b < NKB; b++) sc[b] = mfma(kf[t & 1][b][0], ql[t], sc[b]);
+#pragma unroll
+                for (int b = 0; b < NKB; b++) sc[b] = mfma(kf[t & 1][b][NP - 1], qh[t], sc[b]);
             }
-            const float off = kTop - m_run;
-#pragma unroll
-            for (int b = 0; b < NKB; b++)
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    floatx4 v4 = (floatx4)0.0f;
-                    if constexpr (NP == 2) v4 = *reinterpret_cast<const floatx4 *>(ve + 32 * b + 8 * q + 4 * hf);
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const float p = __builtin_amdgcn_exp2f(sc[b][4 * q + r] + off);
-                        sc[b][4 * q + r] = p;
-                        l_run += NP == 2 ? p * __builtin_amdgcn_exp2f(-v4[r]) : p;
-                    }
-                }
-#pragma unroll
-            for (int st = 0; st < 2 * NKB; st++) {
-                V8 pb, pl;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float p = sc[st >> 1][8 * (st & 1) + e];
-                    pb[e] = (T)p;
-                    if constexpr (NP == 2) pl[e] = (T)(p - (float)pb[e]);
-                }
-                V8 va[NDB], vl[NP == 2 ? NDB : 1];
-#pragma unroll
-                for (int db = 0; db < NDB; db++) {
-                    va[db] = v_operand<T, CPR>(vb, 16 * st, 4 * db, lane);
-                    if constexpr (NP == 2) vl[db] = v_operand<T, CPR>(vb, 16 * st, HD / 8 + 4 * db, lane);
-                }
-                if (mask || NP == 2) {
-                    // 0 times an infinite or NaN value must not reach the sums (0: a masked key's P, or the low
-                    // part of any): what is not finite is added apart, where a visible key brings it.
-                    bool bad = odd_rows;
-                    if constexpr (NP == 1) {
-#pragma unroll
-                        for (int db = 0; db < NDB; db++) bad |= any_bad(va[db], F16);
-                    }
-                    if (__builtin_amdgcn_ballot_w64(bad) != 0) {
-                        V8 see;
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            const int key = base + 16 * st + 8 * (e >> 2) + 4 * hf + (e & 3);
-                            see[e] = key <= qpos ? (T)1.0f : (T)0.0f;
-                        }
-#pragma unroll
-                        for (int db = 0; db < NDB; db++) {
-                            const floatx16 up = mfma(bad_part<T>(va[db], 1), see, (floatx16)0.0f);
-                            const floatx16 dn = mfma(bad_part<T>(va[db], 2), see, (floatx16)0.0f);
-#pragma unroll
-                            for (int e = 0; e < 16; e++) {
-                                o[db][e] += up[e] > 0.0f ? INFINITY : 0.0f;
-                                o[db][e] -= dn[e] > 0.0f ? INFINITY : 0.0f;
-                            }
-                            va[db] = bad_part<T>(va[db], 0);
-                            if constexpr (NP == 2) vl[db] = bad_part<T>(vl[db], 0);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int db = 0; db < NDB; db++) {
-                    o[db] = mfma(va[db], pb, o[db]);
-                    if constexpr (NP == 2) {
-                        o[db] = mfma(va[db], pl, o[db]);
-                        o[db] = mfma(vl[db], pb, o[db]);
-                    }
-                }
-            }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        __syncthreads();
-    }
+        // x: scores in the exp2 domain (two planes: plus the value row's exponent, so that 2^x is the weight P
+        // has to carry); without softcap and planes their scale waits for the exponent's FMA
+        const float *ke = se + (w & 1) * 2 * KT, *ve = ke + KT;
+        float mloc = -INFINITY;
+        bool odd_rows = false;  // two planes: a value row of the tile is not finite (its K scale is negative)
+#pragma unroll
+        for (int b = 0; b < NKB; b++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                floatx4 k4 = (floatx4)qscale, v4 = (floatx4)0.0f;
+                if constexpr (NP == 2) {
+                    const floatx4 s4 = *reinterpret_cast<const floatx4 *>(ke + 32 * b + 8 * q + 4 * hf);
+                    v4 = *reinterpret_cast<const floatx4 *>(ve + 32 * b + 8 * q + 4 * hf);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        odd_rows |= s4[r] < 0.0f;
+                        k4[r] = qscale * fabsf(s4[r]);
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    float x = sc[b][4 * q + r];
+                    if constexpr (!RAW) x *= k4[r];
+                    if constexpr (SOFTCAP) x = tanhf(x / a.softcap) * (a.softcap * kLog2e);
+                    if constexpr (NP == 2) x += v4[r];
+                    if constexpr (MASK)
+                        if (base + 32 * b + 8 * q + 4 * hf + r > qpos) x = -INFINITY;
+                    sc[b][4 * q + r] = x;
+                    mloc = fmaxf(mloc, x);
+                }
+            }
+        mloc = both_max(mloc);
+        if constexpr (RAW) mloc *= qscale;
+        if (__builtin_amdgcn_ballot_w64(mloc - m_run > 8.0f) != 0) {
+            const float m_new = mloc - m_run > 8.0f ? mloc : m_run;
+            const float alpha = exp2f(m_run - m_new);
+            m_run = m_new;
+            l_run *= alpha;
+#pragma unroll
+            for (int db = 0; db < NDB; db++) o[db] *= alpha;
+        }
+        const float off = kTop - m_run;
+        // O^T += V^T P^T, 16 keys at a time: the exponentials of a step run beside the products of the one
+        // before, and V's operands are read one group of products ahead.
+        constexpr int VG = 4 / NP, NVG = NDB < VG ? 1 : NDB / VG, NU = 2 * NKB * NVG;
+        constexpr int DG = NDB < VG ? NDB : VG;  // dim tiles of a group
+        V8 vf[2][DG][NP];
+        auto read_v = [&](int u) __attribute__((always_inline)) {
+#pragma unroll
+            for (int d = 0; d < DG; d++)
+#pragma unroll
+                for (int pl = 0; pl < NP; pl++)
+                    vf[u & 1][d][pl] = v_operand<T, ROWB>(vb + v_at(pl * NDB + DG * (u % NVG) + d) + 16 * (u / NVG) * ROWB);
+        };
+        read_v(0);
+        V8 pb, pl;
+#pragma unroll
+        for (int u = 0; u < NU; u++) {
+            const int st = u / NVG;
+            if (u % NVG == 0) {
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    floatx4 v4 = (floatx4)0.0f;
+                    if constexpr (NP == 2) v4 = *reinterpret_cast<const floatx4 *>(ve + 16 * st + 8 * q + 4 * hf);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const float x = sc[st >> 1][8 * (st & 1) + 4 * q + r];
+                        const float p = __builtin_amdgcn_exp2f(RAW ? __builtin_fmaf(x, qscale, off) : x + off);
+                        l_run += NP == 2 ? p * __builtin_amdgcn_exp2f(-v4[r]) : p;
+                        const T hi = (T)p;
+                        pb[4 * q + r] = hi;
+                        if constexpr (NP == 2) pl[4 * q + r] = (T)(p - (float)hi);
+                    }
+                }
+            }
+            V8 (&va)[DG][NP] = vf[u & 1];
+            floatx16 *const og = o + DG * (u % NVG);
+            if (u + 1 < NU) read_v(u + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (MASK || NP == 2) {
+                // 0 times an infinite or NaN value must not reach the sums (0: a masked key's P, or the low
+                // part of any): what is not finite is added apart, where a visible key brings it.
+                bool bad = odd_rows;
+                if constexpr (NP == 1) {
+#pragma unroll
+                    for (int d = 0; d < DG; d++) bad |= any_bad(va[d][0], F16);
+                }
+                if (__builtin_amdgcn_ballot_w64(bad) != 0) {
+                    V8 see;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const int key = base + 16 * st + 8 * (e >> 2) + 4 * hf + (e & 3);
+                        see[e] = key <= qpos ? (T)1.0f : (T)0.0f;
+                    }
+#pragma unroll
+                    for (int d = 0; d < DG; d++) {
+#pragma unroll
+                        for (int sign = 1; sign <= 2; sign++) {
+                            const floatx16 hit = mfma(bad_part<T>(va[d][0], sign), see, (floatx16)0.0f);
+#pragma unroll
+                            for (int e = 0; e < 16; e++)
+                                og[d][e] += hit[e] > 0.0f ? (sign == 1 ? INFINITY : -INFINITY) : 0.0f;
+                        }
+                        // (in place: these operands are not used again)
+                        va[d][0] = bad_part<T>(va[d][0], 0);
+                        if constexpr (NP == 2) va[d][NP - 1] = bad_part<T>(va[d][NP - 1], 0);
+                    }
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < DG; d++) og[d] = mfma(va[d][0], pb, og[d]);
+            if constexpr (NP == 2) {
+#pragma unroll
+                for (int d = 0; d < DG; d++) og[d] = mfma(va[d][0], pl, og[d]);
+#pragma unroll
+                for (int d = 0; d < DG; d++) og[d] = mfma(va[d][NP - 1], pb, og[d]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+
+    // Tiles that every column of the wave sees whole, then those on its diagonal.  (Two loops: with both
+    // bodies in one, the compiler moves the accumulators between them.)  Every wave passes n_tile barriers.
+    auto step = [&](auto MASKED, int w, bool busy) __attribute__((always_inline)) {
+        tile_barrier();  // tile w is there; nobody reads tile w - 1 any more
+        if (w + 1 < n_tile) fetch(w + 1, (w + 1) & 1);
+        if (busy) tile(MASKED, w);
+        if constexpr (NP == 2)
+            if (w + 1 < n_tile && tid < 2 * KT) se[((w + 1) & 1) * 2 * KT + tid] = pe;
+    };
+    const int n_full = qmax_w < 0 ? 0 : min((qmin_w + 1) / KT, n_tile);
+    int w = 0;
+    for (; w < n_full; w++) step(std::false_type(), w, true);
+    for (; w < n_tile; w++) step(std::true_type(), w, w * KT <= qmax_w);
 
     const float inv = 1.0f / both_sum(l_run);
     O *orow = static_cast<O *>(a.out) + (row0 + tok) * a.os + (int64_t)head * hd;
@@ -467,6 +541,23 @@ void prompt_dims(const PromptArgs &a, bool cap, unsigned blocks, hipStream_t st)
     }
 }
 
+// Sequences seq0 .. of the batch with the longest first, so that the launch ends with short walks (tok:
+// the first row, pos0: the rows).
+void fill_longest_first(PackTable &t, const int32_t *off, int n_seq, int seq0, int G) {
+    int order[kPackSeqs];
+    t.seq0 = seq0;
+    t.n = std::min(n_seq - seq0, kPackSeqs);
+    for (int i = 0; i < t.n; i++) order[i] = seq0 + i;
+    auto len = [&](int s) { return off[s + 1] - off[s]; };
+    std::sort(order, order + t.n, [&](int x, int y) { return len(x) != len(y) ? len(x) > len(y) : x < y; });
+    t.item[0] = 0;
+    for (int i = 0; i < t.n; i++) {
+        t.tok[i] = off[order[i]];
+        t.pos0[i] = len(order[i]);
+        t.item[i + 1] = t.item[i] + (int)(((int64_t)t.pos0[i] * G + kPromptCols - 1) / kPromptCols);
+    }
+}
+
 int padded(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 
 }  // namespace
@@ -513,10 +604,8 @@ hipError_t launch_prompt(const PromptCall &c, hipStream_t st) {
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    const int G = a.G;
     for (int s = 0; s < c.n_seq; s += a.t.n) {
-        pack_fill(a.t, c.off, nullptr, c.n_seq, s,
-                  [G](int n) { return (int)(((int64_t)n * G + kPromptCols - 1) / kPromptCols); });
+        fill_longest_first(a.t, c.off, c.n_seq, s, a.G);
         const int64_t blocks = (int64_t)a.t.item[a.t.n] * c.n_kv;
         if (blocks == 0) continue;
         if (c.dtype == TS_DTYPE_F32)

@@ -4,14 +4,18 @@
 
 namespace ts {
 
-// How a call divides its work: the prefix in n_part pieces of `chunk` keys (a multiple of 64) for
-// every block of 128 (token, head) columns.
+// How a call divides its work.  chain: every block of 128 (token, head) columns of a sequence walks the
+// prefix and then the sequence's own keys, and writes its output.  Otherwise the prefix in n_part pieces
+// of `chunk` keys (a multiple of 64) for every block of columns of the whole batch, and (n_tok > 1)
+// own_blk blocks of each sequence over its own keys, as partials that a last kernel joins.
 struct SharedPlan {
-    int n_blk, n_part, chunk;
+    bool chain;
+    int n_blk, n_part, chunk, own_blk;
+    int groups;  // groups of 4 waves per workgroup
 };
-SharedPlan shared_plan(int n_rows, int G, int n_kv, int prefix_len, int stored_hd, int n_cu);
-// The most pieces of any prefix up to max_prefix.
-int shared_parts_cap(int n_rows, int G, int n_kv, int max_prefix, int stored_hd, int n_cu);
+SharedPlan shared_plan(int n_seq, int n_tok, int G, int n_kv, int prefix_len, int stored_hd, int n_cu);
+// The most partials a row has, of any prefix up to max_prefix (0 for chains).
+int shared_slots_cap(int n_seq, int n_tok, int G, int n_kv, int max_prefix, int n_cu);
 
 struct SharedCall {
     KvLayerView own, pre;
@@ -24,7 +28,7 @@ struct SharedCall {
     float softcap;
     float *out;
     SharedPlan plan;
-    float *part;  // [n_seq n_tok n_head][n_part (+ 1: own keys, n_tok > 1)] of stored_hd + 2 floats
+    float *part;  // [n_seq n_tok n_head][n_part (+ 1 with own_blk)] of stored_hd + 2 floats
     // One token: the partials that the decode kernel wrote of the own keys, its plan, and the length
     // it was given with the launch (or -1).
     const float *own_part;

@@ -22,102 +22,126 @@ struct SharedArgs {
     const int32_t *len;
     const float *q, *rope;
     int rope_pairs, rope_rows, n_head, G, n_tok;
-    int n_blk, n_part, chunk;  // the prefix's jobs: n_blk n_part per kv head
-    int own_blk;               // the own keys' jobs: own_blk per (kv head, sequence); 0 without
+    bool chain;                // one job walks the prefix and then a sequence's own keys
+    int n_blk, n_part, chunk;  // the prefix's jobs: n_blk n_part per kv head (none in a chain)
+    int own_blk;               // the own keys' jobs (or the chains): own_blk per (kv head, sequence)
     int slots;                 // partials per row: n_part, and one of the own keys if own_blk
     float inv_sqrt_hd, softcap;
-    float *part;
+    float *part, *out;
 };
 
-// One job: 128 columns (token, head) of one kv head against a range of one stream's keys, in the
-// window walk of chunked prefill.
-template <int HD, bool SOFTCAP, bool NORM, bool PAD>
-__global__ __launch_bounds__(64 * kPrefillNW, HD > 128 ? 1 : 2) void shared_kernel(SharedArgs a) {
+// The rotations of pairs 4u .. 4u + 3 at table row p, as load_rot8, in two 16-byte loads where the
+// table's rows allow it.
+__device__ inline void load_rot8_wide(const float *rope, int rope_pairs, int u, int p, float2 (&cs)[4]) {
+    if ((rope_pairs & 3) != 0) {
+        load_rot8(rope, rope_pairs, u, p, cs);
+        return;
+    }
+    const bool in = 4 * u < rope_pairs;
+    const float4 *t = reinterpret_cast<const float4 *>(rope + ((size_t)p * rope_pairs + (in ? 4 * u : 0)) * 2);
+    const float4 a = t[0], b = t[1];
+    cs[0] = make_float2(in ? a.x : 1.0f, in ? a.y : 0.0f);
+    cs[1] = make_float2(in ? a.z : 1.0f, in ? a.w : 0.0f);
+    cs[2] = make_float2(in ? b.x : 1.0f, in ? b.y : 0.0f);
+    cs[3] = make_float2(in ? b.z : 1.0f, in ? b.w : 0.0f);
+}
+
+constexpr int kCols = kPrefillNW * kColsPerWave;
+
+// LDS of one workgroup: the window tiles of its groups, afterwards the outputs of all columns.
+template <int HD, int NGRP>
+constexpr size_t shared_lds() {
+    return std::max(NGRP * sizeof(PrefillLds<HD>), NGRP > 1 ? (size_t)kCols * (HD + 4) * sizeof(float) : 0);
+}
+
+// One job: 128 columns (token, head) of one kv head against a range of keys, in the window walk of
+// chunked prefill.  With NGRP 2 two groups of 4 waves take every second window and join through LDS:
+// a job that has a CU for itself then has two waves per SIMD, one's products beside the other's softmax.
+template <int HD, bool SOFTCAP, bool NORM, bool PAD, int NGRP>
+__global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 2) void shared_kernel(SharedArgs a) {
     constexpr int NW = kPrefillNW;
     constexpr int NKS = HD / 16, NDB = HD / 32, NG = NKS / 4, ROWB = HD / 2;
-    constexpr int COLS = NW * kColsPerWave;
     const float *const QN = NORM ? a.own.qn : nullptr;
     const int H = a.own.H, G = a.G, T = a.n_tok, hdr = PAD ? a.own.hdr : HD;
     // Jobs of one kv head go to one XCD where the heads divide the XCDs: its streams share an L2.
     const int h = blockIdx.x % H;
     int job = blockIdx.x / H;
     const bool over_prefix = job < a.n_blk * a.n_part;
-    int row_base, n_cols, blk, slot, k_begin, k_end, s_str;
-    const KvLayerView &L = over_prefix ? a.pre : a.own;
+    // columns: rows (token of a sequence) from row_base on, G heads each; keys: n_pre windows of the
+    // prefix from k_begin to k_end, then n_own windows of sequence s_own's own
+    int row_base, n_cols, blk, slot, k_begin, k_end, s_own = 0, n_own = 0;
     if (over_prefix) {
         blk = job / a.n_part;
         slot = job % a.n_part;
         row_base = 0;
         n_cols = a.own.S * T * G;
-        s_str = a.prefix_seq;
         k_begin = slot * a.chunk;
         k_end = min(k_begin + a.chunk, a.prefix_len);
     } else {
         job -= a.n_blk * a.n_part;
-        s_str = job / a.own_blk;
+        s_own = job / a.own_blk;
         blk = a.own_blk - 1 - job % a.own_blk;  // later tokens first
         slot = a.n_part;
-        row_base = s_str * T;
+        row_base = s_own * T;
         n_cols = T * G;
         k_begin = 0;
-        k_end = min(a.len[s_str] + (min((blk + 1) * COLS, n_cols) - 1) / G + 1, L.P);
+        k_end = a.chain ? a.prefix_len : 0;
+        n_own = (min(a.len[s_own] + (min((blk + 1) * kCols, n_cols) - 1) / G + 1, a.own.P) + kWin - 1) / kWin;
     }
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int n_pre = (k_end - k_begin + kWin - 1) / kWin, n_win = n_pre + n_own;
+    const int tid = threadIdx.x & (64 * NW - 1), lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int grp = NGRP > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * NW)) : 0;
     const int j = lane & 31, hf = lane >> 5;
     extern __shared__ __align__(16) unsigned char sh_smem[];
-    PrefillLds<HD> &sm = *reinterpret_cast<PrefillLds<HD> *>(sh_smem);
-    __shared__ float sm_qb[NW];
+    PrefillLds<HD> &sm = *reinterpret_cast<PrefillLds<HD> *>(sh_smem + grp * sizeof(PrefillLds<HD>));
+    __shared__ float sm_qb[NW * NGRP], sm_m[kCols], sm_l[kCols];
 
-    const size_t stream = (size_t)s_str * H + h;
-    const uint8_t *kbase = L.kp + stream * L.P * ROWB;
-    const uint8_t *vbase = L.vp + stream * (L.P / 32) * (HD * 16);
-    const float *ksb = L.ks + stream * L.P, *vsb = L.vs + stream * L.P;
     const float qmul = SOFTCAP ? a.inv_sqrt_hd : a.inv_sqrt_hd * kLog2e;
     const int krow = qk_row_key(j);
 
-    const int c_blk = blk * COLS, c_wave = c_blk + wave * kColsPerWave, c = c_wave + j;
+    const int c_blk = blk * kCols, c_wave = c_blk + wave * kColsPerWave, c = c_wave + j;
     const bool live = c < n_cols;
     const int cc = live ? c : n_cols - 1;
     const int row = row_base + cc / G, s = row / T, tok = row - s * T;
     const int head = h * G + cc % G;
     const float *qrow = a.q + ((size_t)row * a.n_head + head) * hdr;
-    const int len_s = a.len[s];
-    const int qslot = len_s + tok;  // the token's own slot
-    // the last key this column sees
-    const int qpos = !live ? -1 : over_prefix ? k_end - 1 : qslot;
-    const int len0 = over_prefix ? 0 : len_s;  // (one sequence per own job)
-    const int qmin_w = over_prefix ? k_end - 1 : len0 + c_wave / G;
-    const int qmax_w = c_wave >= n_cols ? -1
-                       : over_prefix    ? k_end - 1
-                                        : len0 + (min(c_wave + kColsPerWave, n_cols) - 1) / G;
 
     Pending<HD, NW> pd;
     const DeqConstV dk;
-    fetch_window<HD, NW>(pd, kbase, vbase, ksb, vsb, k_begin, tid, wave);
+    auto stream_of = [&](const KvLayerView &L, int seq) { return (size_t)seq * H + h; };
+    auto fetch = [&](int w) __attribute__((always_inline)) {
+        const KvLayerView &L = w < n_pre ? a.pre : a.own;
+        const size_t st = stream_of(L, w < n_pre ? a.prefix_seq : s_own);
+        fetch_window<HD, NW>(pd, L.kp + st * L.P * ROWB, L.vp + st * (L.P / 32) * (HD * 16), L.ks + st * L.P, L.vs + st * L.P,
+                             w < n_pre ? k_begin + w * kWin : (w - n_pre) * kWin, tid, wave);
+    };
+    if (grp < n_win) fetch(grp);
 
     // q of this lane's column: norm, rotation at its position, power-of-two scale, hi/lo split
-    const float ns = QN ? qk_norm_scale(qrow, hdr, a.own.norm_eps) : 1.0f;
+    const int len_s = a.len[s], qslot = len_s + tok;  // the token's own slot
     float q_s, inv_s;
     half8 qh[NKS];
     int6v ql1[NG], ql2[NG];
     {
+        const float ns = QN ? qk_norm_scale(qrow, hdr, a.own.norm_eps) : 1.0f;
         float xq[NKS][8];
         float2 cs[NKS][4];
+#pragma unroll
+        for (int t = 0; t < NKS; t++) q_read8(qrow, 2 * t + hf, QN, ns, xq[t], hdr);
         const int qrot = min(rot_of(a.own, s, qslot), a.rope_rows - 1);  // (a graph replayed past the table)
+#pragma unroll
+        for (int t = 0; t < NKS; t++) load_rot8_wide(a.rope, a.rope_pairs, 2 * t + hf, qrot, cs[t]);
         float qb = 0.0f;
 #pragma unroll
-        for (int t = 0; t < NKS; t++) {
-            q_read8(qrow, 2 * t + hf, QN, ns, xq[t], hdr);
-            load_rot8(a.rope, a.rope_pairs, 2 * t + hf, qrot, cs[t]);
+        for (int t = 0; t < NKS; t++)
             qb = fmaxf(qb, fmaxf(fmaxf(fabsf(xq[t][0]) + fabsf(xq[t][1]), fabsf(xq[t][2]) + fabsf(xq[t][3])),
                                  fmaxf(fabsf(xq[t][4]) + fabsf(xq[t][5]), fabsf(xq[t][6]) + fabsf(xq[t][7]))));
-        }
         qb = wave_max(qb);
-        if (lane == 0) sm_qb[wave] = qb;
+        if (lane == 0) sm_qb[NW * grp + wave] = qb;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < NW; w++) qb = fmaxf(qb, sm_qb[w]);
+        for (int w = 0; w < NW; w++) qb = fmaxf(qb, sm_qb[NW * grp + w]);
         q_scale(qb * qmul, q_s, inv_s);
 #pragma unroll
         for (int g = 0; g < NG; g++) {
@@ -141,16 +165,17 @@ __global__ __launch_bounds__(64 * kPrefillNW, HD > 128 ? 1 : 2) void shared_kern
     for (int db = 0; db < NDB; db++) o[db] = (floatx16)0.0f;
     float m_run = 0.0f, l_run = 0.0f;
     bool first = true;
-    const int n_win = (k_end - k_begin + kWin - 1) / kWin;
 
     stage_codes<HD, NW>(sm, 0, pd, tid, wave, dk);
     stage_scales<HD, NW, true>(sm, 0, pd, tid, inv_s);
-    if (n_win > 1) fetch_window<HD, NW>(pd, kbase, vbase, ksb, vsb, k_begin + kWin, tid, wave);
+    if (grp + NGRP < n_win) fetch(grp + NGRP);
     __syncthreads();
 
-    for (int w = 0; w < n_win; w++) {
-        const int buf = w & 1, base = k_begin + w * kWin;
-        const bool more = w + 1 < n_win;
+    // (every group makes the same number of rounds, for the barriers; one without a window left drops
+    // what it computes)
+    const int rounds = (n_win + NGRP - 1) / NGRP;
+    for (int it = 0; it < rounds; it++) {
+        const int buf = it & 1, w = it * NGRP + grp;
         floatx16 sc[2] = {(floatx16)0.0f, (floatx16)0.0f};
         __builtin_amdgcn_s_setprio(3);
         using PD = Pending<HD, NW>;
@@ -185,9 +210,17 @@ __global__ __launch_bounds__(64 * kPrefillNW, HD > 128 ? 1 : 2) void shared_kern
         }
         if constexpr (NPART == 0) stage_codes<HD, NW>(sm, buf ^ 1, pd, tid, wave, dk);
         __builtin_amdgcn_s_setprio(0);
-        if (more) stage_scales<HD, NW, true>(sm, buf ^ 1, pd, tid, inv_s);
-        if (w + 2 < n_win) fetch_window<HD, NW>(pd, kbase, vbase, ksb, vsb, base + 2 * kWin, tid, wave);
-        if (base <= qmax_w) {
+        if (w + NGRP < n_win) stage_scales<HD, NW, true>(sm, buf ^ 1, pd, tid, inv_s);
+        if (w + 2 * NGRP < n_win) fetch(w + 2 * NGRP);
+        // Keys are numbered within their stream: a column sees the prefix up to k_end, its own keys up to
+        // its slot.
+        const bool pre = w < n_pre;
+        const int base = pre ? k_begin + w * kWin : (w - n_pre) * kWin;
+        const int qpos = !live ? -1 : pre ? k_end - 1 : qslot;
+        const int len_w = pre ? 0 : a.len[s_own];
+        const int qmin_w = pre ? k_end - 1 : len_w + c_wave / G;
+        const int qmax_w = pre ? k_end - 1 : len_w + (min(c_wave + kColsPerWave, n_cols) - 1) / G;
+        if (w < n_win && c_wave < n_cols && base <= qmax_w) {
             const bool mask = base + kWin - 1 > qmin_w;
             window_scores<NDB, SOFTCAP>(sc, sm.sk[buf], sm.svlog[buf], a.softcap, mask, first, base, hf, qpos, m_run,
                                         l_run, o);
@@ -213,21 +246,65 @@ __global__ __launch_bounds__(64 * kPrefillNW, HD > 128 ? 1 : 2) void shared_kern
         __syncthreads();
     }
 
-    const float l = half_sum(l_run);
-    if (live) {
-        const size_t rows = (size_t)a.own.S * T * a.n_head;
-        const size_t r = ((size_t)row * a.n_head + head) * a.slots + slot;
-        float *dst = a.part + r * HD;
+    float l = half_sum(l_run);
+    const size_t rows = (size_t)a.own.S * T * a.n_head;
+    const size_t row_head = (size_t)row * a.n_head + head;
+    if constexpr (NGRP == 1) {
+        if (!live) return;
+        float *dst = a.chain ? a.out + row_head * hdr : a.part + (row_head * a.slots + slot) * HD;
+        const float mul = !a.chain ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
         for (int db = 0; db < NDB; db++)
 #pragma unroll
             for (int q = 0; q < 4; q++)
                 if (32 * db + 8 * q + 4 * hf < hdr)
                     *reinterpret_cast<float4 *>(dst + 32 * db + 8 * q + 4 * hf) =
-                        make_float4(o[db][4 * q], o[db][4 * q + 1], o[db][4 * q + 2], o[db][4 * q + 3]);
-        if (hf == 0) {
-            a.part[rows * a.slots * HD + r] = m_run;
-            a.part[rows * a.slots * (HD + 1) + r] = l;
+                        make_float4(o[db][4 * q] * mul, o[db][4 * q + 1] * mul, o[db][4 * q + 2] * mul, o[db][4 * q + 3] * mul);
+        if (!a.chain && hf == 0) {
+            a.part[rows * a.slots * HD + row_head * a.slots + slot] = m_run;
+            a.part[rows * a.slots * (HD + 1) + row_head * a.slots + slot] = l;
+        }
+    } else {
+        // Group 1's outputs through LDS to group 0, the join back through LDS, and whole rows from there.
+        constexpr int OST = HD + 4;
+        float *const mo = reinterpret_cast<float *>(sh_smem);
+        const int col = 32 * wave + j;
+        if (first) m_run = kMinit;  // (a group or wave that had no window)
+        auto cell = [&](int db, int q) { return reinterpret_cast<floatx4 *>(mo + col * OST + 32 * db + 8 * q + 4 * hf); };
+        if (grp == 1) {
+#pragma unroll
+            for (int db = 0; db < NDB; db++)
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                    *cell(db, q) = (floatx4){o[db][4 * q], o[db][4 * q + 1], o[db][4 * q + 2], o[db][4 * q + 3]};
+            if (hf == 0) {
+                sm_m[col] = m_run;
+                sm_l[col] = l;
+            }
+        }
+        __syncthreads();
+        if (grp == 0) {
+            const float m1 = sm_m[col], l1 = sm_l[col], M = fmaxf(m_run, m1);
+            const float e0 = __builtin_amdgcn_exp2f(m_run - M), e1 = __builtin_amdgcn_exp2f(m1 - M);
+#pragma unroll
+            for (int db = 0; db < NDB; db++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const floatx4 mine = {o[db][4 * q], o[db][4 * q + 1], o[db][4 * q + 2], o[db][4 * q + 3]};
+                    *cell(db, q) = e0 * mine + e1 * *cell(db, q);
+                }
+            if (live && hf == 0) {
+                a.part[rows * a.slots * HD + row_head * a.slots + slot] = M;
+                a.part[rows * a.slots * (HD + 1) + row_head * a.slots + slot] = e0 * l + e1 * l1;
+            }
+        }
+        __syncthreads();
+        constexpr int V4 = HD / 4;
+        for (int x = threadIdx.x; x < kCols * V4; x += 64 * NW * NGRP) {
+            const int cl = x / V4, d = 4 * (x % V4), cg = c_blk + cl;
+            if (cg >= n_cols) break;
+            const size_t rh = (size_t)(row_base + cg / G) * a.n_head + h * G + cg % G;
+            *reinterpret_cast<floatx4 *>(a.part + (rh * a.slots + slot) * HD + d) = *reinterpret_cast<floatx4 *>(mo + cl * OST + d);
         }
     }
 }
@@ -241,24 +318,27 @@ struct JoinArgs {
     int own_split, own_chunk, hlen, cap;  // of the decode plan; cap: positions of the own cache
 };
 
-// The join of one (token, head) row's parts, one wave each: lane l holds HD / 64 dims.  The parts'
-// loads do not depend on each other (8 at a time), so a row costs about two memory round trips.
-template <int HD>
+// The join of one (token, head) row's parts by NWR waves: lane l holds HD / 64 dims, wave w every NWR-th
+// group of 8 parts, whose loads do not depend on each other.
+template <int HD, int NWR>
 __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
-    constexpr int D = HD / 64;
-    const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (row >= a.rows) return;
-    const int tok = row / a.n_head, s = tok / a.n_tok;
+    constexpr int D = HD / 64, RPW = 4 / NWR;  // rows per workgroup
+    __shared__ float acc_s[4][HD], l_s[4];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wr = wave % NWR;
+    const int row = blockIdx.x * RPW + wave / NWR;
+    const bool some = row < a.rows;
+    const int r = some ? row : a.rows - 1;
+    const int tok = r / a.n_head, s = tok / a.n_tok;
     const int qpos = (a.hlen >= 0 ? a.hlen : a.len[s]) + tok - s * a.n_tok;
-    // (a graph replayed past the cache's capacity: the own part was not written, nor is the output)
-    if (qpos >= a.cap) return;
-    const float *po = a.part + (size_t)row * a.slots * HD, *pm = a.part + (size_t)a.rows * a.slots * HD + (size_t)row * a.slots;
+    const float *po = a.part + (size_t)r * a.slots * HD, *pm = a.part + (size_t)a.rows * a.slots * HD + (size_t)r * a.slots;
     const float *pl = pm + (size_t)a.rows * a.slots;
-    const int n_own = a.own ? min((qpos + a.own_chunk) / a.own_chunk, a.own_split) : 0;
+    // (a graph replayed past the cache's capacity: the own part was not written, nor is the output)
+    const bool ok = some && qpos < a.cap;
+    const int n_own = a.own && ok ? min((qpos + a.own_chunk) / a.own_chunk, a.own_split) : 0;
     const float *oo = nullptr, *om = nullptr, *ol = nullptr;
     if (a.own) {
-        oo = a.own + (size_t)row * a.own_split * HD;
-        om = a.own + (size_t)a.rows * a.own_split * HD + (size_t)row * a.own_split;
+        oo = a.own + (size_t)r * a.own_split * HD;
+        om = a.own + (size_t)a.rows * a.own_split * HD + (size_t)r * a.own_split;
         ol = om + (size_t)a.rows * a.own_split;
     }
     const int n = a.slots + n_own;
@@ -266,7 +346,7 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
     for (int i = lane; i < n; i += 64) M = fmaxf(M, i < a.slots ? pm[i] : om[i - a.slots]);
     M = wave_max(M);
     float acc[D] = {}, l = 0.0f;
-    for (int i0 = 0; i0 < n; i0 += 8) {
+    for (int i0 = 8 * wr; i0 < n; i0 += 8 * NWR) {
         float x[8][D], w[8], ls[8];
 #pragma unroll
         for (int k = 0; k < 8; k++) {
@@ -287,6 +367,20 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
             l += e2 * ls[k];
         }
     }
+    if constexpr (NWR > 1) {
+#pragma unroll
+        for (int e = 0; e < D; e++) acc_s[wave][D * lane + e] = acc[e];
+        if (lane == 0) l_s[wave] = l;
+        __syncthreads();
+        if (wr != 0) return;
+#pragma unroll
+        for (int k = 1; k < NWR; k++) {
+#pragma unroll
+            for (int e = 0; e < D; e++) acc[e] += acc_s[wave + k][D * lane + e];
+            l += l_s[wave + k];
+        }
+    }
+    if (!ok) return;
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
     float *o = a.out + (size_t)row * a.hdr;
 #pragma unroll
@@ -294,24 +388,44 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
         if (D * lane + e < a.hdr) o[D * lane + e] = acc[e] * inv;
 }
 
-constexpr int kCols = kPrefillNW * kColsPerWave;
-constexpr int kMinPart = 256;  // keys of a piece, at least: a piece costs a row of partials per column
-
 }  // namespace
 
-int shared_parts_cap(int n_rows, int G, int n_kv, int max_prefix, int stored_hd, int n_cu) {
-    const int64_t streams = ((int64_t)n_rows * G + kCols - 1) / kCols * n_kv;
-    const int64_t target = (int64_t)n_cu;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(target / streams, (max_prefix + kMinPart - 1) / kMinPart));
+// A chain needs no partials and no join, but its columns are one sequence's: taken for chunks that fill
+// blocks of 128 to 4/5 and the chip with blocks.
+static bool chains(int n_seq, int n_tok, int G, int n_kv, int n_cu) {
+    const int64_t cols = (int64_t)n_tok * G, blk = (cols + kCols - 1) / kCols;
+    return n_tok > 1 && 5 * cols >= 4 * blk * kCols && blk * n_seq * n_kv >= n_cu;
 }
 
-SharedPlan shared_plan(int n_rows, int G, int n_kv, int prefix_len, int stored_hd, int n_cu) {
+// Two groups of waves wherever one job per CU is all there is (and LDS holds both groups' windows).
+static int groups(int n_blk, int n_kv, int n_part, int stored_hd, int n_cu) {
+    return stored_hd <= 128 && (int64_t)n_blk * n_kv * n_part <= n_cu ? 2 : 1;
+}
+
+SharedPlan shared_plan(int n_seq, int n_tok, int G, int n_kv, int prefix_len, int stored_hd, int n_cu) {
     SharedPlan p;
-    p.n_blk = (int)(((int64_t)n_rows * G + kCols - 1) / kCols);
-    const int n = shared_parts_cap(n_rows, G, n_kv, prefix_len, stored_hd, n_cu);
-    p.chunk = ((prefix_len + n - 1) / n + kWin - 1) / kWin * kWin;
+    p.chain = chains(n_seq, n_tok, G, n_kv, n_cu);
+    p.n_blk = p.n_part = p.chunk = 0;
+    p.groups = 1;
+    p.own_blk = n_tok > 1 ? (n_tok * G + kCols - 1) / kCols : 0;
+    if (p.chain) {
+        p.own_blk = (n_tok * G + kCols - 1) / kCols;
+        return p;
+    }
+    // Pieces of the prefix: one job per CU, and a window at least for each of two groups.
+    p.n_blk = (int)(((int64_t)n_seq * n_tok * G + kCols - 1) / kCols);
+    const int64_t streams = (int64_t)p.n_blk * n_kv;
+    const int64_t n = std::max<int64_t>(1, std::min<int64_t>(n_cu / streams, (prefix_len + 2 * kWin - 1) / (2 * kWin)));
+    p.chunk = (int)((prefix_len + n - 1) / n + kWin - 1) / kWin * kWin;
     p.n_part = (prefix_len + p.chunk - 1) / p.chunk;
+    p.groups = groups(p.n_blk, n_kv, p.n_part, stored_hd, n_cu);
     return p;
+}
+
+int shared_slots_cap(int n_seq, int n_tok, int G, int n_kv, int max_prefix, int n_cu) {
+    if (chains(n_seq, n_tok, G, n_kv, n_cu)) return 0;
+    const int64_t streams = ((int64_t)n_seq * n_tok * G + kCols - 1) / kCols * n_kv;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(n_cu / streams, (max_prefix + 2 * kWin - 1) / (2 * kWin))) + (n_tok > 1);
 }
 
 hipError_t launch_shared(const SharedCall &c, hipStream_t st) {
@@ -328,23 +442,31 @@ hipError_t launch_shared(const SharedCall &c, hipStream_t st) {
     a.n_head = c.n_head;
     a.G = c.n_head / c.own.H;
     a.n_tok = c.n_tok;
+    a.chain = c.plan.chain;
     a.n_blk = c.plan.n_blk;
     a.n_part = c.plan.n_part;
     a.chunk = c.plan.chunk;
-    a.own_blk = c.own_part ? 0 : (c.n_tok * a.G + kCols - 1) / kCols;
+    a.own_blk = c.plan.own_blk;
     a.slots = a.n_part + (a.own_blk ? 1 : 0);
     a.inv_sqrt_hd = 1.0f / sqrtf((float)c.own.hdr);
     a.softcap = c.softcap;
     a.part = c.part;
+    a.out = c.out;
     const unsigned jobs = (unsigned)((a.n_blk * a.n_part + a.own_blk * c.own.S) * c.own.H);
     const bool cap = c.softcap > 0.0f, norm = c.own.qn != nullptr;
+#define TS_SH4(HDV, SC, NM, PD, NGRP)                                                                 \
+    {                                                                                                \
+        constexpr size_t lds = shared_lds<HDV, NGRP>();                                              \
+        static_assert(lds <= 156 * 1024, "a workgroup's windows fit a CU's LDS");                     \
+        if (lds > 64 * 1024)                                                                         \
+            (void)hipFuncSetAttribute((const void *)shared_kernel<HDV, SC, NM, PD, NGRP>,            \
+                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);         \
+        shared_kernel<HDV, SC, NM, PD, NGRP><<<jobs, 64 * kPrefillNW * NGRP, lds, st>>>(a);          \
+    }
 #define TS_SH3(HDV, SC, NM, PD)                                                                      \
     {                                                                                                \
-        constexpr size_t lds = sizeof(PrefillLds<HDV>);                                              \
-        if (lds > 64 * 1024)                                                                         \
-            (void)hipFuncSetAttribute((const void *)shared_kernel<HDV, SC, NM, PD>,                  \
-                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);         \
-        shared_kernel<HDV, SC, NM, PD><<<jobs, 64 * kPrefillNW, lds, st>>>(a);                       \
+        if (HDV <= 128 && c.plan.groups == 2) TS_SH4(HDV, SC, NM, PD, (HDV <= 128 ? 2 : 1))            \
+        else TS_SH4(HDV, SC, NM, PD, 1)                                                              \
     }
 #define TS_SH2(HDV, PD)                                                                              \
     {                                                                                                \
@@ -358,8 +480,9 @@ hipError_t launch_shared(const SharedCall &c, hipStream_t st) {
 #undef TS_SH
 #undef TS_SH2
 #undef TS_SH3
+#undef TS_SH4
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    if (e != hipSuccess || a.chain) return e;
     JoinArgs ja;
     ja.part = c.part;
     ja.own = c.own_part;
@@ -374,10 +497,15 @@ hipError_t launch_shared(const SharedCall &c, hipStream_t st) {
     ja.own_chunk = c.own_plan.chunk;
     ja.hlen = c.hlen;
     ja.cap = c.own.P;
-    const unsigned blocks = (ja.rows + 3) / 4;
-    if (c.own.hd == 256) join_kernel<256><<<blocks, 256, 0, st>>>(ja);
-    else if (c.own.hd == 128) join_kernel<128><<<blocks, 256, 0, st>>>(ja);
-    else join_kernel<64><<<blocks, 256, 0, st>>>(ja);
+    // Many parts of few rows: all four waves of a workgroup on one row.
+    const bool wide = ja.slots > 8 || ja.own_split > 8;
+    const unsigned blocks = wide ? ja.rows : (ja.rows + 3) / 4;
+#define TS_JOIN(HDV) \
+    { if (wide) join_kernel<HDV, 4><<<blocks, 256, 0, st>>>(ja); else join_kernel<HDV, 1><<<blocks, 256, 0, st>>>(ja); }
+    if (c.own.hd == 256) TS_JOIN(256)
+    else if (c.own.hd == 128) TS_JOIN(128)
+    else TS_JOIN(64)
+#undef TS_JOIN
     return hipGetLastError();
 }
 

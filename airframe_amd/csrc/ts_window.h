@@ -5,6 +5,12 @@
 #include "ts_mfma.h"
 
 namespace ts {
+
+// a b, with 0 for a = 0 and any b.  (The compiler's own operation and not inline asm: a transcendental
+// result must not be read by the very next instruction, and the compiler does not see that an asm
+// statement reads it; 64-dim rows came out wrong that way.)
+__device__ float mul_zero(float a, float b) __asm("llvm.amdgcn.fmul.legacy");
+
 namespace {
 
 constexpr int kPrefillNW = 4;  // waves per workgroup
@@ -367,11 +373,6 @@ __device__ inline void window_scores(floatx16 (&sc)[2], const float *sk, float s
             for (int i = 0; i < 16; i++) sc[kb][i] = sc[kb][i] - delta;
     }
 }
-
-// a b, with 0 for a = 0 and any b.  (The compiler's own operation and not inline asm: a transcendental
-// result must not be read by the very next instruction, and the compiler does not see that an asm
-// statement reads it; 64-dim rows came out wrong that way.)
-__device__ float mul_zero(float a, float b) __asm("llvm.amdgcn.fmul.legacy");
 
 // Probabilities of 16-key step st (keys 16st + 8h + 0..7 of the window) times s_v, split
 // hi + lo in f16 in the PV operand's slot order; adds the p to l_run.  p*s_v = hi + lo keeps

@@ -247,7 +247,7 @@ class KVCache:
         is stored as it is (rotated by the caller).  Lengths do not change (increment_packed)."""
         pk, sk = _rows(k, self.n_head_kv, self.head_dim, None, "k")
         pv, sv = _rows(v, self.n_head_kv, self.head_dim, k.dtype, "v")
-        off, keep, _ = _offsets(tok_off, self.n_seq, min(k.shape[0], v.shape[0]))
+        off, keep = _offsets(tok_off, self.n_seq, min(k.shape[0], v.shape[0]))[:2]
         self._check_device(k, v)
         code = _dtype(k.dtype, "k")
         _launch(self.device, stream, lambda raw: check("ts_append_packed", load().ts_append_packed(
@@ -258,7 +258,7 @@ class KVCache:
         """(K, V) of the cache as the values its codes stand for: positions pos0[s] .. (None: 0 ..) of
         sequence s in rows row_off[s] .. row_off[s + 1] - 1 of [rows, n_head_kv, head_dim], K as
         stored (rotated).  out: a pair of such tensors to write into."""
-        off, keep, n_seq = _offsets(row_off, self.n_seq, None, "row_off")
+        off, keep, _, _, rows = _offsets(row_off, self.n_seq, None, "row_off")
         p0 = None
         if pos0 is not None:
             if len(pos0) != self.n_seq:
@@ -269,27 +269,28 @@ class KVCache:
         if out is not None:
             dtype = out[0].dtype
             self._check_device(*out)
+            pk, sk = _rows(out[0], self.n_head_kv, self.head_dim, dtype, "K")
+            pv, sv = _rows(out[1], self.n_head_kv, self.head_dim, dtype, "V")
+            if rows > min(out[0].shape[0], out[1].shape[0]):
+                raise ValueError(f"row_off ends at row {rows} of {min(out[0].shape[0], out[1].shape[0])}")
         code = _dtype(dtype, "dtype")
 
         def call(raw):
-            rows = int(row_off[-1])
             if out is None:
-                k, v = (torch.empty((max(rows, 0), self.n_head_kv, self.head_dim), dtype=dtype, device=self.device)
-                        for _ in range(2))
+                k = torch.empty((max(rows, 0), self.n_head_kv, self.head_dim), dtype=dtype, device=self.device)
+                v = torch.empty_like(k)
+                n = self.n_head_kv * self.head_dim
+                at = (k.data_ptr(), n, v.data_ptr(), n)
             else:
-                k, v = out
-            pk, sk = _rows(k, self.n_head_kv, self.head_dim, dtype, "K")
-            pv, sv = _rows(v, self.n_head_kv, self.head_dim, dtype, "V")
-            if rows > min(k.shape[0], v.shape[0]):
-                raise ValueError(f"row_off ends at row {rows} of {min(k.shape[0], v.shape[0])}")
-            check("ts_read_packed", load().ts_read_packed(self._h, layer, p0, off, code, pk, sk, pv, sv, raw))
+                (k, v), at = out, (pk, sk, pv, sv)
+            check("ts_read_packed", load().ts_read_packed(self._h, layer, p0, off, code, *at, raw))
             return k, v
 
         return _launch(self.device, stream, call)
 
     def increment_packed(self, tok_off, stream=None):
         """increment of a packed batch: sequence s grows by tok_off[s + 1] - tok_off[s]."""
-        off, keep, _ = _offsets(tok_off, self.n_seq, None)
+        off, keep = _offsets(tok_off, self.n_seq, None)[:2]
         _launch(self.device, stream, lambda raw: check("ts_kv_increment_packed", load().ts_kv_increment_packed(self._h, off, raw)))
 
     # ---- a prefix shared by the batch ----------------------------------------------------------

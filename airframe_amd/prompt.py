@@ -29,41 +29,44 @@ def _dtype(dtype: torch.dtype, what: str) -> int:
 
 def _rows(t: torch.Tensor, heads: int | None, head_dim: int | None, dtype: torch.dtype | None, what: str):
     """(address, stride in elements) of [rows, heads, head_dim] with contiguous head rows."""
-    if t.dim() != 3 or (heads is not None and t.shape[1] != heads) or (head_dim is not None and t.shape[2] != head_dim):
-        raise ValueError(f"{what} must be [rows, {heads or 'heads'}, {head_dim or 'head_dim'}], got {tuple(t.shape)}")
+    shape = t.shape
+    if len(shape) != 3 or (heads is not None and shape[1] != heads) or (head_dim is not None and shape[2] != head_dim):
+        raise ValueError(f"{what} must be [rows, {heads or 'heads'}, {head_dim or 'head_dim'}], got {tuple(shape)}")
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{what} must be {dtype}, got {t.dtype}")
     if not t.is_cuda:
         raise ValueError(f"{what} must be a device tensor")
-    n, h, d = t.shape
-    if (d > 1 and t.stride(2) != 1) or (h > 1 and t.stride(1) != d):
+    n, h, d = shape
+    stride = t.stride()
+    if (stride[2] != 1 and d > 1) or (stride[1] != d and h > 1):
         raise ValueError(f"{what}: the heads of a token must be contiguous")
-    return ctypes.c_void_p(t.data_ptr()), t.stride(0) if n > 1 else h * d
+    return t.data_ptr(), stride[0] if n > 1 else h * d
 
 
 def _offsets(off, n_seq: int | None, n_rows: int | None, what: str = "tok_off"):
-    """(host pointer, what keeps it alive, number of sequences) of row offsets; n_rows: the most
-    rows that they may reach."""
+    """(host address, what keeps it alive, number of sequences, first and last offset) of row offsets;
+    n_rows: the most rows that they may reach."""
     if isinstance(off, torch.Tensor):
         if off.dtype != torch.int32 or off.is_cuda or off.dim() != 1 or not off.is_contiguous():
             raise ValueError(f"{what} must be a list of ints or a contiguous int32 CPU tensor")
-        n, last, ptr = off.numel(), None, ctypes.c_void_p(off.data_ptr())
-        if n:
-            last = int(off[-1])
+        n, ptr = off.numel(), off.data_ptr()
     else:
-        off = (ctypes.c_int32 * len(off))(*off)
-        n, last, ptr = len(off), off[-1] if len(off) else None, ctypes.cast(off, ctypes.c_void_p)
+        n = len(off)
+        off = (ctypes.c_int32 * n)(*off)
+        ptr = ctypes.addressof(off)
     if n < 2 or (n_seq is not None and n != n_seq + 1):
         raise ValueError(f"{what} must hold {'at least one sequence' if n_seq is None else n_seq} + 1 offsets, got {n}")
+    first, last = ctypes.c_int32.from_address(ptr).value, ctypes.c_int32.from_address(ptr + 4 * (n - 1)).value
     if n_rows is not None and last > n_rows:
         raise ValueError(f"{what} ends at row {last} of {n_rows}")
-    return ptr, off, n - 1
+    return ptr, off, n - 1, first, last
 
 
 def _same_device(first: torch.Tensor, *others):
+    device = first.device
     for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"tensors on {first.device} and {t.device}")
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors on {device} and {t.device}")
 
 
 @contextlib.contextmanager
@@ -81,7 +84,7 @@ def _on(device: torch.device, stream):
 
 def _plain(device: torch.device, stream) -> bool:
     """Whether a call runs where the thread is already (the usual case: no contexts to enter)."""
-    return stream is None and device.index == torch.cuda.current_device()
+    return stream is None and device.index == torch._C._cuda_getDevice()
 
 
 def _launch(device: torch.device, stream, call):
@@ -103,20 +106,26 @@ def rope_apply(x: torch.Tensor, positions: torch.Tensor, rope, layout: str = "in
     code = _dtype(x.dtype, "x")
     px, sx = _rows(x, None, None, None, "x")
     n, heads, hd = x.shape
-    if positions.dtype != torch.int32 or positions.shape != (n,) or (n > 1 and positions.stride(0) != 1):
+    if positions.dtype != torch.int32 or positions.shape != (n,) or (n > 1 and positions.stride()[0] != 1):
         raise ValueError("positions must be [rows] int32, contiguous")
     _same_device(x, positions, out)
+    if out is not None:
+        po, so = _rows(out, heads, hd, x.dtype, "out")
+        if out.shape[0] != n:
+            raise ValueError(f"out must have x's {n} rows, got {out.shape[0]}")
 
     def call(raw):
-        o = torch.empty((n, heads, hd), dtype=x.dtype, device=x.device) if out is None else out
-        po, so = _rows(o, heads, hd, x.dtype, "out")
-        if o.shape[0] != n:
-            raise ValueError(f"out must have x's {n} rows, got {o.shape[0]}")
+        o, at, stride = (_fresh(x), None, heads * hd) if out is None else (out, po, so)
         check("ts_rope_apply", load().ts_rope_apply(rope.handle, _LAYOUT[layout], code, px, sx, positions.data_ptr(), n,
-                                                    heads, hd, po, so, raw))
+                                                    heads, hd, at or o.data_ptr(), stride, raw))
         return o
 
     return _launch(x.device, stream, call)
+
+
+def _fresh(x: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of x's shape, type and device."""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
 def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tok_off, softcap: float = 0.0,
@@ -131,26 +140,25 @@ def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tok_off, soft
     pk, sk = _rows(k, None, hd, q.dtype, "k")
     kv = k.shape[1]
     pv, sv = _rows(v, kv, hd, q.dtype, "v")
-    off, keep, n_seq = _offsets(tok_off, None, min(n, k.shape[0], v.shape[0]))
+    off, keep, n_seq, first, last = _offsets(tok_off, None, min(n, k.shape[0], v.shape[0]))
     _same_device(q, k, v, out, workspace)
+    if out is not None:
+        po, so = _rows(out, heads, hd, q.dtype, "out")
+        if out.shape[0] < last:
+            raise ValueError(f"out has {out.shape[0]} rows, tok_off ends at {last}")
 
     def call(raw):
-        first, last = int(tok_off[0]), int(tok_off[-1])
-        o = out
-        if o is None:
-            o = torch.empty((n, heads, hd), dtype=q.dtype, device=q.device)
+        o, at, stride = (_fresh(q), None, heads * hd) if out is None else (out, po, so)
+        if out is None:
             if first > 0:
                 o[:first].zero_()
             if last < n:
                 o[max(last, 0):].zero_()
-        po, so = _rows(o, heads, hd, q.dtype, "out")
-        if o.shape[0] < last:
-            raise ValueError(f"out has {o.shape[0]} rows, tok_off ends at {last}")
         ws = workspace
-        if ws is None and q.dtype == torch.float32:
+        if ws is None and code == TS_DTYPE_F32:
             ws = torch.empty(attn_prompt_workspace(q.dtype, max(last - first, 0), kv, hd), dtype=torch.uint8, device=q.device)
-        check("ts_attn_prompt", load().ts_attn_prompt(code, pq, sq, pk, sk, pv, sv, off, n_seq, heads, kv, hd, softcap, po, so,
-                                                      ws.data_ptr() if ws is not None else None,
+        check("ts_attn_prompt", load().ts_attn_prompt(code, pq, sq, pk, sk, pv, sv, off, n_seq, heads, kv, hd, softcap,
+                                                      at or o.data_ptr(), stride, ws.data_ptr() if ws is not None else None,
                                                       ws.numel() if ws is not None else 0, raw))
         return o
 

@@ -12,8 +12,8 @@ INVALID = -1
 
 def test_offsets():
     for off in ([0, 3, 5], torch.tensor([0, 3, 5], dtype=torch.int32)):
-        ptr, keep, n = P._offsets(off, 2, 5)
-        assert n == 2 and [ctypes.cast(ptr, ctypes.POINTER(ctypes.c_int32))[i] for i in range(3)] == [0, 3, 5]
+        ptr, keep, n, first, last = P._offsets(off, 2, 5)
+        assert (n, first, last) == (2, 0, 5) and list((ctypes.c_int32 * 3).from_address(ptr)) == [0, 3, 5]
     for off, n_seq, rows in (([0], None, None), ([], None, None), ([0, 1], 2, None), ([0, 1, 6], 2, 5),
                              (torch.tensor([0, 1]), 1, None), (torch.tensor([[0, 1]], dtype=torch.int32), 1, None),
                              (torch.tensor([0, 9, 1, 9], dtype=torch.int32)[::2], 1, None)):
