@@ -253,6 +253,10 @@ int ts_attn_shared(ts_kv *kv, const ts_kv *prefix, int32_t prefix_seq, int32_t l
     c.own_part = nullptr;
     c.own_plan = DecodePlan{1, 1, false, 4, 1};
     c.hlen = -1;
+    c.own_here = false;
+    c.k_new = d_k;
+    c.v_new = d_v;
+    c.n_cu = kv->n_cu;
     const hipStream_t st = as_stream(stream);
     if (n_tok == 1) {
         float *own = c.part + shared_part_floats(kv, n_head, 1, c.plan.n_part);
@@ -261,9 +265,21 @@ int ts_attn_shared(ts_kv *kv, const ts_kv *prefix, int32_t prefix_seq, int32_t l
         c.own_part = own;
         const int32_t *h_len = capturing(stream) || kv->len_captured ? nullptr : kv->h_len.data();
         if (h_len && kv->d.n_seq == 1) c.hlen = h_len[0];
-        const hipError_t e = launch_decode(c.own, kv->d_len, h_len, d_q, n_head, c.rope, c.rope_pairs, softcap, d_out, own,
-                                           c.own_plan, d_k, d_v, nullptr, st, true);
-        if (e != hipSuccess) return TS_ERR_HIP;
+        // The own keys' splits go out beside the prefix's pieces where they are the 16x16 kernel's (a few
+        // hundred keys: their round trips hide behind the prefix's products); long ones are the integer
+        // kernel's, in a launch of their own.
+        c.own_here = !c.own_plan.g4;
+        if (c.own_here && c.own_plan.nw > 4) {
+            // (a workgroup of its own per sequence is planned 8 or 16 waves wide; here they have 4 or 8)
+            constexpr int kSplit = 512;
+            c.own_plan.n_split = (c.own_plan.chunk + kSplit - 1) / kSplit;
+            c.own_plan.chunk = std::min(c.own_plan.chunk, kSplit);
+        }
+        if (!c.own_here) {
+            const hipError_t e = launch_decode(c.own, kv->d_len, h_len, d_q, n_head, c.rope, c.rope_pairs, softcap, d_out,
+                                               own, c.own_plan, d_k, d_v, nullptr, st, true);
+            if (e != hipSuccess) return TS_ERR_HIP;
+        }
     }
     return hip_status(launch_shared(c, st));
 }

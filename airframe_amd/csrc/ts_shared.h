@@ -11,7 +11,6 @@ namespace ts {
 struct SharedPlan {
     bool chain;
     int n_blk, n_part, chunk, own_blk;
-    int groups;  // groups of 4 waves per workgroup
 };
 SharedPlan shared_plan(int n_seq, int n_tok, int G, int n_kv, int prefix_len, int stored_hd, int n_cu);
 // The most partials a row has, of any prefix up to max_prefix (0 for chains).
@@ -29,11 +28,15 @@ struct SharedCall {
     float *out;
     SharedPlan plan;
     float *part;  // [n_seq n_tok n_head][n_part (+ 1 with own_blk)] of stored_hd + 2 floats
-    // One token: the partials that the decode kernel wrote of the own keys, its plan, and the length
-    // it was given with the launch (or -1).
+    // One token: where the decode kernel's partials of the own keys are, its plan, and the length it is
+    // given with the launch (or -1).  own_here: its workgroups (the 16x16 kernel's, four waves or eight) go
+    // out with the prefix's, with the new token's K and V to append, or null; otherwise they ran before.
     const float *own_part;
     DecodePlan own_plan;
     int hlen;
+    bool own_here;
+    const float *k_new, *v_new;
+    int n_cu;
 };
 hipError_t launch_shared(const SharedCall &c, hipStream_t st);
 

@@ -11,6 +11,7 @@
 // token, of the same window walk for a chunk.
 #include "ts_shared.h"
 
+#include "ts_decode_split.h"
 #include "ts_window.h"
 
 namespace ts {
@@ -25,33 +26,27 @@ struct SharedArgs {
     bool chain;                // one job walks the prefix and then a sequence's own keys
     int n_blk, n_part, chunk;  // the prefix's jobs: n_blk n_part per kv head (none in a chain)
     int own_blk;               // the own keys' jobs (or the chains): own_blk per (kv head, sequence)
+    bool own_decode;           // one token: the own keys' jobs are the decode kernel's splits (dec)
+    DecodeArgs dec;
     int slots;                 // partials per row: n_part, and one of the own keys if own_blk
     float inv_sqrt_hd, softcap;
     float *part, *out;
 };
 
-// The rotations of pairs 4u .. 4u + 3 at table row p, as load_rot8, in two 16-byte loads where the
-// table's rows allow it.
-__device__ inline void load_rot8_wide(const float *rope, int rope_pairs, int u, int p, float2 (&cs)[4]) {
-    if ((rope_pairs & 3) != 0) {
-        load_rot8(rope, rope_pairs, u, p, cs);
-        return;
-    }
-    const bool in = 4 * u < rope_pairs;
-    const float4 *t = reinterpret_cast<const float4 *>(rope + ((size_t)p * rope_pairs + (in ? 4 * u : 0)) * 2);
-    const float4 a = t[0], b = t[1];
-    cs[0] = make_float2(in ? a.x : 1.0f, in ? a.y : 0.0f);
-    cs[1] = make_float2(in ? a.z : 1.0f, in ? a.w : 0.0f);
-    cs[2] = make_float2(in ? b.x : 1.0f, in ? b.y : 0.0f);
-    cs[3] = make_float2(in ? b.z : 1.0f, in ? b.w : 0.0f);
-}
-
 constexpr int kCols = kPrefillNW * kColsPerWave;
 
-// LDS of one workgroup: the window tiles of its groups, afterwards the outputs of all columns.
+// LDS of one workgroup: the columns' rotated q, then the window tiles of its groups, then the outputs of
+// all columns (NGRP 2); or a decode split's.
+template <int HD, int NW>
+struct DecodeLds {
+    DecodeSplitSmem<HD, NW> sm;
+    __align__(16) float kd[HD], vd[HD];
+    float xnew[8];
+};
 template <int HD, int NGRP>
 constexpr size_t shared_lds() {
-    return std::max(NGRP * sizeof(PrefillLds<HD>), NGRP > 1 ? (size_t)kCols * (HD + 4) * sizeof(float) : 0);
+    return std::max(std::max(NGRP * sizeof(PrefillLds<HD>), (size_t)kCols * (HD + 4) * sizeof(float)),
+                    sizeof(DecodeLds<HD, kPrefillNW * NGRP>));
 }
 
 // One job: 128 columns (token, head) of one kv head against a range of keys, in the window walk of
@@ -70,6 +65,15 @@ __global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 
     // columns: rows (token of a sequence) from row_base on, G heads each; keys: n_pre windows of the
     // prefix from k_begin to k_end, then n_own windows of sequence s_own's own
     int row_base, n_cols, blk, slot, k_begin, k_end, s_own = 0, n_own = 0;
+    extern __shared__ __align__(16) unsigned char sh_smem[];
+    if (!over_prefix && a.own_decode) {
+        job -= a.n_blk * a.n_part;
+        const int split = job % a.dec.n_split, gi = job / a.dec.n_split % a.dec.NG;
+        DecodeLds<HD, NW * NGRP> &lds = *reinterpret_cast<DecodeLds<HD, NW * NGRP> *>(sh_smem);
+        decode_split<HD, SOFTCAP, NORM, PAD, NW * NGRP>(a.dec, split, h * a.dec.NG + gi, job / a.dec.n_split / a.dec.NG, lds.sm,
+                                                       lds.kd, lds.vd, lds.xnew);
+        return;
+    }
     if (over_prefix) {
         blk = job / a.n_part;
         slot = job % a.n_part;
@@ -93,9 +97,9 @@ __global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int grp = NGRP > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * NW)) : 0;
     const int j = lane & 31, hf = lane >> 5;
-    extern __shared__ __align__(16) unsigned char sh_smem[];
     PrefillLds<HD> &sm = *reinterpret_cast<PrefillLds<HD> *>(sh_smem + grp * sizeof(PrefillLds<HD>));
     __shared__ float sm_qb[NW * NGRP], sm_m[kCols], sm_l[kCols];
+    __shared__ int sm_pos[kCols];
 
     const float qmul = SOFTCAP ? a.inv_sqrt_hd : a.inv_sqrt_hd * kLog2e;
     const int krow = qk_row_key(j);
@@ -105,7 +109,6 @@ __global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 
     const int cc = live ? c : n_cols - 1;
     const int row = row_base + cc / G, s = row / T, tok = row - s * T;
     const int head = h * G + cc % G;
-    const float *qrow = a.q + ((size_t)row * a.n_head + head) * hdr;
 
     Pending<HD, NW> pd;
     const DeqConstV dk;
@@ -118,47 +121,81 @@ __global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 
     };
     if (grp < n_win) fetch(grp);
 
-    // q of this lane's column: norm, rotation at its position, power-of-two scale, hi/lo split
-    const int len_s = a.len[s], qslot = len_s + tok;  // the token's own slot
-    float q_s, inv_s;
-    half8 qh[NKS];
-    int6v ql1[NG], ql2[NG];
-    {
-        const float ns = QN ? qk_norm_scale(qrow, hdr, a.own.norm_eps) : 1.0f;
-        float xq[NKS][8];
-        float2 cs[NKS][4];
+    // q of all columns: read along their rows (a lane that reads its own column's row alone touches a
+    // line per 16 bytes: 6 us of a 25 us launch), normalized and rotated, and through LDS to the lanes
+    // that multiply it.
+    const int qslot = a.len[s] + tok;  // the token's own slot
+    if (threadIdx.x < 64 * NW && hf == 0) sm_pos[32 * wave + j] = min(rot_of(a.own, s, qslot), a.rope_rows - 1);
+    // (min: a graph replayed past the table)
+    float *const qs = reinterpret_cast<float *>(sh_smem);
+    constexpr int V4 = HD / 4, QST = HD + 4, NT = 64 * NW * NGRP, NQ = kCols * V4 / NT;
+    __syncthreads();
+    float qb = 0.0f;
+    constexpr int QU = NQ < 8 ? NQ : 8;  // (this many rows' loads together)
+#pragma unroll 1
+    for (int i0 = 0; i0 < NQ; i0 += QU) {
+        float4 x[QU];
+        float2 c0[QU], c1[QU];
 #pragma unroll
-        for (int t = 0; t < NKS; t++) q_read8(qrow, 2 * t + hf, QN, ns, xq[t], hdr);
-        const int qrot = min(rot_of(a.own, s, qslot), a.rope_rows - 1);  // (a graph replayed past the table)
+        for (int u = 0; u < QU; u++) {
+            const int at = threadIdx.x + NT * (i0 + u), cl = at / V4, d = 4 * (at % V4);
+            const int cg = c_blk + cl, ce = min(cg, n_cols - 1), rw = row_base + ce / G;
+            const bool in = cg < n_cols && d < hdr;
+            const float4 v = *reinterpret_cast<const float4 *>(a.q + ((size_t)rw * a.n_head + h * G + ce % G) * hdr + (in ? d : 0));
+            x[u] = keep4(in, v);
+            const int pr = min(d / 2, a.rope_pairs - 1), p1 = min(d / 2 + 1, a.rope_pairs - 1);
+            const float *rot = a.rope + (size_t)sm_pos[cl] * a.rope_pairs * 2;
+            c0[u] = *reinterpret_cast<const float2 *>(rot + 2 * pr);
+            c1[u] = *reinterpret_cast<const float2 *>(rot + 2 * p1);
+        }
 #pragma unroll
-        for (int t = 0; t < NKS; t++) load_rot8_wide(a.rope, a.rope_pairs, 2 * t + hf, qrot, cs[t]);
-        float qb = 0.0f;
+        for (int u = 0; u < QU; u++) {
+            const int at = threadIdx.x + NT * (i0 + u), cl = at / V4, d = 4 * (at % V4);
+            float4 v = x[u];
+            if (QN) {
+                float ss = v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w;
 #pragma unroll
-        for (int t = 0; t < NKS; t++)
-            qb = fmaxf(qb, fmaxf(fmaxf(fabsf(xq[t][0]) + fabsf(xq[t][1]), fabsf(xq[t][2]) + fabsf(xq[t][3])),
-                                 fmaxf(fabsf(xq[t][4]) + fabsf(xq[t][5]), fabsf(xq[t][6]) + fabsf(xq[t][7]))));
-        qb = wave_max(qb);
-        if (lane == 0) sm_qb[NW * grp + wave] = qb;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < NW; w++) qb = fmaxf(qb, sm_qb[NW * grp + w]);
-        q_scale(qb * qmul, q_s, inv_s);
-#pragma unroll
-        for (int g = 0; g < NG; g++) {
-            float lo[32];
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const int t = 4 * g + u;
-                split_q8_f32(xq[t], cs[t], 2 * t + hf, a.rope_pairs, qmul * q_s, qh[t], lo + 8 * u);
-                if (!live) {
-                    qh[t] = (half8)(_Float16)0.0f;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) lo[8 * u + e] = 0.0f;
-                }
+                for (int o = 1; o < V4; o <<= 1) ss += __shfl_xor(ss, o, 64);  // (a row's lanes: V4 in a row)
+                const float ns = qk_norm_scale_from_sum(ss, hdr, a.own.norm_eps);
+                const float4 w = *reinterpret_cast<const float4 *>(QN + (d < hdr ? d : 0));
+                v = make_float4(qk_norm_apply(v.x, ns, w.x), qk_norm_apply(v.y, ns, w.y), qk_norm_apply(v.z, ns, w.z),
+                                qk_norm_apply(v.w, ns, w.w));
             }
-            q_lo_terms(lo, ql1[g], ql2[g]);
+            if (d / 2 < a.rope_pairs) rope_rotate(v.x, v.y, c0[u]);
+            if (d / 2 + 1 < a.rope_pairs) rope_rotate(v.z, v.w, c1[u]);
+            qb = fmaxf(qb, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+            *reinterpret_cast<float4 *>(qs + cl * QST + d) = v;
         }
     }
+    qb = wave_max(qb);
+    if (lane == 0) sm_qb[NW * grp + wave] = qb;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW * NGRP; w++) qb = fmaxf(qb, sm_qb[w]);
+    // power-of-two scale, and the hi / lo split of this lane's column
+    float q_s, inv_s;
+    q_scale(qb * qmul, q_s, inv_s);
+    half8 qh[NKS];
+    int6v ql1[NG], ql2[NG];
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+        float lo[32];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int t = 4 * g + u;
+            const float *src = qs + (32 * wave + j) * QST + 8 * (2 * t + hf);
+            const floatx4 x0 = *reinterpret_cast<const floatx4 *>(src), x1 = *reinterpret_cast<const floatx4 *>(src + 4);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float v = opaque((kPerm[e] < 4 ? x0[kPerm[e] & 3] : x1[kPerm[e] & 3]) * (qmul * q_s));
+                const _Float16 hi = (_Float16)v;
+                qh[t][e] = hi;
+                lo[8 * u + e] = v - (float)hi;
+            }
+        }
+        q_lo_terms(lo, ql1[g], ql2[g]);
+    }
+    __syncthreads();  // (the windows' tiles take q's place)
 
     floatx16 o[NDB];
 #pragma unroll
@@ -299,7 +336,6 @@ __global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 
             }
         }
         __syncthreads();
-        constexpr int V4 = HD / 4;
         for (int x = threadIdx.x; x < kCols * V4; x += 64 * NW * NGRP) {
             const int cl = x / V4, d = 4 * (x % V4), cg = c_blk + cl;
             if (cg >= n_cols) break;
@@ -397,16 +433,10 @@ static bool chains(int n_seq, int n_tok, int G, int n_kv, int n_cu) {
     return n_tok > 1 && 5 * cols >= 4 * blk * kCols && blk * n_seq * n_kv >= n_cu;
 }
 
-// Two groups of waves wherever one job per CU is all there is (and LDS holds both groups' windows).
-static int groups(int n_blk, int n_kv, int n_part, int stored_hd, int n_cu) {
-    return stored_hd <= 128 && (int64_t)n_blk * n_kv * n_part <= n_cu ? 2 : 1;
-}
-
 SharedPlan shared_plan(int n_seq, int n_tok, int G, int n_kv, int prefix_len, int stored_hd, int n_cu) {
     SharedPlan p;
     p.chain = chains(n_seq, n_tok, G, n_kv, n_cu);
     p.n_blk = p.n_part = p.chunk = 0;
-    p.groups = 1;
     p.own_blk = n_tok > 1 ? (n_tok * G + kCols - 1) / kCols : 0;
     if (p.chain) {
         p.own_blk = (n_tok * G + kCols - 1) / kCols;
@@ -418,7 +448,6 @@ SharedPlan shared_plan(int n_seq, int n_tok, int G, int n_kv, int prefix_len, in
     const int64_t n = std::max<int64_t>(1, std::min<int64_t>(n_cu / streams, (prefix_len + 2 * kWin - 1) / (2 * kWin)));
     p.chunk = (int)((prefix_len + n - 1) / n + kWin - 1) / kWin * kWin;
     p.n_part = (prefix_len + p.chunk - 1) / p.chunk;
-    p.groups = groups(p.n_blk, n_kv, p.n_part, stored_hd, n_cu);
     return p;
 }
 
@@ -447,13 +476,41 @@ hipError_t launch_shared(const SharedCall &c, hipStream_t st) {
     a.n_part = c.plan.n_part;
     a.chunk = c.plan.chunk;
     a.own_blk = c.plan.own_blk;
+    a.own_decode = c.own_here;
     a.slots = a.n_part + (a.own_blk ? 1 : 0);
     a.inv_sqrt_hd = 1.0f / sqrtf((float)c.own.hdr);
     a.softcap = c.softcap;
     a.part = c.part;
     a.out = c.out;
-    const unsigned jobs = (unsigned)((a.n_blk * a.n_part + a.own_blk * c.own.S) * c.own.H);
-    const bool cap = c.softcap > 0.0f, norm = c.own.qn != nullptr;
+    int own_jobs = a.own_blk * c.own.S;  // per kv head
+    if (c.own_here) {
+        DecodeArgs &d = a.dec;
+        d = {};
+        d.L = c.own;
+        d.len = c.d_len;
+        d.hlen = c.hlen;
+        d.q = c.q;
+        d.rope = c.rope;
+        d.rope_pairs = c.rope_pairs;
+        d.n_head = c.n_head;
+        d.Gt = a.G;
+        d.NG = (a.G + 7) / 8;
+        d.G = std::min(a.G, 8);
+        d.chunk = c.own_plan.chunk;
+        d.n_split = c.own_plan.n_split;
+        d.inv_sqrt_hd = a.inv_sqrt_hd;
+        d.softcap = c.softcap;
+        d.out = c.out;
+        d.ws = const_cast<float *>(c.own_part);
+        d.k_new = c.k_new;
+        d.v_new = c.v_new;
+        d.keep = true;
+        own_jobs = d.n_split * d.NG * c.own.S;
+    }
+    const unsigned jobs = (unsigned)((a.n_blk * a.n_part + own_jobs) * c.own.H);
+    // Two groups of waves where every job has a CU for itself; with more jobs two workgroups share one.
+    const bool pairs = !a.chain && jobs <= (unsigned)c.n_cu;
+    const bool cap = c.softcap > 0.0f, norm = c.own.qn != nullptr || c.own.kn != nullptr;
 #define TS_SH4(HDV, SC, NM, PD, NGRP)                                                                 \
     {                                                                                                \
         constexpr size_t lds = shared_lds<HDV, NGRP>();                                              \
@@ -465,7 +522,7 @@ hipError_t launch_shared(const SharedCall &c, hipStream_t st) {
     }
 #define TS_SH3(HDV, SC, NM, PD)                                                                      \
     {                                                                                                \
-        if (HDV <= 128 && c.plan.groups == 2) TS_SH4(HDV, SC, NM, PD, (HDV <= 128 ? 2 : 1))            \
+        if (HDV <= 128 && pairs) TS_SH4(HDV, SC, NM, PD, (HDV <= 128 ? 2 : 1))            \
         else TS_SH4(HDV, SC, NM, PD, 1)                                                              \
     }
 #define TS_SH2(HDV, PD)                                                                              \
