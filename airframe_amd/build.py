@@ -45,7 +45,7 @@ SOURCES = {
     "ts_prompt.hip": MFMA_VGPR,
     "ts_shared.hip": MFMA_VGPR,
 }
-HEADERS = ["ts_internal.h", "ts_mfma.h", "ts_quant.h", "ts_store.h", "ts_gemm.h", "ts_gemv.h", "ts_kquant.h", "ts_host.h", "ts_packed.h", "ts_prompt.h", "ts_shared.h", "ts_window.h", "ts_decode_split.h", os.path.join("..", "..", "include", "turboshimmy.h")]
+HEADERS = ["ts_internal.h", "ts_mfma.h", "ts_quant.h", "ts_store.h", "ts_gemm.h", "ts_gemv.h", "ts_kquant.h", "ts_host.h", "ts_packed.h", "ts_prompt.h", "ts_shared.h", "ts_window.h", "ts_decode_split.h", "ts_decode_split_body.h", os.path.join("..", "..", "include", "turboshimmy.h")]
 
 
 def _compile(src: str, extra: list[str], objdir: str) -> str:

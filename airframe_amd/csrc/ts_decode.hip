@@ -37,12 +37,27 @@
 namespace ts {
 namespace {
 
+// PAD: the caller's head dim hdr is below the stored HD (rows of q, new K/V and the output are
+// hdr floats; the stored dims past them hold zeros).
+// NW waves per workgroup: 4 (two workgroups per CU up to 128 dims), or 8 / 16 for a plan that
+// gives every (sequence, kv head) stream one workgroup (a CU) of its own and no split: the
+// small-batch case, where the combine launch would be most of the step.
 template <int HD, bool SOFTCAP, bool NORM, bool PAD, int NW>
 __global__ __launch_bounds__(64 * NW, NW > 4 ? 1 : (HD > 128 ? 1 : 2)) void decode_split_kernel(DecodeArgs a) {
-    __shared__ __align__(16) DecodeSplitSmem<HD, NW> sm;
-    __shared__ __align__(16) float kd[HD], vd[HD];
+#define TS_SPLIT_X blockIdx.x
+#define TS_SPLIT_Y blockIdx.y
+#define TS_SPLIT_Z blockIdx.z
+#define TS_SPLIT_KEEP false
+#define TS_SPLIT_LDS                                   \
+    __shared__ __align__(16) DecodeSplitSmem<HD, NW> sm; \
+    __shared__ __align__(16) float kd[HD], vd[HD];       \
     __shared__ float xnew[8];
-    decode_split<HD, SOFTCAP, NORM, PAD, NW>(a, blockIdx.x, blockIdx.y, blockIdx.z, sm, kd, vd, xnew);
+#include "ts_decode_split_body.h"
+#undef TS_SPLIT_X
+#undef TS_SPLIT_Y
+#undef TS_SPLIT_Z
+#undef TS_SPLIT_LDS
+#undef TS_SPLIT_KEEP
 }
 
 // The merge of one (sequence, head) over its ns > 1 splits (body of decode_combine_kernel).
@@ -701,7 +716,7 @@ windows_done:
             lsum += e;
         }
         const size_t head = (size_t)s * a.n_head + h * G + hh;
-        if (n_split_s == 1 && !a.keep) {
+        if (n_split_s == 1) {
             // hdr is a multiple of 8: a float4 of dims lies wholly inside or outside the row
             const float inv = lsum > 0.0f ? 1.0f / lsum : 0.0f;
             if (d < hdr) {
@@ -1028,9 +1043,8 @@ void launch_integer(const DecodeArgs &a, int n_split, bool pad, int Gt, hipStrea
 hipError_t launch_decode(const KvLayerView &L, int32_t *d_len, const int32_t *h_len, const float *q, int n_head,
                          const float *rope, int rope_pairs, float softcap, float *out,
                          float *ws, const DecodePlan &plan, const float *k_new,
-                         const float *v_new, int32_t *adv, hipStream_t st, bool keep) {
+                         const float *v_new, int32_t *adv, hipStream_t st) {
     DecodeArgs a;
-    a.keep = keep;
     a.L = L;
     a.len = d_len;
     a.hlen = h_len && L.S == 1 ? h_len[0] : -1;
@@ -1068,13 +1082,13 @@ hipError_t launch_decode(const KvLayerView &L, int32_t *d_len, const int32_t *h_
          : (norm ? TS_SPLIT(HDV, false, true) : TS_SPLIT(HDV, false, false)))
     if (L.hd == 256) {
         TS_SPLIT_HD(256);
-        if (plan.n_split > 1 && !keep) decode_combine_kernel<256><<<dim3(n_head, L.S), 256, 0, st>>>(a);
+        if (plan.n_split > 1) decode_combine_kernel<256><<<dim3(n_head, L.S), 256, 0, st>>>(a);
     } else if (L.hd == 128) {
         TS_SPLIT_HD(128);
-        if (plan.n_split > 1 && !keep) decode_combine_kernel<128><<<dim3(n_head, L.S), 256, 0, st>>>(a);
+        if (plan.n_split > 1) decode_combine_kernel<128><<<dim3(n_head, L.S), 256, 0, st>>>(a);
     } else if (L.hd == 64) {
         TS_SPLIT_HD(64);
-        if (plan.n_split > 1 && !keep) decode_combine_kernel<64><<<dim3(n_head, L.S), 256, 0, st>>>(a);
+        if (plan.n_split > 1) decode_combine_kernel<64><<<dim3(n_head, L.S), 256, 0, st>>>(a);
     } else {
         return hipErrorInvalidValue;
     }

@@ -180,12 +180,11 @@ int decode_cap(int n_kv, int max_seq, int n_cu);
 // without: a length-update launch after the decode).  h_len: null, or the lengths of the n_seq
 // sequences as the host knows them when they are known to match the device's (an eager
 // call): with one sequence the kernels then take its length as an argument instead of reading
-// d_len first.  keep: the split partials stay in ws, also of a plan without a split, for the caller
-// to join (no combine launch; out is not written).
+// d_len first.
 hipError_t launch_decode(const KvLayerView &L, int32_t *d_len, const int32_t *h_len, const float *q, int n_head,
                          const float *rope, int rope_pairs, float softcap, float *out,
                          float *ws, const DecodePlan &plan, const float *k_new,
-                         const float *v_new, int32_t *adv, hipStream_t st, bool keep = false);
+                         const float *v_new, int32_t *adv, hipStream_t st);
 // n_cu: compute units of the device (the launch staggers its q reads when the grid fits them).
 hipError_t launch_prefill(const KvLayerView &L, const int32_t *d_len, const float *q,
                           int n_head, int n_tok, const float *rope, int rope_pairs,

@@ -251,37 +251,19 @@ int ts_attn_shared(ts_kv *kv, const ts_kv *prefix, int32_t prefix_seq, int32_t l
     c.plan = shared_plan(kv->d.n_seq, n_tok, G, kv->d.n_head_kv, P, kv->hdp, kv->n_cu);
     c.part = static_cast<float *>(d_workspace);
     c.own_part = nullptr;
-    c.own_plan = DecodePlan{1, 1, false, 4, 1};
+    c.own_chunk = c.own_split = 1;
     c.hlen = -1;
-    c.own_here = false;
     c.k_new = d_k;
     c.v_new = d_v;
     c.n_cu = kv->n_cu;
-    const hipStream_t st = as_stream(stream);
     if (n_tok == 1) {
-        float *own = c.part + shared_part_floats(kv, n_head, 1, c.plan.n_part);
+        c.own_part = c.part + shared_part_floats(kv, n_head, 1, c.plan.n_part);
         for (int s = 0; s < kv->d.n_seq; s++) kv->h_ctx[s] = kv->h_len[s] + 1;
-        c.own_plan = decode_plan(kv->h_ctx.data(), kv->d.n_seq, kv->d.n_head_kv, G, kv->n_cu, kv->hdp, d_k != nullptr);
-        c.own_part = own;
-        const int32_t *h_len = capturing(stream) || kv->len_captured ? nullptr : kv->h_len.data();
-        if (h_len && kv->d.n_seq == 1) c.hlen = h_len[0];
-        // The own keys' splits go out beside the prefix's pieces where they are the 16x16 kernel's (a few
-        // hundred keys: their round trips hide behind the prefix's products); long ones are the integer
-        // kernel's, in a launch of their own.
-        c.own_here = !c.own_plan.g4;
-        if (c.own_here && c.own_plan.nw > 4) {
-            // (a workgroup of its own per sequence is planned 8 or 16 waves wide; here they have 4 or 8)
-            constexpr int kSplit = 512;
-            c.own_plan.n_split = (c.own_plan.chunk + kSplit - 1) / kSplit;
-            c.own_plan.chunk = std::min(c.own_plan.chunk, kSplit);
-        }
-        if (!c.own_here) {
-            const hipError_t e = launch_decode(c.own, kv->d_len, h_len, d_q, n_head, c.rope, c.rope_pairs, softcap, d_out,
-                                               own, c.own_plan, d_k, d_v, nullptr, st, true);
-            if (e != hipSuccess) return TS_ERR_HIP;
-        }
+        shared_own_plan(kv->h_ctx.data(), kv->d.n_seq, kv->d.n_head_kv, G, kv->n_cu, &c.own_chunk, &c.own_split);
+        // (an eager call gives a lone sequence's length with the launch, as ts_attn_decode)
+        if (kv->d.n_seq == 1 && !capturing(stream) && !kv->len_captured) c.hlen = kv->h_len[0];
     }
-    return hip_status(launch_shared(c, st));
+    return hip_status(launch_shared(c, as_stream(stream)));
 }
 
 }  // extern "C"

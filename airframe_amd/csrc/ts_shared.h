@@ -13,6 +13,8 @@ struct SharedPlan {
     int n_blk, n_part, chunk, own_blk;
 };
 SharedPlan shared_plan(int n_seq, int n_tok, int G, int n_kv, int prefix_len, int stored_hd, int n_cu);
+// The splits of the own keys (n_ctx of them) for one token.
+void shared_own_plan(const int32_t *n_ctx, int n_seq, int n_kv, int G, int n_cu, int *chunk, int *n_split);
 // The most partials a row has, of any prefix up to max_prefix (0 for chains).
 int shared_slots_cap(int n_seq, int n_tok, int G, int n_kv, int max_prefix, int n_cu);
 
@@ -28,13 +30,12 @@ struct SharedCall {
     float *out;
     SharedPlan plan;
     float *part;  // [n_seq n_tok n_head][n_part (+ 1 with own_blk)] of stored_hd + 2 floats
-    // One token: where the decode kernel's partials of the own keys are, its plan, and the length it is
-    // given with the launch (or -1).  own_here: its workgroups (the 16x16 kernel's, four waves or eight) go
-    // out with the prefix's, with the new token's K and V to append, or null; otherwise they ran before.
-    const float *own_part;
-    DecodePlan own_plan;
+    // One token: the own keys go out as splits of the 16x16 decode kernel beside the prefix's pieces, their
+    // partials in own_part (null for a chunk), with the new token's K and V to append, or null; hlen: the
+    // sequence's length where the launch gives it (or -1).
+    float *own_part;
+    int own_chunk, own_split;
     int hlen;
-    bool own_here;
     const float *k_new, *v_new;
     int n_cu;
 };

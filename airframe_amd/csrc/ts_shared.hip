@@ -451,6 +451,21 @@ SharedPlan shared_plan(int n_seq, int n_tok, int G, int n_kv, int prefix_len, in
     return p;
 }
 
+// One token: the own keys in splits of at least 512 (two rounds of a workgroup's windows), longer ones where
+// the batch has more than fill the chip.
+void shared_own_plan(const int32_t *n_ctx, int n_seq, int n_kv, int G, int n_cu, int *chunk, int *n_split) {
+    constexpr int64_t kMinSplit = 512;
+    int64_t total = 0;
+    int most = 1;
+    for (int s = 0; s < n_seq; s++) {
+        total += n_ctx[s];
+        most = std::max(most, (int)n_ctx[s]);
+    }
+    const int64_t per_cu = (total * n_kv * ((G + 7) / 8) + n_cu - 1) / n_cu;
+    *chunk = (int)(std::max(kMinSplit, per_cu) + 63) / 64 * 64;
+    *n_split = (most + *chunk - 1) / *chunk;
+}
+
 int shared_slots_cap(int n_seq, int n_tok, int G, int n_kv, int max_prefix, int n_cu) {
     if (chains(n_seq, n_tok, G, n_kv, n_cu)) return 0;
     const int64_t streams = ((int64_t)n_seq * n_tok * G + kCols - 1) / kCols * n_kv;
@@ -476,14 +491,14 @@ hipError_t launch_shared(const SharedCall &c, hipStream_t st) {
     a.n_part = c.plan.n_part;
     a.chunk = c.plan.chunk;
     a.own_blk = c.plan.own_blk;
-    a.own_decode = c.own_here;
+    a.own_decode = c.own_part != nullptr;
     a.slots = a.n_part + (a.own_blk ? 1 : 0);
     a.inv_sqrt_hd = 1.0f / sqrtf((float)c.own.hdr);
     a.softcap = c.softcap;
     a.part = c.part;
     a.out = c.out;
     int own_jobs = a.own_blk * c.own.S;  // per kv head
-    if (c.own_here) {
+    if (c.own_part) {
         DecodeArgs &d = a.dec;
         d = {};
         d.L = c.own;
@@ -496,15 +511,14 @@ hipError_t launch_shared(const SharedCall &c, hipStream_t st) {
         d.Gt = a.G;
         d.NG = (a.G + 7) / 8;
         d.G = std::min(a.G, 8);
-        d.chunk = c.own_plan.chunk;
-        d.n_split = c.own_plan.n_split;
+        d.chunk = c.own_chunk;
+        d.n_split = c.own_split;
         d.inv_sqrt_hd = a.inv_sqrt_hd;
         d.softcap = c.softcap;
         d.out = c.out;
-        d.ws = const_cast<float *>(c.own_part);
+        d.ws = c.own_part;
         d.k_new = c.k_new;
         d.v_new = c.v_new;
-        d.keep = true;
         own_jobs = d.n_split * d.NG * c.own.S;
     }
     const unsigned jobs = (unsigned)((a.n_blk * a.n_part + own_jobs) * c.own.H);
@@ -550,8 +564,8 @@ hipError_t launch_shared(const SharedCall &c, hipStream_t st) {
     ja.n_head = c.n_head;
     ja.n_tok = c.n_tok;
     ja.hdr = c.own.hdr;
-    ja.own_split = c.own_plan.n_split;
-    ja.own_chunk = c.own_plan.chunk;
+    ja.own_split = c.own_split;
+    ja.own_chunk = c.own_chunk;
     ja.hlen = c.hlen;
     ja.cap = c.own.P;
     // Many parts of few rows: all four waves of a workgroup on one row.
