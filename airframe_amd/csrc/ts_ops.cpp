@@ -146,8 +146,8 @@ int ts_attn_prompt(int32_t dtype, const void *d_q, int64_t q_stride, const void 
     if (rows == 0) return TS_OK;
     const int64_t qrow = (int64_t)n_head * head_dim, krow = (int64_t)n_head_kv * head_dim;
     if (!rows_ok(d_q, q_stride, qrow, dtype) || !rows_ok(d_k, k_stride, krow, dtype) || !rows_ok(d_v, v_stride, krow, dtype) ||
-        !rows_ok(d_out, out_stride, qrow, dtype))
-        return TS_ERR_INVALID;
+        !rows_ok(d_out, out_stride, qrow, dtype) || std::max(std::max(q_stride, k_stride), v_stride) > (1 << 22))
+        return TS_ERR_INVALID;  // (offsets inside a tile of rows are 32-bit numbers)
     // a token's rows are read by the workgroups of later tokens: the output is apart from all inputs
     const int size = dtype_size(dtype);
     auto span = [&](const void *p, int64_t stride, int64_t row, int end) {

@@ -80,14 +80,16 @@ __device__ inline typename Vec8<T>::type v_operand(const unsigned char *p) {
     return __builtin_bit_cast(typename Vec8<T>::type, s);
 }
 
-// Whether any of 8 elements is infinite or NaN.
+// The largest exponent bits of packed 16-bit floats: m and those of v, and whether they are an infinity's or
+// a NaN's.
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 template <class V>
-__device__ inline bool any_bad(V v, bool f16) {
+__device__ inline void max_bits(u16x2 &m, V v) {
     const u32x4 w = __builtin_bit_cast(u32x4, v);
-    const uint32_t m = f16 ? 0x7C00u : 0x7F80u;
-    auto bad = [&](uint32_t x) { return (x & m) == m || ((x >> 16) & m) == m; };
-    return bad(w.x) || bad(w.y) || bad(w.z) || bad(w.w);
+#pragma unroll
+    for (int i = 0; i < 4; i++) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7FFF7FFFu));
 }
+__device__ inline bool not_finite(u16x2 m, bool f16) { return max(m[0], m[1]) >= (f16 ? 0x7C00 : 0x7F80); }
 // v with every element that is not finite replaced: by 0 (part 0), or all others by 0 and those by 1
 // where they are +inf or NaN (part 1), -inf or NaN (part 2).
 template <class T>
@@ -112,10 +114,10 @@ __device__ inline void load_lds(const u32x4 &rsrc, uint32_t voff, uint32_t lds) 
 // All loads into LDS of this wave have landed, and every wave of the workgroup got here.
 __device__ inline void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// A buffer of `bytes` from p on; reads past it give 0.
+// A buffer of `bytes` from p on (2^31 at most: no offset into it is larger); reads past it give 0.
 __device__ inline u32x4 buffer_of(const void *p, int64_t bytes) {
     const uint64_t a = (uint64_t)p;
-    u32x4 r = {(uint32_t)a, (uint32_t)(a >> 32) & 0xFFFFu, (uint32_t)min(bytes, (int64_t)0xFFFFFFFF), 0x00027000u};
+    u32x4 r = {(uint32_t)a, (uint32_t)(a >> 32) & 0xFFFFu, (uint32_t)min(bytes, (int64_t)0x80000000), 0x00027000u};
 #pragma unroll
     for (int i = 0; i < 4; i++) r[i] = __builtin_amdgcn_readfirstlane(r[i]);
     return r;
@@ -197,6 +199,24 @@ __global__ __launch_bounds__(64 * kPromptNW, HD * NP > 128 ? 1 : 2) void prompt_
                 pe = tid < KT ? a.ke[at] : a.ve[at];
             }
     };
+    // q of the block's columns takes the second buffers' place until the walk begins: read along its rows
+    // (a lane that reads its own column's row touches a line per 32 bytes).
+    constexpr bool QLDS = NP == 1 && kPromptCols * ROWB <= 2 * TILEB;
+    if constexpr (QLDS) {
+        constexpr int NQ = kPromptCols * ROWB / 1024 / NW;
+        const int tok0 = c_blk / G, g0 = c_blk - tok0 * G, last = n_cols - 1 - c_blk;
+        const float inv_g = 1.0f / (float)G;
+        const u32x4 qr = buffer_of(static_cast<const T *>(a.q) + (int64_t)(row0 + tok0) * a.qs + (int64_t)h * G * hd,
+                                   (int64_t)(n - 1 - tok0) * 2 * a.qs + (int64_t)G * hd * 2);
+#pragma unroll
+        for (int p = 0; p < NQ; p++) {
+            const int at = 64 * (wave + NW * p) + lane, cl = at / CPR, qc = kslot<CPR>(cl, at % CPR);
+            // (token and head of a column: an exact division of a small number)
+            const int x = g0 + min(cl, last), t = (int)(((float)x + 0.5f) * inv_g);
+            const uint32_t off = (uint32_t)t * (uint32_t)(2 * a.qs) + (uint32_t)((x - t * G) * hd * 2) + 16 * qc;
+            load_lds(qr, qc < n_chunk ? off : 0xFFFFFFF0u, lds0 + 2 * TILEB + 1024 * (wave + NW * p));
+        }
+    }
     fetch(0, 0);
     if constexpr (NP == 2)
         if (tid < 2 * KT) se[tid] = pe;
@@ -204,7 +224,12 @@ __global__ __launch_bounds__(64 * kPromptNW, HD * NP > 128 ? 1 : 2) void prompt_
     // q of this lane's column: k-step t holds dims 16 t + 8 hf ..
     V8 qh[NKS], ql[NP == 2 ? NKS : 1];
     float qscale = a.scale;
-    if constexpr (NP == 1) {
+    if constexpr (QLDS) {
+        tile_barrier();
+        const unsigned char *src = pr_smem + 2 * TILEB + (32 * wave + j) * ROWB;
+#pragma unroll
+        for (int t = 0; t < NKS; t++) qh[t] = *reinterpret_cast<const V8 *>(src + 16 * kslot<CPR>(j, 2 * t + hf));
+    } else if constexpr (NP == 1) {
         const T *qrow = static_cast<const T *>(a.q) + (row0 + tok) * a.qs + (int64_t)head * hd;
 #pragma unroll
         for (int t = 0; t < NKS; t++) {
@@ -386,8 +411,10 @@ __global__ __launch_bounds__(64 * kPromptNW, HD * NP > 128 ? 1 : 2) void prompt_
                 // part of any): what is not finite is added apart, where a visible key brings it.
                 bool bad = odd_rows;
                 if constexpr (NP == 1) {
+                    u16x2 bits = {0, 0};
 #pragma unroll
-                    for (int d = 0; d < DG; d++) bad |= any_bad(va[d][0], F16);
+                    for (int d = 0; d < DG; d++) max_bits(bits, va[d][0]);
+                    bad = not_finite(bits, F16);
                 }
                 if (__builtin_amdgcn_ballot_w64(bad) != 0) {
                     V8 see;
@@ -438,23 +465,53 @@ __global__ __launch_bounds__(64 * kPromptNW, HD * NP > 128 ? 1 : 2) void prompt_
     for (; w < n_tile; w++) step(std::true_type(), w, w * KT <= qmax_w);
 
     const float inv = 1.0f / both_sum(l_run);
-    O *orow = static_cast<O *>(a.out) + (row0 + tok) * a.os + (int64_t)head * hd;
+    // this lane half's 8 consecutive dims 32 db + 16 q2 + 8 hf .. of its column
+    auto dims8 = [&](int db, int q2, float (&x)[8]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int db = 0; db < NDB; db++)
-#pragma unroll
-        for (int q2 = 0; q2 < 2; q2++) {
-            // this lane half's 8 consecutive dims: 32 db + 16 q2 + 8 hf ..
-            float x[8];
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(o[db][8 * q2 + r] * inv),
-                                                          __float_as_uint(o[db][8 * q2 + 4 + r] * inv), false, false);
-                x[r] = __uint_as_float(s[0]);
-                x[4 + r] = __uint_as_float(s[1]);
-            }
-            const int d = 32 * db + 16 * q2 + 8 * hf;
-            if (live && d < hd) store8(orow + d, x);
+        for (int r = 0; r < 4; r++) {
+            auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(o[db][8 * q2 + r] * inv),
+                                                      __float_as_uint(o[db][8 * q2 + 4 + r] * inv), false, false);
+            x[r] = __uint_as_float(s[0]);
+            x[4 + r] = __uint_as_float(s[1]);
         }
+    };
+    if constexpr (QLDS) {
+        // through LDS (the tiles' place), so that the stores run along the rows
+        tile_barrier();
+        unsigned char *const mine = pr_smem + 32 * wave * ROWB;
+#pragma unroll
+        for (int db = 0; db < NDB; db++)
+#pragma unroll
+            for (int q2 = 0; q2 < 2; q2++) {
+                float x[8];
+                dims8(db, q2, x);
+                store8(reinterpret_cast<T *>(mine + j * ROWB + 16 * kslot<CPR>(j, 4 * db + 2 * q2 + hf)), x);
+            }
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this wave's part is written, and it alone reads it
+        __builtin_amdgcn_wave_barrier();
+        const int tok0 = c_wave / G, g0 = c_wave - tok0 * G;
+        const float inv_g = 1.0f / (float)G;
+#pragma unroll
+        for (int p = 0; p < 32 * CPR / 64; p++) {
+            const int at = 64 * p + lane, cl = at / CPR, ch = kslot<CPR>(cl, at % CPR);
+            const int x = g0 + cl, t = (int)(((float)x + 0.5f) * inv_g);
+            if (c_wave + cl < n_cols && ch < n_chunk)
+                *reinterpret_cast<u32x4 *>(static_cast<T *>(a.out) + (int64_t)(row0 + tok0 + t) * a.os +
+                                           (int64_t)(h * G + x - t * G) * hd + 8 * ch) =
+                    *reinterpret_cast<const u32x4 *>(mine + 16 * at);
+        }
+    } else {
+        O *orow = static_cast<O *>(a.out) + (row0 + tok) * a.os + (int64_t)head * hd;
+#pragma unroll
+        for (int db = 0; db < NDB; db++)
+#pragma unroll
+            for (int q2 = 0; q2 < 2; q2++) {
+                float x[8];
+                dims8(db, q2, x);
+                const int d = 32 * db + 16 * q2 + 8 * hf;
+                if (live && d < hd) store8(orow + d, x);
+            }
+    }
 }
 
 // f32 K and V rows into two f16 planes: x 2^-e = hi + lo with the row's largest |x| 2^-e in [2^13, 2^14),

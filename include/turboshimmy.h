@@ -458,7 +458,7 @@ int ts_attn_prompt_workspace(int32_t dtype, int32_t n_rows, int32_t n_head_kv, i
  * already rotated): out_t = softmax(cap(q_t k_j / sqrt(head_dim))) v_j, cap(x) = softcap tanh(x /
  * softcap) with softcap > 0.  d_q, d_out: rows of [n_head][head_dim], d_k, d_v: of
  * [n_head_kv][head_dim]; n_head a multiple of n_head_kv; head_dim a multiple of 8 up to 256; d_out
- * apart from the inputs (else TS_ERR_INVALID).  f16 and bf16 are multiplied as they are, the
+ * apart from the inputs, strides of the inputs up to 2^22 elements (else TS_ERR_INVALID).  f16 and bf16 are multiplied as they are, the
  * probabilities rounded to the same type; f32 at 22 bits of every factor.  Scores, softmax and sums
  * are f32.  What a token does not attend to has no part in its output, infinities and NaN
  * included.  d_workspace: ts_attn_prompt_workspace bytes of tok_off[n_seq] - tok_off[0] rows. */
