@@ -80,6 +80,15 @@ __device__ inline typename Vec8<T>::type v_operand(const unsigned char *p) {
     return __builtin_bit_cast(typename Vec8<T>::type, s);
 }
 
+// softcap tanh(x / softcap) in the exp2 domain, as c - 2 c / (1 + e^(2 x / softcap)) from two transcendental
+// instructions: within 2^-22 softcap of it, which moves a probability by far less than its rounding to
+// 16 bits does.  (f32 rows take tanhf: with it 373 us of a batch that takes 200 without softcap, with
+// this 235.)
+__device__ inline float cap16(float x, float softcap) {
+    const float c = softcap * kLog2e, e = __builtin_amdgcn_exp2f(x * (2.0f * kLog2e / softcap));
+    return c - 2.0f * c * __builtin_amdgcn_rcpf(e + 1.0f);
+}
+
 // The largest exponent bits of packed 16-bit floats: m and those of v, and whether they are an infinity's or
 // a NaN's.
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
@@ -126,7 +135,7 @@ __device__ inline u32x4 buffer_of(const void *p, int64_t bytes) {
 // T: the matrix cores' type; O: the rows' type (float with two planes); HD: head dims, padded; NP:
 // planes; KT: keys per tile.
 template <class T, class O, int HD, int NP, int KT, bool SOFTCAP>
-__global__ __launch_bounds__(64 * kPromptNW, HD * NP > 128 ? 1 : 2) void prompt_kernel(PromptArgs a) {
+__global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kernel(PromptArgs a) {
     using V8 = typename Vec8<T>::type;
     constexpr int CPR = NP * HD / 8;  // 16-byte chunks of a tile's row
     constexpr int ROWB = 16 * CPR, TILEB = KT * ROWB;
@@ -350,7 +359,7 @@ __global__ __launch_bounds__(64 * kPromptNW, HD * NP > 128 ? 1 : 2) void prompt_
                 for (int r = 0; r < 4; r++) {
                     float x = sc[b][4 * q + r];
                     if constexpr (!RAW) x *= k4[r];
-                    if constexpr (SOFTCAP) x = tanhf(x / a.softcap) * (a.softcap * kLog2e);
+                    if constexpr (SOFTCAP) x = NP == 2 ? tanhf(x / a.softcap) * (a.softcap * kLog2e) : cap16(x, a.softcap);
                     if constexpr (NP == 2) x += v4[r];
                     if constexpr (MASK)
                         if (base + 32 * b + 8 * q + 4 * hf + r > qpos) x = -INFINITY;
@@ -368,10 +377,32 @@ __global__ __launch_bounds__(64 * kPromptNW, HD * NP > 128 ? 1 : 2) void prompt_
 #pragma unroll
             for (int db = 0; db < NDB; db++) o[db] *= alpha;
         }
+        if constexpr (NP == 2)
+            if (__builtin_amdgcn_ballot_w64(odd_rows) != 0) {
+                // value rows that are not finite: the planes hold 0 for those elements, and a key that a column
+                // sees brings them as they are
+#pragma unroll 1
+                for (int kk = 0; kk < KT; kk++) {
+                    if (base + kk >= n || __builtin_amdgcn_readfirstlane(__float_as_int(ke[kk])) >= 0) continue;
+                    const float *vr = static_cast<const float *>(a.v) + (int64_t)(row0 + base + kk) * a.vs + (int64_t)h * hd;
+#pragma unroll
+                    for (int db = 0; db < NDB; db++)
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            const int d = 32 * db + 8 * q + 4 * hf;
+                            const floatx4 x = *reinterpret_cast<const floatx4 *>(vr + (d < hd ? d : 0));
+#pragma unroll
+                            for (int r = 0; r < 4; r++)
+                                o[db][4 * q + r] += base + kk <= qpos && !(fabsf(x[r]) < INFINITY) ? x[r] : 0.0f;
+                        }
+                }
+            }
         const float off = kTop - m_run;
         // O^T += V^T P^T, 16 keys at a time: the exponentials of a step run beside the products of the one
-        // before, and V's operands are read one group of products ahead.
-        constexpr int VG = 4 / NP, NVG = NDB < VG ? 1 : NDB / VG, NU = 2 * NKB * NVG;
+        // before, and V's operands are read one group of products ahead.  (Two planes: one dim tile a group, or
+        // 128 dims take more than the 256 registers that let two workgroups share a CU: 776 against 552 us for
+        // 16 f32 prompts of 300-2048 tokens.)
+        constexpr int VG = NP == 2 ? 1 : 4, NVG = NDB < VG ? 1 : NDB / VG, NU = 2 * NKB * NVG;
         constexpr int DG = NDB < VG ? NDB : VG;  // dim tiles of a group
         V8 vf[2][DG][NP];
         auto read_v = [&](int u) __attribute__((always_inline)) {
@@ -406,16 +437,13 @@ __global__ __launch_bounds__(64 * kPromptNW, HD * NP > 128 ? 1 : 2) void prompt_
             floatx16 *const og = o + DG * (u % NVG);
             if (u + 1 < NU) read_v(u + 1);
             __builtin_amdgcn_sched_barrier(0);
-            if constexpr (MASK || NP == 2) {
-                // 0 times an infinite or NaN value must not reach the sums (0: a masked key's P, or the low
-                // part of any): what is not finite is added apart, where a visible key brings it.
-                bool bad = odd_rows;
-                if constexpr (NP == 1) {
-                    u16x2 bits = {0, 0};
+            if constexpr (MASK && NP == 1) {
+                // 0 times an infinite or NaN value of a masked key must not reach the sums: what is not finite is
+                // added apart, where a visible key brings it.
+                u16x2 bits = {0, 0};
 #pragma unroll
-                    for (int d = 0; d < DG; d++) max_bits(bits, va[d][0]);
-                    bad = not_finite(bits, F16);
-                }
+                for (int d = 0; d < DG; d++) max_bits(bits, va[d][0]);
+                const bool bad = not_finite(bits, F16);
                 if (__builtin_amdgcn_ballot_w64(bad) != 0) {
                     V8 see;
 #pragma unroll
@@ -434,7 +462,6 @@ __global__ __launch_bounds__(64 * kPromptNW, HD * NP > 128 ? 1 : 2) void prompt_
                         }
                         // (in place: these operands are not used again)
                         va[d][0] = bad_part<T>(va[d][0], 0);
-                        if constexpr (NP == 2) va[d][NP - 1] = bad_part<T>(va[d][NP - 1], 0);
                     }
                 }
             }
@@ -516,9 +543,9 @@ __global__ __launch_bounds__(64 * kPromptNW, HD * NP > 128 ? 1 : 2) void prompt_
 
 // f32 K and V rows into two f16 planes: x 2^-e = hi + lo with the row's largest |x| 2^-e in [2^13, 2^14),
 // hi rounded, lo the rest rounded (below 2^2: kept to 2^-9 of it and more).  K's scale is 2^e; of V's
-// the exponent e is kept.  A row of zeros, or one that is not finite throughout, has e = 0 (hi then
-// holds its infinities and NaN); a row of zeros of V e = -64, so that it claims no range of P.
-// A V row with an element that is not finite makes the K scale of its token negative.
+// the exponent e is kept.  A K row that is not finite throughout has e = 0, and hi its infinities and
+// NaN.  Of a V row such elements become 0, and the K scale of its token is made negative; V rows of zeros
+// have e = -64, so that they claim no range of P.
 // One thread per 8 dims of a row, a row's threads in one wave.
 template <int HD>
 __global__ __launch_bounds__(256) void prompt_split_kernel(const float *__restrict__ k, int64_t ks,
@@ -539,16 +566,20 @@ __global__ __launch_bounds__(256) void prompt_split_kernel(const float *__restri
         float x[8];
         load8(src + (int64_t)h * hd + (in ? 8 * l : 0), x);
         float m = 0.0f;
-        bool bad = false;
+        int bad = 0;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             x[e] = in ? x[e] : 0.0f;
-            m = fmaxf(m, fabsf(x[e]));
-            bad |= !(fabsf(x[e]) < INFINITY);
+            const bool fin = fabsf(x[e]) < INFINITY;
+            bad |= !fin;
+            if (which) x[e] = fin ? x[e] : 0.0f;
+            m = fmaxf(m, fin ? fabsf(x[e]) : which ? 0.0f : INFINITY);
         }
-        m = bad ? INFINITY : m;
 #pragma unroll
-        for (int o = 1; o < LPR; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        for (int o = 1; o < LPR; o <<= 1) {
+            m = fmaxf(m, __shfl_xor(m, o, 64));
+            bad |= __shfl_xor(bad, o, 64);
+        }
         int e2 = 0;
         if (m > 0.0f && m < INFINITY) e2 = max(ilogbf(m), -100) - 13;
         const float s = ldexpf(1.0f, -e2);
@@ -558,7 +589,7 @@ __global__ __launch_bounds__(256) void prompt_split_kernel(const float *__restri
             const float y = opaque(x[e] * s);
             hi[e] = (_Float16)y;
             const float rest = y - (float)hi[e];
-            lo[e] = fabsf(y) < INFINITY && fabsf((float)hi[e]) < INFINITY ? (_Float16)rest : (_Float16)0.0f;
+            lo[e] = fabsf(rest) < INFINITY ? (_Float16)rest : (_Float16)0.0f;
         }
         _Float16 *dst = (which ? vp : kp) + idx * (2 * HD) + 8 * l;
         *reinterpret_cast<f16x8 *>(dst) = hi;
@@ -566,7 +597,7 @@ __global__ __launch_bounds__(256) void prompt_split_kernel(const float *__restri
         if (l == 0) {
             if (which) {
                 ve[idx] = m == 0.0f ? -64.0f : (float)e2;
-                ke[idx] = m < INFINITY ? kscale : -kscale;
+                ke[idx] = bad ? -kscale : kscale;
             } else {
                 kscale = ldexpf(1.0f, e2);
             }

@@ -89,6 +89,14 @@ public:
         if (h_) ts_rope_destroy(h_);
     }
 
+    // A table stretched for long contexts, its angles in 64 bits (ts_rope_create_scaled).
+    static RopeTable scaled(int32_t n_pos, int32_t rope_dim, double base, double factor = 1.0, int32_t l_train = 0,
+                            double alpha = 0.0, double beta = 0.0, double mult = 1.0) {
+        ts_rope *h = nullptr;
+        check(ts_rope_create_scaled(n_pos, rope_dim, base, factor, l_train, alpha, beta, mult, &h), "ts_rope_create_scaled");
+        return RopeTable(h);
+    }
+
     // The host table [n_pos][rope_dim / 2][2] (cos, sin), bit-identical to the uploaded one.
     static std::vector<float> host_table(int32_t n_pos, int32_t rope_dim, float base, float scale = 1.0f,
                                          float yarn_alpha = 0.0f, float yarn_beta = 0.0f) {
@@ -104,6 +112,7 @@ public:
     const float *device_table() const { return info().first; }
 
 private:
+    explicit RopeTable(ts_rope *h) : h_(h) {}
     std::pair<const float *, std::pair<int32_t, int32_t>> info() const {
         const float *d = nullptr;
         int32_t n = 0, r = 0;
@@ -264,6 +273,43 @@ public:
         check(ts_kv_set_qk_norm(h_, layer, d_q_norm, d_k_norm, eps), "KVCache::set_qk_norm");
     }
 
+    // ---- packed batches: rows tok_off[s] .. tok_off[s + 1] - 1 of all arrays are sequence s's (host offsets)
+    void append_packed(int32_t layer, int32_t dtype, const void *d_k, int64_t k_stride, const void *d_v, int64_t v_stride,
+                       const int32_t *tok_off, const RopeTable *rope, void *stream = nullptr) {
+        check(ts_append_packed(h_, layer, dtype, d_k, k_stride, d_v, v_stride, tok_off, rope ? rope->get() : nullptr, stream),
+              "KVCache::append_packed");
+    }
+    void read_packed(int32_t layer, const int32_t *pos0, const int32_t *row_off, int32_t dtype, void *d_k, int64_t k_stride,
+                     void *d_v, int64_t v_stride, void *stream = nullptr) const {
+        check(ts_read_packed(h_, layer, pos0, row_off, dtype, d_k, k_stride, d_v, v_stride, stream), "KVCache::read_packed");
+    }
+    void increment_packed(const int32_t *tok_off, void *stream = nullptr) {
+        check(ts_kv_increment_packed(h_, tok_off, stream), "KVCache::increment_packed");
+    }
+
+    // ---- a prefix shared by the batch: every (empty) sequence continues sequence prefix_seq of `prefix`
+    void share_prefix(const KVCache &prefix, int32_t prefix_seq = 0, void *stream = nullptr) {
+        int32_t n = 0;
+        check(ts_kv_seq_len(prefix.h_, prefix_seq, &n), "KVCache::share_prefix");
+        for (int32_t s = 0; s < d_.n_seq; s++)
+            check(get_seq_len(s) == 0 && get_window_base(s) == 0 ? ts_kv_advance_window_base(h_, s, n, stream) : TS_ERR_INVALID,
+                  "KVCache::share_prefix");
+    }
+    uint64_t shared_workspace_bytes(const KVCache &prefix, int32_t n_head, int32_t n_tok = 1) const {
+        uint64_t b = 0;
+        check(ts_attn_shared_workspace(h_, prefix.h_, n_head, n_tok, &b), "ts_attn_shared_workspace");
+        return b;
+    }
+    // Attention of n_tok new tokens over the prefix and the own keys; d_k, d_v: nullptr, or (n_tok 1) the new
+    // token's K and V to append in the same launch.
+    void attn_shared(const KVCache &prefix, int32_t prefix_seq, int32_t layer, const float *d_k, const float *d_v,
+                     const float *d_q, int32_t n_head, int32_t n_tok, const RopeTable &rope, float *d_out,
+                     void *d_workspace, uint64_t workspace_bytes, float softcap = 0.0f, void *stream = nullptr) {
+        check(ts_attn_shared(h_, prefix.h_, prefix_seq, layer, d_k, d_v, d_q, n_head, n_tok, rope.get(), softcap, d_out,
+                             d_workspace, workspace_bytes, stream),
+              "KVCache::attn_shared");
+    }
+
 private:
     KVCache(ts_kv *h, const ts_kv_desc &d) : h_(h), d_(d) {}
     uint32_t max_seq_len_now() const {
@@ -277,6 +323,29 @@ private:
     ts_kv *h_ = nullptr;
     ts_kv_desc d_{};
 };
+
+// Rotary positions of packed head rows (ts_rope_apply).
+inline void rope_apply(const RopeTable &rope, int32_t layout, int32_t dtype, const void *d_x, int64_t x_stride,
+                       const int32_t *d_pos, int32_t n_tok, int32_t n_head, int32_t head_dim, void *d_out,
+                       int64_t out_stride, void *stream = nullptr) {
+    check(ts_rope_apply(rope.get(), layout, dtype, d_x, x_stride, d_pos, n_tok, n_head, head_dim, d_out, out_stride, stream),
+          "rope_apply");
+}
+
+// Causal attention over a packed batch of prompts (ts_attn_prompt).
+inline uint64_t attn_prompt_workspace(int32_t dtype, int32_t n_rows, int32_t n_head_kv, int32_t head_dim) {
+    uint64_t b = 0;
+    check(ts_attn_prompt_workspace(dtype, n_rows, n_head_kv, head_dim, &b), "ts_attn_prompt_workspace");
+    return b;
+}
+inline void attn_prompt(int32_t dtype, const void *d_q, int64_t q_stride, const void *d_k, int64_t k_stride, const void *d_v,
+                        int64_t v_stride, const int32_t *tok_off, int32_t n_seq, int32_t n_head, int32_t n_head_kv,
+                        int32_t head_dim, void *d_out, int64_t out_stride, void *d_workspace = nullptr,
+                        uint64_t workspace_bytes = 0, float softcap = 0.0f, void *stream = nullptr) {
+    check(ts_attn_prompt(dtype, d_q, q_stride, d_k, k_stride, d_v, v_stride, tok_off, n_seq, n_head, n_head_kv, head_dim,
+                         softcap, d_out, out_stride, d_workspace, workspace_bytes, stream),
+          "attn_prompt");
+}
 
 }  // namespace turboshimmy
 
