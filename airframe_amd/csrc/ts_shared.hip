@@ -286,28 +286,14 @@ __global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 
     float l = half_sum(l_run);
     const size_t rows = (size_t)a.own.S * T * a.n_head;
     const size_t row_head = (size_t)row * a.n_head + head;
-    if constexpr (NGRP == 1) {
-        if (!live) return;
-        float *dst = a.chain ? a.out + row_head * hdr : a.part + (row_head * a.slots + slot) * HD;
-        const float mul = !a.chain ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
-#pragma unroll
-        for (int db = 0; db < NDB; db++)
-#pragma unroll
-            for (int q = 0; q < 4; q++)
-                if (32 * db + 8 * q + 4 * hf < hdr)
-                    *reinterpret_cast<float4 *>(dst + 32 * db + 8 * q + 4 * hf) =
-                        make_float4(o[db][4 * q] * mul, o[db][4 * q + 1] * mul, o[db][4 * q + 2] * mul, o[db][4 * q + 3] * mul);
-        if (!a.chain && hf == 0) {
-            a.part[rows * a.slots * HD + row_head * a.slots + slot] = m_run;
-            a.part[rows * a.slots * (HD + 1) + row_head * a.slots + slot] = l;
-        }
-    } else {
-        // Group 1's outputs through LDS to group 0, the join back through LDS, and whole rows from there.
-        constexpr int OST = HD + 4;
-        float *const mo = reinterpret_cast<float *>(sh_smem);
-        const int col = 32 * wave + j;
-        if (first) m_run = kMinit;  // (a group or wave that had no window)
-        auto cell = [&](int db, int q) { return reinterpret_cast<floatx4 *>(mo + col * OST + 32 * db + 8 * q + 4 * hf); };
+    // The outputs go through LDS (the windows' place), whole rows from there: a join of two groups on the
+    // way, group 1's part added to group 0's.
+    constexpr int OST = HD + 4;
+    float *const mo = reinterpret_cast<float *>(sh_smem);
+    const int col = 32 * wave + j;
+    if (first) m_run = kMinit;  // (a group or wave that had no window)
+    auto cell = [&](int db, int q) { return reinterpret_cast<floatx4 *>(mo + col * OST + 32 * db + 8 * q + 4 * hf); };
+    if constexpr (NGRP > 1) {
         if (grp == 1) {
 #pragma unroll
             for (int db = 0; db < NDB; db++)
@@ -320,28 +306,37 @@ __global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 
             }
         }
         __syncthreads();
-        if (grp == 0) {
-            const float m1 = sm_m[col], l1 = sm_l[col], M = fmaxf(m_run, m1);
-            const float e0 = __builtin_amdgcn_exp2f(m_run - M), e1 = __builtin_amdgcn_exp2f(m1 - M);
+    }
+    if (grp == 0) {
+        float M = m_run, e0 = 1.0f, e1 = 0.0f;
+        if constexpr (NGRP > 1) {
+            const float m1 = sm_m[col];
+            M = fmaxf(m_run, m1);
+            e0 = __builtin_amdgcn_exp2f(m_run - M);
+            e1 = __builtin_amdgcn_exp2f(m1 - M);
+            l = e0 * l + e1 * sm_l[col];
+        }
+        if (a.chain) e0 = l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
-            for (int db = 0; db < NDB; db++)
+        for (int db = 0; db < NDB; db++)
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const floatx4 mine = {o[db][4 * q], o[db][4 * q + 1], o[db][4 * q + 2], o[db][4 * q + 3]};
-                    *cell(db, q) = e0 * mine + e1 * *cell(db, q);
-                }
-            if (live && hf == 0) {
-                a.part[rows * a.slots * HD + row_head * a.slots + slot] = M;
-                a.part[rows * a.slots * (HD + 1) + row_head * a.slots + slot] = e0 * l + e1 * l1;
+            for (int q = 0; q < 4; q++) {
+                floatx4 x = e0 * (floatx4){o[db][4 * q], o[db][4 * q + 1], o[db][4 * q + 2], o[db][4 * q + 3]};
+                if constexpr (NGRP > 1) x += e1 * *cell(db, q);
+                *cell(db, q) = x;
             }
+        if (!a.chain && live && hf == 0) {
+            a.part[rows * a.slots * HD + row_head * a.slots + slot] = M;
+            a.part[rows * a.slots * (HD + 1) + row_head * a.slots + slot] = l;
         }
-        __syncthreads();
-        for (int x = threadIdx.x; x < kCols * V4; x += 64 * NW * NGRP) {
-            const int cl = x / V4, d = 4 * (x % V4), cg = c_blk + cl;
-            if (cg >= n_cols) break;
-            const size_t rh = (size_t)(row_base + cg / G) * a.n_head + h * G + cg % G;
-            *reinterpret_cast<floatx4 *>(a.part + (rh * a.slots + slot) * HD + d) = *reinterpret_cast<floatx4 *>(mo + cl * OST + d);
-        }
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < kCols * V4; x += NT) {
+        const int cl = x / V4, d = 4 * (x % V4), cg = c_blk + cl;
+        if (cg >= n_cols) break;
+        const size_t rh = (size_t)(row_base + cg / G) * a.n_head + h * G + cg % G;
+        float *dst = a.chain ? a.out + rh * hdr : a.part + (rh * a.slots + slot) * HD;
+        if (d < hdr) *reinterpret_cast<floatx4 *>(dst + d) = *reinterpret_cast<floatx4 *>(mo + cl * OST + d);
     }
 }
 
@@ -350,7 +345,7 @@ struct JoinArgs {
     const float *own;   // the decode kernel's partials, or null
     const int32_t *len;
     float *out;
-    int rows, slots, n_head, n_tok, hdr;
+    int rows, slots, n_head, H, n_tok, hdr;
     int own_split, own_chunk, hlen, cap;  // of the decode plan; cap: positions of the own cache
 };
 
@@ -361,10 +356,12 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
     constexpr int D = HD / 64, RPW = 4 / NWR;  // rows per workgroup
     __shared__ float acc_s[4][HD], l_s[4];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wr = wave % NWR;
-    const int row = blockIdx.x * RPW + wave / NWR;
-    const bool some = row < a.rows;
-    const int r = some ? row : a.rows - 1;
-    const int tok = r / a.n_head, s = tok / a.n_tok;
+    // (rows of one kv head on the XCD that wrote their parts)
+    const int u = blockIdx.x / a.H * RPW + wave / NWR, G = a.n_head / a.H;
+    const bool some = u < a.rows / a.H;
+    const int uc = some ? u : a.rows / a.H - 1;
+    const int tok = uc / G, s = tok / a.n_tok;
+    const int row = tok * a.n_head + blockIdx.x % a.H * G + uc % G, r = row;
     const int qpos = (a.hlen >= 0 ? a.hlen : a.len[s]) + tok - s * a.n_tok;
     const float *po = a.part + (size_t)r * a.slots * HD, *pm = a.part + (size_t)a.rows * a.slots * HD + (size_t)r * a.slots;
     const float *pl = pm + (size_t)a.rows * a.slots;
@@ -562,6 +559,7 @@ hipError_t launch_shared(const SharedCall &c, hipStream_t st) {
     ja.rows = c.own.S * c.n_tok * c.n_head;
     ja.slots = a.slots;
     ja.n_head = c.n_head;
+    ja.H = c.own.H;
     ja.n_tok = c.n_tok;
     ja.hdr = c.own.hdr;
     ja.own_split = c.own_split;
@@ -570,7 +568,7 @@ hipError_t launch_shared(const SharedCall &c, hipStream_t st) {
     ja.cap = c.own.P;
     // Many parts of few rows: all four waves of a workgroup on one row.
     const bool wide = ja.slots > 8 || ja.own_split > 8;
-    const unsigned blocks = wide ? ja.rows : (ja.rows + 3) / 4;
+    const unsigned blocks = wide ? ja.rows : (ja.rows / ja.H + 3) / 4 * ja.H;
 #define TS_JOIN(HDV) \
     { if (wide) join_kernel<HDV, 4><<<blocks, 256, 0, st>>>(ja); else join_kernel<HDV, 1><<<blocks, 256, 0, st>>>(ja); }
     if (c.own.hd == 256) TS_JOIN(256)
