@@ -124,25 +124,33 @@ __global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 
     // q of all columns: read along their rows (a lane that reads its own column's row alone touches a
     // line per 16 bytes: 6 us of a 25 us launch), normalized and rotated, and through LDS to the lanes
     // that multiply it.
-    const int qslot = a.len[s] + tok;  // the token's own slot
-    if (threadIdx.x < 64 * NW && hf == 0) sm_pos[32 * wave + j] = min(rot_of(a.own, s, qslot), a.rope_rows - 1);
-    // (min: a graph replayed past the table)
     float *const qs = reinterpret_cast<float *>(sh_smem);
     constexpr int V4 = HD / 4, QST = HD + 4, NT = 64 * NW * NGRP, NQ = kCols * V4 / NT;
-    __syncthreads();
-    float qb = 0.0f;
-    constexpr int QU = NQ < 8 ? NQ : 8;  // (this many rows' loads together)
-#pragma unroll 1
-    for (int i0 = 0; i0 < NQ; i0 += QU) {
-        float4 x[QU];
-        float2 c0[QU], c1[QU];
+    constexpr int QU = NQ < 16 ? NQ : 16;  // (this many rows' loads together)
+    float4 x[QU];
+    auto load_q = [&](int i0) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < QU; u++) {
             const int at = threadIdx.x + NT * (i0 + u), cl = at / V4, d = 4 * (at % V4);
             const int cg = c_blk + cl, ce = min(cg, n_cols - 1), rw = row_base + ce / G;
-            const bool in = cg < n_cols && d < hdr;
-            const float4 v = *reinterpret_cast<const float4 *>(a.q + ((size_t)rw * a.n_head + h * G + ce % G) * hdr + (in ? d : 0));
-            x[u] = keep4(in, v);
+            const float4 v = *reinterpret_cast<const float4 *>(a.q + ((size_t)rw * a.n_head + h * G + ce % G) * hdr + (d < hdr ? d : 0));
+            x[u] = keep4(cg < n_cols && d < hdr, v);
+        }
+    };
+    load_q(0);
+    asm volatile("" ::: "memory");  // (on their way before the lengths are waited for)
+    const int qslot = a.len[s] + tok;  // the token's own slot
+    if (threadIdx.x < 64 * NW && hf == 0) sm_pos[32 * wave + j] = min(rot_of(a.own, s, qslot), a.rope_rows - 1);
+    // (min: a graph replayed past the table)
+    __syncthreads();
+    float qb = 0.0f;
+#pragma unroll 1
+    for (int i0 = 0; i0 < NQ; i0 += QU) {
+        if (i0 > 0) load_q(i0);
+        float2 c0[QU], c1[QU];
+#pragma unroll
+        for (int u = 0; u < QU; u++) {
+            const int at = threadIdx.x + NT * (i0 + u), cl = at / V4, d = 4 * (at % V4);
             const int pr = min(d / 2, a.rope_pairs - 1), p1 = min(d / 2 + 1, a.rope_pairs - 1);
             const float *rot = a.rope + (size_t)sm_pos[cl] * a.rope_pairs * 2;
             c0[u] = *reinterpret_cast<const float2 *>(rot + 2 * pr);
