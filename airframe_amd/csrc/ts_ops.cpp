@@ -195,7 +195,8 @@ int ts_attn_shared_workspace(const ts_kv *kv, const ts_kv *prefix, int32_t n_hea
     if (!bytes || !shared_shape_ok(kv, prefix, n_head, n_tok)) return TS_ERR_INVALID;
     *bytes = 0;
     if (n_tok == 0) return TS_OK;
-    const int cap = shared_slots_cap(kv->d.n_seq, n_tok, n_head / kv->d.n_head_kv, kv->d.n_head_kv, prefix->d.max_seq, kv->n_cu);
+    const int cap = shared_slots_cap(kv->d.n_seq, n_tok, n_head / kv->d.n_head_kv, kv->d.n_head_kv, prefix->d.max_seq,
+                                     kv->d.max_seq, kv->n_cu);
     uint64_t n = shared_part_floats(kv, n_head, n_tok, cap) * sizeof(float);
     if (n_tok == 1) {
         uint64_t own;
@@ -248,7 +249,8 @@ int ts_attn_shared(ts_kv *kv, const ts_kv *prefix, int32_t prefix_seq, int32_t l
     c.softcap = softcap;
     c.out = d_out;
     const int G = n_head / kv->d.n_head_kv;
-    c.plan = shared_plan(kv->d.n_seq, n_tok, G, kv->d.n_head_kv, P, kv->hdp, kv->n_cu);
+    const int own_max = *std::max_element(kv->h_len.begin(), kv->h_len.end()) + n_tok;
+    c.plan = shared_plan(kv->d.n_seq, n_tok, G, kv->d.n_head_kv, P, own_max, kv->n_cu);
     c.part = static_cast<float *>(d_workspace);
     c.own_part = nullptr;
     c.own_chunk = c.own_split = 1;

@@ -25,10 +25,11 @@ struct SharedArgs {
     int rope_pairs, rope_rows, n_head, G, n_tok;
     bool chain;                // one job walks the prefix and then a sequence's own keys
     int n_blk, n_part, chunk;  // the prefix's jobs: n_blk n_part per kv head (none in a chain)
-    int own_blk;               // the own keys' jobs (or the chains): own_blk per (kv head, sequence)
+    int own_blk;               // the own keys' jobs (or the chains): own_blk own_pieces per (kv head, sequence),
+    int own_pieces, own_chunk;   // each over own_chunk keys (the last to the end)
     bool own_decode;           // one token: the own keys' jobs are the decode kernel's splits (dec)
     DecodeArgs dec;
-    int slots;                 // partials per row: n_part, and one of the own keys if own_blk
+    int slots;                 // partials per row: n_part, and own_pieces if own_blk
     float inv_sqrt_hd, softcap;
     float *part, *out;
 };
@@ -64,7 +65,7 @@ __global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 
     const bool over_prefix = job < a.n_blk * a.n_part;
     // columns: rows (token of a sequence) from row_base on, G heads each; keys: n_pre windows of the
     // prefix from k_begin to k_end, then n_own windows of sequence s_own's own
-    int row_base, n_cols, blk, slot, k_begin, k_end, s_own = 0, n_own = 0;
+    int row_base, n_cols, blk, slot, k_begin, k_end, s_own = 0, n_own = 0, own_w0 = 0;
     extern __shared__ __align__(16) unsigned char sh_smem[];
     if (!over_prefix && a.own_decode) {
         job -= a.n_blk * a.n_part;
@@ -83,14 +84,28 @@ __global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 
         k_end = min(k_begin + a.chunk, a.prefix_len);
     } else {
         job -= a.n_blk * a.n_part;
+        const int piece = job % a.own_pieces;
+        job /= a.own_pieces;
         s_own = job / a.own_blk;
         blk = a.own_blk - 1 - job % a.own_blk;  // later tokens first
-        slot = a.n_part;
+        slot = a.n_part + piece;
         row_base = s_own * T;
         n_cols = T * G;
         k_begin = 0;
         k_end = a.chain ? a.prefix_len : 0;
         n_own = (min(a.len[s_own] + (min((blk + 1) * kCols, n_cols) - 1) / G + 1, a.own.P) + kWin - 1) / kWin;
+        own_w0 = piece * (a.own_chunk / kWin);
+        n_own = min(n_own - own_w0, piece + 1 < a.own_pieces ? a.own_chunk / kWin : n_own);
+        if (n_own <= 0) {  // (a shorter sequence than the longest: nothing here for the join)
+            const int cg = blk * kCols + threadIdx.x;
+            if (threadIdx.x < kCols && cg < n_cols) {
+                const size_t rows = (size_t)a.own.S * T * a.n_head;
+                const size_t r = ((size_t)(row_base + cg / G) * a.n_head + h * G + cg % G) * a.slots + slot;
+                a.part[rows * a.slots * HD + r] = kMinit;
+                a.part[rows * a.slots * (HD + 1) + r] = 0.0f;
+            }
+            return;
+        }
     }
     const int n_pre = (k_end - k_begin + kWin - 1) / kWin, n_win = n_pre + n_own;
     const int tid = threadIdx.x & (64 * NW - 1), lane = tid & 63;
@@ -117,7 +132,7 @@ __global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 
         const KvLayerView &L = w < n_pre ? a.pre : a.own;
         const size_t st = stream_of(L, w < n_pre ? a.prefix_seq : s_own);
         fetch_window<HD, NW>(pd, L.kp + st * L.P * ROWB, L.vp + st * (L.P / 32) * (HD * 16), L.ks + st * L.P, L.vs + st * L.P,
-                             w < n_pre ? k_begin + w * kWin : (w - n_pre) * kWin, tid, wave);
+                             w < n_pre ? k_begin + w * kWin : (own_w0 + w - n_pre) * kWin, tid, wave);
     };
     if (grp < n_win) fetch(grp);
 
@@ -260,7 +275,7 @@ __global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 
         // Keys are numbered within their stream: a column sees the prefix up to k_end, its own keys up to
         // its slot.
         const bool pre = w < n_pre;
-        const int base = pre ? k_begin + w * kWin : (w - n_pre) * kWin;
+        const int base = pre ? k_begin + w * kWin : (own_w0 + w - n_pre) * kWin;
         const int qpos = !live ? -1 : pre ? k_end - 1 : qslot;
         const int len_w = pre ? 0 : a.len[s_own];
         const int qmin_w = pre ? k_end - 1 : len_w + c_wave / G;
@@ -403,6 +418,7 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
         for (int k = 0; k < 8; k++) {
             if (i0 + k >= n) break;
             const float e2 = __builtin_amdgcn_exp2f(w[k] - M);
+            if (!(w[k] > kMinit)) continue;  // (a part without keys has no output)
 #pragma unroll
             for (int e = 0; e < D; e++) acc[e] += e2 * x[k][e];
             l += e2 * ls[k];
@@ -438,14 +454,24 @@ static bool chains(int n_seq, int n_tok, int G, int n_kv, int n_cu) {
     return n_tok > 1 && 5 * cols >= 4 * blk * kCols && blk * n_seq * n_kv >= n_cu;
 }
 
-SharedPlan shared_plan(int n_seq, int n_tok, int G, int n_kv, int prefix_len, int stored_hd, int n_cu) {
+// Pieces of own keys for a chunk that is no chain: until the jobs fill half the chip, of 256 keys at least.
+static int own_pieces(int n_seq, int own_blk, int n_kv, int own_max, int n_cu) {
+    const int64_t jobs = (int64_t)n_seq * own_blk * n_kv;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(n_cu / 2 / jobs, (own_max + 255) / 256));
+}
+
+SharedPlan shared_plan(int n_seq, int n_tok, int G, int n_kv, int prefix_len, int own_max, int n_cu) {
     SharedPlan p;
     p.chain = chains(n_seq, n_tok, G, n_kv, n_cu);
     p.n_blk = p.n_part = p.chunk = 0;
     p.own_blk = n_tok > 1 ? (n_tok * G + kCols - 1) / kCols : 0;
-    if (p.chain) {
-        p.own_blk = (n_tok * G + kCols - 1) / kCols;
-        return p;
+    p.own_pieces = 1;
+    p.own_chunk = 0;
+    if (p.chain) return p;
+    if (p.own_blk) {
+        const int n = own_pieces(n_seq, p.own_blk, n_kv, own_max, n_cu);
+        p.own_chunk = ((own_max + n - 1) / n + kWin - 1) / kWin * kWin;
+        p.own_pieces = (own_max + p.own_chunk - 1) / p.own_chunk;
     }
     // Pieces of the prefix: one job per CU, and a window at least for each of two groups.
     p.n_blk = (int)(((int64_t)n_seq * n_tok * G + kCols - 1) / kCols);
@@ -471,10 +497,11 @@ void shared_own_plan(const int32_t *n_ctx, int n_seq, int n_kv, int G, int n_cu,
     *n_split = (most + *chunk - 1) / *chunk;
 }
 
-int shared_slots_cap(int n_seq, int n_tok, int G, int n_kv, int max_prefix, int n_cu) {
+int shared_slots_cap(int n_seq, int n_tok, int G, int n_kv, int max_prefix, int own_max, int n_cu) {
     if (chains(n_seq, n_tok, G, n_kv, n_cu)) return 0;
     const int64_t streams = ((int64_t)n_seq * n_tok * G + kCols - 1) / kCols * n_kv;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(n_cu / streams, (max_prefix + 2 * kWin - 1) / (2 * kWin))) + (n_tok > 1);
+    const int pre = (int)std::max<int64_t>(1, std::min<int64_t>(n_cu / streams, (max_prefix + 2 * kWin - 1) / (2 * kWin)));
+    return pre + (n_tok > 1 ? own_pieces(n_seq, (n_tok * G + kCols - 1) / kCols, n_kv, own_max, n_cu) : 0);
 }
 
 hipError_t launch_shared(const SharedCall &c, hipStream_t st) {
@@ -497,12 +524,14 @@ hipError_t launch_shared(const SharedCall &c, hipStream_t st) {
     a.chunk = c.plan.chunk;
     a.own_blk = c.plan.own_blk;
     a.own_decode = c.own_part != nullptr;
-    a.slots = a.n_part + (a.own_blk ? 1 : 0);
+    a.own_pieces = c.plan.own_pieces;
+    a.own_chunk = c.plan.own_chunk;
+    a.slots = a.n_part + (a.own_blk ? a.own_pieces : 0);
     a.inv_sqrt_hd = 1.0f / sqrtf((float)c.own.hdr);
     a.softcap = c.softcap;
     a.part = c.part;
     a.out = c.out;
-    int own_jobs = a.own_blk * c.own.S;  // per kv head
+    int own_jobs = a.own_blk * a.own_pieces * c.own.S;  // per kv head
     if (c.own_part) {
         DecodeArgs &d = a.dec;
         d = {};

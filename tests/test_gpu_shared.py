@@ -114,6 +114,15 @@ def test_shared_long_prefix(gpu, heads, n_kv, hd):
     near(b.kv.attn_shared(1, b.q.cuda(), b.rope, b.pre), b.want(), b)
 
 
+@pytest.mark.parametrize("n_tok", [2, 9])
+@pytest.mark.parametrize("own", [[900, 3, 0, 517], [1400]])
+def test_shared_pieces_of_own_keys(gpu, own, n_tok):
+    """A few tokens over long own keys, in pieces that shorter sequences have nothing in."""
+    b = Batch(200, own, n_tok, 8, 2, 128)
+    b.append()
+    near(b.kv.attn_shared(1, b.q.cuda(), b.rope, b.pre), b.want(), b)
+
+
 def test_shared_equals_unshared(gpu):
     """A whole run: prompts behind a prefix, a chunk and then tokens, against one cache per sequence that
     holds prefix and all; the packed operators feed both."""
