@@ -67,6 +67,7 @@ int ts_rope_apply(const ts_rope *rope, int32_t layout, int32_t dtype, const void
         return TS_ERR_INVALID;
     if (n_tok == 0) return TS_OK;
     const int64_t row = (int64_t)n_head * head_dim;
+    if (row > (1 << 28)) return TS_ERR_INVALID;  // (a token's work items are 32-bit numbers)
     if (!d_pos || ((uintptr_t)d_pos & 3u) != 0 || !rows_ok(d_x, x_stride, row, dtype) || !rows_ok(d_out, out_stride, row, dtype))
         return TS_ERR_INVALID;
     // in place, or apart: a thread reads its rows before it writes them, but not before others write
@@ -144,6 +145,7 @@ int ts_attn_prompt(int32_t dtype, const void *d_q, int64_t q_stride, const void 
     if (head_dim > 256) return TS_ERR_UNSUPPORTED;
     const int64_t rows = (int64_t)tok_off[n_seq] - tok_off[0];
     if (rows == 0) return TS_OK;
+    if (rows * (n_head / n_head_kv) > INT32_MAX - 256) return TS_ERR_INVALID;  // (columns are 32-bit numbers)
     const int64_t qrow = (int64_t)n_head * head_dim, krow = (int64_t)n_head_kv * head_dim;
     if (!rows_ok(d_q, q_stride, qrow, dtype) || !rows_ok(d_k, k_stride, krow, dtype) || !rows_ok(d_v, v_stride, krow, dtype) ||
         !rows_ok(d_out, out_stride, qrow, dtype) || std::max(std::max(q_stride, k_stride), v_stride) > (1 << 22))

@@ -52,6 +52,8 @@ def _offsets(off, n_seq: int | None, n_rows: int | None, what: str = "tok_off"):
         n, ptr = off.numel(), off.data_ptr()
     else:
         n = len(off)
+        if n and not (-2 ** 31 <= min(off) and max(off) < 2 ** 31):
+            raise ValueError(f"{what} must be 32-bit numbers")
         off = (ctypes.c_int32 * n)(*off)
         ptr = ctypes.addressof(off)
     if n < 2 or (n_seq is not None and n != n_seq + 1):

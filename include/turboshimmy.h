@@ -426,8 +426,8 @@ int ts_rope_create_scaled(int32_t n_pos, int32_t rope_dim, double base, double f
 /* Rotary positions: out = x with the first rope_dim dims of every head rotated at the token's
  * position d_pos[t] (device, int32) and the rest copied; x: n_tok rows of [n_head][head_dim].  A
  * position outside the table makes the row's rotated dims NaN.  d_out may be d_x with the same stride
- * (in place); any other overlap is TS_ERR_INVALID.  Products and sums are rounded to f32 one by
- * one, the result once to dtype.  head_dim a multiple of 8. */
+ * (in place); ranges that overlap otherwise, also interleaved ones, are TS_ERR_INVALID.  Products and sums are rounded to f32 one by
+ * one, the result once to dtype.  head_dim a multiple of 8; n_head * head_dim up to 2^28. */
 int ts_rope_apply(const ts_rope *rope, int32_t layout, int32_t dtype, const void *d_x, int64_t x_stride,
                   const int32_t *d_pos, int32_t n_tok, int32_t n_head, int32_t head_dim, void *d_out,
                   int64_t out_stride, void *stream);
@@ -486,7 +486,8 @@ int ts_attn_shared_workspace(const ts_kv *kv, const ts_kv *prefix, int32_t n_hea
  * rotated at its position like there.  With n_tok 1, d_k and d_v: NULL, or the new token's K and V
  * [n_seq][n_head_kv][head_dim], appended in the same launch (ts_attn_decode_append).  Both caches have
  * the same heads, head_dim and device; every window base has to be P or more (TS_ERR_INVALID).  The
- * prefix's length is taken at the call, also into a graph.  d_workspace: ts_attn_shared_workspace
+ * prefix's length is taken at the call, also into a graph; the rope table of a captured call has to
+ * cover the positions its replays reach.  Runs on the caches' device.  d_workspace: ts_attn_shared_workspace
  * bytes, 16-byte aligned. */
 int ts_attn_shared(ts_kv *kv, const ts_kv *prefix, int32_t prefix_seq, int32_t layer, const float *d_k,
                    const float *d_v, const float *d_q, int32_t n_head, int32_t n_tok, const ts_rope *rope,

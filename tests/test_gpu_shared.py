@@ -206,6 +206,14 @@ def test_shared_what_lies_behind(gpu, n_tok):
     bad = torch.full((20, 2, 64), float("inf"), device="cuda")
     b.pre.append_packed(1, bad, bad, [0, 20], b.rope)
     assert torch.equal(b.kv.attn_shared(1, b.q.cuda(), b.rope, b.pre), want)
+    # and in slots of the batch's own, behind what it holds
+    kept = b.kv.seq_lens()
+    b.kv.increment(n_tok)
+    bad = torch.full((2, 20, 2, 64), float("inf"), device="cuda")
+    b.kv.append_quant(1, bad, bad, b.rope)
+    for s, m in enumerate(kept):
+        b.kv.set_seq_len(m, s)
+    assert torch.equal(b.kv.attn_shared(1, b.q.cuda(), b.rope, b.pre), want)
     if n_tok > 1:
         b.nv[:, 4, :, 3] = float("inf")
         b.append()

@@ -14,7 +14,7 @@ def test_offsets():
     for off in ([0, 3, 5], torch.tensor([0, 3, 5], dtype=torch.int32)):
         ptr, keep, n, first, last = P._offsets(off, 2, 5)
         assert (n, first, last) == (2, 0, 5) and list((ctypes.c_int32 * 3).from_address(ptr)) == [0, 3, 5]
-    for off, n_seq, rows in (([0], None, None), ([], None, None), ([0, 1], 2, None), ([0, 1, 6], 2, 5),
+    for off, n_seq, rows in (([0], None, None), ([0, 2 ** 32 + 1], None, None), ([], None, None), ([0, 1], 2, None), ([0, 1, 6], 2, 5),
                              (torch.tensor([0, 1]), 1, None), (torch.tensor([[0, 1]], dtype=torch.int32), 1, None),
                              (torch.tensor([0, 9, 1, 9], dtype=torch.int32)[::2], 1, None)):
         with pytest.raises(ValueError):
@@ -91,7 +91,8 @@ def test_more_null_handles_are_refused():
     assert rc(off=empty) == 0
     for kw in (dict(dtype=5), dict(q=None), dict(q=p + 8), dict(qs=63), dict(qs=68), dict(ks=1 << 23), dict(vs=(1 << 22) + 8),
                dict(n=-1), dict(h=0), dict(h=3, kv=2), dict(hd=62), dict(cap=-1.0), dict(cap=float("nan")), dict(out=p),
-               dict(out=q), dict(off=(ctypes.c_int32 * 2)(1, 0)), dict(off=(ctypes.c_int32 * 2)(-1, 0)), dict(off=None)):
+               dict(out=q), dict(off=(ctypes.c_int32 * 2)(1, 0)), dict(off=(ctypes.c_int32 * 2)(-1, 0)), dict(off=None),
+               dict(h=64, qs=4096, os=4096, off=(ctypes.c_int32 * 2)(0, 1 << 25))):
         assert rc(**kw) == INVALID, kw
     assert rc(hd=264, qs=264, ks=264, vs=264, os=264) == -3
     assert rc(dtype=0) == -6
