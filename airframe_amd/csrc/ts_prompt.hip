@@ -29,6 +29,7 @@ typedef short short8v __attribute__((ext_vector_type(8)));
 
 constexpr int kPromptNW = 4;
 constexpr int kPromptCols = 32 * kPromptNW;
+constexpr float kZeroRow = -200.0f;  // f32: V's exponent of a row of zeros (below any other: out of P's range)
 
 struct PromptArgs {
     const void *q, *k, *v;
@@ -300,6 +301,7 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
 #pragma unroll
     for (int db = 0; db < NDB; db++) o[db] = (floatx16)0.0f;
     float m_run = -3.4e38f, l_run = 0.0f;  // (below every finite score: the first tile sets it)
+    float m_sum = -3.4e38f;                // two planes: l_run's reference
     // P is held up to 2^(8 + kTop) (the maximum is raised lazily, by 2^8), which leaves f16 probabilities
     // 2^-30 of the largest before they are lost; bf16 has f32's range.
     constexpr float kTop = F16 ? 6.0f : 0.0f;
@@ -336,10 +338,12 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-        // x: scores in the exp2 domain (two planes: plus the value row's exponent, so that 2^x is the weight P
-        // has to carry); without softcap and planes their scale waits for the exponent's FMA
+        // x: scores in the exp2 domain; without softcap and planes their scale waits for the exponent's FMA.
+        // Two planes: P carries 2^(x + ve), the probability times its value row's size, and has a maximum of
+        // its own beside the sum's; both references are whole numbers, so that ve (a whole number of any
+        // size) and the reference cancel before x is added, and x keeps its last bits.
         const float *ke = se + (w & 1) * 2 * KT, *ve = ke + KT;
-        float mloc = -INFINITY;
+        float mloc = -INFINITY, msum = -INFINITY;
         bool odd_rows = false;  // two planes: a value row of the tile is not finite (its K scale is negative)
 #pragma unroll
         for (int b = 0; b < NKB; b++)
@@ -360,20 +364,30 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
                     float x = sc[b][4 * q + r];
                     if constexpr (!RAW) x *= k4[r];
                     if constexpr (SOFTCAP) x = NP == 2 ? tanhf(x / a.softcap) * (a.softcap * kLog2e) : cap16(x, a.softcap);
-                    if constexpr (NP == 2) x += v4[r];
                     if constexpr (MASK)
                         if (base + 32 * b + 8 * q + 4 * hf + r > qpos) x = -INFINITY;
                     sc[b][4 * q + r] = x;
-                    mloc = fmaxf(mloc, x);
+                    mloc = fmaxf(mloc, x + v4[r]);
+                    if constexpr (NP == 2) msum = fmaxf(msum, x);
                 }
             }
         mloc = both_max(mloc);
         if constexpr (RAW) mloc *= qscale;
-        if (__builtin_amdgcn_ballot_w64(mloc - m_run > 8.0f) != 0) {
+        if constexpr (NP == 2) {
+            mloc = ceilf(mloc);
+            msum = ceilf(both_max(msum));
+        }
+        if (__builtin_amdgcn_ballot_w64(mloc - m_run > 8.0f || (NP == 2 && msum - m_sum > 8.0f)) != 0) {
             const float m_new = mloc - m_run > 8.0f ? mloc : m_run;
             const float alpha = exp2f(m_run - m_new);
             m_run = m_new;
-            l_run *= alpha;
+            if constexpr (NP == 2) {
+                const float s_new = msum - m_sum > 8.0f ? msum : m_sum;
+                l_run *= exp2f(m_sum - s_new);
+                m_sum = s_new;
+            } else {
+                l_run *= alpha;
+            }
 #pragma unroll
             for (int db = 0; db < NDB; db++) o[db] *= alpha;
         }
@@ -425,8 +439,8 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         const float x = sc[st >> 1][8 * (st & 1) + 4 * q + r];
-                        const float p = __builtin_amdgcn_exp2f(RAW ? __builtin_fmaf(x, qscale, off) : x + off);
-                        l_run += NP == 2 ? p * __builtin_amdgcn_exp2f(-v4[r]) : p;
+                        const float p = __builtin_amdgcn_exp2f(RAW ? __builtin_fmaf(x, qscale, off) : x + (v4[r] + off));
+                        l_run += NP == 2 ? __builtin_amdgcn_exp2f(x - m_sum) : p;
                         const T hi = (T)p;
                         pb[4 * q + r] = hi;
                         if constexpr (NP == 2) pl[4 * q + r] = (T)(p - (float)hi);
@@ -501,6 +515,10 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
             x[r] = __uint_as_float(s[0]);
             x[4 + r] = __uint_as_float(s[1]);
         }
+        if constexpr (NP == 2) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = ldexpf(x[e], (int)(m_run - m_sum) - 13 - (int)kTop);
+        }
     };
     if constexpr (QLDS) {
         // through LDS (the tiles' place), so that the stores run along the rows
@@ -543,9 +561,9 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
 
 // f32 K and V rows into two f16 planes: x 2^-e = hi + lo with the row's largest |x| 2^-e in [2^13, 2^14),
 // hi rounded, lo the rest rounded (below 2^2: kept to 2^-9 of it and more).  K's scale is 2^e; of V's
-// the exponent e is kept.  A K row that is not finite throughout has e = 0, and hi its infinities and
-// NaN.  Of a V row such elements become 0, and the K scale of its token is made negative; V rows of zeros
-// have e = -64, so that they claim no range of P.
+// the exponent e + 13, about log2 of its largest element, is kept (from -90 on; kZeroRow for a row of
+// zeros).  A K row that is not finite throughout has e = 0, and hi its infinities and NaN.  Of a V row such
+// elements become 0, and the K scale of its token is made negative.
 // One thread per 8 dims of a row, a row's threads in one wave.
 template <int HD>
 __global__ __launch_bounds__(256) void prompt_split_kernel(const float *__restrict__ k, int64_t ks,
@@ -581,7 +599,7 @@ __global__ __launch_bounds__(256) void prompt_split_kernel(const float *__restri
             bad |= __shfl_xor(bad, o, 64);
         }
         int e2 = 0;
-        if (m > 0.0f && m < INFINITY) e2 = max(ilogbf(m), -100) - 13;
+        if (m > 0.0f && m < INFINITY) e2 = max(ilogbf(m), which ? -90 : -100) - 13;
         const float s = ldexpf(1.0f, -e2);
         f16x8 hi, lo;
 #pragma unroll
@@ -596,7 +614,7 @@ __global__ __launch_bounds__(256) void prompt_split_kernel(const float *__restri
         *reinterpret_cast<f16x8 *>(dst + HD) = lo;
         if (l == 0) {
             if (which) {
-                ve[idx] = m == 0.0f ? -64.0f : (float)e2;
+                ve[idx] = m == 0.0f ? kZeroRow : (float)(e2 + 13);
                 ke[idx] = bad ? -kscale : kscale;
             } else {
                 kscale = ldexpf(1.0f, e2);

@@ -98,6 +98,29 @@ def test_prompt_magnitudes(gpu, name):
             if dt == torch.float32 else first == v[0]).all()
 
 
+@pytest.mark.parametrize("hd", [64, 256])
+def test_prompt_f32_value_ranges(gpu, hd):
+    """f32 value rows from 1e-25 to 1e30 next to each other: every row's output is within the bound of its
+    own largest value that it sees (2^-18: 22 bits of every factor, and scores of some units)."""
+    n = 130
+    q, k, v = rand((n, 2, hd), 1), rand((n, 1, hd), 2), rand((n, 1, hd), 3)
+    v *= torch.tensor([10.0 ** (-25 + 55 * ((7 * i) % n) / (n - 1)) for i in range(n)])[:, None, None]
+    got = attn_prompt(q.cuda(), k.cuda(), v.cuda(), [0, n]).cpu().double()
+    want = plain(q, k, v, [0, n])
+    seen = v.abs().amax((1, 2)).cummax(0).values.double()[:, None, None]
+    assert ((got - want).abs() <= 2.0 ** -18 * seen).all()
+
+
+@pytest.mark.parametrize("scale", [1e-20, 1e25])
+def test_prompt_f32_small_and_large(gpu, scale):
+    """All values tiny or huge: the relative accuracy stays."""
+    n, hd = 70, 128
+    q, k, v = rand((n, 4, hd), 1), rand((n, 2, hd), 2), rand((n, 2, hd), 3)
+    want = attn_prompt(q.cuda(), k.cuda(), v.cuda(), [0, n]).cpu().double()
+    got = attn_prompt(q.cuda(), k.cuda(), (v * scale).cuda(), [0, n]).cpu().double() / scale
+    assert ((got - want).abs() <= 2.0 ** -20 * 5).all()
+
+
 @pytest.mark.parametrize("hd", [64, 128, 256])
 @pytest.mark.parametrize("name", NAMES)
 def test_prompt_masked_values(gpu, name, hd):
