@@ -209,24 +209,6 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
                 pe = tid < KT ? a.ke[at] : a.ve[at];
             }
     };
-    // q of the block's columns takes the second buffers' place until the walk begins: read along its rows
-    // (a lane that reads its own column's row touches a line per 32 bytes).
-    constexpr bool QLDS = NP == 1 && kPromptCols * ROWB <= 2 * TILEB;
-    if constexpr (QLDS) {
-        constexpr int NQ = kPromptCols * ROWB / 1024 / NW;
-        const int tok0 = c_blk / G, g0 = c_blk - tok0 * G, last = n_cols - 1 - c_blk;
-        const float inv_g = 1.0f / (float)G;
-        const u32x4 qr = buffer_of(static_cast<const T *>(a.q) + (int64_t)(row0 + tok0) * a.qs + (int64_t)h * G * hd,
-                                   (int64_t)(n - 1 - tok0) * 2 * a.qs + (int64_t)G * hd * 2);
-#pragma unroll
-        for (int p = 0; p < NQ; p++) {
-            const int at = 64 * (wave + NW * p) + lane, cl = at / CPR, qc = kslot<CPR>(cl, at % CPR);
-            // (token and head of a column: an exact division of a small number)
-            const int x = g0 + min(cl, last), t = (int)(((float)x + 0.5f) * inv_g);
-            const uint32_t off = (uint32_t)t * (uint32_t)(2 * a.qs) + (uint32_t)((x - t * G) * hd * 2) + 16 * qc;
-            load_lds(qr, qc < n_chunk ? off : 0xFFFFFFF0u, lds0 + 2 * TILEB + 1024 * (wave + NW * p));
-        }
-    }
     fetch(0, 0);
     if constexpr (NP == 2)
         if (tid < 2 * KT) se[tid] = pe;
@@ -234,12 +216,7 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
     // q of this lane's column: k-step t holds dims 16 t + 8 hf ..
     V8 qh[NKS], ql[NP == 2 ? NKS : 1];
     float qscale = a.scale;
-    if constexpr (QLDS) {
-        tile_barrier();
-        const unsigned char *src = pr_smem + 2 * TILEB + (32 * wave + j) * ROWB;
-#pragma unroll
-        for (int t = 0; t < NKS; t++) qh[t] = *reinterpret_cast<const V8 *>(src + 16 * kslot<CPR>(j, 2 * t + hf));
-    } else if constexpr (NP == 1) {
+    if constexpr (NP == 1) {
         const T *qrow = static_cast<const T *>(a.q) + (row0 + tok) * a.qs + (int64_t)head * hd;
 #pragma unroll
         for (int t = 0; t < NKS; t++) {
@@ -520,43 +497,16 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
             for (int e = 0; e < 8; e++) x[e] = ldexpf(x[e], (int)(m_run - m_sum) - 13 - (int)kTop);
         }
     };
-    if constexpr (QLDS) {
-        // through LDS (the tiles' place), so that the stores run along the rows
-        tile_barrier();
-        unsigned char *const mine = pr_smem + 32 * wave * ROWB;
+    O *orow = static_cast<O *>(a.out) + (row0 + tok) * a.os + (int64_t)head * hd;
 #pragma unroll
-        for (int db = 0; db < NDB; db++)
+    for (int db = 0; db < NDB; db++)
 #pragma unroll
-            for (int q2 = 0; q2 < 2; q2++) {
-                float x[8];
-                dims8(db, q2, x);
-                store8(reinterpret_cast<T *>(mine + j * ROWB + 16 * kslot<CPR>(j, 4 * db + 2 * q2 + hf)), x);
-            }
-        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this wave's part is written, and it alone reads it
-        __builtin_amdgcn_wave_barrier();
-        const int tok0 = c_wave / G, g0 = c_wave - tok0 * G;
-        const float inv_g = 1.0f / (float)G;
-#pragma unroll
-        for (int p = 0; p < 32 * CPR / 64; p++) {
-            const int at = 64 * p + lane, cl = at / CPR, ch = kslot<CPR>(cl, at % CPR);
-            const int x = g0 + cl, t = (int)(((float)x + 0.5f) * inv_g);
-            if (c_wave + cl < n_cols && ch < n_chunk)
-                *reinterpret_cast<u32x4 *>(static_cast<T *>(a.out) + (int64_t)(row0 + tok0 + t) * a.os +
-                                           (int64_t)(h * G + x - t * G) * hd + 8 * ch) =
-                    *reinterpret_cast<const u32x4 *>(mine + 16 * at);
+        for (int q2 = 0; q2 < 2; q2++) {
+            float x[8];
+            dims8(db, q2, x);
+            const int d = 32 * db + 16 * q2 + 8 * hf;
+            if (live && d < hd) store8(orow + d, x);
         }
-    } else {
-        O *orow = static_cast<O *>(a.out) + (row0 + tok) * a.os + (int64_t)head * hd;
-#pragma unroll
-        for (int db = 0; db < NDB; db++)
-#pragma unroll
-            for (int q2 = 0; q2 < 2; q2++) {
-                float x[8];
-                dims8(db, q2, x);
-                const int d = 32 * db + 16 * q2 + 8 * hf;
-                if (live && d < hd) store8(orow + d, x);
-            }
-    }
 }
 
 // f32 K and V rows into two f16 planes: x 2^-e = hi + lo with the row's largest |x| 2^-e in [2^13, 2^14),
@@ -636,8 +586,8 @@ void prompt_launch(const PromptArgs &a, unsigned blocks, hipStream_t st) {
 template <class T, class O, int NP>
 void prompt_dims(const PromptArgs &a, bool cap, unsigned blocks, hipStream_t st) {
     if (a.hd <= 64) {
-        if (cap) prompt_launch<T, O, 64, NP, 64, true>(a, blocks, st);
-        else prompt_launch<T, O, 64, NP, 64, false>(a, blocks, st);
+        if (cap) prompt_launch<T, O, 64, NP, 64 / NP, true>(a, blocks, st);
+        else prompt_launch<T, O, 64, NP, 64 / NP, false>(a, blocks, st);
     } else if (a.hd <= 128) {
         if (cap) prompt_launch<T, O, 128, NP, 64 / NP, true>(a, blocks, st);
         else prompt_launch<T, O, 128, NP, 64 / NP, false>(a, blocks, st);

@@ -36,25 +36,24 @@ struct SharedArgs {
 
 constexpr int kCols = kPrefillNW * kColsPerWave;
 
-// LDS of one workgroup: the columns' rotated q, then the window tiles of its groups, then the outputs of
-// all columns (NGRP 2); or a decode split's.
+// LDS of one workgroup: the columns' rotated q, then the window tiles, then the outputs of all columns;
+// or a decode split's.
 template <int HD, int NW>
 struct DecodeLds {
     DecodeSplitSmem<HD, NW> sm;
     __align__(16) float kd[HD], vd[HD];
     float xnew[8];
 };
-template <int HD, int NGRP>
+template <int HD>
 constexpr size_t shared_lds() {
-    return std::max(std::max(NGRP * sizeof(PrefillLds<HD>), (size_t)kCols * (HD + 4) * sizeof(float)),
-                    sizeof(DecodeLds<HD, kPrefillNW * NGRP>));
+    return std::max(std::max(sizeof(PrefillLds<HD>), (size_t)kCols * (HD + 4) * sizeof(float)),
+                    sizeof(DecodeLds<HD, kPrefillNW>));
 }
 
 // One job: 128 columns (token, head) of one kv head against a range of keys, in the window walk of
-// chunked prefill.  With NGRP 2 two groups of 4 waves take every second window and join through LDS:
-// a job that has a CU for itself then has two waves per SIMD, one's products beside the other's softmax.
-template <int HD, bool SOFTCAP, bool NORM, bool PAD, int NGRP>
-__global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 2) void shared_kernel(SharedArgs a) {
+// chunked prefill.
+template <int HD, bool SOFTCAP, bool NORM, bool PAD>
+__global__ __launch_bounds__(64 * kPrefillNW, HD > 128 ? 1 : 2) void shared_kernel(SharedArgs a) {
     constexpr int NW = kPrefillNW;
     constexpr int NKS = HD / 16, NDB = HD / 32, NG = NKS / 4, ROWB = HD / 2;
     const float *const QN = NORM ? a.own.qn : nullptr;
@@ -70,8 +69,8 @@ __global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 
     if (!over_prefix && a.own_decode) {
         job -= a.n_blk * a.n_part;
         const int split = job % a.dec.n_split, gi = job / a.dec.n_split % a.dec.NG;
-        DecodeLds<HD, NW * NGRP> &lds = *reinterpret_cast<DecodeLds<HD, NW * NGRP> *>(sh_smem);
-        decode_split<HD, SOFTCAP, NORM, PAD, NW * NGRP>(a.dec, split, h * a.dec.NG + gi, job / a.dec.n_split / a.dec.NG, lds.sm,
+        DecodeLds<HD, NW> &lds = *reinterpret_cast<DecodeLds<HD, NW> *>(sh_smem);
+        decode_split<HD, SOFTCAP, NORM, PAD, NW>(a.dec, split, h * a.dec.NG + gi, job / a.dec.n_split / a.dec.NG, lds.sm,
                                                        lds.kd, lds.vd, lds.xnew);
         return;
     }
@@ -108,12 +107,11 @@ __global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 
         }
     }
     const int n_pre = (k_end - k_begin + kWin - 1) / kWin, n_win = n_pre + n_own;
-    const int tid = threadIdx.x & (64 * NW - 1), lane = tid & 63;
+    const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int grp = NGRP > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * NW)) : 0;
     const int j = lane & 31, hf = lane >> 5;
-    PrefillLds<HD> &sm = *reinterpret_cast<PrefillLds<HD> *>(sh_smem + grp * sizeof(PrefillLds<HD>));
-    __shared__ float sm_qb[NW * NGRP], sm_m[kCols], sm_l[kCols];
+    PrefillLds<HD> &sm = *reinterpret_cast<PrefillLds<HD> *>(sh_smem);
+    __shared__ float sm_back[kCols];
     __shared__ int sm_pos[kCols];
 
     const float qmul = SOFTCAP ? a.inv_sqrt_hd : a.inv_sqrt_hd * kLog2e;
@@ -134,13 +132,13 @@ __global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 
         fetch_window<HD, NW>(pd, L.kp + st * L.P * ROWB, L.vp + st * (L.P / 32) * (HD * 16), L.ks + st * L.P, L.vs + st * L.P,
                              w < n_pre ? k_begin + w * kWin : (own_w0 + w - n_pre) * kWin, tid, wave);
     };
-    if (grp < n_win) fetch(grp);
+    fetch(0);
 
     // q of all columns: read along their rows (a lane that reads its own column's row alone touches a
     // line per 16 bytes: 6 us of a 25 us launch), normalized and rotated, and through LDS to the lanes
     // that multiply it.
     float *const qs = reinterpret_cast<float *>(sh_smem);
-    constexpr int V4 = HD / 4, QST = HD + 4, NT = 64 * NW * NGRP, NQ = kCols * V4 / NT;
+    constexpr int V4 = HD / 4, QST = HD + 4, NT = 64 * NW, NQ = kCols * V4 / NT;
     constexpr int QU = NQ < 16 ? NQ : 16;  // (this many rows' loads together)
     float4 x[QU];
     auto load_q = [&](int i0) __attribute__((always_inline)) {
@@ -155,10 +153,9 @@ __global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 
     load_q(0);
     asm volatile("" ::: "memory");  // (on their way before the lengths are waited for)
     const int qslot = a.len[s] + tok;  // the token's own slot
-    if (threadIdx.x < 64 * NW && hf == 0) sm_pos[32 * wave + j] = min(rot_of(a.own, s, qslot), a.rope_rows - 1);
+    if (hf == 0) sm_pos[32 * wave + j] = min(rot_of(a.own, s, qslot), a.rope_rows - 1);
     // (min: a graph replayed past the table)
     __syncthreads();
-    float qb = 0.0f;
 #pragma unroll 1
     for (int i0 = 0; i0 < NQ; i0 += QU) {
         if (i0 > 0) load_q(i0);
@@ -186,18 +183,24 @@ __global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 
             }
             if (d / 2 < a.rope_pairs) rope_rotate(v.x, v.y, c0[u]);
             if (d / 2 + 1 < a.rope_pairs) rope_rotate(v.z, v.w, c1[u]);
-            qb = fmaxf(qb, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
             *reinterpret_cast<float4 *>(qs + cl * QST + d) = v;
         }
     }
-    qb = wave_max(qb);
-    if (lane == 0) sm_qb[NW * grp + wave] = qb;
     __syncthreads();
+    // A power-of-two scale of each column for the hi / lo split, taken back from its scores: a column is
+    // another sequence's, whose large, infinite or NaN q must not cost this one its bits.  (Through LDS:
+    // in a register it costs the walk spills.)
+    const float *const qrow = qs + (32 * wave + j) * QST;
+    float mc = 0.0f;
 #pragma unroll
-    for (int w = 0; w < NW * NGRP; w++) qb = fmaxf(qb, sm_qb[w]);
-    // power-of-two scale, and the hi / lo split of this lane's column
-    float q_s, inv_s;
-    q_scale(qb * qmul, q_s, inv_s);
+    for (int t = 0; t < HD / 8; t++) {
+        const floatx4 x = *reinterpret_cast<const floatx4 *>(qrow + 4 * (2 * t + hf));
+        mc = fmaxf(fmaxf(mc, fmaxf(fabsf(x[0]), fabsf(x[1]))), fmaxf(fabsf(x[2]), fabsf(x[3])));
+    }
+    float q_s, q_back;
+    q_scale(half_max(mc) * qmul, q_s, q_back);
+    sm_back[32 * wave + j] = q_back;
+    // the split of this lane's column
     half8 qh[NKS];
     int6v ql1[NG], ql2[NG];
 #pragma unroll
@@ -206,7 +209,7 @@ __global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             const int t = 4 * g + u;
-            const float *src = qs + (32 * wave + j) * QST + 8 * (2 * t + hf);
+            const float *src = qrow + 8 * (2 * t + hf);
             const floatx4 x0 = *reinterpret_cast<const floatx4 *>(src), x1 = *reinterpret_cast<const floatx4 *>(src + 4);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
@@ -227,15 +230,12 @@ __global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 
     bool first = true;
 
     stage_codes<HD, NW>(sm, 0, pd, tid, wave, dk);
-    stage_scales<HD, NW, true>(sm, 0, pd, tid, inv_s);
-    if (grp + NGRP < n_win) fetch(grp + NGRP);
+    stage_scales<HD, NW, true>(sm, 0, pd, tid, 1.0f);
+    if (1 < n_win) fetch(1);
     __syncthreads();
 
-    // (every group makes the same number of rounds, for the barriers; one without a window left drops
-    // what it computes)
-    const int rounds = (n_win + NGRP - 1) / NGRP;
-    for (int it = 0; it < rounds; it++) {
-        const int buf = it & 1, w = it * NGRP + grp;
+    for (int w = 0; w < n_win; w++) {
+        const int buf = w & 1;
         floatx16 sc[2] = {(floatx16)0.0f, (floatx16)0.0f};
         __builtin_amdgcn_s_setprio(3);
         using PD = Pending<HD, NW>;
@@ -270,8 +270,8 @@ __global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 
         }
         if constexpr (NPART == 0) stage_codes<HD, NW>(sm, buf ^ 1, pd, tid, wave, dk);
         __builtin_amdgcn_s_setprio(0);
-        if (w + NGRP < n_win) stage_scales<HD, NW, true>(sm, buf ^ 1, pd, tid, inv_s);
-        if (w + 2 * NGRP < n_win) fetch(w + 2 * NGRP);
+        if (w + 1 < n_win) stage_scales<HD, NW, true>(sm, buf ^ 1, pd, tid, 1.0f);
+        if (w + 2 < n_win) fetch(w + 2);
         // Keys are numbered within their stream: a column sees the prefix up to k_end, its own keys up to
         // its slot.
         const bool pre = w < n_pre;
@@ -280,7 +280,10 @@ __global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 
         const int len_w = pre ? 0 : a.len[s_own];
         const int qmin_w = pre ? k_end - 1 : len_w + c_wave / G;
         const int qmax_w = pre ? k_end - 1 : len_w + (min(c_wave + kColsPerWave, n_cols) - 1) / G;
-        if (w < n_win && c_wave < n_cols && base <= qmax_w) {
+        if (c_wave < n_cols && base <= qmax_w) {
+            const float q_back = sm_back[32 * wave + j];
+            sc[0] *= q_back;
+            sc[1] *= q_back;
             const bool mask = base + kWin - 1 > qmin_w;
             window_scores<NDB, SOFTCAP>(sc, sm.sk[buf], sm.svlog[buf], a.softcap, mask, first, base, hf, qpos, m_run,
                                         l_run, o);
@@ -306,52 +309,22 @@ __global__ __launch_bounds__(64 * kPrefillNW * NGRP, NGRP > 1 || HD > 128 ? 1 : 
         __syncthreads();
     }
 
-    float l = half_sum(l_run);
+    const float l = half_sum(l_run);
     const size_t rows = (size_t)a.own.S * T * a.n_head;
     const size_t row_head = (size_t)row * a.n_head + head;
-    // The outputs go through LDS (the windows' place), whole rows from there: a join of two groups on the
-    // way, group 1's part added to group 0's.
+    // The outputs go through LDS (the windows' place), whole rows from there.
     constexpr int OST = HD + 4;
     float *const mo = reinterpret_cast<float *>(sh_smem);
-    const int col = 32 * wave + j;
-    if (first) m_run = kMinit;  // (a group or wave that had no window)
-    auto cell = [&](int db, int q) { return reinterpret_cast<floatx4 *>(mo + col * OST + 32 * db + 8 * q + 4 * hf); };
-    if constexpr (NGRP > 1) {
-        if (grp == 1) {
+    const float e0 = !a.chain ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-            for (int db = 0; db < NDB; db++)
+    for (int db = 0; db < NDB; db++)
 #pragma unroll
-                for (int q = 0; q < 4; q++)
-                    *cell(db, q) = (floatx4){o[db][4 * q], o[db][4 * q + 1], o[db][4 * q + 2], o[db][4 * q + 3]};
-            if (hf == 0) {
-                sm_m[col] = m_run;
-                sm_l[col] = l;
-            }
-        }
-        __syncthreads();
-    }
-    if (grp == 0) {
-        float M = m_run, e0 = 1.0f, e1 = 0.0f;
-        if constexpr (NGRP > 1) {
-            const float m1 = sm_m[col];
-            M = fmaxf(m_run, m1);
-            e0 = __builtin_amdgcn_exp2f(m_run - M);
-            e1 = __builtin_amdgcn_exp2f(m1 - M);
-            l = e0 * l + e1 * sm_l[col];
-        }
-        if (a.chain) e0 = l > 0.0f ? 1.0f / l : 0.0f;
-#pragma unroll
-        for (int db = 0; db < NDB; db++)
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                floatx4 x = e0 * (floatx4){o[db][4 * q], o[db][4 * q + 1], o[db][4 * q + 2], o[db][4 * q + 3]};
-                if constexpr (NGRP > 1) x += e1 * *cell(db, q);
-                *cell(db, q) = x;
-            }
-        if (!a.chain && live && hf == 0) {
-            a.part[rows * a.slots * HD + row_head * a.slots + slot] = M;
-            a.part[rows * a.slots * (HD + 1) + row_head * a.slots + slot] = l;
-        }
+        for (int q = 0; q < 4; q++)
+            *reinterpret_cast<floatx4 *>(mo + (32 * wave + j) * OST + 32 * db + 8 * q + 4 * hf) =
+                e0 * (floatx4){o[db][4 * q], o[db][4 * q + 1], o[db][4 * q + 2], o[db][4 * q + 3]};
+    if (!a.chain && live && hf == 0) {
+        a.part[rows * a.slots * HD + row_head * a.slots + slot] = first ? kMinit : m_run;  // (a wave without a window)
+        a.part[rows * a.slots * (HD + 1) + row_head * a.slots + slot] = l;
     }
     __syncthreads();
     for (int x = threadIdx.x; x < kCols * V4; x += NT) {
@@ -418,7 +391,7 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
         for (int k = 0; k < 8; k++) {
             if (i0 + k >= n) break;
             const float e2 = __builtin_amdgcn_exp2f(w[k] - M);
-            if (!(w[k] > kMinit)) continue;  // (a part without keys has no output)
+            if (ls[k] == 0.0f) continue;  // (a part without keys has no output; one of a NaN q has)
 #pragma unroll
             for (int e = 0; e < D; e++) acc[e] += e2 * x[k][e];
             l += e2 * ls[k];
@@ -438,7 +411,7 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
         }
     }
     if (!ok) return;
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     float *o = a.out + (size_t)row * a.hdr;
 #pragma unroll
     for (int e = 0; e < D; e++)
@@ -451,13 +424,13 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
 // blocks of 128 to 4/5 and the chip with blocks.
 static bool chains(int n_seq, int n_tok, int G, int n_kv, int n_cu) {
     const int64_t cols = (int64_t)n_tok * G, blk = (cols + kCols - 1) / kCols;
-    return n_tok > 1 && 5 * cols >= 4 * blk * kCols && blk * n_seq * n_kv >= n_cu;
+    return n_tok > 1 && 4 * cols >= 3 * blk * kCols && 2 * blk * n_seq * n_kv > n_cu;
 }
 
 // Pieces of own keys for a chunk that is no chain: until the jobs fill half the chip, of 256 keys at least.
 static int own_pieces(int n_seq, int own_blk, int n_kv, int own_max, int n_cu) {
     const int64_t jobs = (int64_t)n_seq * own_blk * n_kv;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(n_cu / 2 / jobs, (own_max + 255) / 256));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(n_cu / jobs, (own_max + 255) / 256));
 }
 
 SharedPlan shared_plan(int n_seq, int n_tok, int G, int n_kv, int prefix_len, int own_max, int n_cu) {
@@ -476,7 +449,7 @@ SharedPlan shared_plan(int n_seq, int n_tok, int G, int n_kv, int prefix_len, in
     // Pieces of the prefix: one job per CU, and a window at least for each of two groups.
     p.n_blk = (int)(((int64_t)n_seq * n_tok * G + kCols - 1) / kCols);
     const int64_t streams = (int64_t)p.n_blk * n_kv;
-    const int64_t n = std::max<int64_t>(1, std::min<int64_t>(n_cu / streams, (prefix_len + 2 * kWin - 1) / (2 * kWin)));
+    const int64_t n = std::max<int64_t>(1, std::min<int64_t>(n_cu / streams, (prefix_len + kWin - 1) / kWin));
     p.chunk = (int)((prefix_len + n - 1) / n + kWin - 1) / kWin * kWin;
     p.n_part = (prefix_len + p.chunk - 1) / p.chunk;
     return p;
@@ -500,7 +473,7 @@ void shared_own_plan(const int32_t *n_ctx, int n_seq, int n_kv, int G, int n_cu,
 int shared_slots_cap(int n_seq, int n_tok, int G, int n_kv, int max_prefix, int own_max, int n_cu) {
     if (chains(n_seq, n_tok, G, n_kv, n_cu)) return 0;
     const int64_t streams = ((int64_t)n_seq * n_tok * G + kCols - 1) / kCols * n_kv;
-    const int pre = (int)std::max<int64_t>(1, std::min<int64_t>(n_cu / streams, (max_prefix + 2 * kWin - 1) / (2 * kWin)));
+    const int pre = (int)std::max<int64_t>(1, std::min<int64_t>(n_cu / streams, (max_prefix + kWin - 1) / kWin));
     return pre + (n_tok > 1 ? own_pieces(n_seq, (n_tok * G + kCols - 1) / kCols, n_kv, own_max, n_cu) : 0);
 }
 
@@ -556,22 +529,15 @@ hipError_t launch_shared(const SharedCall &c, hipStream_t st) {
         own_jobs = d.n_split * d.NG * c.own.S;
     }
     const unsigned jobs = (unsigned)((a.n_blk * a.n_part + own_jobs) * c.own.H);
-    // Two groups of waves where every job has a CU for itself; with more jobs two workgroups share one.
-    const bool pairs = !a.chain && jobs <= (unsigned)c.n_cu;
     const bool cap = c.softcap > 0.0f, norm = c.own.qn != nullptr || c.own.kn != nullptr;
-#define TS_SH4(HDV, SC, NM, PD, NGRP)                                                                 \
-    {                                                                                                \
-        constexpr size_t lds = shared_lds<HDV, NGRP>();                                              \
-        static_assert(lds <= 156 * 1024, "a workgroup's windows fit a CU's LDS");                     \
-        if (lds > 64 * 1024)                                                                         \
-            (void)hipFuncSetAttribute((const void *)shared_kernel<HDV, SC, NM, PD, NGRP>,            \
-                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);         \
-        shared_kernel<HDV, SC, NM, PD, NGRP><<<jobs, 64 * kPrefillNW * NGRP, lds, st>>>(a);          \
-    }
 #define TS_SH3(HDV, SC, NM, PD)                                                                      \
     {                                                                                                \
-        if (HDV <= 128 && pairs) TS_SH4(HDV, SC, NM, PD, (HDV <= 128 ? 2 : 1))            \
-        else TS_SH4(HDV, SC, NM, PD, 1)                                                              \
+        constexpr size_t lds = shared_lds<HDV>();                                                    \
+        static_assert(lds <= 156 * 1024, "a workgroup's windows fit a CU's LDS");                     \
+        if (lds > 64 * 1024)                                                                         \
+            (void)hipFuncSetAttribute((const void *)shared_kernel<HDV, SC, NM, PD>,                  \
+                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);         \
+        shared_kernel<HDV, SC, NM, PD><<<jobs, 64 * kPrefillNW, lds, st>>>(a);                       \
     }
 #define TS_SH2(HDV, PD)                                                                              \
     {                                                                                                \
@@ -585,7 +551,6 @@ hipError_t launch_shared(const SharedCall &c, hipStream_t st) {
 #undef TS_SH
 #undef TS_SH2
 #undef TS_SH3
-#undef TS_SH4
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.chain) return e;
     JoinArgs ja;
@@ -604,7 +569,7 @@ hipError_t launch_shared(const SharedCall &c, hipStream_t st) {
     ja.hlen = c.hlen;
     ja.cap = c.own.P;
     // Many parts of few rows: all four waves of a workgroup on one row.
-    const bool wide = ja.slots > 8 || ja.own_split > 8;
+    const bool wide = ja.rows <= 4 * c.n_cu;
     const unsigned blocks = wide ? ja.rows : (ja.rows / ja.H + 3) / 4 * ja.H;
 #define TS_JOIN(HDV) \
     { if (wide) join_kernel<HDV, 4><<<blocks, 256, 0, st>>>(ja); else join_kernel<HDV, 1><<<blocks, 256, 0, st>>>(ja); }

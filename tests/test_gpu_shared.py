@@ -283,3 +283,18 @@ def test_shared_refusals(gpu):
         with pytest.raises(TsError) as e:
             bad()
         assert e.value.code == code
+
+
+@pytest.mark.parametrize("n_tok", [1, 2, 40])
+@pytest.mark.parametrize("heads,n_kv,hd", [(8, 2, 128), (4, 2, 256), (8, 8, 64)])
+def test_shared_columns_of_other_scales(gpu, n_tok, heads, n_kv, hd):
+    """Sequences whose q is huge, infinite or NaN stand in one matrix product with ordinary ones, which keep
+    every bit of their accuracy."""
+    b = Batch(300, [40, 3, 0, 11, 25], n_tok, heads, n_kv, hd)
+    b.append()
+    b.q[0] *= 2.0 ** 30
+    b.q[1, :, 0, 5] = float("inf")
+    b.q[2] = float("nan")
+    got = b.kv.attn_shared(1, b.q.cuda(), b.rope, b.pre)
+    assert got[1, :, 0].isnan().all() and got[2].isnan().all() and got[0].isfinite().all()
+    near(got[3:], b.want()[3:], b)
