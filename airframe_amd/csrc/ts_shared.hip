@@ -9,6 +9,11 @@
 // instead of once per sequence.  Its keys are divided among workgroups until they fill the chip;
 // the pieces are joined by a last kernel, with the own keys' parts: of the decode kernel for one
 // token, of the same window walk for a chunk.
+//
+// 32 heads over 8 of 128 dims, 32 sequences of 60 to 500 own keys behind 8192: 28.9 us (shared_kernel 23.3,
+// a CU's four windows with the q before and the partials behind them; join 6), of which the bytes would take
+// 3.4 and the matrix work 4.  Chunks of 256 tokens of 8 sequences behind 4097: 251 us, 142 GFLOP that hi and
+// lo terms of q and P make 240: 0.96 PFLOP/s executed.
 #include "ts_shared.h"
 
 #include "ts_decode_split.h"
@@ -421,13 +426,18 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
 }  // namespace
 
 // A chain needs no partials and no join, but its columns are one sequence's: taken for chunks that fill
-// blocks of 128 to 4/5 and the chip with blocks.
+// blocks of 128 to 3/4 and more than half of the chip with blocks.  32 heads over 8 of 128 dims, 4097 shared
+// keys, with and without: 8 x 256 tokens 254 and 308 us, 8 x 96 164 and 183, 4 x 130 165 and 175, 32 x 24
+// (3/4 filled) 160 and 184; below: 32 x 16 (half filled) 159 and 107, 8 x 64 (half of the chip) 163 and
+// 108, 2 x 256 170 and 110.
 static bool chains(int n_seq, int n_tok, int G, int n_kv, int n_cu) {
     const int64_t cols = (int64_t)n_tok * G, blk = (cols + kCols - 1) / kCols;
     return n_tok > 1 && 4 * cols >= 3 * blk * kCols && 2 * blk * n_seq * n_kv > n_cu;
 }
 
-// Pieces of own keys for a chunk that is no chain: until the jobs fill half the chip, of 256 keys at least.
+// Pieces of own keys for a chunk that is no chain: until the jobs fill the chip, of 256 keys at least.  4 x 3
+// tokens over 2000 own keys 27 us, in one piece 63; 8 x 16 over 1000 49 us, until half of the chip 51, in
+// one piece 69.
 static int own_pieces(int n_seq, int own_blk, int n_kv, int own_max, int n_cu) {
     const int64_t jobs = (int64_t)n_seq * own_blk * n_kv;
     return (int)std::max<int64_t>(1, std::min<int64_t>(n_cu / jobs, (own_max + 255) / 256));
@@ -446,7 +456,9 @@ SharedPlan shared_plan(int n_seq, int n_tok, int G, int n_kv, int prefix_len, in
         p.own_chunk = ((own_max + n - 1) / n + kWin - 1) / kWin * kWin;
         p.own_pieces = (own_max + p.own_chunk - 1) / p.own_chunk;
     }
-    // Pieces of the prefix: one job per CU, and a window at least for each of two groups.
+    // Pieces of the prefix: one job per CU, and a window at least in each.  (Two groups of waves in a workgroup,
+    // each with every second window, were slower from 1000 shared keys on: 8 x 16 tokens 48 us, 42 with one
+    // group and a piece per CU.)
     p.n_blk = (int)(((int64_t)n_seq * n_tok * G + kCols - 1) / kCols);
     const int64_t streams = (int64_t)p.n_blk * n_kv;
     const int64_t n = std::max<int64_t>(1, std::min<int64_t>(n_cu / streams, (prefix_len + kWin - 1) / kWin));
@@ -456,7 +468,8 @@ SharedPlan shared_plan(int n_seq, int n_tok, int G, int n_kv, int prefix_len, in
 }
 
 // One token: the own keys in splits of at least 512 (two rounds of a workgroup's windows), longer ones where
-// the batch has more than fill the chip.
+// the batch has more than fill the chip.  One sequence of 16000 17.2 us, with 1024 20.5; two of 4000 15.3 and
+// 16.2; 16 of 700 to 1500 30.2 and 27.6.  With 256: 32 of 60 to 500 31.2 us, 30.2 with 512, else the same.
 void shared_own_plan(const int32_t *n_ctx, int n_seq, int n_kv, int G, int n_cu, int *chunk, int *n_split) {
     constexpr int64_t kMinSplit = 512;
     int64_t total = 0;
@@ -568,7 +581,9 @@ hipError_t launch_shared(const SharedCall &c, hipStream_t st) {
     ja.own_chunk = c.own_chunk;
     ja.hlen = c.hlen;
     ja.cap = c.own.P;
-    // Many parts of few rows: all four waves of a workgroup on one row.
+    // Few rows: all four waves of a workgroup on one row's parts, where a wave to a row leaves CUs idle.  One
+    // token of 32 heads, with and without: 4 sequences 23.1 and 26.0 us, 32 30.5 and 31.5, 64 42.1 and 41.0, 128
+    // 66.4 and 63.1.
     const bool wide = ja.rows <= 4 * c.n_cu;
     const unsigned blocks = wide ? ja.rows : (ja.rows / ja.H + 3) / 4 * ja.H;
 #define TS_JOIN(HDV) \
