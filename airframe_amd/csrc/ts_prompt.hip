@@ -15,12 +15,12 @@
 //   per row that takes its largest element to [2^13, 2^14); products hi hi + hi lo + lo hi.
 // Scores, maxima, sums and outputs are f32 until the output is rounded once.
 //
-// Matrix work bounds it.  A prompt of 8192 tokens, 32 heads over 8 of 128 dims in f16: 550 GFLOP in 557 us,
-// 0.99 PFLOP/s (a product of 8192^3 reaches 1.15), the matrix cores busy for 53% of the CUs' time and no
+// Matrix work bounds it.  A prompt of 8192 tokens, 32 heads over 8 of 128 dims in f16: 550 GFLOP in 560 us,
+// 0.98 PFLOP/s (a product of 8192^3 reaches 1.15), the matrix cores busy for 53% of the CUs' time and no
 // bank conflicts.  16 ragged prompts of 300 to 2048 in bf16, 150 GFLOP: 197 us; f32 (three products)
-// of 128 dims 550 us.  3 prompts of 501 to 2100, 16 heads over 8 of 256 dims in f32 with softcap: 288 us behind
+// of 128 dims 550 us.  3 prompts of 501 to 2100, 16 heads over 8 of 256 dims in f32 with softcap: 252 us behind
 // 18.6 of the split, one wave per SIMD (o alone takes 128 registers), ended by the longest walk of 66
-// tiles: 0.51 PFLOP/s of the three products' work.
+// tiles: 0.56 PFLOP/s of the three products' work.
 #include "ts_prompt.h"
 
 #include <type_traits>
@@ -48,7 +48,7 @@ struct PromptArgs {
     int64_t row0;
     int G, H, hd;
     float scale;  // 1 / sqrt(hd), times log2(e) without softcap
-    float softcap;
+    float softcap, inv_softcap;
     PackTable t;
 };
 
@@ -90,11 +90,25 @@ __device__ inline typename Vec8<T>::type v_operand(const unsigned char *p) {
 
 // softcap tanh(x / softcap) in the exp2 domain, as c - 2 c / (1 + e^(2 x / softcap)) from two transcendental
 // instructions: within 2^-22 softcap of it, which moves a probability by far less than its rounding to
-// 16 bits does.  (f32 rows take tanhf: with it 373 us of a batch that takes 200 without softcap, with
-// this 235.)
+// 16 bits does.  (With tanhf 373 us of a batch that takes 200 without softcap, with this 235.)
 __device__ inline float cap16(float x, float softcap) {
     const float c = softcap * kLog2e, e = __builtin_amdgcn_exp2f(x * (2.0f * kLog2e / softcap));
     return c - 2.0f * c * __builtin_amdgcn_rcpf(e + 1.0f);
+}
+
+// The same for f32 rows: tanh within 2^-23 of it, relative to it below 0.6 (an odd polynomial, fitted to within
+// 2^-27 there by least squares on Chebyshev nodes), absolute above; the two sides are selected, not
+// branched to.  16 ragged prompts with softcap: 64 dims 412 us, 505 with tanhf; 128 dims 650 and 701; 3 of 256
+// dims 270 and 301.
+__device__ inline float cap32(float x, float softcap, float inv_softcap) {
+    const float y = x * inv_softcap, z = y * y;
+    float p = __builtin_fmaf(z, -5.940939591181278e-03f, 2.0838361233472824e-02f);
+    p = __builtin_fmaf(z, p, -5.379759892821312e-02f);
+    p = __builtin_fmaf(z, p, 1.3332106173038483e-01f);
+    p = __builtin_fmaf(z, p, -3.3333304524421692e-01f);
+    const float near = __builtin_fmaf(y * z, p, y);
+    const float far = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * (2.0f * kLog2e)) + 1.0f), 1.0f);
+    return (fabsf(y) < 0.6f ? near : far) * (softcap * kLog2e);
 }
 
 // The largest exponent bits of packed 16-bit floats: m and those of v, and whether they are an infinity's or
@@ -347,7 +361,7 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
                 for (int r = 0; r < 4; r++) {
                     float x = sc[b][4 * q + r];
                     if constexpr (!RAW) x *= k4[r];
-                    if constexpr (SOFTCAP) x = NP == 2 ? tanhf(x / a.softcap) * (a.softcap * kLog2e) : cap16(x, a.softcap);
+                    if constexpr (SOFTCAP) x = NP == 2 ? cap32(x, a.softcap, a.inv_softcap) : cap16(x, a.softcap);
                     if constexpr (MASK)
                         if (base + 32 * b + 8 * q + 4 * hf + r > qpos) x = -INFINITY;
                     sc[b][4 * q + r] = x;
@@ -650,6 +664,7 @@ hipError_t launch_prompt(const PromptCall &c, hipStream_t st) {
     const bool cap = c.softcap > 0.0f;
     a.scale = (cap ? 1.0f : kLog2e) / sqrtf((float)c.hd);
     a.softcap = c.softcap;
+    a.inv_softcap = cap ? 1.0f / c.softcap : 0.0f;
     a.row0 = c.off[0];
     if (c.dtype == TS_DTYPE_F32) {
         const int64_t n = c.off[c.n_seq] - c.off[0], rows = n * c.n_kv;
