@@ -173,9 +173,11 @@ inline int append_items(int n) { return n > 0 ? (n + 30) / kBlk + 1 : 0; }
 // One workgroup writes the new positions of one 32-position block of one (sequence, kv head), as the
 // append kernels of equal-length rows do (store_block64 / 128 / 256: it owns the block's V words,
 // which interleave 8 positions).  Rows of any type are widened in registers.
-// The quantizer's own sums (in the CPU's order, one rounding each), not HBM, bound it: 15.3k tokens of 8
-// f32 heads of 128 dims (125 + 17 MB) 30.7 us, 4.6 TB/s; 28k tokens of 8 bf16 heads of 80 dims (72 + 30
-// MB) 53.9 us, 1.9 TB/s: the 48 padded dims cost the same work as the others.
+// VALU work bounds it (rotation, maxima, codes that are the CPU's to the bit, V words put together), not HBM:
+// 15.2k tokens of 8 f32 heads of 128 dims (125 + 17 MB) 28.5 us, 5.0 TB/s, in f16 (half the bytes) 28.1; 28k
+// tokens of 8 bf16 heads of 80 dims (72 + 30 MB) 45.6 us, 2.2 TB/s: the 48 padded dims cost the same work
+// as the others.  Eight waves per SIMD instead of six (64 registers) changed nothing for 16-bit rows, and
+// f32 rows spilled.
 template <class T, int HD>
 __global__ __launch_bounds__(256) void append_packed_kernel(KvLayerView L, PackTable t, const int32_t *__restrict__ d_len,
                                                             const T *__restrict__ k, int64_t k_stride,
@@ -220,11 +222,11 @@ __global__ __launch_bounds__(256) void append_packed_kernel(KvLayerView L, PackT
         }
     }
     if constexpr (HD == 64)
-        store_block64(L, s, h, blk, lo, hi, kx[0], vx[0], cs[0], rope_pairs, wave, lane);
+        store_block64<sizeof(T) == 2>(L, s, h, blk, lo, hi, kx[0], vx[0], cs[0], rope_pairs, wave, lane);
     else if constexpr (HD == 128)
-        store_block128(L, s, h, blk, lo, hi, kx, vx, cs, rope_pairs, wave, lane);
+        store_block128<sizeof(T) == 2>(L, s, h, blk, lo, hi, kx, vx, cs, rope_pairs, wave, lane);
     else
-        store_block256(L, s, h, blk, lo, hi, kx, vx, cs, rope_pairs, wave, lane);
+        store_block256<sizeof(T) == 2>(L, s, h, blk, lo, hi, kx, vx, cs, rope_pairs, wave, lane);
 }
 
 // ---- and back ---------------------------------------------------------------------------------------

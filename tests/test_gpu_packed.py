@@ -326,3 +326,28 @@ def test_packed_streams(gpu):
     other.append_packed(0, k, v, off, rope)
     for x, y in zip(got, other.read_packed(0, off)):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("hd", [64, 80, 128, 256])
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+def test_append_packed_quotients_on_half_integers(gpu, name, hd):
+    """16-bit rows whose elements over the scale are half-integers, and neighbours of those, at every size, with
+    NaN, infinite, zero and subnormal rows: the codes of the same rows in f32 (which divide)."""
+    dt, n, n_kv = DTYPES[name], 160, 3
+    g = np.random.default_rng(hd)
+    m = g.integers(1, 37 if name == "bf16" else 293, (n, n_kv, 1)).astype(np.float64)
+    e = g.integers(*((-120, 110) if name == "bf16" else (-10, 3)), (n, n_kv, 1))
+    x = m * (2 * g.integers(0, 7, (n, n_kv, hd)) + 1) / 2 * g.choice([-1.0, 1.0], (n, n_kv, hd))
+    x[..., 0] = 7 * m[..., 0]
+    step = torch.from_numpy(x * 2.0 ** e).to(dt).view(torch.int16)
+    step += torch.from_numpy(g.choice([0, 0, 0, 1, -1], (n, n_kv, hd))).to(torch.int16)  # neighbours in the type
+    v = step.view(dt)
+    v[3, 0, 5:9], v[4, 1], v[5, 2, 7], v[6, 0, 2] = float("nan"), 0.0, float("inf"), float("-inf")
+    v[7] = 1e-38 if name == "bf16" else 6e-8
+    k = v.flip(0).contiguous()
+    caches = [KVCache.new_int4(1, n_kv, hd, 200) for _ in range(2)]
+    for c, (a, b) in zip(caches, ((k, v), (k.float(), v.float()))):
+        c.append_packed(0, a.cuda(), b.cuda(), [0, n], None)
+        c.increment(n)
+    for a, b in zip(*(c.export(0, 0, 0, n) for c in caches)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
