@@ -52,6 +52,7 @@ class RopeTable:
         check("ts_rope_create_yarn", L.ts_rope_create_yarn(n_pos, rope_dim, base, scale, yarn_alpha, yarn_beta,
                                                             ctypes.byref(h)))
         self._h = h
+        self.device = torch.device("cuda", torch.cuda.current_device())
         self.n_pos, self.rope_dim, self.base, self.scale = n_pos, rope_dim, base, scale
 
     @classmethod
@@ -65,6 +66,7 @@ class RopeTable:
                                                                     mult, ctypes.byref(h)))
         t = cls.__new__(cls)
         t._h = h
+        t.device = torch.device("cuda", torch.cuda.current_device())
         t.n_pos, t.rope_dim, t.base, t.scale = n_pos, rope_dim, base, 1.0 / factor
         return t
 
@@ -248,7 +250,7 @@ class KVCache:
         pk, sk = _rows(k, self.n_head_kv, self.head_dim, None, "k")
         pv, sv = _rows(v, self.n_head_kv, self.head_dim, k.dtype, "v")
         off, keep = _offsets(tok_off, self.n_seq, min(k.shape[0], v.shape[0]))[:2]
-        self._check_device(k, v)
+        self._check_device(k, v, rope)
         code = _dtype(k.dtype, "k")
         _launch(self.device, stream, lambda raw: check("ts_append_packed", load().ts_append_packed(
             self._h, layer, code, pk, sk, pv, sv, off, rope.handle if rope else None, raw)))
@@ -327,7 +329,7 @@ class KVCache:
         if k is not None:
             self._check_kv(k, v, 1)
             pk, pv = _ptr(k, torch.float32, "k"), _ptr(v, torch.float32, "v")
-        self._check_device(q, k, v, out, workspace)
+        self._check_device(q, k, v, out, workspace, rope)
 
         def call(raw):
             o = self._out_like(q, out)
@@ -344,7 +346,7 @@ class KVCache:
     def _check_device(self, *tensors):
         for t in tensors:
             if t is not None and t.device != self.device:
-                raise ValueError(f"tensor on {t.device}, cache on {self.device}")
+                raise ValueError(f"{'rope table' if isinstance(t, RopeTable) else 'tensor'} on {t.device}, cache on {self.device}")
 
     def workspace(self, n_head: int) -> torch.Tensor:
         if n_head not in self._ws:

@@ -68,7 +68,7 @@ def _same_device(first: torch.Tensor, *others):
     device = first.device
     for t in others:
         if t is not None and t.device != device:
-            raise ValueError(f"tensors on {device} and {t.device}")
+            raise ValueError(f"arguments on {device} and {t.device}")
 
 
 @contextlib.contextmanager
@@ -110,7 +110,7 @@ def rope_apply(x: torch.Tensor, positions: torch.Tensor, rope, layout: str = "in
     n, heads, hd = x.shape
     if positions.dtype != torch.int32 or positions.shape != (n,) or (n > 1 and positions.stride()[0] != 1):
         raise ValueError("positions must be [rows] int32, contiguous")
-    _same_device(x, positions, out)
+    _same_device(x, positions, out, rope)
     if out is not None:
         po, so = _rows(out, heads, hd, x.dtype, "out")
         if out.shape[0] != n:

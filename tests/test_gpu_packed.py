@@ -351,3 +351,16 @@ def test_append_packed_quotients_on_half_integers(gpu, name, hd):
         c.increment(n)
     for a, b in zip(*(c.export(0, 0, 0, n) for c in caches)):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_rope_table_of_another_device(gpu):
+    """A table lives on one device: calls with tensors or a cache of another refuse it."""
+    x, pos = torch.zeros(2, 2, 64).cuda(), torch.zeros(2, dtype=torch.int32).cuda()
+    rope, kv = RopeTable(16, 64, 1e4), KVCache.new_int4(1, 2, 64, 64)
+    assert rope.device == x.device == RopeTable.scaled(16, 64, 1e4).device
+    rope.device = torch.device("cuda", 1)
+    q = torch.zeros(1, 1, 2, 64).cuda()
+    for bad in (lambda: rope_apply(x, pos, rope), lambda: kv.append_packed(0, x, x, [0, 2], rope),
+                lambda: kv.attn_shared(0, q, rope, KVCache.new_int4(1, 2, 64, 64))):
+        with pytest.raises(ValueError):
+            bad()
