@@ -218,10 +218,12 @@ int ts_attn_shared(ts_kv *kv, const ts_kv *prefix, int32_t prefix_seq, int32_t l
         return TS_ERR_INVALID;
     if (n_tok == 0) return TS_OK;
     if (!d_q || !d_out || !aligned16(d_q) || !aligned16(d_out)) return TS_ERR_INVALID;
-    // the own positions continue the prefix's: slot p of a sequence is position window base + p
+    // the own positions continue the prefix's: slot p of a sequence is position window base + p (of all its
+    // slots: no sinks), and the prefix ends at its length plus its own window base
     const int P = prefix->h_len[prefix_seq];
+    const int64_t end = P > 0 ? (int64_t)P + prefix->h_rot[prefix_seq] : 0;
     for (int s = 0; s < kv->d.n_seq; s++) {
-        if (kv->h_rot[s] < P) return TS_ERR_INVALID;
+        if (kv->h_rot[s] < end || (P > 0 && kv->h_sink[s] != 0)) return TS_ERR_INVALID;
         if ((int64_t)kv->h_len[s] + n_tok > kv->d.max_seq) return TS_ERR_OVERFLOW;
     }
     const int rc = check_rope(rope, kv->d.head_dim, rot_end(kv, n_tok));

@@ -299,8 +299,11 @@ class KVCache:
 
     def share_prefix(self, prefix: "KVCache", prefix_seq: int = 0, stream=None):
         """Makes every (empty) sequence continue sequence prefix_seq of `prefix`: its slot p is
-        position P + p from then on (advance_window_base).  attn_shared then attends over both."""
+        position P + p from then on (advance_window_base), P the prefix's length and window base.
+        attn_shared then attends over both."""
         n = prefix.get_seq_len(prefix_seq)
+        if n:
+            n += prefix.get_window_base(prefix_seq)
         if any(self.seq_lens()) or any(self.get_window_base(s) for s in range(self.n_seq)):
             raise ValueError("share_prefix needs empty sequences (reset)")
         for s in range(self.n_seq):

@@ -471,8 +471,9 @@ int ts_attn_prompt(int32_t dtype, const void *d_q, int64_t q_stride, const void 
  *
  * A long system prompt or document that every sequence of a batch starts with is cached once, as
  * one sequence of a cache of its own (ts_append_quant, ts_append_packed, ts_kv_increment).  The batch's
- * cache holds only what follows: slot p of a sequence is position P + p, P the prefix's length, which
- * ts_kv_advance_window_base(kv, s, P) on an empty sequence sets up; every entry point that appends
+ * cache holds only what follows: slot p of a sequence is position P + p, P the prefix's length (and its
+ * window base, of one that was compacted), which ts_kv_advance_window_base(kv, s, P) on an empty sequence
+ * sets up; every entry point that appends
  * then rotates K there.  (A window compacted later keeps working with keep_sink 0: the prefix stays,
  * the own keys move.) */
 
@@ -485,7 +486,8 @@ int ts_attn_shared_workspace(const ts_kv *kv, const ts_kv *prefix, int32_t n_hea
  * the batch.  d_q, d_out: [n_seq][n_tok][n_head][head_dim]; q is normalized (kv's QK norm) and
  * rotated at its position like there.  With n_tok 1, d_k and d_v: NULL, or the new token's K and V
  * [n_seq][n_head_kv][head_dim], appended in the same launch (ts_attn_decode_append).  Both caches have
- * the same heads, head_dim and device; every window base has to be P or more (TS_ERR_INVALID).  The
+ * the same heads, head_dim and device; every window base has to be P or more, without
+ * sinks (TS_ERR_INVALID).  The
  * prefix's length is taken at the call, also into a graph; the rope table of a captured call has to
  * cover the positions its replays reach.  Runs on the caches' device.  d_workspace: ts_attn_shared_workspace
  * bytes, 16-byte aligned. */

@@ -291,9 +291,11 @@ public:
     void share_prefix(const KVCache &prefix, int32_t prefix_seq = 0, void *stream = nullptr) {
         int32_t n = 0;
         check(ts_kv_seq_len(prefix.h_, prefix_seq, &n), "KVCache::share_prefix");
+        if (n > 0) n += prefix.get_window_base(prefix_seq);
         for (int32_t s = 0; s < d_.n_seq; s++)
-            check(get_seq_len(s) == 0 && get_window_base(s) == 0 ? ts_kv_advance_window_base(h_, s, n, stream) : TS_ERR_INVALID,
-                  "KVCache::share_prefix");
+            check(get_seq_len(s) == 0 && get_window_base(s) == 0 ? TS_OK : TS_ERR_INVALID, "KVCache::share_prefix");
+        for (int32_t s = 0; s < d_.n_seq; s++)
+            check(ts_kv_advance_window_base(h_, s, n, stream), "KVCache::share_prefix");
     }
     uint64_t shared_workspace_bytes(const KVCache &prefix, int32_t n_head, int32_t n_tok = 1) const {
         uint64_t b = 0;

@@ -298,3 +298,37 @@ def test_shared_columns_of_other_scales(gpu, n_tok, heads, n_kv, hd):
     got = b.kv.attn_shared(1, b.q.cuda(), b.rope, b.pre)
     assert got[1, :, 0].isnan().all() and got[2].isnan().all() and got[0].isfinite().all()
     near(got[3:], b.want()[3:], b)
+
+
+def test_shared_compacted_prefix(gpu):
+    """A prefix whose own window was compacted ends at its length plus its window base, and the batch goes on
+    from there: against one cache that went through the same."""
+    rope = RopeTable(400, 64, BASE)
+    pk, pv = rand((90, 2, 64), 1).cuda(), rand((90, 2, 64), 2).cuda()
+    nk, nv, q = (rand((1, 5, h, 64), i).cuda() for h, i in ((2, 3), (2, 4), (4, 5)))
+    pre, kv, whole = KVCache.new_int4(1, 2, 64, 96), KVCache.new_int4(1, 2, 64, 64), KVCache.new_int4(1, 2, 64, 160)
+    for c in (pre, whole):
+        c.append_packed(0, pk, pv, [0, 90], rope)
+        c.increment(90)
+        c.compact(4, 20)
+    kv.advance_window_base(70)  # (its length alone)
+    with pytest.raises(TsError) as e:
+        kv.attn_shared(0, q, rope, pre)
+    assert e.value.code == -1
+    kv.reset()
+    kv.share_prefix(pre)
+    assert kv.get_window_base() == 90
+    for c in (kv, whole):
+        c.append_quant(0, nk, nv, rope)
+    got, want = kv.attn_shared(0, q, rope, pre), whole.attn_prefill(0, q, rope)
+    # both within near()'s bound of the same 64-bit result
+    assert (got - want).abs().max() <= 2 * 4.5 * (2 * 40 * (2.0 ** -20) + 2.0 ** -19)
+    # own sinks would stand at positions of the prefix
+    kv.reset()
+    kv.append_quant(0, nk, nv, rope)
+    kv.increment(5)
+    kv.compact(1, 2)
+    kv.advance_window_base(200)
+    with pytest.raises(TsError) as e:
+        kv.attn_shared(0, q, rope, pre)
+    assert e.value.code == -1
