@@ -18,6 +18,18 @@ static bool rows_ok(const void *p, int64_t stride, int64_t row, int32_t dtype) {
            stride * dtype_size(dtype) % 16 == 0;
 }
 
+// Whether rows first .. last - 1 of `row` bytes at two addresses, a_stride and b_stride bytes apart, share memory (rows
+// that interleave at one stride do not; of different strides, where the ranges do).
+static bool rows_overlap(const void *a, int64_t a_stride, const void *b, int64_t b_stride, int64_t row, int64_t first,
+                         int64_t last) {
+    const int64_t a0 = (int64_t)(uintptr_t)a + first * a_stride, b0 = (int64_t)(uintptr_t)b + first * b_stride;
+    const int64_t n = last - first - 1;
+    if (a0 + n * a_stride + row <= b0 || b0 + n * b_stride + row <= a0) return false;
+    if (a_stride != b_stride) return true;
+    const int64_t d = (a0 > b0 ? a0 - b0 : b0 - a0) % a_stride;
+    return d < row || d > a_stride - row;
+}
+
 // The largest length of a sequence after its rows of a packed batch, and its last rotation position.
 static void packed_ends(const ts_kv *kv, const int32_t *off, int64_t &len_end, int64_t &rot_last) {
     len_end = rot_last = 0;
@@ -107,6 +119,9 @@ int ts_read_packed(const ts_kv *kv, int32_t layer, const int32_t *pos0, const in
     if (row_off[kv->d.n_seq] == row_off[0]) return TS_OK;
     const int64_t row = (int64_t)kv->d.n_head_kv * kv->d.head_dim;
     if (!rows_ok(d_k, k_stride, row, dtype) || !rows_ok(d_v, v_stride, row, dtype)) return TS_ERR_INVALID;
+    const int size = dtype_size(dtype);
+    if (rows_overlap(d_k, k_stride * size, d_v, v_stride * size, row * size, row_off[0], row_off[kv->d.n_seq]))
+        return TS_ERR_INVALID;
     for (int s = 0; s < kv->d.n_seq; s++) {
         const int64_t p = pos0 ? pos0[s] : 0, n = (int64_t)row_off[s + 1] - row_off[s];
         if (n > 0 && (p < 0 || p + n > kv->d.max_seq)) return TS_ERR_INVALID;

@@ -442,7 +442,8 @@ int ts_append_packed(ts_kv *kv, int32_t layer, int32_t dtype, const void *d_k, i
 
 /* The cache read back into packed rows: positions pos0[s] .. of sequence s (host array; NULL: from
  * 0) into rows row_off[s] .. row_off[s + 1] - 1 of K and V, each value (code - 8) * scale rounded to
- * f32 and then to dtype; K as stored, rotated.  A position at or past max_seq is TS_ERR_INVALID;
+ * f32 and then to dtype; K as stored, rotated.  The rows of K and of V may interleave and share no memory
+ * (TS_ERR_INVALID).  A position at or past max_seq is TS_ERR_INVALID;
  * one that nothing was written to reads as whatever the cache holds there (zeros at first). */
 int ts_read_packed(const ts_kv *kv, int32_t layer, const int32_t *pos0, const int32_t *row_off, int32_t dtype,
                    void *d_k, int64_t k_stride, void *d_v, int64_t v_stride, void *stream);

@@ -364,3 +364,24 @@ def test_rope_table_of_another_device(gpu):
                 lambda: kv.attn_shared(0, q, rope, KVCache.new_int4(1, 2, 64, 64))):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_read_packed_rows_apart(gpu):
+    """K and V into the same rows, or into rows that run into each other, is refused; interleaved they are fine."""
+    kv = KVCache.new_int4(1, 2, 64, 64)
+    k, v = rand((9, 2, 64), 1).cuda(), rand((9, 2, 64), 2).cuda()
+    kv.append_packed(0, k, v, [0, 9], None)
+    kv.increment(9)
+    want = kv.read_packed(0, [0, 9])
+    wide = torch.zeros(12, 5, 64, device="cuda")
+    flat = wide.view(30, 2, 64)
+    for a, b in ((wide[:9, :2], wide[:9, :2]), (wide[:9, :2], wide[:9, 1:3]), (wide[:9, :2], wide[1:10, 1:3]),
+                 (flat[:9], flat[8:17])):
+        with pytest.raises(TsError) as e:
+            kv.read_packed(0, [0, 9], out=(a, b))
+        assert e.value.code == -1
+    kv.read_packed(0, [0, 9], out=(wide[:9, :2], wide[:9, 2:4]))
+    assert torch.equal(wide[:9, :2], want[0]) and torch.equal(wide[:9, 2:4], want[1]) and (wide[:, 4] == 0).all()
+    wide.zero_()
+    kv.read_packed(0, [0, 9], out=(wide[:9, 3:], wide[1:10, :2]))  # (V a row further on)
+    assert torch.equal(wide[:9, 3:], want[0]) and torch.equal(wide[1:10, :2], want[1]) and (wide[:, 2] == 0).all()
