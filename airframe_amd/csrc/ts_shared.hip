@@ -12,8 +12,8 @@
 //
 // 32 heads over 8 of 128 dims, 32 sequences of 60 to 500 own keys behind 8192: 28.9 us (shared_kernel 23.3,
 // a CU's four windows with the q before and the partials behind them; join 6), of which the bytes would take
-// 3.4 and the matrix work 4.  Chunks of 256 tokens of 8 sequences behind 4097: 251 us, 142 GFLOP that hi and
-// lo terms of q and P make 240: 0.96 PFLOP/s executed.
+// 3.4 and the matrix work 4.  Chunks of 256 tokens of 8 sequences behind 4097: 254 us, 142 GFLOP that hi and
+// lo terms of q and P make 240: 0.95 PFLOP/s executed.
 #include "ts_shared.h"
 
 #include "ts_decode_split.h"
