@@ -23,6 +23,7 @@
 // tiles: 0.56 PFLOP/s of the three products' work.
 #include "ts_prompt.h"
 
+#include <cfloat>
 #include <type_traits>
 
 #include "ts_mfma.h"
@@ -48,7 +49,7 @@ struct PromptArgs {
     int64_t row0;
     int G, H, hd;
     float scale;  // 1 / sqrt(hd), times log2(e) without softcap
-    float softcap, inv_softcap;
+    float softcap, inv_softcap;  // (inv_softcap: cap_quick's to_exp where that is taken)
     PackTable t;
 };
 
@@ -88,27 +89,38 @@ __device__ inline typename Vec8<T>::type v_operand(const unsigned char *p) {
     return __builtin_bit_cast(typename Vec8<T>::type, s);
 }
 
-// softcap tanh(x / softcap) in the exp2 domain, as c - 2 c / (1 + e^(2 x / softcap)) from two transcendental
-// instructions: within 2^-22 softcap of it, which moves a probability by far less than its rounding to
-// 16 bits does.  (With tanhf 373 us of a batch that takes 200 without softcap, with this 235.)
-__device__ inline float cap16(float x, float softcap) {
-    const float c = softcap * kLog2e, e = __builtin_amdgcn_exp2f(x * (2.0f * kLog2e / softcap));
-    return c - 2.0f * c * __builtin_amdgcn_rcpf(e + 1.0f);
+// softcap tanh(x / softcap) in the exp2 domain, within 2^-20 of it relative to it for any softcap: with y = x /
+// softcap, x (1 + y^2 P(y^2)) near zero, P fitted to (tanh(y) / y - 1) / y^2 by least squares on Chebyshev nodes, and
+// softcap (1 - 2 / (1 + e^(2 y))) beyond, whose error is 2^-22 of softcap and not of x; the two are
+// selected, not branched to.  f32 rows: P of five terms below 0.6 (2^-27), 16-bit rows, whose weights are rounded to
+// 2^-12 and 2^-9, of three below 0.35 (2^-24).
+template <bool F32>
+__device__ inline float cap(float x, float softcap, float inv_softcap) {
+    const float y = x * inv_softcap, z = y * y, xl = x * kLog2e;
+    float p;
+    if constexpr (F32) {
+        p = __builtin_fmaf(z, -5.8939453e-03f, 2.0794618e-02f);
+        p = __builtin_fmaf(z, p, -5.3783293e-02f);
+        p = __builtin_fmaf(z, p, 1.3331915e-01f);
+        p = __builtin_fmaf(z, p, -3.33332975e-01f);
+    } else {
+        p = __builtin_fmaf(z, -4.9134325e-02f, 1.3299560e-01f);
+        p = __builtin_fmaf(z, p, -3.33326515e-01f);
+    }
+    const float near = __builtin_fmaf(xl * z, p, xl);
+    const float rest = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * (2.0f * kLog2e)) + 1.0f);
+    const float far = softcap * __builtin_fmaf(-2.0f * kLog2e, rest, kLog2e);
+    return fabsf(y) < (F32 ? 0.6f : 0.35f) ? near : far;
 }
 
-// The same for f32 rows: tanh within 2^-23 of it, relative to it below 0.6 (an odd polynomial, fitted to within
-// 2^-27 there by least squares on Chebyshev nodes), absolute above; the two sides are selected, not
-// branched to.  16 ragged prompts with softcap: 64 dims 412 us, 505 with tanhf; 128 dims 650 and 701; 3 of 256
-// dims 270 and 301.
-__device__ inline float cap32(float x, float softcap, float inv_softcap) {
-    const float y = x * inv_softcap, z = y * y;
-    float p = __builtin_fmaf(z, -5.940939591181278e-03f, 2.0838361233472824e-02f);
-    p = __builtin_fmaf(z, p, -5.379759892821312e-02f);
-    p = __builtin_fmaf(z, p, 1.3332106173038483e-01f);
-    p = __builtin_fmaf(z, p, -3.3333304524421692e-01f);
-    const float near = __builtin_fmaf(y * z, p, y);
-    const float far = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * (2.0f * kLog2e)) + 1.0f), 1.0f);
-    return (fabsf(y) < 0.6f ? near : far) * (softcap * kLog2e);
+// The same of small softcaps for 16-bit rows, as c - 2 c / (1 + e^(2 y)) from two transcendental instructions: within
+// 2^-21 of softcap and not of x, so up to softcaps of kQuickCap within 2^-15, where f16 weights are rounded by 2^-12.
+// to_exp: 2 log2(e) / softcap.  16 ragged prompts, softcap 50, with this and with cap(): bf16 of 128 dims 242 and 293 us,
+// f16 of 64 dims 161 and 226 (without softcap 205 and 111).
+constexpr float kQuickCap = 64.0f;
+__device__ inline float cap_quick(float x, float softcap, float to_exp) {
+    const float c = softcap * kLog2e;
+    return c - 2.0f * c * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * to_exp) + 1.0f);
 }
 
 // The largest exponent bits of packed 16-bit floats: m and those of v, and whether they are an infinity's or
@@ -155,8 +167,9 @@ __device__ inline u32x4 buffer_of(const void *p, int64_t bytes) {
 }
 
 // T: the matrix cores' type; O: the rows' type (float with two planes); HD: head dims, padded; NP:
-// planes; KT: keys per tile.
-template <class T, class O, int HD, int NP, int KT, bool SOFTCAP>
+// planes; KT: keys per tile; CAP: no softcap, cap_quick or cap.
+enum { kNoCap = 0, kCapQuick = 1, kCap = 2 };
+template <class T, class O, int HD, int NP, int KT, int CAP>
 __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kernel(PromptArgs a) {
     using V8 = typename Vec8<T>::type;
     constexpr int CPR = NP * HD / 8;  // 16-byte chunks of a tile's row
@@ -164,7 +177,7 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
     constexpr int NKS = HD / 16, NDB = HD / 32, NKB = KT / 32;
     constexpr int NW = kPromptNW, NLD = TILEB / 1024 / NW;  // loads of 1 KB of a tile per wave
     constexpr bool F16 = __is_same(T, _Float16);
-    constexpr bool RAW = NP == 1 && !SOFTCAP;  // scores stay unscaled until the exponent's FMA
+    constexpr bool RAW = NP == 1 && CAP == kNoCap;  // scores stay unscaled until the exponent's FMA
     static_assert(TILEB % (1024 * NW) == 0, "a tile's loads spread evenly");
     // [2 buffers] K tile, V tile; then, of two planes, [2][2][KT] K scales and V exponents
     extern __shared__ __align__(1024) unsigned char pr_smem[];
@@ -361,7 +374,8 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
                 for (int r = 0; r < 4; r++) {
                     float x = sc[b][4 * q + r];
                     if constexpr (!RAW) x *= k4[r];
-                    if constexpr (SOFTCAP) x = NP == 2 ? cap32(x, a.softcap, a.inv_softcap) : cap16(x, a.softcap);
+                    if constexpr (CAP == kCapQuick) x = cap_quick(x, a.softcap, a.inv_softcap);
+                    if constexpr (CAP == kCap) x = cap<NP == 2>(x, a.softcap, a.inv_softcap);
                     if constexpr (MASK)
                         if (base + 32 * b + 8 * q + 4 * hf + r > qpos) x = -INFINITY;
                     sc[b][4 * q + r] = x;
@@ -594,32 +608,37 @@ __global__ __launch_bounds__(256) void prompt_split_kernel(const float *__restri
     }
 }
 
-template <class T, class O, int HD, int NP, int KT, bool SC>
+template <class T, class O, int HD, int NP, int KT, int CAP>
 void prompt_launch(const PromptArgs &a, unsigned blocks, hipStream_t st) {
     constexpr size_t lds = (size_t)4 * KT * NP * HD * 2 + (NP == 2 ? 4 * KT * sizeof(float) : 0);
     static_assert(lds <= 160 * 1024, "the tiles fit a CU's LDS");
     if (lds > 64 * 1024)
-        (void)hipFuncSetAttribute((const void *)prompt_kernel<T, O, HD, NP, KT, SC>,
+        (void)hipFuncSetAttribute((const void *)prompt_kernel<T, O, HD, NP, KT, CAP>,
                                   hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    prompt_kernel<T, O, HD, NP, KT, SC><<<blocks, 64 * kPromptNW, lds, st>>>(a);
+    prompt_kernel<T, O, HD, NP, KT, CAP><<<blocks, 64 * kPromptNW, lds, st>>>(a);
 }
 
 // Keys per tile: 64 of one plane and 32 of two up to 128 dims, 32 of 256 dims.  16 ragged prompts of 300 to
 // 2048, 32 heads over 8: bf16 of 128 dims 198 us with 64 and 222 with 32, of 64 dims 114 and 137; f32 of 64
 // dims 351 with 64 and 319 with 32 (one prompt of 500: 30 and 33; of 8192: 951 and 925); bf16 of 256 dims
 // 251 with 64 and 253 with 32, which leaves room for a second workgroup's tiles.
+template <class T, class O, int NP, int CAP>
+void prompt_dims(const PromptArgs &a, unsigned blocks, hipStream_t st) {
+    if (a.hd <= 64)
+        prompt_launch<T, O, 64, NP, 64 / NP, CAP>(a, blocks, st);
+    else if (a.hd <= 128)
+        prompt_launch<T, O, 128, NP, 64 / NP, CAP>(a, blocks, st);
+    else
+        prompt_launch<T, O, 256, NP, 32, CAP>(a, blocks, st);
+}
 template <class T, class O, int NP>
-void prompt_dims(const PromptArgs &a, bool cap, unsigned blocks, hipStream_t st) {
-    if (a.hd <= 64) {
-        if (cap) prompt_launch<T, O, 64, NP, 64 / NP, true>(a, blocks, st);
-        else prompt_launch<T, O, 64, NP, 64 / NP, false>(a, blocks, st);
-    } else if (a.hd <= 128) {
-        if (cap) prompt_launch<T, O, 128, NP, 64 / NP, true>(a, blocks, st);
-        else prompt_launch<T, O, 128, NP, 64 / NP, false>(a, blocks, st);
-    } else {
-        if (cap) prompt_launch<T, O, 256, NP, 32, true>(a, blocks, st);
-        else prompt_launch<T, O, 256, NP, 32, false>(a, blocks, st);
-    }
+void prompt_cap(const PromptArgs &a, int cap, unsigned blocks, hipStream_t st) {
+    if (cap == kNoCap)
+        prompt_dims<T, O, NP, kNoCap>(a, blocks, st);
+    else if (NP == 2 || cap == kCap)
+        prompt_dims<T, O, NP, kCap>(a, blocks, st);
+    else if constexpr (NP == 1)
+        prompt_dims<T, O, NP, kCapQuick>(a, blocks, st);
 }
 
 // Sequences seq0 .. of the batch with the longest first, so that the launch ends with short walks (tok:
@@ -661,10 +680,11 @@ hipError_t launch_prompt(const PromptCall &c, hipStream_t st) {
     a.G = c.n_head / c.n_kv;
     a.H = c.n_kv;
     a.hd = c.hd;
-    const bool cap = c.softcap > 0.0f;
-    a.scale = (cap ? 1.0f : kLog2e) / sqrtf((float)c.hd);
+    const int cap = c.softcap == 0.0f ? kNoCap : c.dtype != TS_DTYPE_F32 && c.softcap <= kQuickCap ? kCapQuick : kCap;
+    a.scale = (cap != kNoCap ? 1.0f : kLog2e) / sqrtf((float)c.hd);
     a.softcap = c.softcap;
-    a.inv_softcap = cap ? 1.0f / c.softcap : 0.0f;
+    // (finite, so that 0 times it stays 0)
+    a.inv_softcap = cap != kNoCap ? std::min((cap == kCapQuick ? 2.0f * kLog2e : 1.0f) / c.softcap, FLT_MAX) : 0.0f;
     a.row0 = c.off[0];
     if (c.dtype == TS_DTYPE_F32) {
         const int64_t n = c.off[c.n_seq] - c.off[0], rows = n * c.n_kv;
@@ -691,11 +711,11 @@ hipError_t launch_prompt(const PromptCall &c, hipStream_t st) {
         const int64_t blocks = (int64_t)a.t.item[a.t.n] * c.n_kv;
         if (blocks == 0) continue;
         if (c.dtype == TS_DTYPE_F32)
-            prompt_dims<_Float16, float, 2>(a, cap, (unsigned)blocks, st);
+            prompt_cap<_Float16, float, 2>(a, cap, (unsigned)blocks, st);
         else if (c.dtype == TS_DTYPE_F16)
-            prompt_dims<_Float16, _Float16, 1>(a, cap, (unsigned)blocks, st);
+            prompt_cap<_Float16, _Float16, 1>(a, cap, (unsigned)blocks, st);
         else
-            prompt_dims<__bf16, __bf16, 1>(a, cap, (unsigned)blocks, st);
+            prompt_cap<__bf16, __bf16, 1>(a, cap, (unsigned)blocks, st);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }

@@ -60,3 +60,24 @@ def attend(q, k, v, hidden, softcap=0.0):
     if softcap > 0:
         x = softcap * torch.tanh(x / softcap)
     return torch.softmax(x.masked_fill(hidden, -math.inf), -1) @ v
+
+
+def attend_bound(q, k, v, hidden, softcap=0.0):
+    """attend()'s output and two lengths per element of it, in 64 bits: sqrt(sum p^2 (v - o)^2), what
+    independent errors of 1 in the scores move it by, and sqrt(sum p^2 v^2), what independent relative errors
+    of 1 in the rounded weights do (their sum is taken before they are rounded)."""
+    q, k, v = q.double(), k.double(), v.double()
+    x = q @ k.T / math.sqrt(q.shape[-1])
+    if softcap > 0:
+        x = softcap * torch.tanh(x / softcap)
+    p = torch.softmax(x.masked_fill(hidden, -math.inf), -1)
+    o, p2 = p @ v, p * p
+    by_weight = p2 @ (v * v)
+    by_score = (by_weight - 2 * o * (p2 @ v) + o * o * p2.sum(-1, keepdim=True)).clamp(min=0)
+    return o, by_score.sqrt(), by_weight.sqrt()
+
+
+def norms(x):
+    """The largest element and the largest root mean square of rows."""
+    x = x.double()
+    return float(x.abs().max()), float(x.square().mean(-1).max().sqrt())
