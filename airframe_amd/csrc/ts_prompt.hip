@@ -311,8 +311,10 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
     floatx16 o[NDB];
 #pragma unroll
     for (int db = 0; db < NDB; db++) o[db] = (floatx16)0.0f;
-    float m_run = -3.4e38f, l_run = 0.0f;  // (below every finite score: the first tile sets it)
-    float m_sum = -3.4e38f;                // two planes: l_run's reference
+    // The softmax's reference: below every finite score, the first tile sets it.  Of two planes that of the scores,
+    // and l_run's; P, which carries the value rows' sizes too, has o_rel above it.
+    float m_run = -3.4e38f, l_run = 0.0f;
+    float o_rel = -3.4e38f;
     // P is held up to 2^(8 + kTop) (the maximum is raised lazily, by 2^8), which leaves f16 probabilities
     // 2^-30 of the largest before they are lost; bf16 has f32's range.
     constexpr float kTop = F16 ? 6.0f : 0.0f;
@@ -350,20 +352,16 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
             __builtin_amdgcn_sched_barrier(0);
         }
         // x: scores in the exp2 domain; without softcap and planes their scale waits for the exponent's FMA.
-        // Two planes: P carries 2^(x + ve), the probability times its value row's size, and has a maximum of
-        // its own beside the sum's; both references are whole numbers, so that ve (a whole number of any
-        // size) and the reference cancel before x is added, and x keeps its last bits.
         const float *ke = se + (w & 1) * 2 * KT, *ve = ke + KT;
-        float mloc = -INFINITY, msum = -INFINITY;
+        float mloc = -INFINITY;
         bool odd_rows = false;  // two planes: a value row of the tile is not finite (its K scale is negative)
 #pragma unroll
         for (int b = 0; b < NKB; b++)
 #pragma unroll
             for (int q = 0; q < 4; q++) {
-                floatx4 k4 = (floatx4)qscale, v4 = (floatx4)0.0f;
+                floatx4 k4 = (floatx4)qscale;
                 if constexpr (NP == 2) {
                     const floatx4 s4 = *reinterpret_cast<const floatx4 *>(ke + 32 * b + 8 * q + 4 * hf);
-                    v4 = *reinterpret_cast<const floatx4 *>(ve + 32 * b + 8 * q + 4 * hf);
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         odd_rows |= s4[r] < 0.0f;
@@ -373,35 +371,54 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     float x = sc[b][4 * q + r];
-                    if constexpr (!RAW) x *= k4[r];
+                    if constexpr (!RAW) x = opaque(x * k4[r]);  // (rounded in every tile: an FMA with the reference in some is not)
                     if constexpr (CAP == kCapQuick) x = cap_quick(x, a.softcap, a.inv_softcap);
                     if constexpr (CAP == kCap) x = cap<NP == 2>(x, a.softcap, a.inv_softcap);
                     if constexpr (MASK)
                         if (base + 32 * b + 8 * q + 4 * hf + r > qpos) x = -INFINITY;
                     sc[b][4 * q + r] = x;
-                    mloc = fmaxf(mloc, x + v4[r]);
-                    if constexpr (NP == 2) msum = fmaxf(msum, x);
+                    mloc = fmaxf(mloc, x);
                 }
             }
         mloc = both_max(mloc);
         if constexpr (RAW) mloc *= qscale;
-        if constexpr (NP == 2) {
-            mloc = ceilf(mloc);
-            msum = ceilf(both_max(msum));
-        }
-        if (__builtin_amdgcn_ballot_w64(mloc - m_run > 8.0f || (NP == 2 && msum - m_sum > 8.0f)) != 0) {
-            const float m_new = mloc - m_run > 8.0f ? mloc : m_run;
-            const float alpha = exp2f(m_run - m_new);
+        if constexpr (NP == 2) mloc = ceilf(mloc);
+        if (__builtin_amdgcn_ballot_w64(mloc - m_run > 8.0f) != 0) {
+            const float m_new = mloc - m_run > 8.0f ? mloc : m_run, d = m_run - m_new;
+            const float alpha = exp2f(d);
             m_run = m_new;
+            l_run *= alpha;
             if constexpr (NP == 2) {
-                const float s_new = msum - m_sum > 8.0f ? msum : m_sum;
-                l_run *= exp2f(m_sum - s_new);
-                m_sum = s_new;
+                o_rel += d;
             } else {
-                l_run *= alpha;
-            }
 #pragma unroll
-            for (int db = 0; db < NDB; db++) o[db] *= alpha;
+                for (int db = 0; db < NDB; db++) o[db] *= alpha;
+            }
+        }
+        // Two planes: P carries 2^(x + ve - o's reference), the probability times its value row's size, and has a maximum
+        // of its own.  The reference of the scores is taken from them first, so that what ve is added to is small where it
+        // counts, whatever their size; all references are whole numbers, as ve is, and moving them is exact.
+        if constexpr (NP == 2) {
+            float ploc = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < NKB; b++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const floatx4 v4 = *reinterpret_cast<const floatx4 *>(ve + 32 * b + 8 * q + 4 * hf);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        sc[b][4 * q + r] -= m_run;
+                        ploc = fmaxf(ploc, sc[b][4 * q + r] + v4[r]);
+                    }
+                }
+            ploc = ceilf(both_max(ploc));
+            if (__builtin_amdgcn_ballot_w64(ploc - o_rel > 8.0f) != 0) {
+                const float o_new = ploc - o_rel > 8.0f ? ploc : o_rel;
+                const float alpha = exp2f(o_rel - o_new);
+                o_rel = o_new;
+#pragma unroll
+                for (int db = 0; db < NDB; db++) o[db] *= alpha;
+            }
         }
         if constexpr (NP == 2)
             if (__builtin_amdgcn_ballot_w64(odd_rows) != 0) {
@@ -423,7 +440,7 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
                         }
                 }
             }
-        const float off = kTop - m_run;
+        const float off = kTop - (NP == 2 ? o_rel : m_run);
         // O^T += V^T P^T, 16 keys at a time: the exponentials of a step run beside the products of the one
         // before, and V's operands are read one group of products ahead.  (Two planes: one dim tile a group, or
         // 128 dims take more than the 256 registers that let two workgroups share a CU: 776 against 552 us for
@@ -452,7 +469,7 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
                     for (int r = 0; r < 4; r++) {
                         const float x = sc[st >> 1][8 * (st & 1) + 4 * q + r];
                         const float p = __builtin_amdgcn_exp2f(RAW ? __builtin_fmaf(x, qscale, off) : x + (v4[r] + off));
-                        l_run += NP == 2 ? __builtin_amdgcn_exp2f(x - m_sum) : p;
+                        l_run += NP == 2 ? __builtin_amdgcn_exp2f(x) : p;
                         const T hi = (T)p;
                         pb[4 * q + r] = hi;
                         if constexpr (NP == 2) pl[4 * q + r] = (T)(p - (float)hi);
@@ -529,7 +546,7 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
         }
         if constexpr (NP == 2) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = ldexpf(x[e], (int)(m_run - m_sum) - 13 - (int)kTop);
+            for (int e = 0; e < 8; e++) x[e] = ldexpf(x[e], (int)o_rel - 13 - (int)kTop);
         }
     };
     O *orow = static_cast<O *>(a.out) + (row0 + tok) * a.os + (int64_t)head * hd;

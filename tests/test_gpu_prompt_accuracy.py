@@ -73,3 +73,37 @@ def test_prompt_softcap_tiny(gpu, name, softcap):
     q, k, v = rand((70, 2, 64), 1, dt), rand((70, 1, 64), 2, dt), rand((70, 1, 64), 3, dt)
     q[5], k[9] = 0.0, 0.0
     close(q, k, v, [0, 70], softcap)
+
+
+def steps(n, hd, size, dt, seed):
+    """q and k whose scores are c_j size^2 sqrt(hd), c_j whole numbers from -3 to 3: apart by far more than 32 bits
+    round them by, or the same."""
+    g = torch.Generator().manual_seed(seed)
+    u = torch.randint(0, 2, (hd,), generator=g) * 2.0 - 1.0
+    c = torch.randint(-3, 4, (n,), generator=g).double()
+    c[:4] = torch.tensor([-3.0, -3.0, -1.0, 2.0])
+    q = (size * u).expand(n, 2, hd).to(dt).contiguous()
+    return q, (size * c[:, None, None] * u).to(dt).contiguous()
+
+
+def largest_take_all(name, size, hd, softcap):
+    """The largest scores take all the weight, in equal parts.  The weights' sum is in 32 bits, the weights of 16-bit rows
+    and the output are rounded once each; those that lose are below 2^-70 (e^-50, with softcap 50)."""
+    dt, n = DTYPES[name], 150
+    q, k = steps(n, hd, size, dt, 5)
+    v = rand((n, 1, hd), 3, dt)
+    got = attn_prompt(q.cuda(), k.cuda(), v.cuda(), [0, n], softcap=softcap).cpu().double()
+    hidden = torch.ones(n, n, dtype=torch.bool).triu(1)
+    eps = torch.finfo(dt).eps / 2
+    for h in range(2):
+        want = attend(q[:, h], k[:, 0], v[:, 0], hidden, softcap)
+        tol = eps * want.abs() + ((0.0 if dt == torch.float32 else eps) + 2.0 ** -20) * float(v.abs().max())
+        assert ((got[:, h] - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("softcap", [0.0, 50.0, 1e12])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("size", [2.0 ** 7, 2.0 ** 10, 2000.0, 2.0 ** 12, 20000.0, 2.0 ** 21, 2.0 ** 40, 2.0 ** 56])
+def test_prompt_large_scores_f32(gpu, size, hd, softcap):
+    """Scores of any finite size."""
+    largest_take_all("f32", size, hd, softcap)
