@@ -37,6 +37,7 @@ typedef short short8v __attribute__((ext_vector_type(8)));
 
 constexpr int kPromptNW = 4;
 constexpr int kPromptCols = 32 * kPromptNW;
+constexpr float kFar = 4194304.0f;   // scores above this: their reference is taken from them first
 constexpr float kZeroRow = -200.0f;  // f32: V's exponent of a row of zeros (below any other: out of P's range)
 
 struct PromptArgs {
@@ -440,7 +441,19 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
                         }
                 }
             }
-        const float off = kTop - (NP == 2 ? o_rel : m_run);
+        // One plane: a weight is 2^(pmul x + off).  Below 2^22 that is one FMA of the scores as they are.  Above, the FMA's
+        // exact product and the rounded reference would be up to half a step of the reference apart (1024 at 2^34),
+        // and off would lose kTop: the scores are rounded, and the reference taken from them first.
+        float pmul = qscale, off = kTop - (NP == 2 ? o_rel : m_run);
+        if constexpr (NP == 1)
+            if (__builtin_amdgcn_ballot_w64(m_run > kFar || (m_run < -kFar && m_run > -3.0e38f)) != 0) {
+#pragma unroll
+                for (int b = 0; b < NKB; b++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) sc[b][e] = opaque(RAW ? sc[b][e] * qscale : sc[b][e]) - m_run;
+                pmul = 1.0f;
+                off = kTop;
+            }
         // O^T += V^T P^T, 16 keys at a time: the exponentials of a step run beside the products of the one
         // before, and V's operands are read one group of products ahead.  (Two planes: one dim tile a group, or
         // 128 dims take more than the 256 registers that let two workgroups share a CU: 776 against 552 us for
@@ -468,7 +481,7 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         const float x = sc[st >> 1][8 * (st & 1) + 4 * q + r];
-                        const float p = __builtin_amdgcn_exp2f(RAW ? __builtin_fmaf(x, qscale, off) : x + (v4[r] + off));
+                        const float p = __builtin_amdgcn_exp2f(RAW ? __builtin_fmaf(x, pmul, off) : x + (v4[r] + off));
                         l_run += NP == 2 ? __builtin_amdgcn_exp2f(x) : p;
                         const T hi = (T)p;
                         pb[4 * q + r] = hi;

@@ -107,3 +107,12 @@ def largest_take_all(name, size, hd, softcap):
 def test_prompt_large_scores_f32(gpu, size, hd, softcap):
     """Scores of any finite size."""
     largest_take_all("f32", size, hd, softcap)
+
+
+@pytest.mark.parametrize("softcap", [0.0, 50.0, 1e12])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("name,size", [(t, s) for t, most in (("f16", 20000.0), ("bf16", 2.0 ** 56)) for s in
+                                       (2.0 ** 7, 2.0 ** 10, 2000.0, 2.0 ** 12, 20000.0, 2.0 ** 21, 2.0 ** 40, 2.0 ** 56) if s <= most])
+def test_prompt_large_scores(gpu, name, size, hd, softcap):
+    """Scores of any finite size, of 16-bit rows."""
+    largest_take_all(name, size, hd, softcap)
