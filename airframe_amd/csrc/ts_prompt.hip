@@ -354,8 +354,30 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
         }
         // x: scores in the exp2 domain; without softcap and planes their scale waits for the exponent's FMA.
         const float *ke = se + (w & 1) * 2 * KT, *ve = ke + KT;
+        // Two planes: K or V of a key in the tile are not finite (its K scale is negative).  The planes hold 0 for those
+        // elements: hi and lo terms of an infinity would meet as NaN.  What they bring is added apart, to the
+        // scores here and to the sums below.
+        bool odd_rows = false;
+        if constexpr (NP == 2) odd_rows = __builtin_amdgcn_ballot_w64(ke[lane % KT] < 0.0f) != 0;
+        if (odd_rows) {
+            const float *qr = static_cast<const float *>(a.q) + (row0 + tok) * a.qs + (int64_t)head * hd;
+#pragma unroll 1
+            for (int kk = 0; kk < KT; kk++) {
+                if (base + kk >= n || __builtin_amdgcn_readfirstlane(__float_as_int(ke[kk])) >= 0) continue;
+                const float *kr = static_cast<const float *>(a.k) + (int64_t)(row0 + base + kk) * a.ks + (int64_t)h * hd;
+                float extra = 0.0f;
+#pragma unroll 1
+                for (int d = 8 * hf; d < hd; d += 16)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) extra += !(fabsf(kr[d + e]) < INFINITY) ? qr[d + e] * kr[d + e] : 0.0f;
+                extra = both_sum(extra);
+#pragma unroll
+                for (int b = 0; b < NKB; b++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) sc[b][e] += 32 * b + 8 * (e >> 2) + 4 * hf + (e & 3) == kk ? extra : 0.0f;
+            }
+        }
         float mloc = -INFINITY;
-        bool odd_rows = false;  // two planes: a value row of the tile is not finite (its K scale is negative)
 #pragma unroll
         for (int b = 0; b < NKB; b++)
 #pragma unroll
@@ -364,10 +386,7 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
                 if constexpr (NP == 2) {
                     const floatx4 s4 = *reinterpret_cast<const floatx4 *>(ke + 32 * b + 8 * q + 4 * hf);
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        odd_rows |= s4[r] < 0.0f;
-                        k4[r] = qscale * fabsf(s4[r]);
-                    }
+                    for (int r = 0; r < 4; r++) k4[r] = qscale * fabsf(s4[r]);
                 }
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
@@ -422,9 +441,8 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
             }
         }
         if constexpr (NP == 2)
-            if (__builtin_amdgcn_ballot_w64(odd_rows) != 0) {
-                // value rows that are not finite: the planes hold 0 for those elements, and a key that a column
-                // sees brings them as they are
+            if (odd_rows) {
+                // value rows that are not finite: a key that a column sees brings those elements as they are
 #pragma unroll 1
                 for (int kk = 0; kk < KT; kk++) {
                     if (base + kk >= n || __builtin_amdgcn_readfirstlane(__float_as_int(ke[kk])) >= 0) continue;
@@ -577,8 +595,7 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
 // f32 K and V rows into two f16 planes: x 2^-e = hi + lo with the row's largest |x| 2^-e in [2^13, 2^14),
 // hi rounded, lo the rest rounded (below 2^2: kept to 2^-9 of it and more).  K's scale is 2^e; of V's
 // the exponent e + 13, about log2 of its largest element, is kept (from -90 on; kZeroRow for a row of
-// zeros).  A K row that is not finite throughout has e = 0, and hi its infinities and NaN.  Of a V row such
-// elements become 0, and the K scale of its token is made negative.
+// zeros).  Elements that are not finite become 0, and the K scale of their token is made negative.
 // One thread per 8 dims of a row, a row's threads in one wave.
 template <int HD>
 __global__ __launch_bounds__(256) void prompt_split_kernel(const float *__restrict__ k, int64_t ks,
@@ -593,20 +610,20 @@ __global__ __launch_bounds__(256) void prompt_split_kernel(const float *__restri
     const int h = (int)(idx - row * H);
     const bool in = 8 * l < hd;
     float kscale = 1.0f;
+    int bad = 0;
 #pragma unroll
     for (int which = 0; which < 2; which++) {
         const float *src = which ? v + (row0 + row) * vs : k + (row0 + row) * ks;
         float x[8];
         load8(src + (int64_t)h * hd + (in ? 8 * l : 0), x);
         float m = 0.0f;
-        int bad = 0;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             x[e] = in ? x[e] : 0.0f;
             const bool fin = fabsf(x[e]) < INFINITY;
             bad |= !fin;
-            if (which) x[e] = fin ? x[e] : 0.0f;
-            m = fmaxf(m, fin ? fabsf(x[e]) : which ? 0.0f : INFINITY);
+            x[e] = fin ? x[e] : 0.0f;
+            m = fmaxf(m, fabsf(x[e]));
         }
 #pragma unroll
         for (int o = 1; o < LPR; o <<= 1) {
@@ -614,15 +631,14 @@ __global__ __launch_bounds__(256) void prompt_split_kernel(const float *__restri
             bad |= __shfl_xor(bad, o, 64);
         }
         int e2 = 0;
-        if (m > 0.0f && m < INFINITY) e2 = max(ilogbf(m), which ? -90 : -100) - 13;
+        if (m > 0.0f) e2 = max(ilogbf(m), which ? -90 : -100) - 13;
         const float s = ldexpf(1.0f, -e2);
         f16x8 hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const float y = opaque(x[e] * s);
             hi[e] = (_Float16)y;
-            const float rest = y - (float)hi[e];
-            lo[e] = fabsf(rest) < INFINITY ? (_Float16)rest : (_Float16)0.0f;
+            lo[e] = (_Float16)(y - (float)hi[e]);
         }
         _Float16 *dst = (which ? vp : kp) + idx * (2 * HD) + 8 * l;
         *reinterpret_cast<f16x8 *>(dst) = hi;

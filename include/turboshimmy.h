@@ -462,7 +462,7 @@ int ts_attn_prompt_workspace(int32_t dtype, int32_t n_rows, int32_t n_head_kv, i
  * apart from the inputs, strides of the inputs up to 2^22 elements (else TS_ERR_INVALID).  f16 and bf16 are multiplied as they are, the
  * probabilities rounded to the same type; f32 at 22 bits of every factor.  Scores, softmax and sums
  * are f32.  What a token does not attend to has no part in its output, infinities and NaN
- * included.  d_workspace: ts_attn_prompt_workspace bytes of tok_off[n_seq] - tok_off[0] rows. */
+ * included (f32: a row of q that is not finite gives NaN).  d_workspace: ts_attn_prompt_workspace bytes of tok_off[n_seq] - tok_off[0] rows. */
 int ts_attn_prompt(int32_t dtype, const void *d_q, int64_t q_stride, const void *d_k, int64_t k_stride,
                    const void *d_v, int64_t v_stride, const int32_t *tok_off, int32_t n_seq, int32_t n_head,
                    int32_t n_head_kv, int32_t head_dim, float softcap, void *d_out, int64_t out_stride,

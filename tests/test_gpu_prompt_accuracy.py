@@ -116,3 +116,40 @@ def test_prompt_large_scores_f32(gpu, size, hd, softcap):
 def test_prompt_large_scores(gpu, name, size, hd, softcap):
     """Scores of any finite size, of 16-bit rows."""
     largest_take_all(name, size, hd, softcap)
+
+
+@pytest.mark.parametrize("softcap", [0.0, 5.0])
+@pytest.mark.parametrize("hd", [64, 80, 128, 256])
+@pytest.mark.parametrize("name", NAMES)
+def test_prompt_infinite_keys(gpu, name, hd, softcap):
+    """A key with infinities that a row sees: a score of -inf takes no weight, one of +inf makes the row NaN, and softcap
+    makes both finite; the key's finite elements of any size change nothing."""
+    dt, n = DTYPES[name], 140
+    q, k, v = rand((n, 4, hd), 1, dt), rand((n, 2, hd), 2, dt), rand((n, 2, hd), 3, dt)
+    for i, at in enumerate((0, 3, 50, 99, 139)):
+        k[at, 0, (7 * i) % hd] = float("-inf") if i % 2 else float("inf")
+    k[50, 0, 5] = 60000.0
+    k[99, 1, hd - 1] = float("nan")
+    got = attn_prompt(q.cuda(), k.cuda(), v.cuda(), [0, 100, n], softcap=softcap).cpu().double()
+    eps = torch.finfo(dt).eps / 2
+    some = False
+    for a, b in ((0, 100), (100, n)):
+        hidden = torch.ones(b - a, b - a, dtype=torch.bool).triu(1)
+        for h in range(4):
+            kh = k[a:b, h // 2].double()
+            x = q[a:b, h].double() @ torch.where(kh.isfinite(), kh, 0.0).T
+            for j in (~kh.isfinite()).any(-1).nonzero()[:, 0].tolist():  # (0 times infinity nowhere: q has no zeros)
+                bad = ~kh[j].isfinite()
+                x[:, j] = (q[a:b, h].double()[:, bad] * kh[j, bad]).sum(-1)
+            x = x / hd ** 0.5
+            x = softcap * torch.tanh(x / softcap) if softcap else x
+            p = torch.softmax(x.masked_fill(hidden, float("-inf")), -1)
+            want = p @ v[a:b, h // 2].double()
+            assert torch.equal(got[a:b, h].isnan(), want.isnan())
+            fine = ~want.isnan()
+            some |= bool(fine[60:].any())
+            # close()'s for rows of unit variance: f32 scores off by 2^-21 (its d below 5e-7), 16-bit weights by eps,
+            # eight standard deviations of each, values below 5
+            tol = 8 * (2.0 ** -21 + (0.0 if dt == torch.float32 else eps)) * 5 + eps * 5
+            assert ((got[a:b, h] - want).abs()[fine] <= tol).all()
+    assert some
