@@ -38,6 +38,7 @@ typedef short short8v __attribute__((ext_vector_type(8)));
 constexpr int kPromptNW = 4;
 constexpr int kPromptCols = 32 * kPromptNW;
 constexpr float kFar = 4194304.0f;   // scores above this: their reference is taken from them first
+constexpr int kLowest = -113;         // f32: least exponent that rows are scaled by (2^(13 - it) and its inverse are normal)
 constexpr float kZeroRow = -200.0f;  // f32: V's exponent of a row of zeros (below any other: out of P's range)
 
 struct PromptArgs {
@@ -273,9 +274,11 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
                 m = fmaxf(m, fabsf(x[t][e]));
             }
         }
-        float s, inv;
-        q_scale(both_max(m), s, inv);
-        qscale = a.scale * inv;
+        // the largest element to [2^13, 2^14), as the planes' rows (and below, from 2^-113 on)
+        m = both_max(m);
+        const int e2 = m > 0.0f ? min(max(ilogbf(m), kLowest), 127) - 13 : 0;
+        const float s = ldexpf(1.0f, -e2);
+        qscale = a.scale * ldexpf(1.0f, e2);
 #pragma unroll
         for (int t = 0; t < NKS; t++)
 #pragma unroll
@@ -594,8 +597,8 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
 
 // f32 K and V rows into two f16 planes: x 2^-e = hi + lo with the row's largest |x| 2^-e in [2^13, 2^14),
 // hi rounded, lo the rest rounded (below 2^2: kept to 2^-9 of it and more).  K's scale is 2^e; of V's
-// the exponent e + 13, about log2 of its largest element, is kept (from -90 on; kZeroRow for a row of
-// zeros).  Elements that are not finite become 0, and the K scale of their token is made negative.
+// the exponent e + 13, about log2 of its largest element, is kept (kZeroRow for a row of zeros).  Elements that are not
+// finite become 0, and the K scale of their token is made negative.
 // One thread per 8 dims of a row, a row's threads in one wave.
 template <int HD>
 __global__ __launch_bounds__(256) void prompt_split_kernel(const float *__restrict__ k, int64_t ks,
@@ -631,7 +634,7 @@ __global__ __launch_bounds__(256) void prompt_split_kernel(const float *__restri
             bad |= __shfl_xor(bad, o, 64);
         }
         int e2 = 0;
-        if (m > 0.0f) e2 = max(ilogbf(m), which ? -90 : -100) - 13;
+        if (m > 0.0f) e2 = max(ilogbf(m), kLowest) - 13;
         const float s = ldexpf(1.0f, -e2);
         f16x8 hi, lo;
 #pragma unroll

@@ -153,3 +153,13 @@ def test_prompt_infinite_keys(gpu, name, hd, softcap):
             tol = 8 * (2.0 ** -21 + (0.0 if dt == torch.float32 else eps)) * 5 + eps * 5
             assert ((got[a:b, h] - want).abs()[fine] <= tol).all()
     assert some
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_prompt_f32_whole_range(gpu, hd):
+    """f32 rows of any normal size: queries of 1e35 against keys of 1e-35, values of 1e-36, keep their bits."""
+    q, k, v = rand((150, 2, hd), 1), rand((150, 1, hd), 2), rand((150, 1, hd), 3)
+    for up in (1e35, 1e-35):
+        close(q * up, k / up, v, [0, 150])
+    close(q, k, v * 1e-36, [0, 150])
+    close(q, k, v * 1e37, [0, 150])
