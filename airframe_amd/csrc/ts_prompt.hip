@@ -151,10 +151,12 @@ __device__ inline typename Vec8<T>::type bad_part(typename Vec8<T>::type v, int 
 
 // One tile of 64 lanes x 16 bytes from memory straight into LDS: lane l's 16 bytes at byte voff of the
 // buffer (0s past its end) go to lds + 16 l.  In asm because the compiler would make every LDS read
-// wait for all such loads; it has no outputs, and tile_barrier() waits for it.
+// wait for all such loads; it has no outputs but M0's old value (put back: the compiler may hold one of its own
+// there), and tile_barrier() waits for it.
 __device__ inline void load_lds(const u32x4 &rsrc, uint32_t voff, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "s"(lds)
-                 : "memory");
+    uint32_t m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0) : "v"(voff), "s"(rsrc), "s"(lds) : "memory");
 }
 // All loads into LDS of this wave have landed, and every wave of the workgroup got here.
 __device__ inline void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
