@@ -259,8 +259,9 @@ class KVCache:
                     stream=None):
         """(K, V) of the cache as the values its codes stand for: positions pos0[s] .. (None: 0 ..) of
         sequence s in rows row_off[s] .. row_off[s + 1] - 1 of [rows, n_head_kv, head_dim], K as
-        stored (rotated).  out: a pair of such tensors to write into."""
-        off, keep, _, _, rows = _offsets(row_off, self.n_seq, None, "row_off")
+        stored (rotated).  out: a pair of such tensors to write into, whose other rows are left as they
+        are (zeros before row_off[0] in tensors allocated here)."""
+        off, keep, _, first, rows = _offsets(row_off, self.n_seq, None, "row_off")
         p0 = None
         if pos0 is not None:
             if len(pos0) != self.n_seq:
@@ -281,6 +282,9 @@ class KVCache:
             if out is None:
                 k = torch.empty((max(rows, 0), self.n_head_kv, self.head_dim), dtype=dtype, device=self.device)
                 v = torch.empty_like(k)
+                if first > 0:
+                    k[:first].zero_()
+                    v[:first].zero_()
                 n = self.n_head_kv * self.head_dim
                 at = (k.data_ptr(), n, v.data_ptr(), n)
             else:

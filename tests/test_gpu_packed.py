@@ -385,3 +385,19 @@ def test_read_packed_rows_apart(gpu):
     wide.zero_()
     kv.read_packed(0, [0, 9], out=(wide[:9, 3:], wide[1:10, :2]))  # (V a row further on)
     assert torch.equal(wide[:9, 3:], want[0]) and torch.equal(wide[1:10, :2], want[1]) and (wide[:, 2] == 0).all()
+
+
+def test_read_packed_leading_rows(gpu):
+    """Tensors that read_packed allocates have zeros in the rows before the first offset."""
+    kv = KVCache.new_int4(1, 2, 64, 64, 2)
+    k, v = rand((9, 2, 64), 1).cuda(), rand((9, 2, 64), 2).cuda()
+    kv.append_packed(0, k, v, [0, 5, 9], None)
+    want = kv.read_packed(0, [0, 5, 9])
+    for dt in DTYPES.values():
+        for first in (1, 300):
+            full = [torch.full((first + 9, 2, 64), 3.0, dtype=dt, device="cuda") for _ in range(4)]
+            del full  # (what the allocator hands out next is not zeros)
+            for got, w in zip(kv.read_packed(0, [first, first + 5, first + 9], dtype=dt), want):
+                assert (got[:first] == 0).all() and torch.equal(got[first:], w.to(dt))
+    got = kv.read_packed(0, [7, 7, 7])  # no rows: all of them before the first
+    assert all(x.shape[0] == 7 and (x == 0).all() for x in got)
