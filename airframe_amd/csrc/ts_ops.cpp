@@ -30,6 +30,11 @@ static bool rows_overlap(const void *a, int64_t a_stride, const void *b, int64_t
     return d < row || d > a_stride - row;
 }
 
+// Whether two ranges of bytes share memory.
+static bool bytes_overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
+    return a && b && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
+
 // The largest length of a sequence after its rows of a packed batch, and its last rotation position.
 static void packed_ends(const ts_kv *kv, const int32_t *off, int64_t &len_end, int64_t &rot_last) {
     len_end = rot_last = 0;
@@ -176,6 +181,12 @@ int ts_attn_prompt(int32_t dtype, const void *d_q, int64_t q_stride, const void 
     const uint64_t need = prompt_workspace(dtype, rows, n_head_kv, head_dim);
     if (need > 0 && (!d_workspace || workspace_bytes < need)) return TS_ERR_WORKSPACE;
     if (need > 0 && !aligned16(d_workspace)) return TS_ERR_INVALID;
+    auto in_ws = [&](const void *p, int64_t stride, int64_t row) {
+        const uintptr_t at = span(p, stride, row, 0);
+        return need > 0 && bytes_overlap(d_workspace, need, (const void *)at, span(p, stride, row, 1) - at);
+    };
+    if (in_ws(d_q, q_stride, qrow) || in_ws(d_k, k_stride, krow) || in_ws(d_v, v_stride, krow) || in_ws(d_out, out_stride, qrow))
+        return TS_ERR_INVALID;
     PromptCall c;
     c.dtype = dtype;
     c.q = d_q;
@@ -233,6 +244,9 @@ int ts_attn_shared(ts_kv *kv, const ts_kv *prefix, int32_t prefix_seq, int32_t l
         return TS_ERR_INVALID;
     if (n_tok == 0) return TS_OK;
     if (!d_q || !d_out || !aligned16(d_q) || !aligned16(d_out)) return TS_ERR_INVALID;
+    // a workgroup reads its rows of q before it writes them, but not before others write theirs
+    const uint64_t q_bytes = (uint64_t)kv->d.n_seq * n_tok * n_head * kv->d.head_dim * sizeof(float);
+    if (d_out != d_q && bytes_overlap(d_q, q_bytes, d_out, q_bytes)) return TS_ERR_INVALID;
     // the own positions continue the prefix's: slot p of a sequence is position window base + p (of all its
     // slots: no sinks), and the prefix ends at its length plus its own window base
     const int P = prefix->h_len[prefix_seq];
@@ -252,6 +266,10 @@ int ts_attn_shared(ts_kv *kv, const ts_kv *prefix, int32_t prefix_seq, int32_t l
     ts_attn_shared_workspace(kv, prefix, n_head, n_tok, &need);
     if (need > 0 && (!d_workspace || workspace_bytes < need)) return TS_ERR_WORKSPACE;
     if (need > 0 && !aligned16(d_workspace)) return TS_ERR_INVALID;
+    const uint64_t kv_bytes = q_bytes / n_head * kv->d.n_head_kv;
+    if (bytes_overlap(d_workspace, need, d_q, q_bytes) || bytes_overlap(d_workspace, need, d_out, q_bytes) ||
+        bytes_overlap(d_workspace, need, d_k, kv_bytes) || bytes_overlap(d_workspace, need, d_v, kv_bytes))
+        return TS_ERR_INVALID;
 
     SharedCall c;
     c.own = kv->layer(layer);

@@ -462,7 +462,8 @@ int ts_attn_prompt_workspace(int32_t dtype, int32_t n_rows, int32_t n_head_kv, i
  * apart from the inputs, strides of the inputs up to 2^22 elements (else TS_ERR_INVALID).  f16 and bf16 are multiplied as they are, the
  * probabilities rounded to the same type; f32 at 22 bits of every factor.  Scores, softmax and sums
  * are f32.  What a token does not attend to has no part in its output, infinities and NaN
- * included (f32: a row of q that is not finite gives NaN).  d_workspace: ts_attn_prompt_workspace bytes of tok_off[n_seq] - tok_off[0] rows. */
+ * included (f32: a row of q that is not finite gives NaN).  d_workspace: ts_attn_prompt_workspace
+ * bytes of tok_off[n_seq] - tok_off[0] rows, 16-byte aligned, apart from all rows (TS_ERR_INVALID). */
 int ts_attn_prompt(int32_t dtype, const void *d_q, int64_t q_stride, const void *d_k, int64_t k_stride,
                    const void *d_v, int64_t v_stride, const int32_t *tok_off, int32_t n_seq, int32_t n_head,
                    int32_t n_head_kv, int32_t head_dim, float softcap, void *d_out, int64_t out_stride,
@@ -490,8 +491,9 @@ int ts_attn_shared_workspace(const ts_kv *kv, const ts_kv *prefix, int32_t n_hea
  * the same heads, head_dim and device; every window base has to be P or more, without
  * sinks (TS_ERR_INVALID).  The
  * prefix's length is taken at the call, also into a graph; the rope table of a captured call has to
- * cover the positions its replays reach.  Runs on the caches' device.  d_workspace: ts_attn_shared_workspace
- * bytes, 16-byte aligned. */
+ * cover the positions its replays reach.  The caches' device is the current one.  d_out may be d_q; ranges that overlap
+ * otherwise are TS_ERR_INVALID.  d_workspace: ts_attn_shared_workspace bytes, 16-byte aligned, apart from the
+ * other arguments (TS_ERR_INVALID). */
 int ts_attn_shared(ts_kv *kv, const ts_kv *prefix, int32_t prefix_seq, int32_t layer, const float *d_k,
                    const float *d_v, const float *d_q, int32_t n_head, int32_t n_tok, const ts_rope *rope,
                    float softcap, float *d_out, void *d_workspace, uint64_t workspace_bytes, void *stream);

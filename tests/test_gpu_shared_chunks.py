@@ -3,6 +3,7 @@ its output, without partials), and every form of it as closely as its roundings 
 import pytest
 import torch
 
+from airframe_amd import TsError
 from airframe_amd.kv_cache import RopeTable
 from tests.packed_util import attend_bound, norms, offsets, rand, rope_angles, rotate
 from tests.test_gpu_shared import BASE, Batch
@@ -174,6 +175,31 @@ def test_shared_accuracy_beside_others(gpu, n_tok, heads, n_kv, hd):
     b.q[1, :, 0, 5] = float("inf")
     b.q[2] = float("nan")
     close(b.kv.attn_shared(1, b.q.cuda(), b.rope, b.pre), b, seqs=[3, 4])
+
+
+@pytest.mark.parametrize("n_tok,own", [(1, [5, 0, 70]), (3, [5, 0, 70]), (75, [3] * 8)])
+def test_shared_output_in_place(gpu, n_tok, own):
+    """The output may be q; another overlap of the two, or of the workspace with any of them, is refused."""
+    b = Exact(100, own, n_tok, 32, 8, 64).refill()
+    b.append()
+    assert b.is_chain() == (n_tok == 75)
+    want = b.kv.attn_shared(1, b.q.cuda(), b.rope, b.pre)
+    n = want.numel()
+    space = torch.zeros(n + 1024 + b.kv.attn_shared_workspace(b.pre, 32, n_tok) // 4, device="cuda")
+    q = space[:n].view(want.shape)
+    q.copy_(b.q)
+    assert torch.equal(b.kv.attn_shared(1, q, b.rope, b.pre, out=q), want)
+    other = torch.zeros_like(want)
+    calls = [lambda: b.kv.attn_shared(1, q, b.rope, b.pre, out=space[64:n + 64].view(want.shape)),
+             lambda: b.kv.attn_shared(1, space[64:n + 64].view(want.shape), b.rope, b.pre, out=q)]
+    if not b.is_chain():
+        ws = space[n - 64:].view(torch.uint8)
+        calls += [lambda: b.kv.attn_shared(1, q, b.rope, b.pre, out=other, workspace=ws),
+                  lambda: b.kv.attn_shared(1, other, b.rope, b.pre, out=q, workspace=ws)]
+    for bad in calls:
+        with pytest.raises(TsError) as e:
+            bad()
+        assert e.value.code == -1
 
 
 @pytest.mark.parametrize("softcap", [1e-39, 1e4, 1e8, 1e20, 3e38])

@@ -96,3 +96,19 @@ def test_more_null_handles_are_refused():
         assert rc(**kw) == INVALID, kw
     assert rc(hd=264, qs=264, ks=264, vs=264, os=264) == -3
     assert rc(dtype=0) == -6
+
+
+def test_prompt_workspace_apart():
+    """A workspace that shares memory with a row of q, k, v or the output is refused, before any device work."""
+    L = load()
+    off = (ctypes.c_int32 * 2)(2, 12)  # rows 2 .. 11
+    need = 10 * 1 * (8 * 64 + 8)
+    row, at = 64 * 4, {"q": 1 << 20, "k": 2 << 20, "v": 3 << 20, "out": 4 << 20}
+
+    def rc(ws, out=at["out"]):
+        return L.ts_attn_prompt(0, at["q"], 64, at["k"], 64, at["v"], 64, off, 1, 1, 1, 64, 0.0, out, 64, ws, need, None)
+    for p in at.values():
+        first, end = p + 2 * row, p + 12 * row
+        for ws in (first, end - 16, first - need + 16):
+            assert rc(ws) == INVALID
+    assert rc(8 << 20, out=at["k"] + 3 * row) == INVALID
