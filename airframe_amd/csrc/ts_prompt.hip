@@ -15,12 +15,12 @@
 //   per row that takes its largest element to [2^13, 2^14); products hi hi + hi lo + lo hi.
 // Scores, maxima, sums and outputs are f32 until the output is rounded once.
 //
-// Matrix work bounds it.  A prompt of 8192 tokens, 32 heads over 8 of 128 dims in f16: 550 GFLOP in 560 us,
-// 0.98 PFLOP/s (a product of 8192^3 reaches 1.15), the matrix cores busy for 53% of the CUs' time and no
-// bank conflicts.  16 ragged prompts of 300 to 2048 in bf16, 150 GFLOP: 197 us; f32 (three products)
-// of 128 dims 550 us.  3 prompts of 501 to 2100, 16 heads over 8 of 256 dims in f32 with softcap: 252 us behind
-// 18.6 of the split, one wave per SIMD (o alone takes 128 registers), ended by the longest walk of 66
-// tiles: 0.56 PFLOP/s of the three products' work.
+// Matrix work bounds it.  A prompt of 8192 tokens, 32 heads over 8 of 128 dims in f16: 550 GFLOP in 555 to 600 us
+// by card, 0.92 to 0.99 PFLOP/s (a product of 8192^3 reaches 1.15), the matrix cores busy for 54% of the CUs' time
+// and no bank conflicts.  16 ragged prompts of 300 to 2048 in bf16, 150 GFLOP: 202 us; f32 (three products) of 128 dims
+// 560 us, of 64 dims 315.  3 prompts of 501 to 2100, 16 heads over 8 of 256 dims in f32 with softcap: 265 us behind 18 of
+// the split, one wave per SIMD (o alone takes 128 registers), ended by the longest walk of 66 tiles (26 on
+// average): 0.53 PFLOP/s of the three products' work.
 #include "ts_prompt.h"
 
 #include <cfloat>
@@ -117,8 +117,8 @@ __device__ inline float cap(float x, float softcap, float inv_softcap) {
 
 // The same of small softcaps for 16-bit rows, as c - 2 c / (1 + e^(2 y)) from two transcendental instructions: within
 // 2^-21 of softcap and not of x, so up to softcaps of kQuickCap within 2^-15, where f16 weights are rounded by 2^-12.
-// to_exp: 2 log2(e) / softcap.  16 ragged prompts, softcap 50, with this and with cap(): bf16 of 128 dims 242 and 293 us,
-// f16 of 64 dims 161 and 226 (without softcap 205 and 111).
+// to_exp: 2 log2(e) / softcap.  16 ragged prompts, softcap 50, with this and with cap(): bf16 of 128 dims 236 and 293 us,
+// f16 of 64 dims 153 and 226 (without softcap 202 and 109).
 constexpr float kQuickCap = 64.0f;
 __device__ inline float cap_quick(float x, float softcap, float to_exp) {
     const float c = softcap * kLog2e;
@@ -479,8 +479,8 @@ __global__ __launch_bounds__(64 * kPromptNW, HD > 128 ? 1 : 2) void prompt_kerne
             }
         // O^T += V^T P^T, 16 keys at a time: the exponentials of a step run beside the products of the one
         // before, and V's operands are read one group of products ahead.  (Two planes: one dim tile a group, or
-        // 128 dims take more than the 256 registers that let two workgroups share a CU: 776 against 552 us for
-        // 16 f32 prompts of 300-2048 tokens.)
+        // 128 dims take more than the 256 registers that let two workgroups share a CU: 1006 against 560 us for
+        // 16 f32 prompts of 300-2048 tokens; 64 dims 349 and 315.)
         constexpr int VG = NP == 2 ? 1 : 4, NVG = NDB < VG ? 1 : NDB / VG, NU = 2 * NKB * NVG;
         constexpr int DG = NDB < VG ? NDB : VG;  // dim tiles of a group
         V8 vf[2][DG][NP];
@@ -670,9 +670,9 @@ void prompt_launch(const PromptArgs &a, unsigned blocks, hipStream_t st) {
 }
 
 // Keys per tile: 64 of one plane and 32 of two up to 128 dims, 32 of 256 dims.  16 ragged prompts of 300 to
-// 2048, 32 heads over 8: bf16 of 128 dims 198 us with 64 and 222 with 32, of 64 dims 114 and 137; f32 of 64
-// dims 351 with 64 and 319 with 32 (one prompt of 500: 30 and 33; of 8192: 951 and 925); bf16 of 256 dims
-// 251 with 64 and 253 with 32, which leaves room for a second workgroup's tiles.
+// 2048, 32 heads over 8: bf16 of 128 dims 202 us with 64 and 228 with 32, f16 of 64 dims 109 and 130; f32 of 64
+// dims 332 with 64 and 315 with 32 (one prompt of 500: 30 and 34; of 8192: 970 and 959), of 128 dims 1382 and
+// 560; bf16 of 256 dims 465 with 64 and 467 with 32 (half the LDS).
 template <class T, class O, int NP, int CAP>
 void prompt_dims(const PromptArgs &a, unsigned blocks, hipStream_t st) {
     if (a.hd <= 64)

@@ -418,7 +418,9 @@ enum { TS_ROPE_INTERLEAVED = 0, TS_ROPE_HALF = 1 };
  * with beta > alpha, by parts: theta_i ((1 - ramp) / factor + ramp) with ramp = clamp((l_train theta_i
  * / (2 pi) - alpha) / (beta - alpha), 0, 1), so that the pairs that turn often within the trained
  * length l_train stay and the slow ones are stretched.  mult scales both parts of the table (a
- * softmax temperature; 1: none).  The handle serves every entry point that takes a ts_rope.
+ * softmax temperature; 1: none).  The ramp is linear in those turns, as in ts_rope_create_yarn, which is the
+ * table of a model that the reference runs, bit for bit; a model trained with a ramp linear in the
+ * pair's index needs a table that neither makes.  The handle serves every entry point that takes a ts_rope.
  * Allocates and waits: not for capture. */
 int ts_rope_create_scaled(int32_t n_pos, int32_t rope_dim, double base, double factor, int32_t l_train,
                           double alpha, double beta, double mult, ts_rope **out);
