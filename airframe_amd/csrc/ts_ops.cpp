@@ -30,9 +30,9 @@ static bool rows_overlap(const void *a, int64_t a_stride, const void *b, int64_t
     return d < row || d > a_stride - row;
 }
 
-// Whether two ranges of bytes share memory.
+// Whether two ranges of bytes share memory (one of no bytes, such as a workspace that is not needed: never).
 static bool bytes_overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
-    return a && b && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+    return a && b && na > 0 && nb > 0 && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
 }
 
 // The largest length of a sequence after its rows of a packed batch, and its last rotation position.

@@ -208,3 +208,13 @@ def test_shared_softcap_range(gpu, n_tok, softcap):
     b = Exact(200, [40, 0, 3, 11, 64, 1, 2, 9], n_tok, 32, 8, 128).refill()
     b.append()
     close(b.kv.attn_shared(1, b.q.cuda(), b.rope, b.pre, softcap=softcap), b, softcap, seqs=[0, 4])
+
+
+def test_shared_workspace_not_needed(gpu):
+    """Where no workspace is needed, what is passed for one is not looked at."""
+    b = Exact(100, [3] * 8, 75, 32, 8, 64).refill()
+    b.append()
+    assert b.is_chain()
+    q = b.q.cuda()
+    want = b.kv.attn_shared(1, q, b.rope, b.pre)
+    assert torch.equal(b.kv.attn_shared(1, q, b.rope, b.pre, workspace=q.view(-1)[1024:].view(torch.uint8)), want)
