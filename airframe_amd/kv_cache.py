@@ -264,7 +264,7 @@ class KVCache:
         off, keep, _, first, rows = _offsets(row_off, self.n_seq, None, "row_off")
         p0 = None
         if pos0 is not None:
-            if len(pos0) != self.n_seq:
+            if len(pos0) != self.n_seq or (isinstance(pos0, torch.Tensor) and pos0.dim() != 1):
                 raise ValueError(f"pos0 must hold {self.n_seq} positions")
             if not (isinstance(pos0, torch.Tensor) and pos0.dtype == torch.int32 and not pos0.is_cuda and pos0.is_contiguous()):
                 pos0 = torch.tensor([int(p) for p in pos0], dtype=torch.int32)

@@ -488,7 +488,7 @@ int ts_attn_shared_workspace(const ts_kv *kv, const ts_kv *prefix, int32_t n_hea
  * prefix_seq of `prefix`) and over the sequence's own keys, causal: token t sits in slot len[s] + t,
  * appended before as for ts_attn_prefill / ts_attn_decode.  The prefix is read and multiplied once for
  * the batch.  d_q, d_out: [n_seq][n_tok][n_head][head_dim]; q is normalized (kv's QK norm) and
- * rotated at its position like there.  With n_tok 1, d_k and d_v: NULL, or the new token's K and V
+ * rotated at its position like there, its elements below 2^100.  With n_tok 1, d_k and d_v: NULL, or the new token's K and V
  * [n_seq][n_head_kv][head_dim], appended in the same launch (ts_attn_decode_append).  Both caches have
  * the same heads, head_dim and device; every window base has to be P or more, without
  * sinks (TS_ERR_INVALID).  The

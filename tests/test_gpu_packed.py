@@ -401,3 +401,10 @@ def test_read_packed_leading_rows(gpu):
                 assert (got[:first] == 0).all() and torch.equal(got[first:], w.to(dt))
     got = kv.read_packed(0, [7, 7, 7])  # no rows: all of them before the first
     assert all(x.shape[0] == 7 and (x == 0).all() for x in got)
+
+
+def test_read_packed_positions_of_another_shape(gpu):
+    """pos0 is one position a sequence: a table of them is refused, not read as its first numbers."""
+    kv = KVCache.new_int4(1, 2, 64, 64, 2)
+    with pytest.raises(ValueError):
+        kv.read_packed(0, [0, 1, 2], torch.zeros(2, 3, dtype=torch.int32))
