@@ -15,8 +15,8 @@
 //   per row that takes its largest element to [2^13, 2^14); products hi hi + hi lo + lo hi.
 // Scores, maxima, sums and outputs are f32 until the output is rounded once.
 //
-// Matrix work bounds it.  A prompt of 8192 tokens, 32 heads over 8 of 128 dims in f16: 550 GFLOP in 555 to 600 us
-// by card, 0.92 to 0.99 PFLOP/s (a product of 8192^3 reaches 1.15), the matrix cores busy for 54% of the CUs' time
+// Matrix work bounds it.  A prompt of 8192 tokens, 32 heads over 8 of 128 dims in f16: 550 GFLOP in 550 to 600 us
+// by card, 0.92 to 1.00 PFLOP/s (a product of 8192^3 reaches 1.15), the matrix cores busy for 54% of the CUs' time
 // and no bank conflicts.  16 ragged prompts of 300 to 2048 in bf16, 150 GFLOP: 202 us; f32 (three products) of 128 dims
 // 560 us, of 64 dims 315.  3 prompts of 501 to 2100, 16 heads over 8 of 256 dims in f32 with softcap: 265 us behind 18 of
 // the split, one wave per SIMD (o alone takes 128 registers), ended by the longest walk of 66 tiles (26 on

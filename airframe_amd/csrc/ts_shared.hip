@@ -13,7 +13,7 @@
 // 32 heads over 8 of 128 dims, 32 sequences of 60 to 500 own keys behind 8192: 29.5 us (shared_kernel 24.4,
 // a CU's four windows with the q before and the partials behind them; join 6), of which the bytes would take
 // 3.4 and the matrix work 4; the same with the new tokens' append in the launch.  Chunks of 256 tokens of 8 sequences
-// behind 4097: 261 us, 142 GFLOP that hi and lo terms of q and P make 240: 0.92 PFLOP/s executed.
+// behind 4097: 252 to 269 us by card, 142 GFLOP that hi and lo terms of q and P make 240: 0.89 to 0.95 PFLOP/s executed.
 #include "ts_shared.h"
 
 #include "ts_decode_split.h"
