@@ -1,6 +1,7 @@
 """airframe_amd -- MI355X (gfx950) INT4 KV-cache path: RoPE-fused quantize-on-append, split-K
 GQA decode attention and chunked-prefill attention over the INT4 cache, rotary positions, attention
-and cache rows of packed prompts, attention behind a shared prefix, behind the C ABI in
+and cache rows of packed prompts, attention behind a shared prefix, eviction by accumulated
+attention, behind the C ABI in
 include/turboshimmy.h."""
 from ._lib import LIB_PATH, TsError, load  # noqa: F401
 

@@ -101,6 +101,10 @@ SIGNATURES = {
     "ts_attn_prompt_workspace": (ctypes.c_int, [_i32, _i32, _i32, _i32, _u64p]),
     "ts_attn_prompt": (ctypes.c_int, [_i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _f, _vp, _i64,
                                       _vp, ctypes.c_uint64, _vp]),
+    "ts_attn_weigh_workspace": (ctypes.c_int, [_vp, _i32, _i32, _u64p]),
+    "ts_attn_weigh": (ctypes.c_int, [_vp, _i32, _vp, _vp, _vp, _i32, _i32, _vp, _f, _vp, _i32, _vp, _vp, ctypes.c_uint64, _vp]),
+    "ts_kv_select": (ctypes.c_int, [_vp, _vp, _i32, _i32, _i32, _vp, _vp]),
+    "ts_kv_keep": (ctypes.c_int, [_vp, _i32, _vp, _i32, _i32, _vp, _i32, _vp, _vp, _vp]),
 }
 
 _lib = None

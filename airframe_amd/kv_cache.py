@@ -350,6 +350,104 @@ class KVCache:
 
         return _launch(self.device, stream, call)
 
+    # ---- eviction by accumulated attention ------------------------------------------------------
+
+    def new_weights(self) -> torch.Tensor:
+        """What every slot has received, zeros: [n_layers, n_seq, n_head_kv, max_seq_len] f32."""
+        return torch.zeros((self.n_layers, self.n_seq, self.n_head_kv, self.max_seq_len), dtype=torch.float32, device=self.device)
+
+    def attn_weigh_workspace(self, n_head: int, n_tok: int = 1) -> int:
+        """Bytes of scratch attn_weigh needs for this shape."""
+        b = ctypes.c_uint64()
+        check("ts_attn_weigh_workspace", load().ts_attn_weigh_workspace(self._h, n_head, n_tok, ctypes.byref(b)))
+        return b.value
+
+    def attn_weigh(self, layer: int, q: torch.Tensor, rope: RopeTable, weights: torch.Tensor, fresh: bool = False,
+                   k: torch.Tensor | None = None, v: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                   softcap: float = 0.0, workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+        """attn_prefill (of one token attn_decode) that adds to weights [n_seq, n_head_kv, max_seq_len], one
+        layer's part of new_weights(), what every slot receives (ts_attn_weigh); fresh: the sums start at
+        zero.  q: [n_seq, n_tok, n_head, head_dim] f32, the tokens appended before; or, with n_tok 1, k
+        and v [n_seq, 1, n_head_kv, head_dim] to append in the same call.  Returns the attention's output."""
+        if q.dim() != 4 or q.shape[0] != self.n_seq or q.shape[3] != self.head_dim:
+            raise ValueError("q must be [n_seq, n_tok, n_head, head_dim]")
+        if (k is None) != (v is None):
+            raise ValueError("k and v come together")
+        n_tok, n_head = q.shape[1], q.shape[2]
+        pq, pw = _ptr(q, torch.float32, "q"), self._weights(weights, 1)
+        pk = pv = None
+        if k is not None:
+            self._check_kv(k, v, 1)
+            pk, pv = _ptr(k, torch.float32, "k"), _ptr(v, torch.float32, "v")
+        self._check_device(q, k, v, out, weights, workspace, rope)
+
+        def call(raw):
+            o = self._out_like(q, out)
+            ws = workspace
+            if ws is None:
+                ws = torch.empty(self.attn_weigh_workspace(n_head, n_tok), dtype=torch.uint8, device=self.device)
+            check("ts_attn_weigh", load().ts_attn_weigh(self._h, layer, pk, pv, pq, n_head, n_tok, rope.handle, softcap, pw,
+                                                        int(fresh), _ptr(o, torch.float32, "out"), ws.data_ptr(), ws.numel(), raw))
+            return o
+
+        return _launch(self.device, stream, call)
+
+    def select_slots(self, weights: torch.Tensor, keep: int, n_sink: int = 0, n_recent: int = 0,
+                     out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+        """The slots that stay when every sequence is cut to `keep`: [n_layers, n_seq, n_head_kv, keep]
+        int32, ascending, -1 behind the last of a shorter sequence (ts_kv_select).  The first n_sink and the
+        last n_recent stay, and of the others those with the largest weights (new_weights()), ties from the
+        lowest."""
+        pw = self._weights(weights, self.n_layers)
+        shape = (self.n_layers, self.n_seq, self.n_head_kv, keep)
+        if out is not None and tuple(out.shape) != shape:
+            raise ValueError(f"out must be {shape}, got {tuple(out.shape)}")
+        self._check_device(weights, out)
+
+        def call(raw):
+            o = torch.empty([max(n, 0) for n in shape], dtype=torch.int32, device=self.device) if out is None else out
+            check("ts_kv_select", load().ts_kv_select(self._h, pw, keep, n_sink, n_recent, _ptr(o, torch.int32, "out"), raw))
+            return o
+
+        return _launch(self.device, stream, call)
+
+    def keep_slots(self, slots: torch.Tensor, weights: torch.Tensor | None = None, src: "KVCache | None" = None,
+                   src_weights: torch.Tensor | None = None, seq: int = 0, src_seq: int = 0, n_seq: int | None = None,
+                   stream=None):
+        """The rows of `slots` [n_layers, n_seq, n_head_kv, keep] (select_slots) moved together
+        (ts_kv_keep): in place, or sequences src_seq .. of the cache src into sequences seq .. of this one.
+        n_seq: how many (all of src's).  Lengths become what was kept, new tokens go on at the positions
+        they would have had.  weights, src_weights: this cache's and src's weights, to move along (in place:
+        weights alone)."""
+        src = self if src is None else src
+        n = src.n_seq if n_seq is None else n_seq
+        if slots.dim() != 4 or tuple(slots.shape[:3]) != (src.n_layers, n, src.n_head_kv):
+            raise ValueError(f"slots must be [{src.n_layers}, {n}, {src.n_head_kv}, keep], got {tuple(slots.shape)}")
+        if src is self and src_weights is None:
+            src_weights = weights
+        if (weights is None) != (src_weights is None):
+            raise ValueError("weights and src_weights come together")
+        ps, pw, psw = _ptr(slots, torch.int32, "slots"), None, None
+        if weights is not None:
+            pw, psw = self._weights(weights, self.n_layers), src._weights(src_weights, src.n_layers)
+        self._check_device(slots, weights, src_weights)
+        _launch(self.device, stream, lambda raw: check("ts_kv_keep", load().ts_kv_keep(
+            self._h, seq, src.handle, src_seq, n, ps, slots.shape[3], psw, pw, raw)))
+
+    def evict(self, weights: torch.Tensor, keep: int, n_sink: int = 0, n_recent: int = 0, stream=None) -> torch.Tensor:
+        """Every sequence cut to the `keep` slots of each layer and kv head that select_slots names, in
+        place, weights with them.  Returns the slots."""
+        slots = self.select_slots(weights, keep, n_sink, n_recent, stream=stream)
+        self.keep_slots(slots, weights, stream=stream)
+        return slots
+
+    def _weights(self, w: torch.Tensor, layers: int) -> ctypes.c_void_p:
+        """Address of weights of `layers` layers."""
+        shape = (self.n_seq, self.n_head_kv, self.max_seq_len)
+        if tuple(w.shape) not in ((layers, *shape), *((shape,) if layers == 1 else ())):
+            raise ValueError(f"weights must be {(layers, *shape)}, got {tuple(w.shape)}")
+        return _ptr(w, torch.float32, "weights")
+
     def _check_device(self, *tensors):
         for t in tensors:
             if t is not None and t.device != self.device:

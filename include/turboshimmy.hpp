@@ -312,6 +312,41 @@ public:
               "KVCache::attn_shared");
     }
 
+    // ---- eviction by accumulated attention; weights: [n_layers][n_seq][n_head_kv][max_seq] f32 on the device
+    size_t weights_count() const {
+        return (size_t)d_.n_layers * d_.n_seq * d_.n_head_kv * d_.max_seq;
+    }
+    size_t slots_count(int32_t keep) const { return (size_t)d_.n_layers * d_.n_seq * d_.n_head_kv * keep; }
+    uint64_t weigh_workspace_bytes(int32_t n_head, int32_t n_tok = 1) const {
+        uint64_t b = 0;
+        check(ts_attn_weigh_workspace(h_, n_head, n_tok, &b), "ts_attn_weigh_workspace");
+        return b;
+    }
+    // attn_prefill or attn_decode (with d_k and d_v attn_decode_append) that adds what every slot receives to one
+    // layer's weights.
+    void attn_weigh(int32_t layer, const float *d_k, const float *d_v, const float *d_q, int32_t n_head, int32_t n_tok,
+                    const RopeTable &rope, float *d_weights, bool fresh, float *d_out, void *d_workspace,
+                    uint64_t workspace_bytes, float softcap = 0.0f, void *stream = nullptr) {
+        check(ts_attn_weigh(h_, layer, d_k, d_v, d_q, n_head, n_tok, rope.get(), softcap, d_weights, fresh, d_out,
+                            d_workspace, workspace_bytes, stream),
+              "KVCache::attn_weigh");
+    }
+    void select_slots(const float *d_weights, int32_t keep, int32_t n_sink, int32_t n_recent, int32_t *d_slots,
+                      void *stream = nullptr) const {
+        check(ts_kv_select(h_, d_weights, keep, n_sink, n_recent, d_slots, stream), "KVCache::select_slots");
+    }
+    // Rows of n_seq sequences of src (which may be this cache: in place with seq = src_seq) into sequences seq ..
+    void keep_slots(int32_t seq, const KVCache &src, int32_t src_seq, int32_t n_seq, const int32_t *d_slots, int32_t keep,
+                    const float *d_src_weights = nullptr, float *d_weights = nullptr, void *stream = nullptr) {
+        check(ts_kv_keep(h_, seq, src.h_, src_seq, n_seq, d_slots, keep, d_src_weights, d_weights, stream),
+              "KVCache::keep_slots");
+    }
+    // Every sequence cut to `keep` slots in place; d_slots: slots_count(keep) ints, written.
+    void evict(float *d_weights, int32_t keep, int32_t n_sink, int32_t n_recent, int32_t *d_slots, void *stream = nullptr) {
+        select_slots(d_weights, keep, n_sink, n_recent, d_slots, stream);
+        keep_slots(0, *this, 0, d_.n_seq, d_slots, keep, d_weights, d_weights, stream);
+    }
+
 private:
     KVCache(ts_kv *h, const ts_kv_desc &d) : h_(h), d_(d) {}
     uint32_t max_seq_len_now() const {
