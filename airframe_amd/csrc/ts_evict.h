@@ -8,16 +8,24 @@ namespace ts {
 struct WeighCall {
     KvLayerView L;
     const int32_t *d_len;
+    int own_max;  // the longest sequence, the new tokens' slots included, as the host knows it
+    bool captured;  // (replays go past own_max)
     const float *q;
     int n_head, n_tok;
     const float *rope;
     int rope_pairs, rope_rows;
     float softcap;
+    float *out;
     int max_seq;  // a row of weights
     float *w;     // [n_seq][n_head_kv][max_seq]
     bool fresh;
-    float *ws;
+    int n_cu;
+    uint8_t *ws;
 };
+// Chunks (n_tok > 1).
+uint64_t weigh_chunk_workspace(int n_seq, int n_tok, int n_head, int n_kv, int stored_hd, int max_seq, int n_cu);
+hipError_t launch_weigh_chunk(const WeighCall &c, hipStream_t st);
+
 uint64_t weigh_workspace(int n_seq, int n_tok, int n_head, int stored_hd);
 hipError_t launch_weigh(const WeighCall &c, hipStream_t st);
 

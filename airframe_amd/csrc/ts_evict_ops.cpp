@@ -30,8 +30,12 @@ int ts_attn_weigh_workspace(const ts_kv *kv, int32_t n_head, int32_t n_tok, uint
     if (!bytes || !weigh_shape_ok(kv, n_head, n_tok)) return TS_ERR_INVALID;
     *bytes = 0;
     if (n_tok == 0) return TS_OK;
+    if (n_tok > 1) {
+        *bytes = weigh_chunk_workspace(kv->d.n_seq, n_tok, n_head, kv->d.n_head_kv, kv->hdp, kv->d.max_seq, kv->n_cu);
+        return TS_OK;
+    }
     uint64_t dec = 0;
-    if (n_tok == 1) ts_attn_decode_workspace(kv, n_head, &dec);
+    ts_attn_decode_workspace(kv, n_head, &dec);
     *bytes = dec + weigh_workspace(kv->d.n_seq, n_tok, n_head, kv->hdp);
     return TS_OK;
 }
@@ -61,14 +65,11 @@ int ts_attn_weigh(ts_kv *kv, int32_t layer, const float *d_k, const float *d_v, 
         for (int j = i + 1; j < 6; j++)
             if (shares(arg[i].p, arg[i].n, arg[j].p, arg[j].n)) return TS_ERR_INVALID;
 
-    if (n_tok == 1) ts_attn_decode_workspace(kv, n_head, &dec);
-    const int ra = n_tok > 1 ? ts_attn_prefill(kv, layer, d_q, n_head, n_tok, rope, softcap, d_out, stream)
-                   : d_k     ? ts_attn_decode_append(kv, layer, d_k, d_v, d_q, n_head, rope, softcap, d_out, d_workspace, dec, stream)
-                             : ts_attn_decode(kv, layer, d_q, n_head, rope, softcap, d_out, d_workspace, dec, stream);
-    if (ra) return ra;
     WeighCall c;
     c.L = kv->layer(layer);
     c.d_len = kv->d_len;
+    c.own_max = max_len + n_tok;
+    c.captured = capturing(stream) || kv->len_captured;
     c.q = d_q;
     c.n_head = n_head;
     c.n_tok = n_tok;
@@ -76,10 +77,18 @@ int ts_attn_weigh(ts_kv *kv, int32_t layer, const float *d_k, const float *d_v, 
     c.rope_pairs = rope->rope_dim / 2;
     c.rope_rows = rope->n_pos;
     c.softcap = softcap;
+    c.out = d_out;
     c.max_seq = kv->d.max_seq;
     c.w = d_weights;
     c.fresh = fresh != 0;
-    c.ws = reinterpret_cast<float *>(static_cast<uint8_t *>(d_workspace) + dec);
+    c.n_cu = kv->n_cu;
+    c.ws = static_cast<uint8_t *>(d_workspace);
+    if (n_tok > 1) return hip_status(launch_weigh_chunk(c, as_stream(stream)));
+    ts_attn_decode_workspace(kv, n_head, &dec);
+    const int ra = d_k ? ts_attn_decode_append(kv, layer, d_k, d_v, d_q, n_head, rope, softcap, d_out, d_workspace, dec, stream)
+                       : ts_attn_decode(kv, layer, d_q, n_head, rope, softcap, d_out, d_workspace, dec, stream);
+    if (ra) return ra;
+    c.ws += dec;
     return hip_status(launch_weigh(c, as_stream(stream)));
 }
 

@@ -37,6 +37,7 @@ struct SharedArgs {
     int slots;                 // partials per row: n_part, and own_pieces if own_blk
     float inv_sqrt_hd, softcap;
     float *part, *out;
+    float *stats;              // a chain's m and l per row, or null
 };
 
 constexpr int kCols = kPrefillNW * kColsPerWave;
@@ -331,6 +332,10 @@ __global__ __launch_bounds__(64 * kPrefillNW, HD > 128 ? 1 : 2) void shared_kern
         a.part[rows * a.slots * HD + row_head * a.slots + slot] = first ? kMinit : m_run;  // (a wave without a window)
         a.part[rows * a.slots * (HD + 1) + row_head * a.slots + slot] = l;
     }
+    if (a.stats && live && hf == 0) {
+        a.stats[row_head] = m_run;
+        a.stats[rows + row_head] = l;
+    }
     __syncthreads();
     for (int x = threadIdx.x; x < kCols * V4; x += NT) {
         const int cl = x / V4, d = 4 * (x % V4), cg = c_blk + cl;
@@ -467,6 +472,26 @@ SharedPlan shared_plan(int n_seq, int n_tok, int G, int n_kv, int prefix_len, in
     return p;
 }
 
+// Pieces of a chunk's own keys where nothing else runs beside them: two jobs per CU, of 256 keys at least.
+static int lone_pieces(int64_t jobs, int own_max, int n_cu) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>(2 * n_cu / jobs, (own_max + 255) / 256));
+}
+
+SharedPlan own_plan(int n_seq, int n_tok, int G, int n_kv, int own_max, int n_cu) {
+    SharedPlan p;
+    p.n_blk = p.n_part = p.chunk = 0;
+    p.own_blk = (n_tok * G + kCols - 1) / kCols;
+    const int n = lone_pieces((int64_t)n_seq * p.own_blk * n_kv, own_max, n_cu);
+    p.own_chunk = ((own_max + n - 1) / n + kWin - 1) / kWin * kWin;
+    p.own_pieces = (own_max + p.own_chunk - 1) / p.own_chunk;
+    p.chain = p.own_pieces == 1;
+    return p;
+}
+
+int own_pieces_cap(int n_seq, int n_tok, int G, int n_kv, int own_max, int n_cu) {
+    return lone_pieces((int64_t)n_seq * ((n_tok * G + kCols - 1) / kCols) * n_kv, own_max, n_cu);
+}
+
 // One token: the own keys in splits of at least 512 (two rounds of a workgroup's windows), longer ones where
 // the batch has more than fill the chip.  One sequence of 16000 17.2 us, with 1024 20.5; two of 4000 15.3 and
 // 16.2; 16 of 700 to 1500 30.2 and 27.6.  With 256: 32 of 60 to 500 31.2 us, 30.2 with 512, else the same.
@@ -517,6 +542,7 @@ hipError_t launch_shared(const SharedCall &c, hipStream_t st) {
     a.softcap = c.softcap;
     a.part = c.part;
     a.out = c.out;
+    a.stats = c.plan.chain ? c.stats : nullptr;
     int own_jobs = a.own_blk * a.own_pieces * c.own.S;  // per kv head
     if (c.own_part) {
         DecodeArgs &d = a.dec;

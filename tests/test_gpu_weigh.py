@@ -106,7 +106,7 @@ def test_append_in_the_call(lens, heads, n_kv, hd, norm):
     b.check(out, b.w)
 
 
-@pytest.mark.parametrize("n_tok", [1])
+@pytest.mark.parametrize("n_tok", [1, 6, 150])
 @pytest.mark.parametrize("hd", [64, 128, 256])
 def test_what_is_not_seen_has_no_part(n_tok, hd):
     """Rows that a shortened sequence left behind, with infinite and NaN scales, change nothing."""
