@@ -36,6 +36,9 @@ struct DecodeArgs {
     // and the arrival counter of the kernel that does it, or null.
     int32_t *adv_len;
     int32_t *adv_ctr;
+
+    // Scores of every head and slot in the exp2 domain, [S][n_head][P] (the kernels with SCORES).
+    float *scores;
 };
 
 // Every workgroup of the launch's last kernel calls this once, after its last read of the
@@ -159,11 +162,12 @@ struct QLds {
 
 // live: this lane's column carries a head (n < 2G); lo_col: it carries the low parts (G <= n);
 // partner4: byte address (for ds_bpermute) of the lane holding the other part of its scores.
-template <int HD, bool SOFTCAP>
+// scores (SCORES): this lane's head's row.
+template <int HD, bool SOFTCAP, bool SCORES = false>
 __device__ __forceinline__ void process_window(const Window<HD> &w, WaveState<HD> &st,
                                                const QLds<HD> &qs, float *stage, int base, int end,
                                                int lane, int g, bool live, bool lo_col, int partner4,
-                                               float inv_s, float softcap, const DeqConst &dc) {
+                                               float inv_s, float softcap, const DeqConst &dc, float *scores = nullptr) {
     constexpr int WPG = HD / 32, NTD = HD / 16;
     // Scales: one per lane in registers -> this wave's LDS stage -> the 4 positions each lane
     // holds per tile (16kt + 4g + r).  Same-wave LDS traffic is ordered: no barrier needed.
@@ -211,6 +215,21 @@ __device__ __forceinline__ void process_window(const Window<HD> &w, WaveState<HD
         if (pos >= end) {
             x[i] = -INFINITY;
             sv[i] = 0.0f;
+        }
+    }
+    if constexpr (SCORES) {
+        if (live && !lo_col) {
+#pragma unroll
+            for (int kt = 0; kt < 4; kt++) {
+                const int pos = base + 16 * kt + 4 * g;
+                if (pos + 3 < end) {
+                    *reinterpret_cast<float4 *>(scores + pos) = make_float4(x[4 * kt], x[4 * kt + 1], x[4 * kt + 2], x[4 * kt + 3]);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (pos + r < end) scores[pos + r] = x[4 * kt + r];
+                }
+            }
         }
     }
     float xm = x[0], sm = sv[0];
@@ -467,6 +486,13 @@ __device__ inline void store_partial(const DecodeArgs &a, size_t head, int split
     }
 }
 
+// The reference and the sum alone, of a sequence that is not split (its output is whole already).
+__device__ inline void store_stats(const DecodeArgs &a, size_t head, int split, int HD, float M, float lsum) {
+    const size_t rows = (size_t)a.L.S * a.n_head * a.n_split, r = head * a.n_split + split;
+    a.ws[rows * HD + r] = M;
+    a.ws[rows * (HD + 1) + r] = lsum;
+}
+
 // LDS: q operands, per-wave scale stages; and the merge area, apart from them so that a
 // wave writes its share of the merge as soon as its windows are done.
 template <int HD, int NW>
@@ -493,12 +519,14 @@ __device__ __forceinline__ void decode_split(const DecodeArgs &a, int split_x, i
 #define TS_SPLIT_Z seq
 #define TS_SPLIT_LDS
 #define TS_SPLIT_KEEP true
+#define TS_SPLIT_SCORES false
 #include "ts_decode_split_body.h"
 #undef TS_SPLIT_X
 #undef TS_SPLIT_Y
 #undef TS_SPLIT_Z
 #undef TS_SPLIT_LDS
 #undef TS_SPLIT_KEEP
+#undef TS_SPLIT_SCORES
 }
 
 }  // namespace

@@ -4,7 +4,8 @@
 // slower (16 sequences of 2801-4403 256-dim positions, 26.7 -> 27.7 us).
 // In scope: HD, SOFTCAP, NORM, PAD, NW, a; TS_SPLIT_X, _Y, _Z: the split, the kv head and group of query
 // heads, the sequence; TS_SPLIT_LDS: declares sm (DecodeSplitSmem), kd, vd and xnew; TS_SPLIT_KEEP: partials
-// also of a sequence without a split (a flag in the arguments cost the decode kernels 2%).
+// also of a sequence without a split (a flag in the arguments cost the decode kernels 2%); TS_SPLIT_SCORES:
+// every score into a.scores, and the references and sums of sequences without a split.
     constexpr int SPAN = 64 * NW;     // positions one round of windows covers
     constexpr int WPG = HD / 32;   // K words per lane group = MFMA k-steps per 16-row tile
     constexpr int NTD = HD / 16;   // 16-dim output tiles
@@ -132,6 +133,7 @@
     st.m = kMinit;
     st.l = 0.0f;
     float *stage = sm.run.stage[wave];
+    float *const scores = TS_SPLIT_SCORES ? a.scores + ((size_t)s * a.n_head + hb + qhead) * L.P : nullptr;
 
     // Register double buffering: window i+1 is in flight while window i is computed.  One form
     // for every window, the tail mask included (a masked and an unmasked copy cost 70 VGPRs
@@ -142,7 +144,7 @@
         /* keep the prefetch here: the scheduler would otherwise sink it below CUR's use */     \
         asm volatile("" ::: "memory");                                                         \
         __builtin_amdgcn_sched_barrier(0);                                                     \
-        process_window<HD, SOFTCAP>(CUR, st, sm.run.q, stage, base, end, lane, g, live, lo_col, partner4, inv_s, a.softcap, dc); \
+        process_window<HD, SOFTCAP, TS_SPLIT_SCORES>(CUR, st, sm.run.q, stage, base, end, lane, g, live, lo_col, partner4, inv_s, a.softcap, dc, scores); \
         base += SPAN;                                                                           \
         if (base >= end) break;                                                                \
     }
@@ -192,6 +194,10 @@
             lsum += e;
         }
         const size_t head = (size_t)s * a.n_head + hb + hh;
+        if constexpr (TS_SPLIT_SCORES) {
+            if (fused && d == 0) a.scores[head * L.P + qpos] = xnew[hh];
+            if (n_split_s == 1 && d == 0) store_stats(a, head, split, HD, M, lsum);
+        }
         if (n_split_s == 1 && !TS_SPLIT_KEEP) {
             // hdr is a multiple of 8: a float4 of dims lies wholly inside or outside the row
             if (d < hdr) {

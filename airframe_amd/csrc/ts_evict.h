@@ -21,13 +21,16 @@ struct WeighCall {
     bool fresh;
     int n_cu;
     uint8_t *ws;
+    // one token: its K and V to append, or null; the sequence's length where the launch gives it (or -1)
+    const float *k_new, *v_new;
+    int hlen;
 };
+// One token.
+uint64_t weigh_token_workspace(int n_seq, int n_head, int n_kv, int P, int max_seq, int stored_hd, int n_cu);
+hipError_t launch_weigh_token(const WeighCall &c, const DecodePlan &plan, hipStream_t st);
 // Chunks (n_tok > 1).
 uint64_t weigh_chunk_workspace(int n_seq, int n_tok, int n_head, int n_kv, int stored_hd, int max_seq, int n_cu);
 hipError_t launch_weigh_chunk(const WeighCall &c, hipStream_t st);
-
-uint64_t weigh_workspace(int n_seq, int n_tok, int n_head, int stored_hd);
-hipError_t launch_weigh(const WeighCall &c, hipStream_t st);
 
 // Which slots stay: d_slots [n_layers][n_seq][H][keep] from w [n_layers][n_seq][H][max_seq].
 hipError_t launch_select(const float *w, const int32_t *d_len, int n_layers, int n_seq, int H, int max_seq, int keep,

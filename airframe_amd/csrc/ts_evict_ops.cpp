@@ -23,7 +23,7 @@ extern "C" {
 
 // (columns and launch sizes are 32-bit numbers)
 static bool weigh_shape_ok(const ts_kv *kv, int32_t n_head, int32_t n_tok) {
-    return kv && heads_ok(kv, n_head) && n_head <= 65536 && n_tok >= 0 && (int64_t)kv->d.n_seq * n_tok * n_head <= INT32_MAX / 64;
+    return kv && heads_ok(kv, n_head) && n_head / kv->d.n_head_kv <= 4096 && n_tok >= 0 && (int64_t)kv->d.n_seq * n_tok * n_head <= INT32_MAX / 64;
 }
 
 int ts_attn_weigh_workspace(const ts_kv *kv, int32_t n_head, int32_t n_tok, uint64_t *bytes) {
@@ -34,9 +34,7 @@ int ts_attn_weigh_workspace(const ts_kv *kv, int32_t n_head, int32_t n_tok, uint
         *bytes = weigh_chunk_workspace(kv->d.n_seq, n_tok, n_head, kv->d.n_head_kv, kv->hdp, kv->d.max_seq, kv->n_cu);
         return TS_OK;
     }
-    uint64_t dec = 0;
-    ts_attn_decode_workspace(kv, n_head, &dec);
-    *bytes = dec + weigh_workspace(kv->d.n_seq, n_tok, n_head, kv->hdp);
+    *bytes = weigh_token_workspace(kv->d.n_seq, n_head, kv->d.n_head_kv, kv->P, kv->d.max_seq, kv->hdp, kv->n_cu);
     return TS_OK;
 }
 
@@ -53,7 +51,7 @@ int ts_attn_weigh(ts_kv *kv, int32_t layer, const float *d_k, const float *d_v, 
     if ((int64_t)max_len + n_tok > kv->d.max_seq) return TS_ERR_OVERFLOW;
     const int rc = check_rope(rope, kv->d.head_dim, rot_end(kv, n_tok));
     if (rc) return rc;
-    uint64_t need = 0, dec = 0;
+    uint64_t need = 0;
     ts_attn_weigh_workspace(kv, n_head, n_tok, &need);
     if (!d_workspace || workspace_bytes < need) return TS_ERR_WORKSPACE;
     if (!aligned16(d_workspace)) return TS_ERR_INVALID;
@@ -84,12 +82,14 @@ int ts_attn_weigh(ts_kv *kv, int32_t layer, const float *d_k, const float *d_v, 
     c.n_cu = kv->n_cu;
     c.ws = static_cast<uint8_t *>(d_workspace);
     if (n_tok > 1) return hip_status(launch_weigh_chunk(c, as_stream(stream)));
-    ts_attn_decode_workspace(kv, n_head, &dec);
-    const int ra = d_k ? ts_attn_decode_append(kv, layer, d_k, d_v, d_q, n_head, rope, softcap, d_out, d_workspace, dec, stream)
-                       : ts_attn_decode(kv, layer, d_q, n_head, rope, softcap, d_out, d_workspace, dec, stream);
-    if (ra) return ra;
-    c.ws += dec;
-    return hip_status(launch_weigh(c, as_stream(stream)));
+    c.k_new = d_k;
+    c.v_new = d_v;
+    // (an eager call gives a lone sequence's length with the launch, as ts_attn_decode)
+    c.hlen = kv->d.n_seq == 1 && !c.captured ? kv->h_len[0] : -1;
+    for (int s = 0; s < kv->d.n_seq; s++) kv->h_ctx[s] = kv->h_len[s] + 1;
+    const DecodePlan plan = decode_plan(kv->h_ctx.data(), kv->d.n_seq, kv->d.n_head_kv, n_head / kv->d.n_head_kv, kv->n_cu,
+                                        kv->hdp, d_k != nullptr);
+    return hip_status(launch_weigh_token(c, plan, as_stream(stream)));
 }
 
 int ts_kv_select(const ts_kv *kv, const float *d_weights, int32_t keep, int32_t n_sink, int32_t n_recent, int32_t *d_slots,

@@ -518,7 +518,8 @@ int ts_attn_weigh_workspace(const ts_kv *kv, int32_t n_head, int32_t n_tok, uint
  * the softmax probabilities that it received from the tokens and the query heads of its kv head.  fresh 1:
  * the sums start at zero, and slots behind the newest token become 0; fresh 0: they are added to what is
  * there.  A slot that a token does not see receives nothing from it.  d_out, d_weights and the workspace are
- * apart from each other and from the inputs (TS_ERR_INVALID); n_seq * n_tok * n_head up to 2^25; the rope table
+ * apart from each other and from the inputs (TS_ERR_INVALID); n_seq * n_tok * n_head up to 2^25, up to 4096 query
+ * heads per kv head; the rope table
  * of a captured call has to cover the positions its replays reach.  d_workspace: ts_attn_weigh_workspace
  * bytes, 16-byte aligned. */
 int ts_attn_weigh(ts_kv *kv, int32_t layer, const float *d_k, const float *d_v, const float *d_q, int32_t n_head,
