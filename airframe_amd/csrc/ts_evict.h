@@ -32,9 +32,10 @@ hipError_t launch_weigh_token(const WeighCall &c, const DecodePlan &plan, hipStr
 uint64_t weigh_chunk_workspace(int n_seq, int n_tok, int n_head, int n_kv, int stored_hd, int max_seq, int n_cu);
 hipError_t launch_weigh_chunk(const WeighCall &c, hipStream_t st);
 
-// Which slots stay: d_slots [n_layers][n_seq][H][keep] from w [n_layers][n_seq][H][max_seq].
-hipError_t launch_select(const float *w, const int32_t *d_len, int n_layers, int n_seq, int H, int max_seq, int keep,
-                         int n_sink, int n_recent, int32_t *d_slots, hipStream_t st);
+// Which slots stay: d_slots [n_layers][n_seq][H][keep] from w [n_layers][n_seq][H][max_seq].  max_len: the longest
+// sequence as far as the host knows it (the choice of a kernel; any is right).
+hipError_t launch_select(const float *w, const int32_t *d_len, int max_len, int n_layers, int n_seq, int H, int max_seq,
+                         int keep, int n_sink, int n_recent, int32_t *d_slots, hipStream_t st);
 
 struct KeepCall {
     KvLayerView src, dst;  // layer 0 of each

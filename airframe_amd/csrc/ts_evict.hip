@@ -20,157 +20,318 @@ __device__ inline uint32_t order_key(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelThreads = 256;
-
-__device__ inline int block_sum(int v, int *s, int tid) {
+// Workgroup sums of one number per wave: the sum over the waves before this one, and over all.
+template <int NW>
+__device__ inline int wave_base(int mine, int *s, int wave, int lane, int &all) {
+    __syncthreads();
+    if (lane == 0) s[wave] = mine;
+    __syncthreads();
+    int base = 0;
+    all = 0;
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-    __syncthreads();
-    if ((tid & 63) == 0) s[tid >> 6] = v;
-    __syncthreads();
-    int sum = 0;
-    for (int i = 0; i < kSelThreads / 64; i++) sum += s[i];
-    return sum;
+    for (int i = 0; i < NW; i++) {
+        const int v = s[i];
+        base += i < wave ? v : 0;
+        all += v;
+    }
+    return base;
 }
 
-__global__ __launch_bounds__(kSelThreads) void select_kernel(const float *w, const int32_t *len, int n_seq, int H, int max_seq,
-                                                             int keep, int n_sink, int n_recent, int32_t *slots) {
-    __shared__ int s_sum[kSelThreads / 64], s_gt[kSelThreads / 64], s_eq[kSelThreads / 64];
+// One workgroup a row.  The keys stay in registers (of a row longer than NT * kSelPer they are read again
+// for every pass).  The `need`-th largest key is found in passes over ever smaller ranges of keys: a
+// histogram of kBins bins between the smallest and the largest, the bin that holds it, and so on into that bin,
+// until the bin is taken whole or holds one key only.  Keys are logarithmic in the weight, so a row's spread over
+// the bins also when a few slots hold most of the weight, and two passes nearly always do.
+constexpr int kSelPer = 16, kBins = 2048;
+
+template <int NT>
+__global__ __launch_bounds__(NT) void select_kernel(const float *w, const int32_t *len, int n_seq, int H, int max_seq, int keep,
+                                                    int n_sink, int n_recent, int32_t *slots) {
+    constexpr int NW = NT / 64, E = kSelPer, TILE = NT * E, BPT = kBins / NT;
+    __shared__ int hist[kBins], s_wave[NW], found[3];
+    __shared__ uint32_t s_min[NW], s_max[NW];
     const size_t row = blockIdx.x;
     const int s = (int)(row / H % n_seq), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int n = min(len[s], max_seq);
     w += row * max_seq;
     slots += row * keep;
     if (n <= keep) {
-        for (int j = tid; j < keep; j += kSelThreads) slots[j] = j < n ? j : -1;
+        for (int j = tid; j < keep; j += NT) slots[j] = j < n ? j : -1;
         return;
     }
-    const int lo = n_sink, hi = n - n_recent, need = keep - n_sink - n_recent;
-    // the need-th largest key: its bits from the highest down
-    uint32_t t = 0;
-    for (int b = 31; b >= 0 && need > 0; b--) {
-        const uint32_t c = t | 1u << b;
-        int cnt = 0;
-        for (int p = lo + tid; p < hi; p += kSelThreads) cnt += order_key(w[p]) >= c;
-        if (block_sum(cnt, s_sum, tid) >= need) t = c;
-    }
-    int above = 0;
-    for (int p = lo + tid; p < hi; p += kSelThreads) above += order_key(w[p]) > t;
-    const int ties = need > 0 ? need - block_sum(above, s_sum, tid) : 0;  // of those equal to it
-    int out = 0, eq = 0;
-    for (int p0 = 0; p0 < n; p0 += kSelThreads) {
-        const int p = p0 + tid;
-        const bool mid = p >= lo && p < hi;
-        const uint32_t k = mid && need > 0 ? order_key(w[p]) : 0;
-        const bool is_eq = mid && need > 0 && k == t, sure = p < n && (!mid || (need > 0 && k > t));
-        const uint64_t beq = __ballot(is_eq);
-        __syncthreads();
-        if (lane == 0) s_eq[wave] = __popcll(beq);
-        __syncthreads();
-        int rank = eq + __popcll(beq & ((1ull << lane) - 1));
-        for (int i = 0; i < wave; i++) rank += s_eq[i];
-        const bool take = sure || (is_eq && rank < ties);
-        const uint64_t bt = __ballot(take);
-        if (lane == 0) s_gt[wave] = __popcll(bt);
-        __syncthreads();
-        int at = out + __popcll(bt & ((1ull << lane) - 1));
-        for (int i = 0; i < wave; i++) at += s_gt[i];
-        if (take && at < keep) slots[at] = p;
-        for (int i = 0; i < kSelThreads / 64; i++) {
-            out += s_gt[i];
-            eq += s_eq[i];
+    const int lo = n_sink, hi = n - n_recent, tiles = (n + TILE - 1) / TILE;
+    int need = keep - n_sink - n_recent;
+    // element e of a tile: wave w holds slots 64 E w .. of it, in order
+    const int p_lane = wave * 64 * E + lane;
+    uint32_t k[E];
+    auto load = [&](int t) __attribute__((always_inline)) {
+        float x[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) x[e] = w[min(t * TILE + p_lane + 64 * e, n - 1)];
+#pragma unroll
+        for (int e = 0; e < E; e++) k[e] = order_key(x[e]);
+    };
+    auto mid = [&](int t, int e) __attribute__((always_inline)) {
+        return (unsigned)(t * TILE + p_lane + 64 * e - lo) < (unsigned)(hi - lo);
+    };
+    if (tiles == 1) load(0);
+    uint64_t sure = 0;      // keys from here on stay
+    uint32_t tie = 0;       // and the first `need` of this one
+    if (need > 0) {
+        uint32_t base = 0xFFFFFFFFu, top = 0;
+        for (int t = 0; t < tiles; t++) {
+            if (tiles > 1) load(t);
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (mid(t, e)) {
+                    base = min(base, k[e]);
+                    top = max(top, k[e]);
+                }
         }
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) {
+            base = min(base, (uint32_t)__shfl_xor((int)base, o, 64));
+            top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+        }
+        if (lane == 0) {
+            s_min[wave] = base;
+            s_max[wave] = top;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NW; i++) {
+            base = min(base, s_min[i]);
+            top = max(top, s_max[i]);
+        }
+        while (true) {
+            if (base == top) {
+                sure = (uint64_t)base + 1;
+                tie = base;
+                break;
+            }
+            const int shift = max(0, 32 - __clz(top - base) - 11);
+#pragma unroll
+            for (int i = 0; i < BPT; i++) hist[tid + NT * i] = 0;
+            __syncthreads();
+            for (int t = 0; t < tiles; t++) {
+                if (tiles > 1) load(t);
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (mid(t, e) && k[e] >= base && k[e] <= top) atomicAdd(&hist[(k[e] - base) >> shift], 1);
+            }
+            __syncthreads();
+            // thread t holds bins BPT t .. from the top one down
+            int c[BPT], sum = 0;
+#pragma unroll
+            for (int i = 0; i < BPT; i++) {
+                c[i] = hist[kBins - 1 - (BPT * tid + i)];
+                sum += c[i];
+            }
+            int upto = sum;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int v = __shfl_up(upto, o, 64);
+                upto += lane >= o ? v : 0;
+            }
+            int all;
+            int above = wave_base<NW>(__shfl(upto, 63, 64), s_wave, wave, lane, all) + upto - sum;
+            if (above < need && need <= above + sum) {
+#pragma unroll
+                for (int i = 0; i < BPT; i++) {
+                    if (above < need && need <= above + c[i]) {
+                        found[0] = kBins - 1 - (BPT * tid + i);
+                        found[1] = above;
+                        found[2] = c[i];
+                    }
+                    above += c[i];
+                }
+            }
+            __syncthreads();
+            const uint32_t from = base + ((uint32_t)found[0] << shift);
+            need -= found[1];
+            if (found[2] == need) {  // the whole bin
+                sure = from;
+                need = 0;
+                break;
+            }
+            top = from + min(top - from, (1u << shift) - 1);  // (from + 2^shift may pass 2^32)
+            base = from;
+        }
+    }
+    const uint64_t below = (1ull << lane) - 1;
+    int out = 0, ties = 0;
+    for (int t = 0; t < tiles; t++) {
+        if (tiles > 1) load(t);
+        uint32_t take = 0;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const int p = t * TILE + p_lane + 64 * e;
+            const bool m = mid(t, e);
+            take |= (uint32_t)(m ? keep > n_sink + n_recent && k[e] >= sure : p < n) << e;
+        }
+        if (need > 0) {  // (uniform)
+            int cnt = 0, all;
+#pragma unroll
+            for (int e = 0; e < E; e++) cnt += __popcll(__ballot(mid(t, e) && k[e] == tie));
+            int rank = ties + wave_base<NW>(cnt, s_wave, wave, lane, all);
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const bool eq = mid(t, e) && k[e] == tie;
+                const uint64_t b = __ballot(eq);
+                take |= (uint32_t)(eq && rank + __popcll(b & below) < need) << e;
+                rank += __popcll(b);
+            }
+            ties += all;
+        }
+        int cnt = 0, all;
+#pragma unroll
+        for (int e = 0; e < E; e++) cnt += __popcll(__ballot(take >> e & 1));
+        int at = out + wave_base<NW>(cnt, s_wave, wave, lane, all);
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const uint64_t b = __ballot(take >> e & 1);
+            const int j = at + __popcll(b & below);
+            if ((take >> e & 1) && j < keep) slots[j] = t * TILE + p_lane + 64 * e;
+            at += __popcll(b);
+        }
+        out += all;
     }
 }
 
 // ---- the rows ------------------------------------------------------------------------------------
 //
 // Slots are ascending, so a row never moves up: the source of slot j is j or a later one.  One wave
-// takes one slice of the rows of one (layer, sequence, kv head) and walks the slots in windows of 64:
+// takes one slice of the rows of one (layer, sequence, kv head) and walks the slots in windows:
 // it reads a window's sources before it writes the window, and no later window reads a slot that an
 // earlier one has written, so the move needs no second copy, also in place.  Slices: the K words of
-// each lane group g, 16-byte chunks of V's lane groups, the scales with the weights.
+// each lane group g, 16-byte chunks of V's lane groups, the scales with the weights; they share no
+// memory.  In place a slice is one wave's from its first slot to its last; into another cache the slots
+// are divided among waves too.
 
 template <int HD>
 constexpr int kKeepSlices = 4 + HD / 64 + 1;
+constexpr int kKeepPart = 128;  // slots of a wave that does not move in place
 
-template <int HD>
-__global__ __launch_bounds__(64) void keep_kernel(KeepCall a) {
-    const unsigned slice = blockIdx.x % kKeepSlices<HD>, row = blockIdx.x / kKeepSlices<HD>;
+// Windows of STEP slots from j0 to j1, D of them in registers: window i + D - 1 goes out before window i is
+// written, its slots' sources one window earlier.
+template <int STEP, int D, class Reg, class Source, class Load, class Store>
+__device__ __forceinline__ void walk(int j0, int j1, Source source, Load load, Store store) {
+    if (j0 >= j1) return;
+    Reg r[D];
+    int next = source(j0);
+#pragma unroll
+    for (int d = 0; d < D - 1; d++) {
+        const int now = next;
+        next = source(j0 + STEP * (d + 1));
+        if (j0 + STEP * d < j1) load(r[d], now);
+    }
+    int j = j0;
+    while (true) {
+#pragma unroll
+        for (int d = 0; d < D; d++) {
+            const int now = next;
+            next = source(j + STEP * D);
+            if (j + STEP * (D - 1) < j1) load(r[(d + D - 1) % D], now);
+            store(r[d], j);
+            j += STEP;
+            if (j >= j1) return;
+        }
+    }
+}
+
+template <int HD, bool IN_PLACE>
+__global__ __launch_bounds__(64) void keep_kernel(KeepCall a, int n_part) {
+    constexpr int NS = kKeepSlices<HD>;
+    const unsigned slice = blockIdx.x % NS, part = IN_PLACE ? 0 : blockIdx.x / NS % n_part;
+    const unsigned row = blockIdx.x / NS / (IN_PLACE ? 1 : n_part);
     const int lane = threadIdx.x, H = a.src.H;
     const int h = row % H, i = row / H % a.n_seq, layer = row / H / a.n_seq;
     const int len = min(a.src_len[a.src_seq + i], a.src_max), n = min(len, a.keep);
+    const int j0 = IN_PLACE ? 0 : part * kKeepPart, j1 = IN_PLACE ? n : min(n, j0 + kKeepPart);
     const size_t srow = (size_t)(a.src_seq + i) * H + h, drow = (size_t)(a.dst_seq + i) * H + h;
     const int sP = a.src.P, dP = a.dst.P;
     const int32_t *slots = a.slots + (size_t)row * a.slot_row;
     const size_t so = a.src_layer * layer, dof = a.dst_layer * layer;
     // (a slot outside the source reads one inside it)
-    auto source = [&](int j) { return j < n ? min(max(slots[j], 0), len - 1) : 0; };
+    auto source = [&](int j) __attribute__((always_inline)) { return j < n ? min(max(slots[j], 0), len - 1) : 0; };
     if (slice < 4) {
-        constexpr int W = HD / 32;  // words of a slot in lane group g
+        constexpr int W = HD / 32, V = W < 4 ? W : 4, NV = W / V;  // words of a slot in lane group g, in vectors
+        typedef uint32_t vec __attribute__((ext_vector_type(V)));
+        struct Reg { vec x[NV]; };
         const int g = slice;
         const uint32_t *src = reinterpret_cast<const uint32_t *>(a.src.kp + so + srow * sP * (HD / 2));
         uint32_t *dst = reinterpret_cast<uint32_t *>(a.dst.kp + dof + drow * dP * (HD / 2));
-        for (int j0 = 0; j0 < n; j0 += 64) {
-            const int j = j0 + lane, p = source(j);
-            uint32_t x[W];
+        walk<64, 4, Reg>(j0, j1, [&](int j) { return source(j + lane); },
+            [&](Reg &r, int p) {
 #pragma unroll
-            for (int e = 0; e < W; e++) x[e] = src[k_word_idx<HD>(p, 8 * (e >> 1) + 2 * g + (e & 1))];
-            if (j < n) {
+                for (int c = 0; c < NV; c++) r.x[c] = *reinterpret_cast<const vec *>(src + k_word_idx<HD>(p, 16 * c + 2 * g));
+            },
+            [&](const Reg &r, int j) {
+                if (j + lane < n) {
 #pragma unroll
-                for (int e = 0; e < W; e++) dst[k_word_idx<HD>(j, 8 * (e >> 1) + 2 * g + (e & 1))] = x[e];
-            }
-        }
+                    for (int c = 0; c < NV; c++) *reinterpret_cast<vec *>(dst + k_word_idx<HD>(j + lane, 16 * c + 2 * g)) = r.x[c];
+                }
+            });
     } else if (slice < 4 + HD / 64) {
-        const int td4 = slice - 4;
+        struct Reg { u32x4 x[8]; int p; };
+        const int td4 = slice - 4, g = lane >> 4, dl = lane & 15;
         const u32x4 *src = reinterpret_cast<const u32x4 *>(a.src.vp + so + srow * (sP / 32) * (HD * 16));
         u32x4 *dst = reinterpret_cast<u32x4 *>(a.dst.vp + dof + drow * (dP / 32) * (HD * 16));
-        const int g = lane >> 4, dl = lane & 15;
-        for (int j0 = 0; j0 < n; j0 += 32) {
-            const int mine = source(j0 + (lane & 31));
-            u32x4 x = {0, 0, 0, 0};
-            uint32_t left = 0;  // nibbles of slots from n on stay
+        // slot of nibble e of this lane's words, in a block of 32
+        auto slot = [&](int e) __attribute__((always_inline)) { return (e < 4 ? 0 : 16) + 4 * g + (e & 3); };
+        walk<32, 3, Reg>(j0, j1, [&](int j) { return source(j + (lane & 31)); },
+            [&](Reg &r, int mine) {
+                r.p = mine;
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int jj = (e < 4 ? 0 : 16) + 4 * g + (e & 3);
-                const int p = __shfl(mine, jj, 64), r = p & 31;
-                const u32x4 w = src[(size_t)(p >> 5) * HD + td4 * 64 + 16 * ((r & 15) >> 2) + dl];
-                const int sh = 4 * ((r & 3) + 4 * (r >> 4));
-                if (j0 + jj < n) {
-#pragma unroll
-                    for (int c = 0; c < 4; c++) x[c] |= (w[c] >> sh & 15) << (4 * e);
-                } else {
-                    left |= 15u << (4 * e);
+                for (int e = 0; e < 8; e++) {
+                    const int p = __shfl(mine, slot(e), 64);
+                    r.x[e] = src[(size_t)(p >> 5) * HD + td4 * 64 + 16 * ((p & 15) >> 2) + dl];
                 }
-            }
-            u32x4 *to = dst + (size_t)(j0 >> 5) * HD + td4 * 64 + lane;
-            if (left) {
-                const u32x4 old = *to;
+            },
+            [&](const Reg &r, int j) {
+                u32x4 x = {0, 0, 0, 0};
+                uint32_t left = 0;  // nibbles of slots from n on stay
 #pragma unroll
-                for (int c = 0; c < 4; c++) x[c] = (x[c] & ~left) | (old[c] & left);
-            }
-            *to = x;
-        }
+                for (int e = 0; e < 8; e++) {
+                    const int p = __shfl(r.p, slot(e), 64), sh = 4 * ((p & 3) + ((p & 16) >> 2));
+                    const bool in = j + slot(e) < n;
+                    left |= in ? 0 : 15u << (4 * e);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) x[c] |= (r.x[e][c] >> sh & 15) << (4 * e);
+                }
+                u32x4 *to = dst + (size_t)(j >> 5) * HD + td4 * 64 + lane;
+                if (left) {
+                    const u32x4 old = *to;
+#pragma unroll
+                    for (int c = 0; c < 4; c++) x[c] = (x[c] & ~left) | (old[c] & left);
+                }
+                *to = x;
+            });
     } else {
+        struct Reg { float k, v, w; };
         const float *ks = reinterpret_cast<const float *>(reinterpret_cast<const uint8_t *>(a.src.ks) + so) + srow * sP;
         const float *vs = reinterpret_cast<const float *>(reinterpret_cast<const uint8_t *>(a.src.vs) + so) + srow * sP;
         float *kd = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(a.dst.ks) + dof) + drow * dP;
         float *vd = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(a.dst.vs) + dof) + drow * dP;
         const float *ws = a.src_w ? a.src_w + ((size_t)layer * a.src.S * H + srow) * a.src_max : nullptr;
         float *wd = a.dst_w ? a.dst_w + ((size_t)layer * a.dst.S * H + drow) * a.dst_max : nullptr;
-        for (int j0 = 0; j0 < n; j0 += 64) {
-            const int j = j0 + lane, p = source(j);
-            const float k = ks[p], v = vs[p], w = wd ? ws[p] : 0.0f;
-            if (j < n) {
-                kd[j] = k;
-                vd[j] = v;
-                if (wd) wd[j] = w;
-            }
-        }
+        walk<64, 4, Reg>(j0, j1, [&](int j) { return source(j + lane); },
+            [&](Reg &r, int p) {
+                r.k = ks[p];
+                r.v = vs[p];
+                r.w = wd ? ws[p] : 0.0f;
+            },
+            [&](const Reg &r, int j) {
+                if (j + lane < n) {
+                    kd[j + lane] = r.k;
+                    vd[j + lane] = r.v;
+                    if (wd) wd[j + lane] = r.w;
+                }
+            });
         // slots behind the kept ones have received nothing
-        const int end = a.in_place ? len : a.dst_max;
+        const int end = IN_PLACE ? len : a.dst_max;
         if (wd)
-            for (int j = n + lane; j < end; j += 64) wd[j] = 0.0f;
+            for (int j = n + 64 * part + lane; j < end; j += 64 * (IN_PLACE ? 1 : n_part)) wd[j] = 0.0f;
     }
 }
 
@@ -185,17 +346,29 @@ __global__ void keep_len_kernel(KeepCall a) {
 
 }  // namespace
 
-hipError_t launch_select(const float *w, const int32_t *d_len, int n_layers, int n_seq, int H, int max_seq, int keep,
-                         int n_sink, int n_recent, int32_t *d_slots, hipStream_t st) {
-    select_kernel<<<(unsigned)(n_layers * n_seq * H), kSelThreads, 0, st>>>(w, d_len, n_seq, H, max_seq, keep, n_sink, n_recent, d_slots);
+hipError_t launch_select(const float *w, const int32_t *d_len, int max_len, int n_layers, int n_seq, int H, int max_seq,
+                         int keep, int n_sink, int n_recent, int32_t *d_slots, hipStream_t st) {
+    const unsigned rows = (unsigned)(n_layers * n_seq * H);
+    // A workgroup whose registers hold the longest row, and no larger: several of the smaller one share a CU.
+    if (max_len <= 256 * kSelPer)
+        select_kernel<256><<<rows, 256, 0, st>>>(w, d_len, n_seq, H, max_seq, keep, n_sink, n_recent, d_slots);
+    else
+        select_kernel<1024><<<rows, 1024, 0, st>>>(w, d_len, n_seq, H, max_seq, keep, n_sink, n_recent, d_slots);
     return hipGetLastError();
 }
 
 hipError_t launch_keep(const KeepCall &c, hipStream_t st) {
     const unsigned rows = (unsigned)(c.n_layers * c.n_seq * c.src.H);
-    if (c.src.hd == 256) keep_kernel<256><<<rows * kKeepSlices<256>, 64, 0, st>>>(c);
-    else if (c.src.hd == 128) keep_kernel<128><<<rows * kKeepSlices<128>, 64, 0, st>>>(c);
-    else keep_kernel<64><<<rows * kKeepSlices<64>, 64, 0, st>>>(c);
+    const int n_part = (c.keep + kKeepPart - 1) / kKeepPart;
+#define TS_KEEP(HDV)                                                                                          \
+    {                                                                                                         \
+        if (c.in_place) keep_kernel<HDV, true><<<rows * kKeepSlices<HDV>, 64, 0, st>>>(c, 1);                   \
+        else keep_kernel<HDV, false><<<rows * kKeepSlices<HDV> * n_part, 64, 0, st>>>(c, n_part);               \
+    }
+    if (c.src.hd == 256) TS_KEEP(256)
+    else if (c.src.hd == 128) TS_KEEP(128)
+    else TS_KEEP(64)
+#undef TS_KEEP
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     keep_len_kernel<<<(c.n_seq + 63) / 64, 64, 0, st>>>(c);

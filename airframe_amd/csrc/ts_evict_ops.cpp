@@ -100,7 +100,8 @@ int ts_kv_select(const ts_kv *kv, const float *d_weights, int32_t keep, int32_t 
     const uint64_t rows = (uint64_t)kv->d.n_layers * kv->d.n_seq * kv->d.n_head_kv;
     if (rows > INT32_MAX / 64) return TS_ERR_INVALID;
     if (shares(d_weights, weight_bytes(kv) * kv->d.n_layers, d_slots, rows * keep * sizeof(int32_t))) return TS_ERR_INVALID;
-    return hip_status(launch_select(d_weights, kv->d_len, kv->d.n_layers, kv->d.n_seq, kv->d.n_head_kv, kv->d.max_seq, keep,
+    const int max_len = *std::max_element(kv->h_len.begin(), kv->h_len.end());
+    return hip_status(launch_select(d_weights, kv->d_len, max_len, kv->d.n_layers, kv->d.n_seq, kv->d.n_head_kv, kv->d.max_seq, keep,
                                     n_sink, n_recent, d_slots, as_stream(stream)));
 }
 
@@ -115,7 +116,8 @@ int ts_kv_keep(ts_kv *dst, int32_t dst_seq, const ts_kv *src, int32_t src_seq, i
     const bool in_place = dst == src && dst_seq == src_seq;
     if (dst == src && !in_place && dst_seq < src_seq + n_seq && src_seq < dst_seq + n_seq) return TS_ERR_INVALID;
     const uint64_t rows = (uint64_t)src->d.n_layers * n_seq * src->d.n_head_kv, slot_bytes = rows * keep * sizeof(int32_t);
-    if (rows > INT32_MAX / 64) return TS_ERR_INVALID;
+    // (workgroups are 32-bit numbers)
+    if (rows * ((keep + 127) / 128) > INT32_MAX / 64) return TS_ERR_INVALID;
     const uint64_t sb = weight_bytes(src) * src->d.n_layers, db = weight_bytes(dst) * dst->d.n_layers;
     if (!(dst == src && d_weights == d_src_weights) && shares(d_src_weights, sb, d_weights, db)) return TS_ERR_INVALID;
     if (shares(d_slots, slot_bytes, d_weights, db)) return TS_ERR_INVALID;
