@@ -49,7 +49,7 @@ SOURCES = {
     "ts_weigh.hip": MFMA_VGPR,
     "ts_weigh_token.hip": MFMA_VGPR,
 }
-HEADERS = ["ts_internal.h", "ts_mfma.h", "ts_quant.h", "ts_store.h", "ts_gemm.h", "ts_gemv.h", "ts_kquant.h", "ts_host.h", "ts_packed.h", "ts_prompt.h", "ts_shared.h", "ts_evict.h", "ts_window.h", "ts_decode_split.h", "ts_decode_int.h", "ts_decode_split_body.h", os.path.join("..", "..", "include", "turboshimmy.h")]
+HEADERS = ["ts_internal.h", "ts_mfma.h", "ts_quant.h", "ts_store.h", "ts_gemm.h", "ts_gemv.h", "ts_kquant.h", "ts_host.h", "ts_packed.h", "ts_prompt.h", "ts_shared.h", "ts_evict.h", "ts_window.h", "ts_columns.h", "ts_decode_split.h", "ts_decode_int.h", "ts_decode_split_body.h", os.path.join("..", "..", "include", "turboshimmy.h")]
 
 
 def _compile(src: str, extra: list[str], objdir: str) -> str:

@@ -8,7 +8,8 @@ namespace ts {
 struct WeighCall {
     KvLayerView L;
     const int32_t *d_len;
-    int own_max;  // the longest sequence, the new tokens' slots included, as the host knows it
+    const int32_t *n_ctx;  // slots of every sequence with the new tokens', as the host knows them, and the most of them
+    int own_max;
     bool captured;  // (replays go past own_max)
     const float *q;
     int n_head, n_tok;

@@ -20,10 +20,26 @@ __device__ inline uint32_t order_key(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Workgroup sums of one number per wave: the sum over the waves before this one, and over all.
+// op over the 64 lanes of a wave, every lane getting the result: DPP within each 16-lane row, then two permlane swaps.
+template <int CTRL>
+__device__ inline uint32_t dpp_u(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
+}
+template <class Op>
+__device__ inline uint32_t wave_all(uint32_t v, Op op) {
+    v = op(v, dpp_u<0xB1>(v));   // quad_perm(1,0,3,2)
+    v = op(v, dpp_u<0x4E>(v));   // quad_perm(2,3,0,1)
+    v = op(v, dpp_u<0x141>(v));  // row_half_mirror
+    v = op(v, dpp_u<0x140>(v));  // row_mirror
+    auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = op(a[0], a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return op(b[0], b[1]);
+}
+
+// One number per wave: the sum over the waves before this one, and over all.  (A barrier between two calls.)
 template <int NW>
 __device__ inline int wave_base(int mine, int *s, int wave, int lane, int &all) {
-    __syncthreads();
     if (lane == 0) s[wave] = mine;
     __syncthreads();
     int base = 0;
@@ -37,164 +53,163 @@ __device__ inline int wave_base(int mine, int *s, int wave, int lane, int &all) 
     return base;
 }
 
-// One workgroup a row.  The keys stay in registers (of a row longer than NT * kSelPer they are read again
-// for every pass).  The `need`-th largest key is found in passes over ever smaller ranges of keys: a
-// histogram of kBins bins between the smallest and the largest, the bin that holds it, and so on into that bin,
-// until the bin is taken whole or holds one key only.  Keys are logarithmic in the weight, so a row's spread over
-// the bins also when a few slots hold most of the weight, and two passes nearly always do.
+// One workgroup a row; the slots between the first n_sink and the last n_recent compete.  Their keys stay in
+// registers (of a row longer than NT * kSelPer they are read again for every pass).  The `need`-th largest key is found in
+// passes over ever smaller ranges of keys: a histogram of kBins bins between the smallest and the largest, the bin that
+// holds it, and so on into that bin, until the bin is taken whole or holds one key only.  Keys are logarithmic in the
+// weight, so a row's spread over the bins also when a few slots hold most of the weight, and two passes nearly
+// always do.
 constexpr int kSelPer = 16, kBins = 2048;
 
 template <int NT>
-__global__ __launch_bounds__(NT) void select_kernel(const float *w, const int32_t *len, int n_seq, int H, int max_seq, int keep,
-                                                    int n_sink, int n_recent, int32_t *slots) {
+__global__ __launch_bounds__(NT, NT == 1024 ? 8 : 7) void select_kernel(const float *weights, const int32_t *len, int n_seq, int H, int max_seq,
+                                                       int keep, int n_sink, int n_recent, int32_t *slots) {
     constexpr int NW = NT / 64, E = kSelPer, TILE = NT * E, BPT = kBins / NT;
-    __shared__ int hist[kBins], s_wave[NW], found[3];
+    __shared__ int hist[kBins], s_wave[3][NW], found[3];
     __shared__ uint32_t s_min[NW], s_max[NW];
     const size_t row = blockIdx.x;
-    const int s = (int)(row / H % n_seq), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int s = (int)(row / H % n_seq), tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = min(len[s], max_seq);
-    w += row * max_seq;
     slots += row * keep;
     if (n <= keep) {
         for (int j = tid; j < keep; j += NT) slots[j] = j < n ? j : -1;
         return;
     }
-    const int lo = n_sink, hi = n - n_recent, tiles = (n + TILE - 1) / TILE;
+    const int m = n - n_sink - n_recent;  // slots that compete
     int need = keep - n_sink - n_recent;
-    // element e of a tile: wave w holds slots 64 E w .. of it, in order
-    const int p_lane = wave * 64 * E + lane;
+    for (int j = tid; j < n_sink; j += NT) slots[j] = j;
+    for (int j = tid; j < n_recent; j += NT) slots[keep - n_recent + j] = n - n_recent + j;
+    if (need == 0) return;
+    const __amdgpu_buffer_rsrc_t w =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(weights + row * max_seq + n_sink), (short)0, m * 4, 0x00020000);
+    const int tiles = (m + TILE - 1) / TILE;
+    // element e of a tile: wave w holds slots 64 E w .. of it, in order; 0, which is no key, past the last one
     uint32_t k[E];
+    const int p_lane = wave * 64 * E + lane;
     auto load = [&](int t) __attribute__((always_inline)) {
-        float x[E];
+        const int p = t * TILE + p_lane;
 #pragma unroll
-        for (int e = 0; e < E; e++) x[e] = w[min(t * TILE + p_lane + 64 * e, n - 1)];
+        for (int e = 0; e < E; e++) k[e] = __builtin_amdgcn_raw_buffer_load_b32(w, 4 * p + 256 * e, 0, 0);
 #pragma unroll
-        for (int e = 0; e < E; e++) k[e] = order_key(x[e]);
+        for (int e = 0; e < E; e++) k[e] = p + 64 * e < m ? order_key(__uint_as_float(k[e])) : 0;
     };
-    auto mid = [&](int t, int e) __attribute__((always_inline)) {
-        return (unsigned)(t * TILE + p_lane + 64 * e - lo) < (unsigned)(hi - lo);
-    };
-    if (tiles == 1) load(0);
-    uint64_t sure = 0;      // keys from here on stay
-    uint32_t tie = 0;       // and the first `need` of this one
-    if (need > 0) {
-        uint32_t base = 0xFFFFFFFFu, top = 0;
+    load(0);
+    uint32_t base = 0xFFFFFFFFu, top = 0;
+    for (int t = 0; t < tiles; t++) {
+        if (t > 0) load(t);
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            base = min(base, k[e] - 1);  // (0 becomes the largest)
+            top = max(top, k[e]);
+        }
+    }
+    base = wave_all(base, [](uint32_t a, uint32_t b) { return min(a, b); });
+    top = wave_all(top, [](uint32_t a, uint32_t b) { return max(a, b); });
+    if (lane == 0) {
+        s_min[wave] = base;
+        s_max[wave] = top;
+    }
+#pragma unroll
+    for (int i = 0; i < BPT; i++) hist[tid + NT * i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NW; i++) {
+        base = min(base, s_min[i]);
+        top = max(top, s_max[i]);
+    }
+    base++;
+    uint32_t tie = 0;   // the first `need` of this key stay,
+    uint32_t over = 0;  // and all above this one (at least 1 below the smallest key)
+    while (true) {
+        if (base == top) {
+            over = tie = base;
+            break;
+        }
+        const uint32_t span = top - base;
+        const int shift = max(0, 32 - __clz(span) - 11);
         for (int t = 0; t < tiles; t++) {
             if (tiles > 1) load(t);
 #pragma unroll
             for (int e = 0; e < E; e++)
-                if (mid(t, e)) {
-                    base = min(base, k[e]);
-                    top = max(top, k[e]);
-                }
-        }
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) {
-            base = min(base, (uint32_t)__shfl_xor((int)base, o, 64));
-            top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
-        }
-        if (lane == 0) {
-            s_min[wave] = base;
-            s_max[wave] = top;
+                if (k[e] - base <= span) atomicAdd(&hist[(k[e] - base) >> shift], 1);
         }
         __syncthreads();
+        // thread t holds bins BPT t .. from the top one down
+        int c[BPT], sum = 0;
 #pragma unroll
-        for (int i = 0; i < NW; i++) {
-            base = min(base, s_min[i]);
-            top = max(top, s_max[i]);
+        for (int i = 0; i < BPT; i++) {
+            int *b = &hist[kBins - 1 - (BPT * tid + i)];
+            c[i] = *b;
+            *b = 0;  // (for the next pass)
+            sum += c[i];
         }
-        while (true) {
-            if (base == top) {
-                sure = (uint64_t)base + 1;
-                tie = base;
-                break;
-            }
-            const int shift = max(0, 32 - __clz(top - base) - 11);
+        int upto = sum;
 #pragma unroll
-            for (int i = 0; i < BPT; i++) hist[tid + NT * i] = 0;
-            __syncthreads();
-            for (int t = 0; t < tiles; t++) {
-                if (tiles > 1) load(t);
-#pragma unroll
-                for (int e = 0; e < E; e++)
-                    if (mid(t, e) && k[e] >= base && k[e] <= top) atomicAdd(&hist[(k[e] - base) >> shift], 1);
-            }
-            __syncthreads();
-            // thread t holds bins BPT t .. from the top one down
-            int c[BPT], sum = 0;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(upto, o, 64);
+            upto += lane >= o ? v : 0;
+        }
+        int all;
+        int above = wave_base<NW>(__builtin_amdgcn_readlane(upto, 63), s_wave[0], wave, lane, all) + upto - sum;
+        if (above < need && need <= above + sum) {
 #pragma unroll
             for (int i = 0; i < BPT; i++) {
-                c[i] = hist[kBins - 1 - (BPT * tid + i)];
-                sum += c[i];
-            }
-            int upto = sum;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int v = __shfl_up(upto, o, 64);
-                upto += lane >= o ? v : 0;
-            }
-            int all;
-            int above = wave_base<NW>(__shfl(upto, 63, 64), s_wave, wave, lane, all) + upto - sum;
-            if (above < need && need <= above + sum) {
-#pragma unroll
-                for (int i = 0; i < BPT; i++) {
-                    if (above < need && need <= above + c[i]) {
-                        found[0] = kBins - 1 - (BPT * tid + i);
-                        found[1] = above;
-                        found[2] = c[i];
-                    }
-                    above += c[i];
+                if (above < need && need <= above + c[i]) {
+                    found[0] = kBins - 1 - (BPT * tid + i);
+                    found[1] = above;
+                    found[2] = c[i];
                 }
+                above += c[i];
             }
-            __syncthreads();
-            const uint32_t from = base + ((uint32_t)found[0] << shift);
-            need -= found[1];
-            if (found[2] == need) {  // the whole bin
-                sure = from;
-                need = 0;
-                break;
-            }
-            top = from + min(top - from, (1u << shift) - 1);  // (from + 2^shift may pass 2^32)
-            base = from;
         }
+        __syncthreads();
+        base += (uint32_t)found[0] << shift;
+        need -= found[1];
+        if (found[2] == need) {  // the whole bin
+            over = base - 1;
+            need = 0;
+            break;
+        }
+        top = base + min(top - base, (1u << shift) - 1);  // (base + 2^shift may pass 2^32)
     }
-    const uint64_t below = (1ull << lane) - 1;
+    slots += n_sink;
+    const int most = keep - n_sink - n_recent;
     int out = 0, ties = 0;
     for (int t = 0; t < tiles; t++) {
         if (tiles > 1) load(t);
         uint32_t take = 0;
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-            const int p = t * TILE + p_lane + 64 * e;
-            const bool m = mid(t, e);
-            take |= (uint32_t)(m ? keep > n_sink + n_recent && k[e] >= sure : p < n) << e;
-        }
+        for (int e = 0; e < E; e++) take |= (uint32_t)(k[e] > over) << e;
         if (need > 0) {  // (uniform)
-            int cnt = 0, all;
+            uint32_t eq = 0;
 #pragma unroll
-            for (int e = 0; e < E; e++) cnt += __popcll(__ballot(mid(t, e) && k[e] == tie));
-            int rank = ties + wave_base<NW>(cnt, s_wave, wave, lane, all);
+            for (int e = 0; e < E; e++) eq |= (uint32_t)(k[e] == tie) << e;
+            const int cnt = wave_all(__popc(eq), [](uint32_t a, uint32_t b) { return a + b; });
+            int all, rank = ties + wave_base<NW>(cnt, s_wave[1], wave, lane, all);
 #pragma unroll
             for (int e = 0; e < E; e++) {
-                const bool eq = mid(t, e) && k[e] == tie;
-                const uint64_t b = __ballot(eq);
-                take |= (uint32_t)(eq && rank + __popcll(b & below) < need) << e;
+                const bool mine = eq >> e & 1;
+                const uint64_t b = __ballot(mine);
+                const int r = rank + __builtin_amdgcn_mbcnt_hi(b >> 32, __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+                take |= (uint32_t)(mine && r < need) << e;
                 rank += __popcll(b);
             }
             ties += all;
         }
-        int cnt = 0, all;
-#pragma unroll
-        for (int e = 0; e < E; e++) cnt += __popcll(__ballot(take >> e & 1));
-        int at = out + wave_base<NW>(cnt, s_wave, wave, lane, all);
+        const int cnt = wave_all(__popc(take), [](uint32_t a, uint32_t b) { return a + b; });
+        int all, at = out + wave_base<NW>(cnt, s_wave[2], wave, lane, all);
+        const int p0 = n_sink + t * TILE + p_lane;
 #pragma unroll
         for (int e = 0; e < E; e++) {
-            const uint64_t b = __ballot(take >> e & 1);
-            const int j = at + __popcll(b & below);
-            if ((take >> e & 1) && j < keep) slots[j] = t * TILE + p_lane + 64 * e;
+            const bool mine = take >> e & 1;
+            const uint64_t b = __ballot(mine);
+            const int j = at + __builtin_amdgcn_mbcnt_hi(b >> 32, __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+            if (mine && j < most) slots[j] = p0 + 64 * e;
             at += __popcll(b);
         }
         out += all;
+        __syncthreads();  // (the waves' counts are read before the next tile's)
     }
 }
 

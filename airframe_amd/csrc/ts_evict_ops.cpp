@@ -66,6 +66,8 @@ int ts_attn_weigh(ts_kv *kv, int32_t layer, const float *d_k, const float *d_v, 
     WeighCall c;
     c.L = kv->layer(layer);
     c.d_len = kv->d_len;
+    for (int s = 0; s < kv->d.n_seq; s++) kv->h_ctx[s] = kv->h_len[s] + n_tok;
+    c.n_ctx = kv->h_ctx.data();
     c.own_max = max_len + n_tok;
     c.captured = capturing(stream) || kv->len_captured;
     c.q = d_q;
@@ -86,7 +88,6 @@ int ts_attn_weigh(ts_kv *kv, int32_t layer, const float *d_k, const float *d_v, 
     c.v_new = d_v;
     // (an eager call gives a lone sequence's length with the launch, as ts_attn_decode)
     c.hlen = kv->d.n_seq == 1 && !c.captured ? kv->h_len[0] : -1;
-    for (int s = 0; s < kv->d.n_seq; s++) kv->h_ctx[s] = kv->h_len[s] + 1;
     const DecodePlan plan = decode_plan(kv->h_ctx.data(), kv->d.n_seq, kv->d.n_head_kv, n_head / kv->d.n_head_kv, kv->n_cu,
                                         kv->hdp, d_k != nullptr);
     return hip_status(launch_weigh_token(c, plan, as_stream(stream)));
@@ -98,7 +99,7 @@ int ts_kv_select(const ts_kv *kv, const float *d_weights, int32_t keep, int32_t 
         !d_weights || !d_slots || !aligned4(d_weights) || !aligned4(d_slots))
         return TS_ERR_INVALID;
     const uint64_t rows = (uint64_t)kv->d.n_layers * kv->d.n_seq * kv->d.n_head_kv;
-    if (rows > INT32_MAX / 64) return TS_ERR_INVALID;
+    if (rows > INT32_MAX / 64 || kv->d.max_seq > (1 << 29)) return TS_ERR_INVALID;  // (a row's bytes are a 32-bit number)
     if (shares(d_weights, weight_bytes(kv) * kv->d.n_layers, d_slots, rows * keep * sizeof(int32_t))) return TS_ERR_INVALID;
     const int max_len = *std::max_element(kv->h_len.begin(), kv->h_len.end());
     return hip_status(launch_select(d_weights, kv->d_len, max_len, kv->d.n_layers, kv->d.n_seq, kv->d.n_head_kv, kv->d.max_seq, keep,

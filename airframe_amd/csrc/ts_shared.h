@@ -20,9 +20,9 @@ void shared_own_plan(const int32_t *n_ctx, int n_seq, int n_kv, int G, int n_cu,
 // The most partials a row has, of any prefix up to max_prefix and own keys up to own_max (0 for chains).
 int shared_slots_cap(int n_seq, int n_tok, int G, int n_kv, int max_prefix, int own_max, int n_cu);
 
-// The plan of a chunk over its own keys alone (no prefix; weighed attention): as many pieces as fill the chip, a
-// chain if that is one.  pieces_cap: the most of any own keys up to own_max.
-SharedPlan own_plan(int n_seq, int n_tok, int G, int n_kv, int own_max, int n_cu);
+// The plan of a chunk over its own keys alone (no prefix; weighed attention), n_ctx of them with the new tokens: as
+// many pieces as fill the chip, a chain if that is one.  own_pieces_cap: the most pieces of any lengths up to own_max.
+SharedPlan own_plan(const int32_t *n_ctx, int n_seq, int n_tok, int G, int n_kv, int n_cu);
 int own_pieces_cap(int n_seq, int n_tok, int G, int n_kv, int own_max, int n_cu);
 
 struct SharedCall {
@@ -45,8 +45,10 @@ struct SharedCall {
     int hlen;
     const float *k_new, *v_new;
     int n_cu;
-    // A chain's references and sums, [rows], [rows] (null: not wanted).
-    float *stats = nullptr;
+    // [n_seq][n_head_kv][n_blk32] ColBlock: the columns are left there too, a chain's with their log2 sums, and
+    // the partials of pieces are the caller's to join (null: not wanted).
+    void *cols = nullptr;
+    int n_blk32 = 0;
 };
 hipError_t launch_shared(const SharedCall &c, hipStream_t st);
 

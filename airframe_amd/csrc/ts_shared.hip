@@ -17,7 +17,7 @@
 #include "ts_shared.h"
 
 #include "ts_decode_split.h"
-#include "ts_window.h"
+#include "ts_columns.h"
 
 namespace ts {
 namespace {
@@ -37,7 +37,8 @@ struct SharedArgs {
     int slots;                 // partials per row: n_part, and own_pieces if own_blk
     float inv_sqrt_hd, softcap;
     float *part, *out;
-    float *stats;              // a chain's m and l per row, or null
+    void *cols;                // (COLS)
+    int n_blk32;
 };
 
 constexpr int kCols = kPrefillNW * kColsPerWave;
@@ -57,8 +58,8 @@ constexpr size_t shared_lds() {
 }
 
 // One job: 128 columns (token, head) of one kv head against a range of keys, in the window walk of
-// chunked prefill.
-template <int HD, bool SOFTCAP, bool NORM, bool PAD>
+// chunked prefill.  COLS (no prefix): the first piece's jobs leave their columns' operands in a.cols.
+template <int HD, bool SOFTCAP, bool NORM, bool PAD, bool COLS = false>
 __global__ __launch_bounds__(64 * kPrefillNW, HD > 128 ? 1 : 2) void shared_kernel(SharedArgs a) {
     constexpr int NW = kPrefillNW;
     constexpr int NKS = HD / 16, NDB = HD / 32, NG = NKS / 4, ROWB = HD / 2;
@@ -227,6 +228,22 @@ __global__ __launch_bounds__(64 * kPrefillNW, HD > 128 ? 1 : 2) void shared_kern
         }
         q_lo_terms(lo, ql1[g], ql2[g]);
     }
+    auto col_block = [&] { return static_cast<ColBlock<HD> *>(a.cols) + ((size_t)s_own * H + h) * a.n_blk32 + 4 * blk + wave; };
+    if constexpr (COLS) {
+        if (slot == 0 && c_wave < n_cols) {
+            ColBlock<HD> *to = col_block();
+#pragma unroll
+            for (int t = 0; t < NKS; t++) to->hi[t][lane] = qh[t];
+#pragma unroll
+            for (int g = 0; g < NG; g++)
+#pragma unroll
+                for (int e = 0; e < 3; e++) {
+                    to->lo[g][0][e][lane] = (uint32_t)ql1[g][2 * e] | (uint64_t)(uint32_t)ql1[g][2 * e + 1] << 32;
+                    to->lo[g][1][e][lane] = (uint32_t)ql2[g][2 * e] | (uint64_t)(uint32_t)ql2[g][2 * e + 1] << 32;
+                }
+            if (hf == 0) to->back[j] = q_back;
+        }
+    }
     __syncthreads();  // (the windows' tiles take q's place)
 
     floatx16 o[NDB];
@@ -332,9 +349,8 @@ __global__ __launch_bounds__(64 * kPrefillNW, HD > 128 ? 1 : 2) void shared_kern
         a.part[rows * a.slots * HD + row_head * a.slots + slot] = first ? kMinit : m_run;  // (a wave without a window)
         a.part[rows * a.slots * (HD + 1) + row_head * a.slots + slot] = l;
     }
-    if (a.stats && live && hf == 0) {
-        a.stats[row_head] = m_run;
-        a.stats[rows + row_head] = l;
+    if constexpr (COLS) {
+        if (a.chain && c_wave < n_cols && hf == 0) col_block()->lse[j] = m_run + __log2f(l);
     }
     __syncthreads();
     for (int x = threadIdx.x; x < kCols * V4; x += NT) {
@@ -472,24 +488,33 @@ SharedPlan shared_plan(int n_seq, int n_tok, int G, int n_kv, int prefix_len, in
     return p;
 }
 
-// Pieces of a chunk's own keys where nothing else runs beside them: two jobs per CU, of 256 keys at least.
-static int lone_pieces(int64_t jobs, int own_max, int n_cu) {
-    return (int)std::max<int64_t>(1, std::min<int64_t>(2 * n_cu / jobs, (own_max + 255) / 256));
+// Own keys alone: pieces of the same length, two jobs per CU over the batch's keys (a ragged batch's longest gets
+// more of them), of 256 keys at least and kMaxPieces n_cu / jobs at most (which bounds the partials' scratch);
+// one piece, a chain, once the blocks of columns fill the chip.
+static constexpr int64_t kMaxPieces = 8;
+
+int own_pieces_cap(int n_seq, int n_tok, int G, int n_kv, int own_max, int n_cu) {
+    const int64_t jobs = (int64_t)n_seq * ((n_tok * G + kCols - 1) / kCols) * n_kv;
+    if (jobs >= n_cu) return 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(kMaxPieces * n_cu / jobs, (own_max + 255) / 256));
 }
 
-SharedPlan own_plan(int n_seq, int n_tok, int G, int n_kv, int own_max, int n_cu) {
+SharedPlan own_plan(const int32_t *n_ctx, int n_seq, int n_tok, int G, int n_kv, int n_cu) {
     SharedPlan p;
     p.n_blk = p.n_part = p.chunk = 0;
     p.own_blk = (n_tok * G + kCols - 1) / kCols;
-    const int n = lone_pieces((int64_t)n_seq * p.own_blk * n_kv, own_max, n_cu);
-    p.own_chunk = ((own_max + n - 1) / n + kWin - 1) / kWin * kWin;
-    p.own_pieces = (own_max + p.own_chunk - 1) / p.own_chunk;
+    int64_t total = 0;
+    int most = 1;
+    for (int s = 0; s < n_seq; s++) {
+        total += n_ctx[s];
+        most = std::max(most, (int)n_ctx[s]);
+    }
+    const int64_t cap = own_pieces_cap(n_seq, n_tok, G, n_kv, most, n_cu);
+    const int64_t even = (total * p.own_blk * n_kv + 2 * n_cu - 1) / (2 * n_cu);
+    p.own_chunk = (int)((std::max<int64_t>(std::max<int64_t>(256, even), (most + cap - 1) / cap) + kWin - 1) / kWin * kWin);
+    p.own_pieces = cap == 1 ? 1 : (most + p.own_chunk - 1) / p.own_chunk;
     p.chain = p.own_pieces == 1;
     return p;
-}
-
-int own_pieces_cap(int n_seq, int n_tok, int G, int n_kv, int own_max, int n_cu) {
-    return lone_pieces((int64_t)n_seq * ((n_tok * G + kCols - 1) / kCols) * n_kv, own_max, n_cu);
 }
 
 // One token: the own keys in splits of at least 512 (two rounds of a workgroup's windows), longer ones where
@@ -542,7 +567,8 @@ hipError_t launch_shared(const SharedCall &c, hipStream_t st) {
     a.softcap = c.softcap;
     a.part = c.part;
     a.out = c.out;
-    a.stats = c.plan.chain ? c.stats : nullptr;
+    a.cols = c.cols;
+    a.n_blk32 = c.n_blk32;
     int own_jobs = a.own_blk * a.own_pieces * c.own.S;  // per kv head
     if (c.own_part) {
         DecodeArgs &d = a.dec;
@@ -573,10 +599,10 @@ hipError_t launch_shared(const SharedCall &c, hipStream_t st) {
     {                                                                                                \
         constexpr size_t lds = shared_lds<HDV>();                                                    \
         static_assert(lds <= 156 * 1024, "a workgroup's windows fit a CU's LDS");                     \
+        auto kernel = c.cols ? shared_kernel<HDV, SC, NM, PD, true> : shared_kernel<HDV, SC, NM, PD>; \
         if (lds > 64 * 1024)                                                                         \
-            (void)hipFuncSetAttribute((const void *)shared_kernel<HDV, SC, NM, PD>,                  \
-                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);         \
-        shared_kernel<HDV, SC, NM, PD><<<jobs, 64 * kPrefillNW, lds, st>>>(a);                       \
+            (void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds); \
+        kernel<<<jobs, 64 * kPrefillNW, lds, st>>>(a);                                               \
     }
 #define TS_SH2(HDV, PD)                                                                              \
     {                                                                                                \
@@ -591,7 +617,7 @@ hipError_t launch_shared(const SharedCall &c, hipStream_t st) {
 #undef TS_SH2
 #undef TS_SH3
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || a.chain) return e;
+    if (e != hipSuccess || a.chain || c.cols) return e;
     JoinArgs ja;
     ja.part = c.part;
     ja.own = c.own_part;

@@ -3,140 +3,324 @@
 // For the new tokens t and query heads h of one kv head, P[t,h,p] = softmax over the slots p the token
 // sees: w[p] = (w[p]) + sum over t and h of P[t,h,p].  The sums over columns need each softmax's final
 // reference and sum, so they come behind the attention itself (one token: ts_weigh_token.hip).
+//
+// A chunk: the attention itself is the window walk of ts_shared.hip over the own keys.  It leaves its columns' rotated q
+// in the operand layout of the matrix cores, and every column's log2 sum lse, its own or (of pieces of the keys)
+// the join's.  Then the scores are computed a second time with the keys held in registers and the columns streaming
+// past, so that a slot's sum stays in its lane: w[p] += sum over the columns of 2^(x - lse).
+#include "ts_columns.h"
 #include "ts_evict.h"
 #include "ts_shared.h"
-#include "ts_window.h"
 
 namespace ts {
-
-// The attention itself is the window walk of ts_shared.hip over the own keys (its outputs, and every
-// column's reference and sum).  Then the columns' rotated q goes into the operand layout of the matrix
-// cores once (weigh_prep_kernel), and the scores are computed a second time with the keys held in registers
-// and the columns streaming past (weigh_cols_kernel), so that a slot's sum stays in its lane.
 namespace {
-
-constexpr int kColBlk = 32;  // columns of one operand block
-
-// One block: q's high halves [k-step][lane][16 bytes], its low terms [group][term][3][lane][8 bytes], then
-// q's scale back and the softmax's log2 sum of each column.
-template <int HD>
-struct ColBlock {
-    half8 hi[HD / 16][64];
-    uint64_t lo[HD / 64][2][3][64];
-    float back[kColBlk], lse[kColBlk];
-};
 
 struct ChunkArgs {
     KvLayerView L;
     const int32_t *len;
-    const float *q, *rope;
-    int rope_pairs, rope_rows, n_head, G, n_tok, n_blk32;
-    float inv_sqrt_hd, softcap;
-    const float *pm, *pl;  // references and sums of the walk, [rows][slots]
-    int slots;
+    int n_head, G, n_tok, n_blk32;
+    float softcap;
+    const float *part;  // of pieces: [rows][slots][HD], references and sums [rows][slots]
+    int slots, own_chunk;
+    float *out;
     void *cols;  // [S][H][n_blk32] ColBlock
     int max_seq;
     float *w;
     bool fresh;
+    int tiles;  // weigh_window_kernel: tiles of keys per workgroup
 };
 
-// 128 columns (token, head) of one kv head and sequence.
-template <int HD, bool NORM, bool PAD>
-__global__ __launch_bounds__(256) void weigh_prep_kernel(ChunkArgs a) {
-    constexpr int NKS = HD / 16, NG = NKS / 4, V4 = HD / 4, QST = HD + 4, BC = 128, NQ = BC * V4 / 256;
-    extern __shared__ __align__(16) unsigned char prep_smem[];
-    float *const qs = reinterpret_cast<float *>(prep_smem);
-    const int h = blockIdx.y, s = blockIdx.z, G = a.G, hdr = PAD ? a.L.hdr : HD, n_cols = a.n_tok * G;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, j = lane & 31, hf = lane >> 5;
-    const int c_blk = blockIdx.x * BC, len = a.len[s];
-    const float *const QN = NORM ? a.L.qn : nullptr;
-    const float qmul = a.softcap > 0.0f ? a.inv_sqrt_hd : a.inv_sqrt_hd * kLog2e;
-#pragma unroll 4
-    for (int i = 0; i < NQ; i++) {
-        const int at = tid + 256 * i, cl = at / V4, d = 4 * (at % V4);
-        const int cg = c_blk + cl, ce = min(cg, n_cols - 1), tok = ce / G;
-        const float *qrow = a.q + (((size_t)s * a.n_tok + tok) * a.n_head + h * G + ce % G) * hdr;
-        float4 v = keep4(cg < n_cols && d < hdr, *reinterpret_cast<const float4 *>(qrow + (d < hdr ? d : 0)));
-        if (QN) {
-            float ss = v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w;
+// The join of one (token, head) row's pieces by a wave, lane l holding HD / 64 dims: the output, and the row's lse into its
+// column.
+template <int HD>
+__global__ __launch_bounds__(256) void weigh_join_kernel(ChunkArgs a) {
+    constexpr int D = HD / 64;
+    const int lane = threadIdx.x & 63, H = a.L.H, G = a.G;
+    // (rows of one kv head on the XCD that wrote their parts)
+    const int h = blockIdx.x % H, u = blockIdx.x / H * 4 + (threadIdx.x >> 6), rows = a.L.S * a.n_tok * a.n_head;
+    if (u >= rows / H) return;
+    const int t = u / G, g = u - t * G, s = t / a.n_tok, tok = t - s * a.n_tok, row = t * a.n_head + h * G + g;
+    const int n = min((min(a.len[s] + a.n_tok, a.L.P) + a.own_chunk - 1) / a.own_chunk, a.slots);
+    const float *po = a.part + (size_t)row * a.slots * HD, *pm = a.part + (size_t)rows * a.slots * HD + (size_t)row * a.slots;
+    const float *pl = pm + (size_t)rows * a.slots;
+    float M = kMinit;
+    for (int i = lane; i < n; i += 64) M = fmaxf(M, pm[i]);
+    M = wave_max(M);
+    float acc[D] = {}, l = 0.0f;
+    for (int i0 = 0; i0 < n; i0 += 8) {
+        float x[8][D], m[8], ls[8];
 #pragma unroll
-            for (int o = 1; o < V4; o <<= 1) ss += __shfl_xor(ss, o, 64);
-            const float ns = qk_norm_scale_from_sum(ss, hdr, a.L.norm_eps);
-            const float4 w = *reinterpret_cast<const float4 *>(QN + (d < hdr ? d : 0));
-            v = make_float4(qk_norm_apply(v.x, ns, w.x), qk_norm_apply(v.y, ns, w.y), qk_norm_apply(v.z, ns, w.z),
-                            qk_norm_apply(v.w, ns, w.w));
+        for (int k = 0; k < 8; k++) {
+            const int i = min(i0 + k, n - 1);
+#pragma unroll
+            for (int e = 0; e < D; e++) x[k][e] = po[(size_t)i * HD + D * lane + e];
+            m[k] = pm[i];
+            ls[k] = pl[i];
         }
-        const float *rot = a.rope + (size_t)min(rot_of(a.L, s, len + tok), a.rope_rows - 1) * a.rope_pairs * 2;
-        if (d / 2 < a.rope_pairs) rope_rotate(v.x, v.y, *reinterpret_cast<const float2 *>(rot + d));
-        if (d / 2 + 1 < a.rope_pairs) rope_rotate(v.z, v.w, *reinterpret_cast<const float2 *>(rot + d + 2));
-        *reinterpret_cast<float4 *>(qs + cl * QST + d) = v;
-    }
-    __syncthreads();
-    const int b32 = blockIdx.x * 4 + wave;
-    if (b32 >= a.n_blk32) return;
-    ColBlock<HD> &out = static_cast<ColBlock<HD> *>(a.cols)[((size_t)s * a.L.H + h) * a.n_blk32 + b32];
-    const float *const qrow = qs + (32 * wave + j) * QST;
-    float mc = 0.0f;
 #pragma unroll
-    for (int t = 0; t < NKS; t++) {
+        for (int k = 0; k < 8; k++) {
+            if (i0 + k >= n) break;
+            if (ls[k] == 0.0f) continue;  // (a piece without keys has no output; one of a NaN q has)
+            const float e2 = __builtin_amdgcn_exp2f(m[k] - M);
 #pragma unroll
-        for (int e = 0; e < 8; e++) mc = fmaxf(mc, fabsf(qrow[8 * (2 * t + hf) + e]));
-    }
-    float q_s, q_back;
-    q_scale(half_max(mc) * qmul, q_s, q_back);
-#pragma unroll
-    for (int g = 0; g < NG; g++) {
-        float lo[32];
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int t = 4 * g + u;
-            const float *src = qrow + 8 * (2 * t + hf);
-            half8 hi;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float v = opaque(src[kPerm[e]] * (qmul * q_s));
-                const _Float16 x = (_Float16)v;
-                hi[e] = x;
-                lo[8 * u + e] = v - (float)x;
-            }
-            out.hi[t][lane] = hi;
-        }
-        int6v t1, t2;
-        q_lo_terms(lo, t1, t2);
-#pragma unroll
-        for (int e = 0; e < 3; e++) {
-            out.lo[g][0][e][lane] = (uint32_t)t1[2 * e] | (uint64_t)(uint32_t)t1[2 * e + 1] << 32;
-            out.lo[g][1][e][lane] = (uint32_t)t2[2 * e] | (uint64_t)(uint32_t)t2[2 * e + 1] << 32;
+            for (int e = 0; e < D; e++) acc[e] += e2 * x[k][e];
+            l += e2 * ls[k];
         }
     }
-    // the softmax's log2 sum over all pieces of the walk
-    const int c = c_blk + 32 * wave + j, ce = min(c, n_cols - 1);
-    const size_t row = ((size_t)s * a.n_tok + ce / G) * a.n_head + h * G + ce % G;
-    float M = kMinit, l = 0.0f;
-    for (int i = 0; i < a.slots; i++) M = fmaxf(M, a.pm[row * a.slots + i]);
-    for (int i = 0; i < a.slots; i++) {
-        const float li = a.pl[row * a.slots + i];
-        l += li == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(a.pm[row * a.slots + i] - M) * li;
-    }
-    if (hf == 0) {
-        out.back[j] = q_back;
-        out.lse[j] = M + __log2f(l);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    float *o = a.out + (size_t)row * a.L.hdr;
+#pragma unroll
+    for (int e = 0; e < D; e++)
+        if (D * lane + e < a.L.hdr) o[D * lane + e] = acc[e] * inv;
+    const int c = tok * G + g;
+    if (lane == 0)
+        static_cast<ColBlock<HD> *>(a.cols)[((size_t)s * H + h) * a.n_blk32 + c / kColBlk].lse[c % kColBlk] = M + __log2f(l);
+}
+
+// A wave's tile: NT x 32 keys as the matrix cores' first operand (row j of part i is key 32 i + j), the codes in f16 and fp6.
+template <int HD>
+struct KeyTile {
+    static constexpr int NT = HD > 128 ? 1 : 2, KEYS = 32 * NT, NKS = HD / 16, NG = NKS / 4;
+    static constexpr int V = HD / 32 < 4 ? HD / 32 : 4, NV = HD / 32 / V;  // words of a slot and lane group, in vectors
+    typedef uint32_t vec __attribute__((ext_vector_type(V)));
+    typedef half8 F16[NT][NKS];
+    typedef int6v F6[NT][NG];
+    typedef vec Raw[NT][4][NV];
+};
+
+// Slots base .. of one stream (past P: slot P - 1).
+template <int HD>
+__device__ __forceinline__ void fetch_keys(typename KeyTile<HD>::Raw &r, const uint32_t *kw, int P, int base, int j) {
+    using T = KeyTile<HD>;
+#pragma unroll
+    for (int i = 0; i < T::NT; i++) {
+        const int p = min(base + 32 * i + j, P - 1);
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+#pragma unroll
+            for (int c = 0; c < T::NV; c++)
+                r[i][g][c] = *reinterpret_cast<const typename T::vec *>(kw + k_word_idx<HD>(p, 16 * c + 2 * g));
     }
 }
 
-// Slots of one (sequence, kv head) in blocks of KEYS: wave w of each group of four holds KEYS / 4 keys as
-// matrix operands in registers; the two groups take every second column block.  Grid: kv head first, so that the
-// workgroups that read one head's columns share an XCD where the heads divide the XCDs.
+// k-step t takes word 2 t + hf of the slot: lane group t % 4, word 2 (t / 4) + hf of its words.
 template <int HD>
-constexpr int kColKeys = HD > 128 ? 128 : 256;
+__device__ __forceinline__ void set_keys(const typename KeyTile<HD>::Raw &r, typename KeyTile<HD>::F16 &ka,
+                                         typename KeyTile<HD>::F6 &k6, int hf, const DeqConst &dk) {
+    using T = KeyTile<HD>;
+#pragma unroll
+    for (int i = 0; i < T::NT; i++) {
+#pragma unroll
+        for (int g = 0; g < T::NG; g++) {
+            // (the fp6 operand element by element: as a copy of four half8 the compiler keeps all of ka in memory)
+            half32 all;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int t = 4 * g + u, at = 2 * g % T::V;
+                const typename T::vec v = r[i][u][2 * g / T::V];
+                const uint32_t w0 = v[at], w1 = v[at + 1];
+                const half8 x = dequant8_c(hf ? w1 : w0, dk);
+                ka[i][t] = x;
+#pragma unroll
+                for (int e = 0; e < 8; e++) all[8 * u + e] = x[e];
+            }
+            k6[i][g] = __builtin_amdgcn_cvt_scalef32_pk32_fp6_f16(all, 1.0f);
+        }
+    }
+    // (pinned: the compiler would otherwise keep the codes and unpack them for every column block)
+#pragma unroll
+    for (int i = 0; i < T::NT; i++) {
+#pragma unroll
+        for (int t = 0; t < T::NKS; t++) {
+            u32x4 x = __builtin_bit_cast(u32x4, ka[i][t]);
+            asm volatile("" : "+v"(x));
+            ka[i][t] = __builtin_bit_cast(half8, x);
+        }
+#pragma unroll
+        for (int g = 0; g < T::NG; g++) asm volatile("" : "+v"(k6[i][g]));
+    }
+}
 
+// Scores of one column block: lane (j, hf) holds column j and keys 32 i + 8 (e / 4) + 4 hf + e % 4.
+template <int HD>
+__device__ __forceinline__ void tile_scores(const typename KeyTile<HD>::F16 &ka, const typename KeyTile<HD>::F6 &k6,
+                                            const ColBlock<HD> &b, int lane, floatx16 (&sc)[KeyTile<HD>::NT]) {
+    using T = KeyTile<HD>;
+#pragma unroll
+    for (int i = 0; i < T::NT; i++) sc[i] = (floatx16)0.0f;
+#pragma unroll
+    for (int t = 0; t < T::NKS; t++) {
+        const half8 q = b.hi[t][lane];
+#pragma unroll
+        for (int i = 0; i < T::NT; i++) sc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[i][t], q, sc[i], 0, 0, 0);
+    }
+#pragma unroll
+    for (int g = 0; g < T::NG; g++)
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            int6v q;
+#pragma unroll
+            for (int e = 0; e < 3; e++) {
+                const uint64_t x = b.lo[g][u][e][lane];
+                q[2 * e] = (int)(uint32_t)x;
+                q[2 * e + 1] = (int)(x >> 32);
+            }
+#pragma unroll
+            for (int i = 0; i < T::NT; i++) sc[i] = mfma_lo6(k6[i][g], q, sc[i], u ? kQlo2E8 : kQlo1E8);
+        }
+    // the columns' reads run four ahead of the matrix instructions that take them
+    constexpr int READS = T::NKS + 3 * T::NG, MFMAS = T::NT * (T::NKS + 2 * T::NG);
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (int k = 0; k < READS - 4; k++) {
+        __builtin_amdgcn_sched_group_barrier(0x8, T::NT, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, MFMAS, 0);
+}
+
+// Probabilities of one column block added to acc.  sk: the tile's K scales in LDS; cb: the block, of n_cols columns in
+// all; base: the tile's first key.
 template <int HD, bool SOFTCAP>
-__global__ __launch_bounds__(512, 2) void weigh_cols_kernel(ChunkArgs a) {
-    constexpr int KEYS = kColKeys<HD>, NT = KEYS / 128, NKS = HD / 16, NG = NKS / 4;  // NT: tiles of 32 keys per wave
-    extern __shared__ __align__(16) unsigned char cols_smem[];
+__device__ __forceinline__ void add_probs(floatx16 (&sc)[KeyTile<HD>::NT], float (&acc)[KeyTile<HD>::NT][16], const ColBlock<HD> &b,
+                                          const float *sk, int cb, int n_cols, int G, int len, int base, int j, int hf,
+                                          float softcap) {
+    constexpr int NT = KeyTile<HD>::NT;
+    const float back = b.back[j], lse = b.lse[j];
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const floatx4 s4 = *reinterpret_cast<const floatx4 *>(sk + 32 * i + 8 * q + 4 * hf);
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                float x = sc[i][4 * q + r] * s4[r];
+                if constexpr (SOFTCAP) x = tanhf(x * back / softcap) * softcap * kLog2e - lse;
+                else x = __builtin_fmaf(x, back, -lse);
+                sc[i][4 * q + r] = __builtin_amdgcn_exp2f(x);
+            }
+        }
+    // (uniform: some column of the block does not see some key of the tile)
+    if (base + 32 * NT - 1 > len + kColBlk * cb / G || kColBlk * (cb + 1) > n_cols) {
+        asm volatile("");  // (a branch: the compares are the rare case)
+        const int c = kColBlk * cb + j;
+        const int qpos = c < n_cols ? len + c / G : -1;  // the last slot the column sees
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                if (base + 32 * i + 8 * (e >> 2) + 4 * hf + (e & 3) > qpos) sc[i][e] = 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) acc[i][e] += sc[i][e];
+}
+
+// The sums over the 32 columns' lanes into the tile's row of LDS.
+template <int HD>
+__device__ __forceinline__ void sum_columns(const float (&acc)[KeyTile<HD>::NT][16], float *row, int j, int hf) {
+#pragma unroll
+    for (int i = 0; i < KeyTile<HD>::NT; i++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            float v = acc[i][e];
+            v += dpp_f<0xB1>(v);
+            v += dpp_f<0x4E>(v);
+            v += dpp_f<0x141>(v);
+            v += dpp_f<0x140>(v);
+            auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+            v = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+            if (j == 0) row[32 * i + 8 * (e >> 2) + 4 * hf + (e & 3)] = v;
+        }
+}
+
+constexpr int kWaves = 8;  // of a workgroup
+
+// Few columns: all of them in LDS, and every wave takes tiles of keys of its own, the next one's codes on their way.
+// No barrier but the one behind the columns.  Grid: kv head first, so that the workgroups that read one head's
+// columns share an XCD where the heads divide the XCDs.
+template <int HD, bool SOFTCAP>
+__global__ __launch_bounds__(64 * kWaves, 2) void weigh_window_kernel(ChunkArgs a) {
+    using Tile = KeyTile<HD>;
     using Block = ColBlock<HD>;
+    constexpr int NT = Tile::NT, KEYS = Tile::KEYS;
+    extern __shared__ __align__(16) unsigned char win_smem[];
+    Block *const blk = reinterpret_cast<Block *>(win_smem);  // [n_blk32]
+    __shared__ __align__(16) float sks[kWaves][KEYS], sums[kWaves][KEYS];
+    const int H = a.L.H, h = blockIdx.x % H, s = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 63, j = lane & 31, hf = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const size_t st = (size_t)s * H + h;
+    const int len = a.len[s], n = len + a.n_tok, n_cols = a.n_tok * a.G;
+    const int first = blockIdx.x / H * a.tiles, last = first + a.tiles;
+    float *const w = a.w + st * a.max_seq;
+    if (n > a.max_seq) return;  // (a graph replayed past the capacity)
+    const float *ks = a.L.ks + st * a.L.P;
+    const uint32_t *const kw = reinterpret_cast<const uint32_t *>(a.L.kp + st * a.L.P * (HD / 2));
+    typename Tile::Raw raw;
+    float scale = 0.0f;
+    auto fetch = [&](int tile) __attribute__((always_inline)) {
+        fetch_keys<HD>(raw, kw, a.L.P, tile * KEYS, j);
+        scale = ks[min(tile * KEYS + (lane & (KEYS - 1)), a.L.P - 1)];
+    };
+    if (first * KEYS < n) {
+        fetch(min(first + wave, (n - 1) / KEYS));
+        const u32x4 *src = reinterpret_cast<const u32x4 *>(static_cast<const Block *>(a.cols) + st * a.n_blk32);
+        u32x4 *to = reinterpret_cast<u32x4 *>(blk);
+        const int pieces = a.n_blk32 * (int)(sizeof(Block) / 16);
+#pragma unroll 4
+        for (int i = tid; i < pieces; i += 64 * kWaves) to[i] = src[i];
+    }
+    __syncthreads();
+    const DeqConstV dk;
+    for (int tile = first + wave; tile < last; tile += kWaves) {
+        const int base = tile * KEYS, p = base + lane;
+        if (base >= a.max_seq) break;
+        const bool mine = lane < KEYS && p < a.max_seq;
+        if (base >= n) {
+            if (a.fresh && mine) w[p] = 0.0f;
+            continue;
+        }
+        const float old = !a.fresh && mine && p < n ? w[p] : 0.0f;
+        typename Tile::F16 ka;
+        typename Tile::F6 k6;
+        set_keys<HD>(raw, ka, k6, hf, dk);
+        sks[wave][lane & (KEYS - 1)] = scale;
+        fetch(min(tile + kWaves, (n - 1) / KEYS));
+        asm volatile("" ::: "memory");
+        float acc[NT][16];
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[i][e] = 0.0f;
+        // (the first columns that see a key of the tile; all blocks behind them do too)
+        for (int cb = max(0, base - len) * a.G / kColBlk; cb < a.n_blk32; cb++) {
+            floatx16 sc[NT];
+            tile_scores<HD>(ka, k6, blk[cb], lane, sc);
+            add_probs<HD, SOFTCAP>(sc, acc, blk[cb], sks[wave], cb, n_cols, a.G, len, base, j, hf, a.softcap);
+        }
+        sum_columns<HD>(acc, sums[wave], j, hf);
+        asm volatile("" ::: "memory");  // (the wave's LDS writes are ordered before its reads)
+        if (mine) {
+            const float v = sums[wave][lane & (KEYS - 1)];
+            if (p < n) w[p] = old + v;
+            else if (a.fresh) w[p] = 0.0f;
+        }
+    }
+}
+
+// Many columns: four waves hold four tiles of keys for as long as the columns stream past through LDS; the workgroup's
+// two groups of four take every second column block.  (With the groups half a step apart, one's matrix instructions
+// beside the other's exponentials: 70 us, 68 without, 512 tokens of 4 sequences of 1-1.5K slots.)
+template <int HD, bool SOFTCAP>
+__global__ __launch_bounds__(64 * kWaves, 2) void weigh_cols_kernel(ChunkArgs a) {
+    using Tile = KeyTile<HD>;
+    using Block = ColBlock<HD>;
+    constexpr int NT = Tile::NT, TK = Tile::KEYS, KEYS = 4 * TK;
+    extern __shared__ __align__(16) unsigned char cols_smem[];
     Block *const buf = reinterpret_cast<Block *>(cols_smem);  // [group][2]
-    __shared__ float part[2][KEYS];
+    __shared__ __align__(16) float part[2][KEYS], sks[KEYS];
     const int H = a.L.H, h = blockIdx.x % H, kb = blockIdx.x / H, s = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 63, j = lane & 31, hf = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), grp = wave >> 2, wk = wave & 3;
@@ -146,10 +330,10 @@ __global__ __launch_bounds__(512, 2) void weigh_cols_kernel(ChunkArgs a) {
     if (n > a.max_seq) return;  // (a graph replayed past the capacity)
     if (key0 >= n) {
         if (a.fresh)
-            for (int p = key0 + tid; p < min(key0 + KEYS, a.max_seq); p += 512) w[p] = 0.0f;
+            for (int p = key0 + tid; p < min(key0 + KEYS, a.max_seq); p += 64 * kWaves) w[p] = 0.0f;
         return;
     }
-    const int base = key0 + wk * (KEYS / 4), n_cols = a.n_tok * a.G;
+    const int base = key0 + wk * TK, n_cols = a.n_tok * a.G;
     // (the first columns that see a key of the block; all blocks behind them do too)
     const int first = max(0, key0 - len) * a.G / kColBlk;
     const int n_it = (a.n_blk32 - first + 1) / 2;
@@ -170,27 +354,14 @@ __global__ __launch_bounds__(512, 2) void weigh_cols_kernel(ChunkArgs a) {
             if ((tid & 255) + 256 * i < PIECES) p[(tid & 255) + 256 * i] = next[i];
     };
     fetch(0);
-    // this wave's keys: row j of tile i is key base + 32 i + j
-    half8 ka[NT][NKS];
-    int6v k6[NT][NG];
-    float sk[NT][16];
+    typename Tile::F16 ka;
+    typename Tile::F6 k6;
     {
         const DeqConstV dk;
-        const uint32_t *kw = reinterpret_cast<const uint32_t *>(a.L.kp + st * a.L.P * (HD / 2));
-        const float *ks = a.L.ks + st * a.L.P;
-#pragma unroll
-        for (int i = 0; i < NT; i++) {
-            const int p = min(base + 32 * i + j, a.L.P - 1);
-#pragma unroll
-            for (int t = 0; t < NKS; t++) ka[i][t] = dequant8_c(kw[k_word_idx<HD>(p, 2 * t + hf)], dk);
-#pragma unroll
-            for (int g = 0; g < NG; g++) {
-                const half8 x[4] = {ka[i][4 * g], ka[i][4 * g + 1], ka[i][4 * g + 2], ka[i][4 * g + 3]};
-                k6[i][g] = fp6_of(x, 1.0f);
-            }
-#pragma unroll
-            for (int e = 0; e < 16; e++) sk[i][e] = ks[min(base + 32 * i + 8 * (e >> 2) + 4 * hf + (e & 3), a.L.P - 1)];
-        }
+        typename Tile::Raw raw;
+        fetch_keys<HD>(raw, reinterpret_cast<const uint32_t *>(a.L.kp + st * a.L.P * (HD / 2)), a.L.P, base, j);
+        if (tid < KEYS) sks[tid] = a.L.ks[st * a.L.P + min(key0 + tid, a.L.P - 1)];
+        set_keys<HD>(raw, ka, k6, hf, dk);
     }
     float acc[NT][16];
 #pragma unroll
@@ -202,80 +373,18 @@ __global__ __launch_bounds__(512, 2) void weigh_cols_kernel(ChunkArgs a) {
     __syncthreads();
     for (int it = 0; it < n_it; it++) {
         const Block &b = buf[2 * grp + (it & 1)];
+        const int cb = first + 2 * it + grp;
+        floatx16 sc[NT];
+        tile_scores<HD>(ka, k6, b, lane, sc);
         if (it + 1 < n_it) stage(it + 1);
         if (it + 2 < n_it) fetch(it + 2);
-        const int cb = first + 2 * it + grp;
-        if (cb < a.n_blk32) {
-            floatx16 sc[NT];
-#pragma unroll
-            for (int i = 0; i < NT; i++) sc[i] = (floatx16)0.0f;
-#pragma unroll
-            for (int t = 0; t < NKS; t++) {
-                const half8 q = b.hi[t][lane];
-#pragma unroll
-                for (int i = 0; i < NT; i++) sc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[i][t], q, sc[i], 0, 0, 0);
-            }
-#pragma unroll
-            for (int g = 0; g < NG; g++)
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    int6v q;
-#pragma unroll
-                    for (int e = 0; e < 3; e++) {
-                        const uint64_t x = b.lo[g][u][e][lane];
-                        q[2 * e] = (int)(uint32_t)x;
-                        q[2 * e + 1] = (int)(x >> 32);
-                    }
-#pragma unroll
-                    for (int i = 0; i < NT; i++) sc[i] = mfma_lo6(k6[i][g], q, sc[i], u ? kQlo2E8 : kQlo1E8);
-                }
-            const float back = b.back[j], lse = b.lse[j];
-            const int c = kColBlk * cb + j;
-            const int qpos = c < n_cols ? len + c / a.G : -1;  // the last slot the column sees
-            // (uniform: some column of the block does not see some key of the wave)
-            const bool mask = base + KEYS / 4 - 1 > len + kColBlk * cb / a.G || kColBlk * (cb + 1) > n_cols;
-#pragma unroll
-            for (int i = 0; i < NT; i++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    float x = sc[i][e] * sk[i][e];
-                    if constexpr (SOFTCAP) {
-                        x = tanhf(x * back / a.softcap) * a.softcap * kLog2e - lse;
-                    } else {
-                        x = __builtin_fmaf(x, back, -lse);
-                    }
-                    sc[i][e] = __builtin_amdgcn_exp2f(x);
-                }
-            if (mask) {
-#pragma unroll
-                for (int i = 0; i < NT; i++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        if (base + 32 * i + 8 * (e >> 2) + 4 * hf + (e & 3) > qpos) sc[i][e] = 0.0f;
-            }
-#pragma unroll
-            for (int i = 0; i < NT; i++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) acc[i][e] += sc[i][e];
-        }
+        // (a block behind the last has no columns: nothing is added)
+        add_probs<HD, SOFTCAP>(sc, acc, b, sks + wk * TK, cb, n_cols, a.G, len, base, j, hf, a.softcap);
         __syncthreads();
     }
-    // the sums of the 32 columns' lanes
-#pragma unroll
-    for (int i = 0; i < NT; i++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-            float v = acc[i][e];
-            v += dpp_f<0xB1>(v);
-            v += dpp_f<0x4E>(v);
-            v += dpp_f<0x141>(v);
-            v += dpp_f<0x140>(v);
-            auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-            v = __uint_as_float(x[0]) + __uint_as_float(x[1]);
-            if (j == 0) part[grp][wk * (KEYS / 4) + 32 * i + 8 * (e >> 2) + 4 * hf + (e & 3)] = v;
-        }
+    sum_columns<HD>(acc, part[grp] + wk * TK, j, hf);
     __syncthreads();
-    for (int x = tid; x < KEYS; x += 512) {
+    for (int x = tid; x < KEYS; x += 64 * kWaves) {
         const int p = key0 + x;
         if (p >= a.max_seq) break;
         const float v = part[0][x] + part[1][x];
@@ -286,20 +395,22 @@ __global__ __launch_bounds__(512, 2) void weigh_cols_kernel(ChunkArgs a) {
     }
 }
 
-uint64_t col_block_bytes(int hd) {
+size_t col_block_bytes(int hd) {
     return hd == 256 ? sizeof(ColBlock<256>) : hd == 128 ? sizeof(ColBlock<128>) : sizeof(ColBlock<64>);
 }
 
-uint64_t part_floats(int rows, int pieces, int hd) { return pieces > 1 ? (uint64_t)rows * pieces * (hd + 2) : (uint64_t)rows * 2; }
+uint64_t part_bytes(uint64_t rows, int pieces, int hd) { return pieces > 1 ? (rows * pieces * (hd + 2) * sizeof(float) + 15) / 16 * 16 : 0; }
+
+// The columns' blocks and the waves' rows in a CU's LDS.
+constexpr size_t kWindowLds = 150 * 1024;
 
 }  // namespace
 
 uint64_t weigh_chunk_workspace(int n_seq, int n_tok, int n_head, int n_kv, int stored_hd, int max_seq, int n_cu) {
-    const int G = n_head / n_kv, rows = n_seq * n_tok * n_head;
-    // (a chain of a call whose longest sequence is short needs less than pieces do, one piece's sums alone)
-    const uint64_t parts = part_floats(rows, own_pieces_cap(n_seq, n_tok, G, n_kv, max_seq, n_cu), stored_hd) * sizeof(float);
+    const int G = n_head / n_kv;
     const uint64_t blocks = (uint64_t)n_seq * n_kv * ((n_tok * G + kColBlk - 1) / kColBlk);
-    return (parts + 15) / 16 * 16 + blocks * col_block_bytes(stored_hd);
+    return part_bytes((uint64_t)n_seq * n_tok * n_head, own_pieces_cap(n_seq, n_tok, G, n_kv, max_seq, n_cu), stored_hd) +
+           blocks * col_block_bytes(stored_hd);
 }
 
 hipError_t launch_weigh_chunk(const WeighCall &c, hipStream_t st) {
@@ -316,53 +427,51 @@ hipError_t launch_weigh_chunk(const WeighCall &c, hipStream_t st) {
     sc.rope_rows = c.rope_rows;
     sc.softcap = c.softcap;
     sc.out = c.out;
-    sc.plan = own_plan(c.L.S, c.n_tok, G, c.L.H, c.own_max, c.n_cu);
+    sc.plan = own_plan(c.n_ctx, c.L.S, c.n_tok, G, c.L.H, c.n_cu);
     sc.part = reinterpret_cast<float *>(c.ws);
     sc.own_part = nullptr;
     sc.own_chunk = sc.own_split = 1;
     sc.hlen = -1;
     sc.k_new = sc.v_new = nullptr;
     sc.n_cu = c.n_cu;
-    sc.stats = sc.part;
+    sc.cols = c.ws + part_bytes(rows, sc.plan.own_pieces, c.L.hd);
+    sc.n_blk32 = (c.n_tok * G + kColBlk - 1) / kColBlk;
     const hipError_t e = launch_shared(sc, st);
     if (e != hipSuccess) return e;
-    const uint64_t parts = part_floats(rows, sc.plan.own_pieces, c.L.hd) * sizeof(float);
 
     ChunkArgs a;
     a.L = c.L;
     a.len = c.d_len;
-    a.q = c.q;
-    a.rope = c.rope;
-    a.rope_pairs = c.rope_pairs;
-    a.rope_rows = c.rope_rows;
     a.n_head = c.n_head;
     a.G = G;
     a.n_tok = c.n_tok;
-    a.n_blk32 = (c.n_tok * G + kColBlk - 1) / kColBlk;
-    a.inv_sqrt_hd = 1.0f / sqrtf((float)c.L.hdr);
+    a.n_blk32 = sc.n_blk32;
     a.softcap = c.softcap;
+    a.part = sc.part;
     a.slots = sc.plan.own_pieces;
-    a.pm = sc.plan.chain ? sc.part : sc.part + (size_t)rows * a.slots * c.L.hd;
-    a.pl = a.pm + (size_t)rows * a.slots;
-    a.cols = c.ws + (parts + 15) / 16 * 16;
+    a.own_chunk = sc.plan.own_chunk;
+    a.out = c.out;
+    a.cols = sc.cols;
     a.max_seq = c.max_seq;
     a.w = c.w;
     a.fresh = c.fresh;
-    const dim3 prep((a.n_blk32 + 3) / 4, c.L.H, c.L.S);
     const int slots = c.fresh || c.captured ? c.max_seq : c.own_max;
-    const bool norm = c.L.qn != nullptr, pad = c.L.hdr != c.L.hd;
-#define TS_COLS(HDV)                                                                                                     \
-    {                                                                                                                    \
-        constexpr size_t lp = (size_t)128 * (HDV + 4) * sizeof(float), lc = 4 * sizeof(ColBlock<HDV>);                     \
-        static_assert(lc <= 156 * 1024 && lp <= 156 * 1024, "LDS of the column kernels");                                 \
-        auto prep_k = norm ? (pad ? weigh_prep_kernel<HDV, true, true> : weigh_prep_kernel<HDV, true, false>)             \
-                           : (pad ? weigh_prep_kernel<HDV, false, true> : weigh_prep_kernel<HDV, false, false>);          \
-        auto cols_k = c.softcap > 0.0f ? weigh_cols_kernel<HDV, true> : weigh_cols_kernel<HDV, false>;                    \
-        (void)hipFuncSetAttribute((const void *)prep_k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lp);             \
-        (void)hipFuncSetAttribute((const void *)cols_k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lc);             \
-        prep_k<<<prep, 256, lp, st>>>(a);                                                                                 \
-        const dim3 grid((unsigned)((slots + kColKeys<HDV> - 1) / kColKeys<HDV> * c.L.H), c.L.S);                          \
-        cols_k<<<grid, 512, lc, st>>>(a);                                                                                 \
+    const bool window = a.n_blk32 * col_block_bytes(c.L.hd) <= kWindowLds;
+    // tiles of keys per workgroup: one for every wave at least, and a workgroup per CU over the batch's keys
+    const int tk = c.L.hd > 128 ? 32 : 64;
+    int64_t total = 0;
+    for (int s = 0; s < c.L.S; s++) total += (c.n_ctx[s] + tk - 1) / tk;
+    a.tiles = (int)(((total * c.L.H + c.n_cu - 1) / c.n_cu + kWaves - 1) / kWaves * kWaves);
+#define TS_COLS(HDV)                                                                                                  \
+    {                                                                                                                 \
+        if (!sc.plan.chain) weigh_join_kernel<HDV><<<(unsigned)((rows / c.L.H + 3) / 4 * c.L.H), 256, 0, st>>>(a);      \
+        constexpr int TK = KeyTile<HDV>::KEYS;                                                                        \
+        auto kernel = window ? (c.softcap > 0.0f ? weigh_window_kernel<HDV, true> : weigh_window_kernel<HDV, false>)   \
+                             : (c.softcap > 0.0f ? weigh_cols_kernel<HDV, true> : weigh_cols_kernel<HDV, false>);      \
+        const int lds = (int)sizeof(ColBlock<HDV>) * (window ? a.n_blk32 : 4), per = window ? TK * a.tiles : 4 * TK;   \
+        (void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,                    \
+                                  window ? (int)kWindowLds : lds);                                                    \
+        kernel<<<dim3((unsigned)((slots + per - 1) / per * c.L.H), c.L.S), 64 * kWaves, lds, st>>>(a);                 \
     }
     if (c.L.hd == 256) TS_COLS(256)
     else if (c.L.hd == 128) TS_COLS(128)
