@@ -14,10 +14,9 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // unsigned keys in their order (-0 as 0, NaN above all).
 
 __device__ inline uint32_t order_key(float w) {
-    const uint32_t u = __float_as_uint(w);
-    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return 0xFFFFFFFFu;
-    if (u == 0x80000000u) return 0x80000000u;
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+    const uint32_t u = __float_as_uint(w + 0.0f);  // (-0 + 0 is 0)
+    const uint32_t k = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+    return w != w ? 0xFFFFFFFFu : k;
 }
 
 // op over the 64 lanes of a wave, every lane getting the result: DPP within each 16-lane row, then two permlane swaps.
@@ -37,20 +36,25 @@ __device__ inline uint32_t wave_all(uint32_t v, Op op) {
     return op(b[0], b[1]);
 }
 
+// The sum over the lanes up to this one.
+__device__ inline int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr 1, 2, 4, 8: within 16 lanes
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast 15 into rows 1 and 3, 31 into 2 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+
 // One number per wave: the sum over the waves before this one, and over all.  (A barrier between two calls.)
 template <int NW>
 __device__ inline int wave_base(int mine, int *s, int wave, int lane, int &all) {
     if (lane == 0) s[wave] = mine;
     __syncthreads();
-    int base = 0;
-    all = 0;
-#pragma unroll
-    for (int i = 0; i < NW; i++) {
-        const int v = s[i];
-        base += i < wave ? v : 0;
-        all += v;
-    }
-    return base;
+    const int v = wave_scan(lane < NW ? s[lane] : 0);
+    all = __builtin_amdgcn_readlane(v, NW - 1);
+    return wave > 0 ? __builtin_amdgcn_readlane(v, wave - 1) : 0;
 }
 
 // One workgroup a row; the slots between the first n_sink and the last n_recent compete.  Their keys stay in
@@ -84,15 +88,18 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 8 : 7) void select_kernel(const fl
     const __amdgpu_buffer_rsrc_t w =
         __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(weights + row * max_seq + n_sink), (short)0, m * 4, 0x00020000);
     const int tiles = (m + TILE - 1) / TILE;
-    // element e of a tile: wave w holds slots 64 E w .. of it, in order; 0, which is no key, past the last one
+    // thread i of a tile holds slots E i .., in order; 0, which is no key, past the last one
     uint32_t k[E];
-    const int p_lane = wave * 64 * E + lane;
     auto load = [&](int t) __attribute__((always_inline)) {
-        const int p = t * TILE + p_lane;
+        const int p = t * TILE + tid * E;
 #pragma unroll
-        for (int e = 0; e < E; e++) k[e] = __builtin_amdgcn_raw_buffer_load_b32(w, 4 * p + 256 * e, 0, 0);
+        for (int e = 0; e < E; e += 4) {
+            const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(w, 4 * p + 4 * e, 0, 0);
 #pragma unroll
-        for (int e = 0; e < E; e++) k[e] = p + 64 * e < m ? order_key(__uint_as_float(k[e])) : 0;
+            for (int c = 0; c < 4; c++) k[e + c] = x[c];
+        }
+#pragma unroll
+        for (int e = 0; e < E; e++) k[e] = p + e < m ? order_key(__uint_as_float(k[e])) : 0;
     };
     load(0);
     uint32_t base = 0xFFFFFFFFu, top = 0;
@@ -144,12 +151,7 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 8 : 7) void select_kernel(const fl
             *b = 0;  // (for the next pass)
             sum += c[i];
         }
-        int upto = sum;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(upto, o, 64);
-            upto += lane >= o ? v : 0;
-        }
+        const int upto = wave_scan(sum);
         int all;
         int above = wave_base<NW>(__builtin_amdgcn_readlane(upto, 63), s_wave[0], wave, lane, all) + upto - sum;
         if (above < need && need <= above + sum) {
@@ -185,29 +187,17 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 8 : 7) void select_kernel(const fl
             uint32_t eq = 0;
 #pragma unroll
             for (int e = 0; e < E; e++) eq |= (uint32_t)(k[e] == tie) << e;
-            const int cnt = wave_all(__popc(eq), [](uint32_t a, uint32_t b) { return a + b; });
-            int all, rank = ties + wave_base<NW>(cnt, s_wave[1], wave, lane, all);
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                const bool mine = eq >> e & 1;
-                const uint64_t b = __ballot(mine);
-                const int r = rank + __builtin_amdgcn_mbcnt_hi(b >> 32, __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
-                take |= (uint32_t)(mine && r < need) << e;
-                rank += __popcll(b);
-            }
+            const int upto = wave_scan(__popc(eq));
+            int all, rank = ties + upto - __popc(eq);
+            rank += wave_base<NW>(__builtin_amdgcn_readlane(upto, 63), s_wave[1], wave, lane, all);
+            for (; eq && rank < need; eq &= eq - 1, rank++) take |= eq & -eq;
             ties += all;
         }
-        const int cnt = wave_all(__popc(take), [](uint32_t a, uint32_t b) { return a + b; });
-        int all, at = out + wave_base<NW>(cnt, s_wave[2], wave, lane, all);
-        const int p0 = n_sink + t * TILE + p_lane;
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            const bool mine = take >> e & 1;
-            const uint64_t b = __ballot(mine);
-            const int j = at + __builtin_amdgcn_mbcnt_hi(b >> 32, __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
-            if (mine && j < most) slots[j] = p0 + 64 * e;
-            at += __popcll(b);
-        }
+        const int upto = wave_scan(__popc(take));
+        int all, at = out + upto - __popc(take);
+        at += wave_base<NW>(__builtin_amdgcn_readlane(upto, 63), s_wave[2], wave, lane, all);
+        const int p0 = n_sink + t * TILE + tid * E;
+        for (; take && at < most; take &= take - 1) slots[at++] = p0 + __builtin_ctz(take);
         out += all;
         __syncthreads();  // (the waves' counts are read before the next tile's)
     }
