@@ -352,7 +352,9 @@ hipError_t launch_decode(const KvLayerView &L, int32_t *d_len, const int32_t *h_
     a.ws = ws;
     a.k_new = k_new;
     a.v_new = v_new;
-    a.scores = nullptr;
+    a.scores = a.w = nullptr;
+    a.max_seq = 0;
+    a.fresh = false;
     // with a split the combine kernel advances the lengths (the last of its workgroups to
     // arrive); without one a length update follows the decode launch
     // (the 16x16 kernel does it itself when there is no split)

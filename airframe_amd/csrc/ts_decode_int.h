@@ -387,6 +387,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void decode_split4_kernel(DecodeAr
     __shared__ float mm_[NW][4 * GH], ml_[NW][4 * GH];
     __shared__ __align__(16) float kd[HD], vd[HD];
     __shared__ float xnew[4 * GH * HG < 8 ? 8 : 4 * GH * HG];
+    __shared__ float lse_s[SCORES ? 16 : 1];
     __shared__ int32_t qsum[NW][GH][16];  // per wave and half: digit sums of the 16 q rows
     __shared__ float qinv_s[NW][GH][4];   // per wave and half: 2^-e of each head's q scale
 
@@ -667,12 +668,13 @@ windows_done:
         }
         const size_t head = (size_t)s * a.n_head + h * G + hh;
         if constexpr (SCORES) {
-            if (fused && d == 0) a.scores[head * L.P + qpos] = xnew[hh];
+            if (d == 0) {
+                if (fused) a.scores[head * L.P + qpos] = xnew[hh];
+                if (n_split_s == 1 && !a.w) store_stats(a, head, split, HD, M, lsum);
+                lse_s[hh] = M + __log2f(lsum);
+            }
         }
         if (n_split_s == 1) {
-            if constexpr (SCORES) {
-                if (d == 0) store_stats(a, head, split, HD, M, lsum);
-            }
             // hdr is a multiple of 8: a float4 of dims lies wholly inside or outside the row
             const float inv = lsum > 0.0f ? 1.0f / lsum : 0.0f;
             if (d < hdr) {
@@ -682,6 +684,12 @@ windows_done:
         } else {
 #pragma unroll
             for (int k = 0; k < 4; k++) store_partial(a, head, split, HD, d + k, acc[k], M, lsum);
+        }
+    }
+    if constexpr (SCORES) {
+        if (a.w) {  // (every slot of the stream is this workgroup's)
+            __syncthreads();
+            add_weights<4 * GH * HG, 64 * NW>(a, row, (size_t)s * a.n_head + h * G, G, n_ctx, lse_s, tid);
         }
     }
 }

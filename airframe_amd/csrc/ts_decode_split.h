@@ -37,8 +37,13 @@ struct DecodeArgs {
     int32_t *adv_len;
     int32_t *adv_ctr;
 
-    // Scores of every head and slot in the exp2 domain, [S][n_head][P] (the kernels with SCORES).
+    // The kernels with SCORES: scores of every head and slot in the exp2 domain, [S][n_head][P]; and, if not null (n_split 1,
+    // one head group), the weights [S][H][max_seq] that the launch itself brings up to date: added to, or with fresh
+    // written, zeros behind the last slot.
     float *scores;
+    float *w;
+    int max_seq;
+    bool fresh;
 };
 
 // Every workgroup of the launch's last kernel calls this once, after its last read of the
@@ -491,6 +496,50 @@ __device__ inline void store_stats(const DecodeArgs &a, size_t head, int split, 
     const size_t rows = (size_t)a.L.S * a.n_head * a.n_split, r = head * a.n_split + split;
     a.ws[rows * HD + r] = M;
     a.ws[rows * (HD + 1) + r] = lsum;
+}
+
+// The weights of slots p .. p + 3 (p a multiple of 4 below P) of U groups of slots, `step` apart, from scores x of G <= GM
+// heads (rows P apart) and the heads' log2 sums lse (LDS).  The scores of all groups are on their way together.
+template <int GM, int U>
+__device__ __forceinline__ void sum_scores(const DecodeArgs &a, const float *x, float *w, int G, int n_ctx, const float *lse,
+                                           int p, int step) {
+    floatx4 v[GM][U];
+#pragma unroll
+    for (int g = 0; g < GM; g++)
+        if (g < G) {
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                v[g][u] = *reinterpret_cast<const floatx4 *>(x + (size_t)g * a.L.P + min(p + u * step, a.L.P - 4));
+        }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        floatx4 sum = (floatx4)0.0f;
+#pragma unroll
+        for (int g = 0; g < GM; g++)
+            if (g < G) {
+                const float l = lse[g];
+#pragma unroll
+                for (int e = 0; e < 4; e++) sum[e] += __builtin_amdgcn_exp2f(v[g][u][e] - l);
+            }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {  // (a row of weights is 4-byte aligned)
+            const int at = p + u * step + e;
+            if (at < n_ctx) w[at] = a.fresh ? sum[e] : w[at] + sum[e];
+            else if (a.fresh && at < a.max_seq) w[at] = 0.0f;
+        }
+    }
+}
+
+// The weights of one (sequence, kv head) by the workgroup that holds all of its slots.  All threads call it, behind a
+// barrier that follows the last score.
+template <int GM, int NT>
+__device__ __forceinline__ void add_weights(const DecodeArgs &a, size_t row, size_t head0, int G, int n_ctx, const float *lse, int tid) {
+    constexpr int U = GM <= 4 ? 4 : GM <= 8 ? 2 : 1;
+    if (n_ctx > a.max_seq) return;  // (a graph replayed past the capacity)
+    const int end = a.fresh ? a.max_seq : n_ctx;
+    float *w = a.w + row * a.max_seq;
+    for (int p = 4 * tid; p < end; p += 4 * NT * U)
+        sum_scores<GM, U>(a, a.scores + head0 * a.L.P, w, G, n_ctx, lse, p, 4 * NT);
 }
 
 // LDS: q operands, per-wave scale stages; and the merge area, apart from them so that a

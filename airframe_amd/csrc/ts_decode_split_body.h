@@ -5,7 +5,8 @@
 // In scope: HD, SOFTCAP, NORM, PAD, NW, a; TS_SPLIT_X, _Y, _Z: the split, the kv head and group of query
 // heads, the sequence; TS_SPLIT_LDS: declares sm (DecodeSplitSmem), kd, vd and xnew; TS_SPLIT_KEEP: partials
 // also of a sequence without a split (a flag in the arguments cost the decode kernels 2%); TS_SPLIT_SCORES:
-// every score into a.scores, and the references and sums of sequences without a split.
+// every score into a.scores, the references and sums of sequences without a split among others, and with a.w the
+// weights; lse_s [8] in LDS.
     constexpr int SPAN = 64 * NW;     // positions one round of windows covers
     constexpr int WPG = HD / 32;   // K words per lane group = MFMA k-steps per 16-row tile
     constexpr int NTD = HD / 16;   // 16-dim output tiles
@@ -194,10 +195,13 @@
             lsum += e;
         }
         const size_t head = (size_t)s * a.n_head + hb + hh;
-        if constexpr (TS_SPLIT_SCORES) {
-            if (fused && d == 0) a.scores[head * L.P + qpos] = xnew[hh];
-            if (n_split_s == 1 && d == 0) store_stats(a, head, split, HD, M, lsum);
+#if TS_SPLIT_SCORES
+        if (d == 0) {
+            if (fused) a.scores[head * L.P + qpos] = xnew[hh];
+            if (n_split_s == 1 && !a.w) store_stats(a, head, split, HD, M, lsum);
+            lse_s[hh] = M + __log2f(lsum);
         }
+#endif
         if (n_split_s == 1 && !TS_SPLIT_KEEP) {
             // hdr is a multiple of 8: a float4 of dims lies wholly inside or outside the row
             if (d < hdr) {
@@ -210,5 +214,11 @@
             for (int k = 0; k < 4; k++) store_partial(a, head, split, HD, d + k, acc[k], M, lsum);
         }
     }
+#if TS_SPLIT_SCORES
+    if (a.w) {  // (every slot of the stream is this workgroup's)
+        __syncthreads();
+        add_weights<8, SPAN>(a, row, (size_t)s * a.n_head + hb, G, n_ctx, lse_s, tid);
+    }
+#endif
     // without a split this is the launch's last kernel: it advances the lengths itself
     if (a.n_split == 1) arrive_and_advance(a);

@@ -3,7 +3,8 @@
 //
 // A slot's probability needs the final reference and sum of its head's softmax, which no split of the keys has.
 // The decode kernels therefore leave every score beside their partials (4 bytes per query head and slot; the cached
-// row behind it has hd + 8 per kv head), and one launch joins the partials and turns the scores into sums:
+// row behind it has hd + 8 per kv head).  A workgroup that holds all slots of its kv head turns them into sums itself,
+// from L2; otherwise one more launch joins the partials and does:
 //   w[p] = (w[p]) + sum over the query heads g of one kv head of 2^(x_g[p] - lse_g),
 //   lse = M + log2(sum over the splits of 2^(m - M) l).
 #include "ts_decode_int.h"
@@ -22,7 +23,7 @@ __global__ __launch_bounds__(64 * NW, NW > 4 ? 1 : (HD > 128 ? 1 : 2)) void weig
 #define TS_SPLIT_LDS                                   \
     __shared__ __align__(16) DecodeSplitSmem<HD, NW> sm; \
     __shared__ __align__(16) float kd[HD], vd[HD];       \
-    __shared__ float xnew[8];
+    __shared__ float xnew[8], lse_s[8];
 #include "ts_decode_split_body.h"
 #undef TS_SPLIT_X
 #undef TS_SPLIT_Y
@@ -35,8 +36,6 @@ __global__ __launch_bounds__(64 * NW, NW > 4 ? 1 : (HD > 128 ? 1 : 2)) void weig
 struct SumArgs {
     DecodeArgs d;
     float *w;
-    int max_seq;
-    bool fresh;
     int n_join, n_chunk;  // workgroups that join a head's splits, then n_chunk per (sequence, kv head)
 };
 
@@ -54,8 +53,8 @@ __global__ __launch_bounds__(256) void weigh_sum_token_kernel(SumArgs a) {
     }
     const int b = blockIdx.x - a.n_join, h = b % H, s = b / H % d.L.S, p0 = b / H / d.L.S * kSumSlots;
     const int n = (d.hlen >= 0 ? d.hlen : d.len[s]) + 1;
-    float *const w = a.w + ((size_t)s * H + h) * a.max_seq;
-    if (n > a.max_seq) return;  // (a graph replayed past the capacity)
+    float *const w = a.w + ((size_t)s * H + h) * d.max_seq;
+    if (n > d.max_seq) return;  // (a graph replayed past the capacity)
     const int ns = min((n + d.chunk - 1) / d.chunk, d.n_split), G = d.Gt;
     extern __shared__ float lse[];  // [G]
     const size_t rows = (size_t)d.L.S * d.n_head * d.n_split, head0 = (size_t)s * d.n_head + h * G;
@@ -73,14 +72,20 @@ __global__ __launch_bounds__(256) void weigh_sum_token_kernel(SumArgs a) {
     }
     __syncthreads();
     const float *x = d.scores + head0 * d.L.P;
-    for (int p = p0 + tid; p < min(p0 + kSumSlots, a.max_seq); p += 256) {
-        float sum = 0.0f;
-        if (p < n) {
-            for (int g = 0; g < G; g++) sum += __builtin_amdgcn_exp2f(x[(size_t)g * d.L.P + p] - lse[g]);
-            w[p] = a.fresh ? sum : w[p] + sum;
-        } else if (a.fresh) {
-            w[p] = 0.0f;
+    const int p = p0 + 4 * tid;
+    if (p >= (d.fresh ? d.max_seq : n)) return;
+    if (G <= 8) return sum_scores<8, 1>(d, x, w, G, n, lse, p, 0);
+    floatx4 sum = (floatx4)0.0f;
+    if (p < n)
+        for (int g = 0; g < G; g++) {
+            const floatx4 v = *reinterpret_cast<const floatx4 *>(x + (size_t)g * d.L.P + p);
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum[e] += __builtin_amdgcn_exp2f(v[e] - lse[g]);
         }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        if (p + e < n) w[p + e] = d.fresh ? sum[e] : w[p + e] + sum[e];
+        else if (d.fresh && p + e < d.max_seq) w[p + e] = 0.0f;
     }
 }
 
@@ -108,7 +113,7 @@ void launch_token(const SumArgs &a, const DecodePlan &plan, unsigned blocks, hip
     const bool cap = a.d.softcap > 0.0f, norm = a.d.L.qn != nullptr || a.d.L.kn != nullptr;
     if (cap) norm ? launch_scores<HD, true, true>(a.d, plan, st) : launch_scores<HD, true, false>(a.d, plan, st);
     else norm ? launch_scores<HD, false, true>(a.d, plan, st) : launch_scores<HD, false, false>(a.d, plan, st);
-    weigh_sum_token_kernel<HD><<<blocks, 256, a.d.Gt * sizeof(float), st>>>(a);
+    if (!a.d.w) weigh_sum_token_kernel<HD><<<blocks, 256, a.d.Gt * sizeof(float), st>>>(a);
 }
 
 uint64_t token_part_floats(int n_seq, int n_head, int n_split, int hd) { return (uint64_t)n_seq * n_head * n_split * (hd + 2); }
@@ -144,9 +149,11 @@ hipError_t launch_weigh_token(const WeighCall &c, const DecodePlan &plan, hipStr
     d.adv_len = d.adv_ctr = nullptr;
     const uint64_t parts = token_part_floats(c.L.S, c.n_head, plan.n_split, c.L.hd) * sizeof(float);
     d.scores = reinterpret_cast<float *>(c.ws + (parts + 15) / 16 * 16);
+    d.max_seq = c.max_seq;
+    d.fresh = c.fresh;
     a.w = c.w;
-    a.max_seq = c.max_seq;
-    a.fresh = c.fresh;
+    // no sequence split, one workgroup for all query heads of a kv head: it adds up itself
+    d.w = plan.n_split == 1 && d.NG == 1 ? c.w : nullptr;
     const int slots = c.fresh || c.captured ? c.max_seq : c.own_max;
     a.n_join = plan.n_split > 1 ? c.n_head * c.L.S : 0;
     a.n_chunk = (slots + kSumSlots - 1) / kSumSlots;

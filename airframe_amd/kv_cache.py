@@ -358,9 +358,12 @@ class KVCache:
 
     def attn_weigh_workspace(self, n_head: int, n_tok: int = 1) -> int:
         """Bytes of scratch attn_weigh needs for this shape."""
-        b = ctypes.c_uint64()
-        check("ts_attn_weigh_workspace", load().ts_attn_weigh_workspace(self._h, n_head, n_tok, ctypes.byref(b)))
-        return b.value
+        n = self._ws.get(("weigh", n_head, n_tok))  # (the same for any lengths)
+        if n is None:
+            b = ctypes.c_uint64()
+            check("ts_attn_weigh_workspace", load().ts_attn_weigh_workspace(self._h, n_head, n_tok, ctypes.byref(b)))
+            n = self._ws["weigh", n_head, n_tok] = b.value
+        return n
 
     def attn_weigh(self, layer: int, q: torch.Tensor, rope: RopeTable, weights: torch.Tensor, fresh: bool = False,
                    k: torch.Tensor | None = None, v: torch.Tensor | None = None, out: torch.Tensor | None = None,
