@@ -724,7 +724,7 @@ void launch_split4(const DecodeArgs &a, int n_split, hipStream_t st) {
 // waves measured slower: 1.970 vs 1.888.)
 template <int HD, bool SC, bool NM, bool SCORES = false>
 void launch_integer(const DecodeArgs &a, int n_split, bool pad, int Gt, hipStream_t st) {
-    constexpr int NW = HD == 64 ? 8 : 4;
+    constexpr int NW = HD == 64 || (SCORES && HD == 128) ? 8 : 4;
     if constexpr (HD <= 128) {
         // More than 8 query heads per kv head (the plan allows them up to 128-dim rows).  On
         // 64-dim rows: two head groups of 4 waves, two halves each (config-3 shape with 128 q

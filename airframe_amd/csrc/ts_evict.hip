@@ -215,7 +215,7 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 8 : 7) void select_kernel(const fl
 
 template <int HD>
 constexpr int kKeepSlices = 4 + HD / 64 + 1;
-constexpr int kKeepPart = 128;  // slots of a wave that does not move in place
+constexpr int kKeepPart = 64;  // slots of a wave that does not move in place
 
 // Windows of STEP slots from j0 to j1, D of them in registers: window i + D - 1 goes out before window i is
 // written, its slots' sources one window earlier.
@@ -244,6 +244,13 @@ __device__ __forceinline__ void walk(int j0, int j1, Source source, Load load, S
     }
 }
 
+// Sequence i's length, window base (new tokens go on at the positions they would have had) and sinks.
+__device__ inline void set_length(const KeepCall &a, int i, int len, int n) {
+    a.dst_len[a.dst_seq + i] = n;
+    a.dst_rot[a.dst_seq + i] = a.src_rot[a.src_seq + i] + len - n;
+    a.dst_sink[a.dst_seq + i] = 0;
+}
+
 template <int HD, bool IN_PLACE>
 __global__ __launch_bounds__(64) void keep_kernel(KeepCall a, int n_part) {
     constexpr int NS = kKeepSlices<HD>;
@@ -257,6 +264,8 @@ __global__ __launch_bounds__(64) void keep_kernel(KeepCall a, int n_part) {
     const int sP = a.src.P, dP = a.dst.P;
     const int32_t *slots = a.slots + (size_t)row * a.slot_row;
     const size_t so = a.src_layer * layer, dof = a.dst_layer * layer;
+    // (in place the lengths change behind the launch: its other workgroups read them)
+    if (!IN_PLACE && slice == 0 && part == 0 && layer == 0 && h == 0 && lane == 0) set_length(a, i, len, n);
     // (a slot outside the source reads one inside it)
     auto source = [&](int j) __attribute__((always_inline)) { return j < n ? min(max(slots[j], 0), len - 1) : 0; };
     if (slice < 4) {
@@ -266,7 +275,7 @@ __global__ __launch_bounds__(64) void keep_kernel(KeepCall a, int n_part) {
         const int g = slice;
         const uint32_t *src = reinterpret_cast<const uint32_t *>(a.src.kp + so + srow * sP * (HD / 2));
         uint32_t *dst = reinterpret_cast<uint32_t *>(a.dst.kp + dof + drow * dP * (HD / 2));
-        walk<64, 4, Reg>(j0, j1, [&](int j) { return source(j + lane); },
+        walk<64, IN_PLACE ? 4 : 1, Reg>(j0, j1, [&](int j) { return source(j + lane); },
             [&](Reg &r, int p) {
 #pragma unroll
                 for (int c = 0; c < NV; c++) r.x[c] = *reinterpret_cast<const vec *>(src + k_word_idx<HD>(p, 16 * c + 2 * g));
@@ -284,7 +293,7 @@ __global__ __launch_bounds__(64) void keep_kernel(KeepCall a, int n_part) {
         u32x4 *dst = reinterpret_cast<u32x4 *>(a.dst.vp + dof + drow * (dP / 32) * (HD * 16));
         // slot of nibble e of this lane's words, in a block of 32
         auto slot = [&](int e) __attribute__((always_inline)) { return (e < 4 ? 0 : 16) + 4 * g + (e & 3); };
-        walk<32, 3, Reg>(j0, j1, [&](int j) { return source(j + (lane & 31)); },
+        walk<32, IN_PLACE ? 3 : 1, Reg>(j0, j1, [&](int j) { return source(j + (lane & 31)); },
             [&](Reg &r, int mine) {
                 r.p = mine;
 #pragma unroll
@@ -320,7 +329,7 @@ __global__ __launch_bounds__(64) void keep_kernel(KeepCall a, int n_part) {
         float *vd = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(a.dst.vs) + dof) + drow * dP;
         const float *ws = a.src_w ? a.src_w + ((size_t)layer * a.src.S * H + srow) * a.src_max : nullptr;
         float *wd = a.dst_w ? a.dst_w + ((size_t)layer * a.dst.S * H + drow) * a.dst_max : nullptr;
-        walk<64, 4, Reg>(j0, j1, [&](int j) { return source(j + lane); },
+        walk<64, IN_PLACE ? 4 : 1, Reg>(j0, j1, [&](int j) { return source(j + lane); },
             [&](Reg &r, int p) {
                 r.k = ks[p];
                 r.v = vs[p];
@@ -343,10 +352,8 @@ __global__ __launch_bounds__(64) void keep_kernel(KeepCall a, int n_part) {
 __global__ void keep_len_kernel(KeepCall a) {
     const int i = blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= a.n_seq) return;
-    const int len = min(a.src_len[a.src_seq + i], a.src_max), n = min(len, a.keep), rot = a.src_rot[a.src_seq + i];
-    a.dst_len[a.dst_seq + i] = n;
-    a.dst_rot[a.dst_seq + i] = rot + len - n;
-    a.dst_sink[a.dst_seq + i] = 0;
+    const int len = min(a.src_len[a.src_seq + i], a.src_max);
+    set_length(a, i, len, min(len, a.keep));
 }
 
 }  // namespace
@@ -375,7 +382,7 @@ hipError_t launch_keep(const KeepCall &c, hipStream_t st) {
     else TS_KEEP(64)
 #undef TS_KEEP
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    if (e != hipSuccess || !c.in_place) return e;
     keep_len_kernel<<<(c.n_seq + 63) / 64, 64, 0, st>>>(c);
     return hipGetLastError();
 }

@@ -88,8 +88,20 @@ int ts_attn_weigh(ts_kv *kv, int32_t layer, const float *d_k, const float *d_v, 
     c.v_new = d_v;
     // (an eager call gives a lone sequence's length with the launch, as ts_attn_decode)
     c.hlen = kv->d.n_seq == 1 && !c.captured ? kv->h_len[0] : -1;
-    const DecodePlan plan = decode_plan(kv->h_ctx.data(), kv->d.n_seq, kv->d.n_head_kv, n_head / kv->d.n_head_kv, kv->n_cu,
-                                        kv->hdp, d_k != nullptr);
+    DecodePlan plan = decode_plan(kv->h_ctx.data(), kv->d.n_seq, kv->d.n_head_kv, n_head / kv->d.n_head_kv, kv->n_cu,
+                                  kv->hdp, d_k != nullptr);
+    // The integer kernel runs a workgroup per CU, those past a short sequence's end too: of a ragged batch, longer
+    // splits that fit the CUs in one round, if no longer than 5/2 of the plan's.  4 sequences of 700-6001 slots of
+    // 256-dim heads 28.5 us, 19.6 so; 8 of 1001-16003 with 128 dims 30.7 and 26.2, with 8 query heads per kv head 42.6
+    // and 34.7.
+    const int round = kv->n_cu / (kv->d.n_seq * kv->d.n_head_kv);
+    if (plan.g4 && round > 1 && plan.n_split > round) {
+        const int chunk = ((c.own_max + round - 1) / round + 63) / 64 * 64;
+        if (2 * (int64_t)chunk <= 5 * (int64_t)plan.chunk) {
+            plan.chunk = chunk;
+            plan.n_split = (c.own_max + chunk - 1) / chunk;
+        }
+    }
     return hip_status(launch_weigh_token(c, plan, as_stream(stream)));
 }
 
@@ -118,7 +130,7 @@ int ts_kv_keep(ts_kv *dst, int32_t dst_seq, const ts_kv *src, int32_t src_seq, i
     if (dst == src && !in_place && dst_seq < src_seq + n_seq && src_seq < dst_seq + n_seq) return TS_ERR_INVALID;
     const uint64_t rows = (uint64_t)src->d.n_layers * n_seq * src->d.n_head_kv, slot_bytes = rows * keep * sizeof(int32_t);
     // (workgroups are 32-bit numbers)
-    if (rows * ((keep + 127) / 128) > INT32_MAX / 64) return TS_ERR_INVALID;
+    if (rows * ((keep + 63) / 64) > INT32_MAX / 16) return TS_ERR_INVALID;
     const uint64_t sb = weight_bytes(src) * src->d.n_layers, db = weight_bytes(dst) * dst->d.n_layers;
     if (!(dst == src && d_weights == d_src_weights) && shares(d_src_weights, sb, d_weights, db)) return TS_ERR_INVALID;
     if (shares(d_slots, slot_bytes, d_weights, db)) return TS_ERR_INVALID;
