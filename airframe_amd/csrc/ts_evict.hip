@@ -343,7 +343,7 @@ __global__ __launch_bounds__(64) void keep_kernel(KeepCall a, int n_part) {
                 }
             });
         // slots behind the kept ones have received nothing
-        const int end = IN_PLACE ? len : a.dst_max;
+        const int end = IN_PLACE && a.src_w == a.dst_w ? len : a.dst_max;
         if (wd)
             for (int j = n + 64 * part + lane; j < end; j += 64 * (IN_PLACE ? 1 : n_part)) wd[j] = 0.0f;
     }

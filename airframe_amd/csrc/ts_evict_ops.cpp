@@ -111,7 +111,7 @@ int ts_kv_select(const ts_kv *kv, const float *d_weights, int32_t keep, int32_t 
         !d_weights || !d_slots || !aligned4(d_weights) || !aligned4(d_slots))
         return TS_ERR_INVALID;
     const uint64_t rows = (uint64_t)kv->d.n_layers * kv->d.n_seq * kv->d.n_head_kv;
-    if (rows > INT32_MAX / 64 || kv->d.max_seq > (1 << 29)) return TS_ERR_INVALID;  // (a row's bytes are a 32-bit number)
+    if (rows > INT32_MAX / 64 || kv->d.max_seq > (1 << 28)) return TS_ERR_INVALID;  // (a row's bytes are a 32-bit number)
     if (shares(d_weights, weight_bytes(kv) * kv->d.n_layers, d_slots, rows * keep * sizeof(int32_t))) return TS_ERR_INVALID;
     const int max_len = *std::max_element(kv->h_len.begin(), kv->h_len.end());
     return hip_status(launch_select(d_weights, kv->d_len, max_len, kv->d.n_layers, kv->d.n_seq, kv->d.n_head_kv, kv->d.max_seq, keep,
@@ -122,9 +122,11 @@ int ts_kv_keep(ts_kv *dst, int32_t dst_seq, const ts_kv *src, int32_t src_seq, i
                int32_t keep, const float *d_src_weights, float *d_weights, void *stream) {
     if (!dst || !src || n_seq < 0 || dst_seq < 0 || src_seq < 0 || (int64_t)dst_seq + n_seq > dst->d.n_seq ||
         (int64_t)src_seq + n_seq > src->d.n_seq || dst->d.n_layers != src->d.n_layers || dst->d.n_head_kv != src->d.n_head_kv ||
-        dst->d.head_dim != src->d.head_dim || dst->device != src->device || keep <= 0 || !d_slots || !aligned4(d_slots) ||
+        dst->d.head_dim != src->d.head_dim || dst->device != src->device || keep <= 0 || !aligned4(d_slots) ||
         (d_src_weights == nullptr) != (d_weights == nullptr) || !aligned4(d_src_weights) || !aligned4(d_weights))
         return TS_ERR_INVALID;
+    if (n_seq == 0) return TS_OK;
+    if (!d_slots) return TS_ERR_INVALID;
     // in place, or into sequences apart from those that are read
     const bool in_place = dst == src && dst_seq == src_seq;
     if (dst == src && !in_place && dst_seq < src_seq + n_seq && src_seq < dst_seq + n_seq) return TS_ERR_INVALID;
@@ -140,7 +142,6 @@ int ts_kv_keep(ts_kv *dst, int32_t dst_seq, const ts_kv *src, int32_t src_seq, i
         if (src->h_sink[s] != 0) return TS_ERR_INVALID;  // (sinks are rotated at their own slot, the others past the window base)
         if (n > dst->d.max_seq || (int64_t)src->h_rot[s] + src->h_len[s] - n > INT32_MAX / 2) return TS_ERR_OVERFLOW;
     }
-    if (n_seq == 0) return TS_OK;
     KeepCall c;
     c.src = src->layer(0);
     c.dst = dst->layer(0);

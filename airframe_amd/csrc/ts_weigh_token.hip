@@ -122,7 +122,7 @@ uint64_t token_part_floats(int n_seq, int n_head, int n_split, int hd) { return 
 
 uint64_t weigh_token_workspace(int n_seq, int n_head, int n_kv, int P, int max_seq, int stored_hd, int n_cu) {
     const uint64_t parts = token_part_floats(n_seq, n_head, decode_cap(n_kv, max_seq, n_cu), stored_hd) * sizeof(float);
-    return (parts + 15) / 16 * 16 + (uint64_t)n_seq * n_head * P * sizeof(float);
+    return parts + 256 + (uint64_t)n_seq * n_head * P * sizeof(float);
 }
 
 hipError_t launch_weigh_token(const WeighCall &c, const DecodePlan &plan, hipStream_t st) {
@@ -148,7 +148,8 @@ hipError_t launch_weigh_token(const WeighCall &c, const DecodePlan &plan, hipStr
     d.v_new = c.v_new;
     d.adv_len = d.adv_ctr = nullptr;
     const uint64_t parts = token_part_floats(c.L.S, c.n_head, plan.n_split, c.L.hd) * sizeof(float);
-    d.scores = reinterpret_cast<float *>(c.ws + (parts + 15) / 16 * 16);
+    // (whole cache lines: a head's scores are read back by the workgroup that wrote them, and by no other before)
+    d.scores = reinterpret_cast<float *>(((uintptr_t)c.ws + parts + 255) / 256 * 256);
     d.max_seq = c.max_seq;
     d.fresh = c.fresh;
     a.w = c.w;

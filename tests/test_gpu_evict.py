@@ -197,6 +197,52 @@ def test_weigh_evict_and_go_on(hd):
     assert alone.shape == (2, heads, hd) and bool(torch.isfinite(alone).all())
 
 
+def test_weights_of_their_own_in_place():
+    """In place with another array for the kept weights: whole rows of it are written."""
+    lens, keep = [90, 30], 40
+    kv = cache(lens, 2, 2, 64, 120)
+    w, to = rand((2, 2, 2, 120), 1).cuda(), torch.full((2, 2, 2, 120), 5.0, device="cuda")
+    slots = picked(lens, 2, 2, keep, 2)
+    kv.keep_slots(slots.cuda(), to, src_weights=w)
+    for i in range(2):
+        for s, n in enumerate([40, 30]):
+            for h in range(2):
+                want = torch.zeros(120)
+                want[:n] = w[i, s, h].cpu()[slots[i, s, h, :n].long()]
+                assert torch.equal(to[i, s, h].cpu(), want)
+
+
+def test_captured_choice():
+    """select_slots in a graph reads the lengths and weights of its replays."""
+    kv = KVCache.new_int4(1, 2, 64, 5000, 2)
+    for s, m in enumerate([3000, 50]):
+        kv.set_seq_len(m, s)
+    w, out = kv.new_weights(), torch.empty((1, 2, 2, 64), dtype=torch.int32, device="cuda")
+    kv.select_slots(w, 64, 2, 4, out=out)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        kv.select_slots(w, 64, 2, 4, out=out)
+    for i, lens in enumerate(([3000, 50], [4900, 700], [64, 4100])):
+        for s, m in enumerate(lens):
+            kv.set_seq_len(m, s)
+        w.copy_(rand(w.shape, 70 + i).cuda())
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.cpu(), chosen(w.cpu(), lens, 64, 2, 4))
+
+
+def test_another_stream():
+    kv = cache([400, 30], 1, 2, 128)
+    w, st = rand((1, 2, 2, 400), 1).cuda(), torch.cuda.Stream()
+    before = rows_of(kv, [400, 30])
+    st.wait_stream(torch.cuda.current_stream())
+    wc = w.cpu()
+    slots = kv.evict(w, 50, 1, 5, stream=st)
+    st.synchronize()
+    assert torch.equal(slots.cpu(), chosen(wc, [400, 30], 50, 1, 5))
+    check_rows(rows_of(kv, [50, 30]), before, slots.cpu(), [400, 30], 50)
+
+
 def test_refusals():
     kv, other = cache([50, 20], 2, 2, 64), KVCache.new_int4(2, 2, 64, 16, 2)
     w, ow = kv.new_weights(), other.new_weights()
@@ -230,6 +276,7 @@ def test_refusals():
     kv.reset()
     for s, m in enumerate((50, 20)):
         kv.set_seq_len(m, s)
+    kv.keep_slots(slots[:, :0].contiguous(), n_seq=0)  # no sequence: nothing happens
     kv.keep_slots(slots, w)
     assert kv.seq_lens() == [8, 8]
     g = torch.cuda.CUDAGraph()

@@ -180,6 +180,54 @@ def test_captured_steps(n_tok, heads, hd):
         total = w.cpu()
 
 
+@pytest.mark.parametrize("n_tok", [1, 6])
+def test_two_calls_at_once(n_tok):
+    """Two caches on two streams, each with a workspace of its own."""
+    pair = [Batch([700, 300], n_tok, 8, 2, 128, seed=40 + i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in pair]
+    for b in pair:
+        b.append()
+    args = [(b.q.cuda(), torch.empty(b.kv.attn_weigh_workspace(8, n_tok), dtype=torch.uint8, device="cuda")) for b in pair]
+    torch.cuda.synchronize()
+    outs = [None, None]
+    for _ in range(5):
+        for i, b in enumerate(pair):
+            outs[i] = b.kv.attn_weigh(b.layer, args[i][0], b.rope, b.w, fresh=True, workspace=args[i][1], stream=streams[i])
+    torch.cuda.synchronize()
+    for b, out in zip(pair, outs):
+        b.check(out, b.w)
+
+
+@pytest.mark.parametrize("n_tok", [1, 3])
+def test_offsets_past_32_bits(n_tok):
+    """The last sequences of a layer of 10 GB."""
+    n_seq, cap = 70, 131072
+    kv = KVCache.new_int4(1, 8, 128, cap, n_seq)
+    rope = RopeTable.scaled(512, 128, BASE)
+    lens = [0] * (n_seq - 2) + [77, 300]
+    off = offsets(lens)
+    kv.append_packed(0, rand((377, 8, 128), 1).cuda(), rand((377, 8, 128), 2).cuda(), off, rope)
+    kv.increment_packed(off)
+    k, v = (rand((n_seq, n_tok, 8, 128), i).cuda() for i in (3, 4))
+    kv.append_quant(0, k, v, rope)
+    q, w = rand((n_seq, n_tok, 16, 128), 5, scale=2.0), torch.zeros((n_seq, 8, cap), device="cuda")
+    out = kv.attn_weigh(0, q.cuda(), rope, w).cpu()
+    ends = [m + n_tok for m in lens]
+    want, far, weights = weigh(cached(kv, 0, ends), q, lens, [0] * n_seq, 128, 128, BASE)
+    assert bool(((out.double() - want).abs() <= far).all())
+    for s in (0, n_seq - 3, n_seq - 2, n_seq - 1):
+        ws, ws_far = weights[s]
+        got = w[s].cpu().double()
+        assert bool(((got[:, :ends[s]] - ws).abs() <= ws_far + 2.0 ** -23 * ws).all()) and not bool(got[:, ends[s]:].any())
+    kv.increment(n_tok)
+    before, slots = cached(kv, 0, ends), kv.evict(w[None], 40, 1, 2).cpu()
+    after = cached(kv, 0, [min(e, 40) for e in ends])
+    for s in (n_seq - 2, n_seq - 1):
+        for h in range(8):
+            at = slots[0, s, h].long()
+            assert torch.equal(after[s][0][:, h], before[s][0][at, h]) and torch.equal(after[s][1][:, h], before[s][1][at, h])
+
+
 def test_refusals():
     b = Batch([20, 8], 1, 8, 2, 64)
     kv, q = b.kv, b.q.cuda()
