@@ -352,6 +352,7 @@ hipError_t launch_decode(const KvLayerView &L, int32_t *d_len, const int32_t *h_
     a.ws = ws;
     a.k_new = k_new;
     a.v_new = v_new;
+    a.inv_softcap = 0.0f;
     a.scores = a.w = nullptr;
     a.max_seq = 0;
     a.fresh = false;

@@ -207,7 +207,7 @@ __device__ __forceinline__ void process_window8(const Window8<HD> &w, WaveState8
                                                 const i32x4 (&qa)[GH][HD / 64], const i32x4 (&bias)[GH],
                                                 const float (&qinv)[GH], _Float16 (*pt)[64], int base, int end,
                                                 int lane, const bool (&live)[GH], float softcap, const DeqConst &dc,
-                                                float *scores = nullptr, int score_ld = 0) {
+                                                float *scores = nullptr, int score_ld = 0, float inv_softcap = 0.0f) {
     constexpr int NTD = HD / 16, NM = HD / 64;
     const int n = lane & 15, hg = lane >> 4;
     // ---- S = Q K^T, exact -----------------------------------------------------------------
@@ -239,7 +239,8 @@ __device__ __forceinline__ void process_window8(const Window8<HD> &w, WaveState8
             const int dhi = acc[hf][t][0] * 128 + acc[hf][t][1], dlo = acc[hf][t][2] * 128 + acc[hf][t][3];
             float v = fmaf((float)dhi, 16384.0f, (float)dlo);
             v *= qinv[hf] * w.sk[t];
-            if constexpr (SOFTCAP) v = tanhf(v * (1.0f / kLog2e) / softcap) * softcap * kLog2e;
+            if constexpr (SOFTCAP && SCORES) v = cap<true>(v * (1.0f / kLog2e), softcap, inv_softcap);
+            else if constexpr (SOFTCAP) v = tanhf(v * (1.0f / kLog2e) / softcap) * softcap * kLog2e;
             x[hf][t] = base + 4 * n + t >= end ? -INFINITY : v;
         }
     }
@@ -612,7 +613,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void decode_split4_kernel(DecodeAr
                 // (one form for every window, the tail mask included: a branch between a masked
                 // and an unmasked copy made the compiler shuffle the accumulators at the join,
                 // ~30 moves per window; config 4 1.396 vs 1.408 ms per step)
-                process_window8<HD, SOFTCAP, GH, SCORES>(w[d], st, qa, bias, qinv, pt, win_base(it), end, lane, live, a.softcap, dc, scores, L.P);
+                process_window8<HD, SOFTCAP, GH, SCORES>(w[d], st, qa, bias, qinv, pt, win_base(it), end, lane, live, a.softcap, dc, scores, L.P, a.inv_softcap);
                 if (++it >= cnt) goto windows_done;
             }
         }

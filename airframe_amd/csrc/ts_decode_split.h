@@ -39,7 +39,8 @@ struct DecodeArgs {
 
     // The kernels with SCORES: scores of every head and slot in the exp2 domain, [S][n_head][P]; and, if not null (n_split 1,
     // one head group), the weights [S][H][max_seq] that the launch itself brings up to date: added to, or with fresh
-    // written, zeros behind the last slot.
+    // written, zeros behind the last slot.  The softcap by cap().
+    float inv_softcap;  // 1 / softcap, at most the largest float
     float *scores;
     float *w;
     int max_seq;
@@ -172,7 +173,7 @@ template <int HD, bool SOFTCAP, bool SCORES = false>
 __device__ __forceinline__ void process_window(const Window<HD> &w, WaveState<HD> &st,
                                                const QLds<HD> &qs, float *stage, int base, int end,
                                                int lane, int g, bool live, bool lo_col, int partner4,
-                                               float inv_s, float softcap, const DeqConst &dc, float *scores = nullptr) {
+                                               float inv_s, float softcap, const DeqConst &dc, float *scores = nullptr, float inv_softcap = 0.0f) {
     constexpr int WPG = HD / 32, NTD = HD / 16;
     // Scales: one per lane in registers -> this wave's LDS stage -> the 4 positions each lane
     // holds per tile (16kt + 4g + r).  Same-wave LDS traffic is ordered: no barrier needed.
@@ -209,7 +210,8 @@ __device__ __forceinline__ void process_window(const Window<HD> &w, WaveState<HD
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             float v = sc[kt][r] * sk4[r];
-            if constexpr (SOFTCAP) v = tanhf(v * (1.0f / kLog2e) / softcap) * softcap * kLog2e;
+            if constexpr (SOFTCAP && SCORES) v = cap<true>(v * (1.0f / kLog2e), softcap, inv_softcap);
+            else if constexpr (SOFTCAP) v = tanhf(v * (1.0f / kLog2e) / softcap) * softcap * kLog2e;
             x[4 * kt + r] = v;
             sv[4 * kt + r] = sv4[r];
         }

@@ -145,7 +145,7 @@
         /* keep the prefetch here: the scheduler would otherwise sink it below CUR's use */     \
         asm volatile("" ::: "memory");                                                         \
         __builtin_amdgcn_sched_barrier(0);                                                     \
-        process_window<HD, SOFTCAP, TS_SPLIT_SCORES>(CUR, st, sm.run.q, stage, base, end, lane, g, live, lo_col, partner4, inv_s, a.softcap, dc, scores); \
+        process_window<HD, SOFTCAP, TS_SPLIT_SCORES>(CUR, st, sm.run.q, stage, base, end, lane, g, live, lo_col, partner4, inv_s, a.softcap, dc, scores, a.inv_softcap); \
         base += SPAN;                                                                           \
         if (base >= end) break;                                                                \
     }

@@ -215,5 +215,29 @@ __device__ inline void load_q8(const float *rope, int rope_pairs, const float *q
     split_q8(x, cs, u, rope_pairs, mul, hi, lo);
 }
 
+// softcap tanh(x / softcap) in the exp2 domain, within 2^-20 of it relative to it for any softcap: with y = x /
+// softcap, x (1 + y^2 P(y^2)) near zero, P fitted to (tanh(y) / y - 1) / y^2 by least squares on Chebyshev nodes, and
+// softcap (1 - 2 / (1 + e^(2 y))) beyond, whose error is 2^-22 of softcap and not of x; the two are
+// selected, not branched to.  f32 rows: P of five terms below 0.6 (2^-27), 16-bit rows, whose weights are rounded to
+// 2^-12 and 2^-9, of three below 0.35 (2^-24).
+template <bool F32>
+__device__ inline float cap(float x, float softcap, float inv_softcap) {
+    const float y = x * inv_softcap, z = y * y, xl = x * kLog2e;
+    float p;
+    if constexpr (F32) {
+        p = __builtin_fmaf(z, -5.8939453e-03f, 2.0794618e-02f);
+        p = __builtin_fmaf(z, p, -5.3783293e-02f);
+        p = __builtin_fmaf(z, p, 1.3331915e-01f);
+        p = __builtin_fmaf(z, p, -3.33332975e-01f);
+    } else {
+        p = __builtin_fmaf(z, -4.9134325e-02f, 1.3299560e-01f);
+        p = __builtin_fmaf(z, p, -3.33326515e-01f);
+    }
+    const float near = __builtin_fmaf(xl * z, p, xl);
+    const float rest = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * (2.0f * kLog2e)) + 1.0f);
+    const float far = softcap * __builtin_fmaf(-2.0f * kLog2e, rest, kLog2e);
+    return fabsf(y) < (F32 ? 0.6f : 0.35f) ? near : far;
+}
+
 }  // namespace
 }  // namespace ts

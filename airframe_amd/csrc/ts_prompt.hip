@@ -91,31 +91,7 @@ __device__ inline typename Vec8<T>::type v_operand(const unsigned char *p) {
     return __builtin_bit_cast(typename Vec8<T>::type, s);
 }
 
-// softcap tanh(x / softcap) in the exp2 domain, within 2^-20 of it relative to it for any softcap: with y = x /
-// softcap, x (1 + y^2 P(y^2)) near zero, P fitted to (tanh(y) / y - 1) / y^2 by least squares on Chebyshev nodes, and
-// softcap (1 - 2 / (1 + e^(2 y))) beyond, whose error is 2^-22 of softcap and not of x; the two are
-// selected, not branched to.  f32 rows: P of five terms below 0.6 (2^-27), 16-bit rows, whose weights are rounded to
-// 2^-12 and 2^-9, of three below 0.35 (2^-24).
-template <bool F32>
-__device__ inline float cap(float x, float softcap, float inv_softcap) {
-    const float y = x * inv_softcap, z = y * y, xl = x * kLog2e;
-    float p;
-    if constexpr (F32) {
-        p = __builtin_fmaf(z, -5.8939453e-03f, 2.0794618e-02f);
-        p = __builtin_fmaf(z, p, -5.3783293e-02f);
-        p = __builtin_fmaf(z, p, 1.3331915e-01f);
-        p = __builtin_fmaf(z, p, -3.33332975e-01f);
-    } else {
-        p = __builtin_fmaf(z, -4.9134325e-02f, 1.3299560e-01f);
-        p = __builtin_fmaf(z, p, -3.33326515e-01f);
-    }
-    const float near = __builtin_fmaf(xl * z, p, xl);
-    const float rest = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * (2.0f * kLog2e)) + 1.0f);
-    const float far = softcap * __builtin_fmaf(-2.0f * kLog2e, rest, kLog2e);
-    return fabsf(y) < (F32 ? 0.6f : 0.35f) ? near : far;
-}
-
-// The same of small softcaps for 16-bit rows, as c - 2 c / (1 + e^(2 y)) from two transcendental instructions: within
+// cap() (ts_mfma.h) of small softcaps for 16-bit rows, as c - 2 c / (1 + e^(2 y)) from two transcendental instructions: within
 // 2^-21 of softcap and not of x, so up to softcaps of kQuickCap within 2^-15, where f16 weights are rounded by 2^-12.
 // to_exp: 2 log2(e) / softcap.  16 ragged prompts, softcap 50, with this and with cap(): bf16 of 128 dims 236 and 293 us,
 // f16 of 64 dims 153 and 226 (without softcap 202 and 109).

@@ -16,6 +16,8 @@
 // behind 4097: 252 to 269 us by card, 142 GFLOP that hi and lo terms of q and P make 240: 0.89 to 0.95 PFLOP/s executed.
 #include "ts_shared.h"
 
+#include <cfloat>
+
 #include "ts_decode_split.h"
 #include "ts_columns.h"
 
@@ -39,6 +41,7 @@ struct SharedArgs {
     float *part, *out;
     void *cols;                // (COLS)
     int n_blk32;
+    float inv_softcap;         // 1 / softcap, at most the largest float
 };
 
 constexpr int kCols = kPrefillNW * kColsPerWave;
@@ -308,8 +311,8 @@ __global__ __launch_bounds__(64 * kPrefillNW, HD > 128 ? 1 : 2) void shared_kern
             sc[0] *= q_back;
             sc[1] *= q_back;
             const bool mask = base + kWin - 1 > qmin_w;
-            window_scores<NDB, SOFTCAP>(sc, sm.sk[buf], sm.svlog[buf], a.softcap, mask, first, base, hf, qpos, m_run,
-                                        l_run, o);
+            window_scores<NDB, SOFTCAP, COLS>(sc, sm.sk[buf], sm.svlog[buf], a.softcap, mask, first, base, hf, qpos, m_run,
+                                              l_run, o, a.inv_softcap);
             first = false;
 #pragma unroll
             for (int st = 0; st < 4; st++) {
@@ -569,6 +572,7 @@ hipError_t launch_shared(const SharedCall &c, hipStream_t st) {
     a.out = c.out;
     a.cols = c.cols;
     a.n_blk32 = c.n_blk32;
+    a.inv_softcap = c.softcap > 0.0f ? std::min(1.0f / c.softcap, FLT_MAX) : 0.0f;
     int own_jobs = a.own_blk * a.own_pieces * c.own.S;  // per kv head
     if (c.own_part) {
         DecodeArgs &d = a.dec;

@@ -8,6 +8,8 @@
 // in the operand layout of the matrix cores, and every column's log2 sum lse, its own or (of pieces of the keys)
 // the join's.  Then the scores are computed a second time with the keys held in registers and the columns streaming
 // past, so that a slot's sum stays in its lane: w[p] += sum over the columns of 2^(x - lse).
+#include <cfloat>
+
 #include "ts_columns.h"
 #include "ts_evict.h"
 #include "ts_shared.h"
@@ -19,7 +21,7 @@ struct ChunkArgs {
     KvLayerView L;
     const int32_t *len;
     int n_head, G, n_tok, n_blk32;
-    float softcap;
+    float softcap, inv_softcap;
     const float *part;  // of pieces: [rows][slots][HD], references and sums [rows][slots]
     int slots, own_chunk;
     float *out;
@@ -184,7 +186,7 @@ __device__ __forceinline__ void tile_scores(const typename KeyTile<HD>::F16 &ka,
 template <int HD, bool SOFTCAP>
 __device__ __forceinline__ void add_probs(floatx16 (&sc)[KeyTile<HD>::NT], float (&acc)[KeyTile<HD>::NT][16], const ColBlock<HD> &b,
                                           const float *sk, int cb, int n_cols, int G, int len, int base, int j, int hf,
-                                          float softcap) {
+                                          float softcap, float inv_softcap) {
     constexpr int NT = KeyTile<HD>::NT;
     const float back = b.back[j], lse = b.lse[j];
 #pragma unroll
@@ -195,7 +197,7 @@ __device__ __forceinline__ void add_probs(floatx16 (&sc)[KeyTile<HD>::NT], float
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 float x = sc[i][4 * q + r] * s4[r];
-                if constexpr (SOFTCAP) x = tanhf(x * back / softcap) * softcap * kLog2e - lse;
+                if constexpr (SOFTCAP) x = cap<true>(x * back, softcap, inv_softcap) - lse;
                 else x = __builtin_fmaf(x, back, -lse);
                 sc[i][4 * q + r] = __builtin_amdgcn_exp2f(x);
             }
@@ -298,7 +300,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_window_kernel(ChunkArgs 
         for (int cb = max(0, base - len) * a.G / kColBlk; cb < a.n_blk32; cb++) {
             floatx16 sc[NT];
             tile_scores<HD>(ka, k6, blk[cb], lane, sc);
-            add_probs<HD, SOFTCAP>(sc, acc, blk[cb], sks[wave], cb, n_cols, a.G, len, base, j, hf, a.softcap);
+            add_probs<HD, SOFTCAP>(sc, acc, blk[cb], sks[wave], cb, n_cols, a.G, len, base, j, hf, a.softcap, a.inv_softcap);
         }
         sum_columns<HD>(acc, sums[wave], j, hf);
         asm volatile("" ::: "memory");  // (the wave's LDS writes are ordered before its reads)
@@ -379,7 +381,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_cols_kernel(ChunkArgs a)
         if (it + 1 < n_it) stage(it + 1);
         if (it + 2 < n_it) fetch(it + 2);
         // (a block behind the last has no columns: nothing is added)
-        add_probs<HD, SOFTCAP>(sc, acc, b, sks + wk * TK, cb, n_cols, a.G, len, base, j, hf, a.softcap);
+        add_probs<HD, SOFTCAP>(sc, acc, b, sks + wk * TK, cb, n_cols, a.G, len, base, j, hf, a.softcap, a.inv_softcap);
         __syncthreads();
     }
     sum_columns<HD>(acc, part[grp] + wk * TK, j, hf);
@@ -447,6 +449,7 @@ hipError_t launch_weigh_chunk(const WeighCall &c, hipStream_t st) {
     a.n_tok = c.n_tok;
     a.n_blk32 = sc.n_blk32;
     a.softcap = c.softcap;
+    a.inv_softcap = c.softcap > 0.0f ? std::min(1.0f / c.softcap, FLT_MAX) : 0.0f;
     a.part = sc.part;
     a.slots = sc.plan.own_pieces;
     a.own_chunk = sc.plan.own_chunk;

@@ -7,6 +7,8 @@
 // from L2; otherwise one more launch joins the partials and does:
 //   w[p] = (w[p]) + sum over the query heads g of one kv head of 2^(x_g[p] - lse_g),
 //   lse = M + log2(sum over the splits of 2^(m - M) l).
+#include <cfloat>
+
 #include "ts_decode_int.h"
 #include "ts_evict.h"
 
@@ -142,6 +144,7 @@ hipError_t launch_weigh_token(const WeighCall &c, const DecodePlan &plan, hipStr
     d.n_split = plan.n_split;
     d.inv_sqrt_hd = 1.0f / sqrtf((float)c.L.hdr);
     d.softcap = c.softcap;
+    d.inv_softcap = c.softcap > 0.0f ? std::min(1.0f / c.softcap, FLT_MAX) : 0.0f;
     d.out = c.out;
     d.ws = reinterpret_cast<float *>(c.ws);
     d.k_new = c.k_new;

@@ -318,10 +318,11 @@ __device__ inline float half_sum(float v) {
 // online-softmax state update.  The reference is raised only when the window breaks
 // p <= 2^8 or p*s_v <= 2^15 (f16 range), and the scores move down with it; the first window
 // (first, uniform; m_run = 0 and nothing accumulated yet) sets it from its own max.
-template <int NDB, bool SOFTCAP>
+// FAST: the softcap by cap() with inv_softcap = 1 / softcap, at most the largest float.
+template <int NDB, bool SOFTCAP, bool FAST = false>
 __device__ inline void window_scores(floatx16 (&sc)[2], const float *sk, float svl, float softcap,
                                      bool mask, bool first, int base, int h, int qpos, float &m_run,
-                                     float &l_run, floatx16 (&o)[NDB]) {
+                                     float &l_run, floatx16 (&o)[NDB], float inv_softcap = 0.0f) {
 #pragma unroll
     for (int kb = 0; kb < 2; kb++) {
 #pragma unroll
@@ -332,7 +333,8 @@ __device__ inline void window_scores(floatx16 (&sc)[2], const float *sk, float s
                 float x;
                 if constexpr (SOFTCAP) {
                     x = sc[kb][4 * q + r] * sk4[r];
-                    x = tanhf(x / softcap) * softcap * kLog2e - m_run;
+                    if constexpr (FAST) x = cap<true>(x, softcap, inv_softcap) - m_run;
+                    else x = tanhf(x / softcap) * softcap * kLog2e - m_run;
                 } else {
                     x = __builtin_fmaf(sc[kb][4 * q + r], sk4[r], -m_run);
                 }

@@ -93,6 +93,14 @@ def test_softcap_norm_and_window_base(n_tok, hd):
         b.check(b.kv.attn_weigh(b.layer, b.q.cuda(), b.rope, b.w, fresh=True, softcap=softcap), b.w, softcap=softcap)
 
 
+@pytest.mark.parametrize("n_tok", [1, 6, 140])
+@pytest.mark.parametrize("softcap", [1e-38, 1e-3, 0.7, 1e6, 3e38])
+def test_softcaps_large_and_tiny(n_tok, softcap):
+    b = Batch([150, 700], n_tok, 8, 2, 128, seed=6)
+    b.append()
+    b.check(b.kv.attn_weigh(b.layer, b.q.cuda(), b.rope, b.w, fresh=True, softcap=softcap), b.w, softcap=softcap)
+
+
 @pytest.mark.parametrize("lens,heads,n_kv,hd", [([0, 700], 8, 2, 128), ([511], 32, 8, 64), ([64, 3], 20, 2, 64), ([1025], 16, 8, 256),
                                                 ([95, 2000], 24, 8, 128), ([128], 12, 4, 96)])
 @pytest.mark.parametrize("norm", [False, True])
