@@ -312,20 +312,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_window_kernel(ChunkArgs 
     }
 }
 
-// Many columns: four waves hold four tiles of keys for as long as the columns stream past through LDS; the workgroup's
-// two groups of four take every second column block.  (With the groups half a step apart, one's matrix instructions
+// Many columns: KW waves hold KW tiles of keys for as long as the columns stream past through LDS; the workgroup's
+// groups of KW waves take the column blocks in turn.  (Two groups half a step apart, one's matrix instructions
 // beside the other's exponentials: 70 us, 68 without, 512 tokens of 4 sequences of 1-1.5K slots.)
-template <int HD, bool SOFTCAP>
+template <int HD, bool SOFTCAP, int KW>
 __global__ __launch_bounds__(64 * kWaves, 2) void weigh_cols_kernel(ChunkArgs a) {
     using Tile = KeyTile<HD>;
     using Block = ColBlock<HD>;
-    constexpr int NT = Tile::NT, TK = Tile::KEYS, KEYS = 4 * TK;
+    constexpr int NT = Tile::NT, TK = Tile::KEYS, KEYS = KW * TK, GROUPS = kWaves / KW, GT = 64 * KW;
     extern __shared__ __align__(16) unsigned char cols_smem[];
     Block *const buf = reinterpret_cast<Block *>(cols_smem);  // [group][2]
-    __shared__ __align__(16) float part[2][KEYS], sks[KEYS];
+    __shared__ __align__(16) float part[GROUPS][KEYS], sks[KEYS];
     const int H = a.L.H, h = blockIdx.x % H, kb = blockIdx.x / H, s = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 63, j = lane & 31, hf = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), grp = wave >> 2, wk = wave & 3;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), grp = wave / KW, wk = wave % KW, gt = tid % GT;
     const size_t st = (size_t)s * H + h;
     const int len = a.len[s], n = len + a.n_tok, key0 = kb * KEYS;
     float *const w = a.w + st * a.max_seq;
@@ -338,22 +338,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_cols_kernel(ChunkArgs a)
     const int base = key0 + wk * TK, n_cols = a.n_tok * a.G;
     // (the first columns that see a key of the block; all blocks behind them do too)
     const int first = max(0, key0 - len) * a.G / kColBlk;
-    const int n_it = (a.n_blk32 - first + 1) / 2;
+    const int n_it = (a.n_blk32 - first + GROUPS - 1) / GROUPS;
     const Block *const src = static_cast<const Block *>(a.cols) + st * a.n_blk32;
-    constexpr int PIECES = sizeof(Block) / 16, PER = (PIECES + 255) / 256;
+    constexpr int PIECES = sizeof(Block) / 16, PER = (PIECES + GT - 1) / GT;
     static_assert(sizeof(Block) % 16 == 0, "blocks move in 16-byte pieces");
     u32x4 next[PER];
     auto fetch = [&](int it) __attribute__((always_inline)) {
-        const int b = min(first + 2 * it + grp, a.n_blk32 - 1);
+        const int b = min(first + GROUPS * it + grp, a.n_blk32 - 1);
         const u32x4 *p = reinterpret_cast<const u32x4 *>(src + b);
 #pragma unroll
-        for (int i = 0; i < PER; i++) next[i] = p[min((tid & 255) + 256 * i, PIECES - 1)];
+        for (int i = 0; i < PER; i++) next[i] = p[min(gt + GT * i, PIECES - 1)];
     };
     auto stage = [&](int it) __attribute__((always_inline)) {
         u32x4 *p = reinterpret_cast<u32x4 *>(buf + 2 * grp + (it & 1));
 #pragma unroll
         for (int i = 0; i < PER; i++)
-            if ((tid & 255) + 256 * i < PIECES) p[(tid & 255) + 256 * i] = next[i];
+            if (gt + GT * i < PIECES) p[gt + GT * i] = next[i];
     };
     fetch(0);
     typename Tile::F16 ka;
@@ -375,7 +375,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_cols_kernel(ChunkArgs a)
     __syncthreads();
     for (int it = 0; it < n_it; it++) {
         const Block &b = buf[2 * grp + (it & 1)];
-        const int cb = first + 2 * it + grp;
+        const int cb = first + GROUPS * it + grp;
         floatx16 sc[NT];
         tile_scores<HD>(ka, k6, b, lane, sc);
         if (it + 1 < n_it) stage(it + 1);
@@ -389,7 +389,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_cols_kernel(ChunkArgs a)
     for (int x = tid; x < KEYS; x += 64 * kWaves) {
         const int p = key0 + x;
         if (p >= a.max_seq) break;
-        const float v = part[0][x] + part[1][x];
+        float v = part[0][x];
+#pragma unroll
+        for (int i = 1; i < GROUPS; i++) v += part[i][x];
         if (p < n)
             w[p] = a.fresh ? v : w[p] + v;
         else if (a.fresh)
@@ -460,21 +462,36 @@ hipError_t launch_weigh_chunk(const WeighCall &c, hipStream_t st) {
     a.fresh = c.fresh;
     const int slots = c.fresh || c.captured ? c.max_seq : c.own_max;
     const bool window = a.n_blk32 * col_block_bytes(c.L.hd) <= kWindowLds;
-    // tiles of keys per workgroup: one for every wave at least, and a workgroup per CU over the batch's keys
+    // Few columns: tiles of keys per workgroup, one for every wave at least and a workgroup per CU over the batch's keys;
+    // where that leaves CUs idle, one for every second wave (11 sequences of 4-726 slots, 37 tokens of 64 heads with
+    // softcap: 44 us with eight tiles, 32 with four).
     const int tk = c.L.hd > 128 ? 32 : 64;
-    int64_t total = 0;
-    for (int s = 0; s < c.L.S; s++) total += (c.n_ctx[s] + tk - 1) / tk;
-    a.tiles = (int)(((total * c.L.H + c.n_cu - 1) / c.n_cu + kWaves - 1) / kWaves * kWaves);
-#define TS_COLS(HDV)                                                                                                  \
-    {                                                                                                                 \
-        if (!sc.plan.chain) weigh_join_kernel<HDV><<<(unsigned)((rows / c.L.H + 3) / 4 * c.L.H), 256, 0, st>>>(a);      \
-        constexpr int TK = KeyTile<HDV>::KEYS;                                                                        \
-        auto kernel = window ? (c.softcap > 0.0f ? weigh_window_kernel<HDV, true> : weigh_window_kernel<HDV, false>)   \
-                             : (c.softcap > 0.0f ? weigh_cols_kernel<HDV, true> : weigh_cols_kernel<HDV, false>);      \
-        const int lds = (int)sizeof(ColBlock<HDV>) * (window ? a.n_blk32 : 4), per = window ? TK * a.tiles : 4 * TK;   \
-        (void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,                    \
-                                  window ? (int)kWindowLds : lds);                                                    \
-        kernel<<<dim3((unsigned)((slots + per - 1) / per * c.L.H), c.L.S), 64 * kWaves, lds, st>>>(a);                 \
+    int64_t tiles = 0, wg4 = 0, wg2 = 0;
+    for (int s = 0; s < c.L.S; s++) {
+        tiles += (c.n_ctx[s] + tk - 1) / tk * c.L.H;
+        wg4 += (c.n_ctx[s] + 4 * tk - 1) / (4 * tk) * c.L.H;
+        wg2 += (c.n_ctx[s] + 2 * tk - 1) / (2 * tk) * c.L.H;
+    }
+    const int64_t per_cu = (tiles + c.n_cu - 1) / c.n_cu;
+    a.tiles = (int)(per_cu <= kWaves / 2 ? kWaves / 2 : (per_cu + kWaves - 1) / kWaves * kWaves);
+    // Many columns: four tiles of keys per workgroup, or two, whose column groups then have half as many steps, if that
+    // takes less than twice as many rounds of the CUs.  4 sequences of 434 slots, 505 tokens, 64-dim heads with softcap:
+    // 112 and 63 us (the launch).
+    const bool two = 2 * ((wg4 + c.n_cu - 1) / c.n_cu) > (wg2 + c.n_cu - 1) / c.n_cu && c.L.hd <= 128;
+#define TS_COLS(HDV)                                                                                                     \
+    {                                                                                                                    \
+        if (!sc.plan.chain) weigh_join_kernel<HDV><<<(unsigned)((rows / c.L.H + 3) / 4 * c.L.H), 256, 0, st>>>(a);         \
+        constexpr int TK = KeyTile<HDV>::KEYS, KW2 = HDV <= 128 ? 2 : 4;                                                 \
+        const bool cap = c.softcap > 0.0f;                                                                               \
+        auto kernel = window ? (cap ? weigh_window_kernel<HDV, true> : weigh_window_kernel<HDV, false>)                   \
+                      : two  ? (cap ? weigh_cols_kernel<HDV, true, KW2> : weigh_cols_kernel<HDV, false, KW2>)             \
+                             : (cap ? weigh_cols_kernel<HDV, true, 4> : weigh_cols_kernel<HDV, false, 4>);                \
+        const int kw = two ? KW2 : 4, per = TK * (window ? a.tiles : kw);                                                \
+        const int lds = (int)sizeof(ColBlock<HDV>) * (window ? a.n_blk32 : 2 * kWaves / kw);                             \
+        static_assert(sizeof(ColBlock<HDV>) * 2 * kWaves / KW2 <= kWindowLds, "the column groups' blocks fit a CU's LDS"); \
+        (void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,                       \
+                                  window ? (int)kWindowLds : lds);                                                       \
+        kernel<<<dim3((unsigned)((slots + per - 1) / per * c.L.H), c.L.S), 64 * kWaves, lds, st>>>(a);                    \
     }
     if (c.L.hd == 256) TS_COLS(256)
     else if (c.L.hd == 128) TS_COLS(128)

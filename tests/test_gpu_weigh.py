@@ -65,7 +65,7 @@ SHAPES = [
     ([1300], 1, 16, 8, 256), ([200, 31], 1, 12, 4, 96), ([77], 1, 8, 8, 8), ([250], 1, 4, 2, 40), ([333, 1], 1, 16, 8, 80),
     ([0], 2, 4, 2, 64), ([0], 33, 6, 2, 128), ([5, 64], 3, 32, 8, 128), ([1000, 7, 0], 32, 8, 2, 128), ([63], 130, 4, 1, 64),
     ([400, 100], 65, 3, 3, 256), ([31], 70, 5, 1, 80), ([500], 17, 16, 1, 64), ([2500, 900], 9, 8, 2, 128), ([100], 40, 34, 2, 128),
-    ([40, 300, 7, 64], 160, 8, 2, 96), ([0, 130], 257, 4, 1, 128),
+    ([40, 300, 7, 64], 160, 8, 2, 96), ([0, 130], 257, 4, 1, 128), ([120, 30], 200, 2, 1, 256), ([3000, 2900, 3100, 3050], 330, 16, 8, 64),
 ]
 
 
