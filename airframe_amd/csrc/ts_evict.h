@@ -44,6 +44,7 @@ struct KeepCall {
     const int32_t *src_len, *src_rot;
     int32_t *dst_len, *dst_rot, *dst_sink;
     int src_seq, dst_seq, n_seq, n_layers, keep, src_max, dst_max;
+    int first_layer;  // of a launch; slots and weights begin at it
     int slot_row;  // slots of a row of d_slots (keep, or more than fit the destination)
     bool in_place;
     const int32_t *slots;

@@ -2,6 +2,8 @@
 // received, and their rows moved together.
 #include "ts_evict.h"
 
+#include <algorithm>
+
 namespace ts {
 namespace {
 
@@ -263,7 +265,7 @@ __global__ __launch_bounds__(64) void keep_kernel(KeepCall a, int n_part) {
     const size_t srow = (size_t)(a.src_seq + i) * H + h, drow = (size_t)(a.dst_seq + i) * H + h;
     const int sP = a.src.P, dP = a.dst.P;
     const int32_t *slots = a.slots + (size_t)row * a.slot_row;
-    const size_t so = a.src_layer * layer, dof = a.dst_layer * layer;
+    const size_t so = a.src_layer * (a.first_layer + layer), dof = a.dst_layer * (a.first_layer + layer);
     // (in place the lengths change behind the launch: its other workgroups read them)
     if (!IN_PLACE && slice == 0 && part == 0 && layer == 0 && h == 0 && lane == 0) set_length(a, i, len, n);
     // (a slot outside the source reads one inside it)
@@ -358,30 +360,51 @@ __global__ void keep_len_kernel(KeepCall a) {
 
 }  // namespace
 
+// Layers of one launch: its work-items are a 32-bit number.
+static int layers_per_launch(int64_t items, int n_layers) { return (int)std::min<int64_t>(std::max<int64_t>(1, UINT32_MAX / items), n_layers); }
+
 hipError_t launch_select(const float *w, const int32_t *d_len, int max_len, int n_layers, int n_seq, int H, int max_seq,
                          int keep, int n_sink, int n_recent, int32_t *d_slots, hipStream_t st) {
-    const unsigned rows = (unsigned)(n_layers * n_seq * H);
+    const int64_t rows = (int64_t)n_seq * H;
     // A workgroup whose registers hold the longest row, and no larger: several of the smaller one share a CU.
-    if (max_len <= 256 * kSelPer)
-        select_kernel<256><<<rows, 256, 0, st>>>(w, d_len, n_seq, H, max_seq, keep, n_sink, n_recent, d_slots);
-    else
-        select_kernel<1024><<<rows, 1024, 0, st>>>(w, d_len, n_seq, H, max_seq, keep, n_sink, n_recent, d_slots);
-    return hipGetLastError();
+    const bool small = max_len <= 256 * kSelPer;
+    const int per = layers_per_launch(rows * (small ? 256 : 1024), n_layers);
+    for (int i = 0; i < n_layers; i += per) {
+        const unsigned wgs = (unsigned)(std::min(per, n_layers - i) * rows);
+        const float *wi = w + i * rows * max_seq;
+        int32_t *to = d_slots + i * rows * keep;
+        if (small) select_kernel<256><<<wgs, 256, 0, st>>>(wi, d_len, n_seq, H, max_seq, keep, n_sink, n_recent, to);
+        else select_kernel<1024><<<wgs, 1024, 0, st>>>(wi, d_len, n_seq, H, max_seq, keep, n_sink, n_recent, to);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+template <int HD>
+static hipError_t launch_rows(KeepCall c, hipStream_t st) {
+    const int64_t rows = (int64_t)c.n_seq * c.src.H;
+    const int n_part = c.in_place ? 1 : (c.keep + kKeepPart - 1) / kKeepPart, n_layers = c.n_layers;
+    const int per = layers_per_launch(rows * kKeepSlices<HD> * n_part * 64, n_layers);
+    for (int i = 0; i < n_layers; i += per) {
+        c.n_layers = std::min(per, n_layers - i);
+        const unsigned wgs = (unsigned)(c.n_layers * rows * kKeepSlices<HD> * n_part);
+        if (c.in_place) keep_kernel<HD, true><<<wgs, 64, 0, st>>>(c, 1);
+        else keep_kernel<HD, false><<<wgs, 64, 0, st>>>(c, n_part);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        c.first_layer += per;
+        c.slots += per * rows * c.slot_row;
+        if (c.dst_w) {
+            c.src_w += (int64_t)per * c.src.S * c.src.H * c.src_max;
+            c.dst_w += (int64_t)per * c.dst.S * c.dst.H * c.dst_max;
+        }
+    }
+    return hipSuccess;
 }
 
 hipError_t launch_keep(const KeepCall &c, hipStream_t st) {
-    const unsigned rows = (unsigned)(c.n_layers * c.n_seq * c.src.H);
-    const int n_part = (c.keep + kKeepPart - 1) / kKeepPart;
-#define TS_KEEP(HDV)                                                                                          \
-    {                                                                                                         \
-        if (c.in_place) keep_kernel<HDV, true><<<rows * kKeepSlices<HDV>, 64, 0, st>>>(c, 1);                   \
-        else keep_kernel<HDV, false><<<rows * kKeepSlices<HDV> * n_part, 64, 0, st>>>(c, n_part);               \
-    }
-    if (c.src.hd == 256) TS_KEEP(256)
-    else if (c.src.hd == 128) TS_KEEP(128)
-    else TS_KEEP(64)
-#undef TS_KEEP
-    hipError_t e = hipGetLastError();
+    const hipError_t e = c.src.hd == 256 ? launch_rows<256>(c, st) : c.src.hd == 128 ? launch_rows<128>(c, st) : launch_rows<64>(c, st);
     if (e != hipSuccess || !c.in_place) return e;
     keep_len_kernel<<<(c.n_seq + 63) / 64, 64, 0, st>>>(c);
     return hipGetLastError();

@@ -21,9 +21,10 @@ static uint64_t weight_bytes(const ts_kv *kv) { return (uint64_t)kv->d.n_seq * k
 
 extern "C" {
 
-// (columns and launch sizes are 32-bit numbers)
+// (work-items of a launch are a 32-bit number, sequences its second dimension)
 static bool weigh_shape_ok(const ts_kv *kv, int32_t n_head, int32_t n_tok) {
-    return kv && heads_ok(kv, n_head) && n_head / kv->d.n_head_kv <= 4096 && n_tok >= 0 && (int64_t)kv->d.n_seq * n_tok * n_head <= INT32_MAX / 64;
+    return kv && heads_ok(kv, n_head) && n_head / kv->d.n_head_kv <= 4096 && n_tok >= 0 && kv->d.n_seq <= 65535 &&
+           (int64_t)kv->d.n_seq * n_tok * n_head <= (n_tok == 1 ? UINT32_MAX / 256 : UINT32_MAX / 128);
 }
 
 int ts_attn_weigh_workspace(const ts_kv *kv, int32_t n_head, int32_t n_tok, uint64_t *bytes) {
@@ -111,7 +112,8 @@ int ts_kv_select(const ts_kv *kv, const float *d_weights, int32_t keep, int32_t 
         !d_weights || !d_slots || !aligned4(d_weights) || !aligned4(d_slots))
         return TS_ERR_INVALID;
     const uint64_t rows = (uint64_t)kv->d.n_layers * kv->d.n_seq * kv->d.n_head_kv;
-    if (rows > INT32_MAX / 64 || kv->d.max_seq > (1 << 28)) return TS_ERR_INVALID;  // (a row's bytes are a 32-bit number)
+    // (a row's bytes and a layer's work-items are 32-bit numbers)
+    if (rows / kv->d.n_layers > UINT32_MAX / 1024 || kv->d.max_seq > (1 << 28)) return TS_ERR_INVALID;
     if (shares(d_weights, weight_bytes(kv) * kv->d.n_layers, d_slots, rows * keep * sizeof(int32_t))) return TS_ERR_INVALID;
     const int max_len = *std::max_element(kv->h_len.begin(), kv->h_len.end());
     return hip_status(launch_select(d_weights, kv->d_len, max_len, kv->d.n_layers, kv->d.n_seq, kv->d.n_head_kv, kv->d.max_seq, keep,
@@ -131,8 +133,8 @@ int ts_kv_keep(ts_kv *dst, int32_t dst_seq, const ts_kv *src, int32_t src_seq, i
     const bool in_place = dst == src && dst_seq == src_seq;
     if (dst == src && !in_place && dst_seq < src_seq + n_seq && src_seq < dst_seq + n_seq) return TS_ERR_INVALID;
     const uint64_t rows = (uint64_t)src->d.n_layers * n_seq * src->d.n_head_kv, slot_bytes = rows * keep * sizeof(int32_t);
-    // (workgroups are 32-bit numbers)
-    if (rows * ((keep + 63) / 64) > INT32_MAX / 16) return TS_ERR_INVALID;
+    // (a layer's work-items are a 32-bit number: 64 of each of up to 9 slices of 64 slots)
+    if (rows / src->d.n_layers * (((uint64_t)keep + 63) / 64) > UINT32_MAX / (9 * 64)) return TS_ERR_INVALID;
     const uint64_t sb = weight_bytes(src) * src->d.n_layers, db = weight_bytes(dst) * dst->d.n_layers;
     if (!(dst == src && d_weights == d_src_weights) && shares(d_src_weights, sb, d_weights, db)) return TS_ERR_INVALID;
     if (shares(d_slots, slot_bytes, d_weights, db)) return TS_ERR_INVALID;
@@ -156,6 +158,7 @@ int ts_kv_keep(ts_kv *dst, int32_t dst_seq, const ts_kv *src, int32_t src_seq, i
     c.dst_seq = dst_seq;
     c.n_seq = n_seq;
     c.n_layers = src->d.n_layers;
+    c.first_layer = 0;
     c.keep = std::min(keep, dst->d.max_seq);
     c.slot_row = keep;
     c.src_max = src->d.max_seq;

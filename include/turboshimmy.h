@@ -520,7 +520,7 @@ int ts_attn_weigh_workspace(const ts_kv *kv, int32_t n_head, int32_t n_tok, uint
  * there, and slots behind the newest token are left.  A slot that a token does not see receives nothing from it,
  * whatever it holds.  The cache alone is attended to (no shared prefix).  q's elements are finite and below 2^100.
  * d_out, d_weights and the workspace are apart from each other and from the inputs (TS_ERR_INVALID);
- * n_seq * n_tok * n_head up to 2^25, up to 4096 query heads per kv head; the rope table of a captured call
+ * n_seq up to 65535, n_seq * n_tok * n_head below 2^25 (one token: 2^24), up to 4096 query heads per kv head; the rope table of a captured call
  * has to cover the positions its replays reach.  d_workspace: ts_attn_weigh_workspace bytes, 16-byte aligned,
  * one call's at a time. */
 int ts_attn_weigh(ts_kv *kv, int32_t layer, const float *d_k, const float *d_v, const float *d_q, int32_t n_head,
@@ -530,7 +530,7 @@ int ts_attn_weigh(ts_kv *kv, int32_t layer, const float *d_k, const float *d_v, 
 /* Which slots stay when every sequence is cut to `keep`: d_slots [n_layers][n_seq][n_head_kv][keep],
  * ascending.  The first n_sink and the last n_recent slots stay (n_sink + n_recent <= keep), and of those
  * between the ones with the largest weights, of equal ones the lowest; a NaN counts as the largest, -0 as 0.
- * A sequence of up to `keep` slots keeps all, with -1 behind them.  max_seq up to 2^28. */
+ * A sequence of up to `keep` slots keeps all, with -1 behind them.  max_seq up to 2^28, n_seq * n_head_kv below 2^22. */
 int ts_kv_select(const ts_kv *kv, const float *d_weights, int32_t keep, int32_t n_sink, int32_t n_recent, int32_t *d_slots,
                  void *stream);
 
@@ -538,12 +538,12 @@ int ts_kv_select(const ts_kv *kv, const float *d_weights, int32_t keep, int32_t 
  * src_seq + i, in every layer and kv head (d_slots: [n_layers][n_seq][n_head_kv][keep], as ts_kv_select
  * writes them: ascending, inside the sequence; others leave rows unspecified).  n = min(length, keep) slots are taken, which become
  * the sequence's length; its window base becomes the source's and what was left out, so that new tokens go on
- * at the positions they would have had.  In place (dst = src, dst_seq = src_seq), or into sequences of the
+ * at the positions they would have had (ts_kv_shift goes on with keep_sink 0).  In place (dst = src, dst_seq = src_seq), or into sequences of the
  * same or another cache (the same n_layers, n_head_kv, head_dim and device) apart from those read, whose old content goes.
  * d_src_weights, d_weights: NULL, or the weights of src and dst, which move along, 0 behind the last (in place: the
  * same array, or one apart).  The lengths are the host's too: after replays of a captured call that changes
  * them, ts_kv_set_seq_len first.  TS_ERR_INVALID: src sequences with sinks (ts_kv_shift); a stream being
- * captured.  TS_ERR_OVERFLOW: n slots do not fit dst. */
+ * captured; n_seq * n_head_kv * keep past 4.7e8.  TS_ERR_OVERFLOW: n slots do not fit dst. */
 int ts_kv_keep(ts_kv *dst, int32_t dst_seq, const ts_kv *src, int32_t src_seq, int32_t n_seq, const int32_t *d_slots,
                int32_t keep, const float *d_src_weights, float *d_weights, void *stream);
 

@@ -197,6 +197,35 @@ def test_weigh_evict_and_go_on(hd):
     assert alone.shape == (2, heads, hd) and bool(torch.isfinite(alone).all())
 
 
+def test_more_rows_than_one_launch_takes():
+    """12.6 million rows in six slices: 4.8e9 work-items, where a launch takes 2^32, 21 layers of them."""
+    n_layers, n_seq, heads, hd = 24, 32768, 16, 8
+    rope = RopeTable.scaled(8, hd, 10000.0)
+    kv = KVCache.new_int4(n_layers, heads, hd, 3, n_seq)
+    w = torch.rand((n_layers, n_seq, heads, 3), device="cuda")
+    k = torch.rand((n_seq, 3, heads, hd), device="cuda")
+    some = (0, 1, 16, 23)  # layers of either launch
+    for i in some:
+        kv.append_quant(i, k + i, k - i, rope)
+    kv.increment(3)
+    off = [3 * s for s in range(n_seq + 1)]
+    before = {i: [x.view(n_seq, 3, heads, hd) for x in kv.read_packed(i, off)] for i in some}
+    wc = w.clone()
+    slots = kv.evict(w, 2)
+    # (of equal weights the lowest slots stay: the last of the smallest goes)
+    lowest = torch.where(wc == wc.amin(-1, keepdim=True), torch.arange(3, device="cuda"), -1).amax(-1, keepdim=True)
+    want = torch.arange(2, device="cuda").expand(slots.shape)
+    want = want + (want >= lowest)
+    assert torch.equal(slots.long(), want)
+    assert torch.equal(w[..., :2], wc.gather(-1, want)) and not bool(w[..., 2].any())
+    assert kv.seq_lens() == [2] * n_seq
+    off = [2 * s for s in range(n_seq + 1)]
+    for i in some:
+        at = want[i].transpose(1, 2)[..., None].expand(n_seq, 2, heads, hd)
+        for old, new in zip(before[i], kv.read_packed(i, off)):
+            assert torch.equal(new.view(n_seq, 2, heads, hd), old.gather(1, at))
+
+
 def test_weights_of_their_own_in_place():
     """In place with another array for the kept weights: whole rows of it are written."""
     lens, keep = [90, 30], 40

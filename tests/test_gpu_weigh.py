@@ -188,6 +188,40 @@ def test_captured_steps(n_tok, heads, hd):
         total = w.cpu()
 
 
+@pytest.mark.parametrize("n_tok,heads,n_kv,hd", [(1, 8, 2, 64), (1, 16, 8, 128), (1, 12, 1, 128), (1, 8, 4, 256), (4, 8, 2, 128), (150, 8, 2, 64),
+                                                 (40, 32, 8, 256)])
+def test_replays_far_past_the_capture(n_tok, heads, n_kv, hd):
+    """A graph of attention captured over a few slots and replayed over thousands, and over a few again."""
+    lens = [2900, 1700, 40]
+    b = Batch(lens, n_tok, heads, n_kv, hd, seed=8)
+    b.append()
+    q, out = b.q.cuda(), torch.empty_like(b.q, device="cuda")
+    ws = torch.empty(b.kv.attn_weigh_workspace(heads, n_tok), dtype=torch.uint8, device="cuda")
+    b.kv.attn_weigh(b.layer, q, b.rope, b.w, out=out, workspace=ws)
+    for s in range(3):
+        b.kv.set_seq_len(20 + s, s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        b.kv.attn_weigh(b.layer, q, b.rope, b.w, fresh=True, out=out, workspace=ws)
+    for now in (lens, [20, 21, 22], lens):
+        for s, m in enumerate(now):
+            b.kv.set_seq_len(m, s)
+        g.replay()
+        torch.cuda.synchronize()
+        b.check(out, b.w, lens=now)
+
+
+@pytest.mark.parametrize("n_tok", [1, 7, 140])
+def test_a_sequence_with_sinks(n_tok):
+    """Sequences that a shift has cut: their keys keep their rotations, the new tokens go on past the window base."""
+    b = Batch([300, 90], n_tok, 8, 2, 128, seed=12)
+    b.kv.compact(4, 100, 0)
+    b.lens[0] -= 100
+    b.base[0] += 100
+    b.append()
+    b.check(b.kv.attn_weigh(b.layer, b.q.cuda(), b.rope, b.w, fresh=True), b.w)
+
+
 @pytest.mark.parametrize("n_tok", [1, 6])
 def test_two_calls_at_once(n_tok):
     """Two caches on two streams, each with a workspace of its own."""
