@@ -723,6 +723,8 @@ void launch_split4(const DecodeArgs &a, int n_split, hipStream_t st) {
 // shape with 64-dim rows: 1.170 vs 1.378 ms per step at 8 query heads per kv head, 1.017 vs
 // 1.030 at 4; ragged config 4: 0.837 vs 0.886.  (With 128-dim rows and two halves of heads 8
 // waves measured slower: 1.970 vs 1.888.)
+// With the scores (SCORES) 128-dim rows run 8 waves too, one storing while the other loads: 32 sequences of 4096-8192
+// slots 56 us, with 4 waves 60; 8 of 1001-16003 26.6 and 27.5.
 template <int HD, bool SC, bool NM, bool SCORES = false>
 void launch_integer(const DecodeArgs &a, int n_split, bool pad, int Gt, hipStream_t st) {
     constexpr int NW = HD == 64 || (SCORES && HD == 128) ? 8 : 4;

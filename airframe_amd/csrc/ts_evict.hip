@@ -64,14 +64,17 @@ __device__ inline int wave_base(int mine, int *s, int wave, int lane, int &all) 
 // passes over ever smaller ranges of keys: a histogram of kBins bins between the smallest and the largest, the bin that
 // holds it, and so on into that bin, until the bin is taken whole or holds one key only.  Keys are logarithmic in the
 // weight, so a row's spread over the bins also when a few slots hold most of the weight, and two passes nearly
-// always do.
+// always do.  The chosen slots go through LDS, so that a wave writes lines: written by the thread that found them, 4096
+// of 4352 slots of 2304 rows took 53 us, 26 so.
+//   A few rows are bound by that chain (28 of 4096 slots: 9 us), many by HBM and the rounds of the CUs: 2304 rows
+// of 16000 slots 47 us, 3.1 TB/s.
 constexpr int kSelPer = 16, kBins = 2048;
 
 template <int NT>
-__global__ __launch_bounds__(NT, NT == 1024 ? 8 : 7) void select_kernel(const float *weights, const int32_t *len, int n_seq, int H, int max_seq,
+__global__ __launch_bounds__(NT, NT == 256 ? 7 : 8) void select_kernel(const float *weights, const int32_t *len, int n_seq, int H, int max_seq,
                                                        int keep, int n_sink, int n_recent, int32_t *slots) {
     constexpr int NW = NT / 64, E = kSelPer, TILE = NT * E, BPT = kBins / NT;
-    __shared__ int hist[kBins], s_wave[3][NW], found[3];
+    __shared__ int hist[kBins > TILE / 2 ? kBins : TILE / 2], s_wave[3][NW], found[3];  // hist: then a tile's chosen slots
     __shared__ uint32_t s_min[NW], s_max[NW];
     const size_t row = blockIdx.x;
     const int s = (int)(row / H % n_seq), tid = threadIdx.x, lane = tid & 63;
@@ -196,12 +199,15 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 8 : 7) void select_kernel(const fl
             ties += all;
         }
         const int upto = wave_scan(__popc(take));
-        int all, at = out + upto - __popc(take);
+        int all, at = upto - __popc(take);
         at += wave_base<NW>(__builtin_amdgcn_readlane(upto, 63), s_wave[2], wave, lane, all);
-        const int p0 = n_sink + t * TILE + tid * E;
-        for (; take && at < most; take &= take - 1) slots[at++] = p0 + __builtin_ctz(take);
+        uint16_t *const list = reinterpret_cast<uint16_t *>(hist);
+        for (; take; take &= take - 1) list[at++] = (uint16_t)(tid * E + __builtin_ctz(take));
+        __syncthreads();
+        const int now = min(all, most - out);
+        for (int i = tid; i < now; i += NT) slots[out + i] = n_sink + t * TILE + list[i];
         out += all;
-        __syncthreads();  // (the waves' counts are read before the next tile's)
+        __syncthreads();  // (the list and the waves' counts are read before the next tile's)
     }
 }
 
@@ -214,12 +220,17 @@ __global__ __launch_bounds__(NT, NT == 1024 ? 8 : 7) void select_kernel(const fl
 // each lane group g, 16-byte chunks of V's lane groups, the scales with the weights; they share no
 // memory.  In place a slice is one wave's from its first slot to its last; into another cache the slots
 // are divided among waves too.
+//   Elsewhere it is bound by HBM, whose lines a gather reads for the slots between too: 2048 of 2048-8192 slots of 4
+// layers, 8 sequences, 8 heads of 128 dims 56 us for the 143 MB of the kept rows (2.5 TB/s).  In place each wave's chain of
+// windows bounds a lone layer (4096 of 4352 slots: 105 us, 64 windows), HBM many (36 layers of 8 sequences: 814 us, 3.2 TB/s).
 
 template <int HD>
 constexpr int kKeepSlices = 4 + HD / 64 + 1;
-constexpr int kKeepPart = 64;  // slots of a wave that does not move in place
+// Slots of a wave that does not move in place: one window of K, so that the launch's waves and not a wave's registers hold what
+// is on its way (128 slots: 59.5 us against 56 in the case above, 6.9 and 6.5 of 4 sequences of 2 layers).
+constexpr int kKeepPart = 64;
 
-// Windows of STEP slots from j0 to j1, D of them in registers: window i + D - 1 goes out before window i is
+// Windows of STEP slots from j0 to j1, D of them in registers: window i + D - 1 is asked for before window i is
 // written, its slots' sources one window earlier.
 template <int STEP, int D, class Reg, class Source, class Load, class Store>
 __device__ __forceinline__ void walk(int j0, int j1, Source source, Load load, Store store) {
@@ -366,14 +377,16 @@ static int layers_per_launch(int64_t items, int n_layers) { return (int)std::min
 hipError_t launch_select(const float *w, const int32_t *d_len, int max_len, int n_layers, int n_seq, int H, int max_seq,
                          int keep, int n_sink, int n_recent, int32_t *d_slots, hipStream_t st) {
     const int64_t rows = (int64_t)n_seq * H;
-    // A workgroup whose registers hold the longest row, and no larger: several of the smaller one share a CU.
-    const bool small = max_len <= 256 * kSelPer;
-    const int per = layers_per_launch(rows * (small ? 256 : 1024), n_layers);
+    // A workgroup whose registers hold the longest row, and no larger: several of the smaller ones share a CU.  2304 rows
+    // with 256, 512 and 1024 threads: of 4096 slots 22.8, 25.2, 40.1 us, of 8192 50.4, 25.4, 40.7, of 16000 99.7, 89.6, 47.1.
+    const int nt = max_len <= 256 * kSelPer ? 256 : max_len <= 512 * kSelPer ? 512 : 1024;
+    const int per = layers_per_launch(rows * nt, n_layers);
     for (int i = 0; i < n_layers; i += per) {
         const unsigned wgs = (unsigned)(std::min(per, n_layers - i) * rows);
         const float *wi = w + i * rows * max_seq;
         int32_t *to = d_slots + i * rows * keep;
-        if (small) select_kernel<256><<<wgs, 256, 0, st>>>(wi, d_len, n_seq, H, max_seq, keep, n_sink, n_recent, to);
+        if (nt == 256) select_kernel<256><<<wgs, 256, 0, st>>>(wi, d_len, n_seq, H, max_seq, keep, n_sink, n_recent, to);
+        else if (nt == 512) select_kernel<512><<<wgs, 512, 0, st>>>(wi, d_len, n_seq, H, max_seq, keep, n_sink, n_recent, to);
         else select_kernel<1024><<<wgs, 1024, 0, st>>>(wi, d_len, n_seq, H, max_seq, keep, n_sink, n_recent, to);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;

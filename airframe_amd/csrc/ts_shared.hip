@@ -493,7 +493,9 @@ SharedPlan shared_plan(int n_seq, int n_tok, int G, int n_kv, int prefix_len, in
 
 // Own keys alone: pieces of the same length, two jobs per CU over the batch's keys (a ragged batch's longest gets
 // more of them), of 256 keys at least and kMaxPieces n_cu / jobs at most (which bounds the partials' scratch);
-// one piece, a chain, once the blocks of columns fill the chip.
+// one piece, a chain, once the blocks of columns fill the chip.  Walk and join with one job per CU and with two: 32 tokens of 4
+// sequences of 1003-8003 slots, 32 heads over 8 of 128 dims, 50 and 43 us; 64 tokens behind 32704 slots, 24 heads, 109
+// and 83 (with four 100).  With 512 keys at least the first takes 50 us too.
 static constexpr int64_t kMaxPieces = 8;
 
 int own_pieces_cap(int n_seq, int n_tok, int G, int n_kv, int own_max, int n_cu) {

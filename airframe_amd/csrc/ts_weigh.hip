@@ -7,7 +7,13 @@
 // A chunk: the attention itself is the window walk of ts_shared.hip over the own keys.  It leaves its columns' rotated q
 // in the operand layout of the matrix cores, and every column's log2 sum lse, its own or (of pieces of the keys)
 // the join's.  Then the scores are computed a second time with the keys held in registers and the columns streaming
-// past, so that a slot's sum stays in its lane: w[p] += sum over the columns of 2^(x - lse).
+// past, so that a slot's sum stays in its lane: w[p] += sum over the columns of 2^(x - lse).  The products are the walk's
+// (q in f16 and two fp6 terms, the codes exact in f16), so P here is what the output was made of but for its rounding.
+//   4 sequences of 1024-1536 slots, 512 tokens, 32 heads over 8 of 128 dims: walk 129 us, sums 68 (26 GFLOP of
+// scores, 0.38 PFLOP/s; the low terms double the products).  Of its 159K cycles a SIMD 40K go to the matrix cores and 50K to
+// the exponentials and their sums, the rest to the waits between them: two waves a SIMD is what the keys' registers allow.
+//   32 tokens of 4 sequences of 1003-8003 slots: walk 35 us, join 8.4, sums 18.6; 64 tokens behind 32704 slots 75, 8.2 and 33.
+// (The sums' launch joining the pieces itself: 43 us and 41.5 before or behind its tiles, the two launches 41.4.)
 #include <cfloat>
 
 #include "ts_columns.h"
@@ -33,7 +39,7 @@ struct ChunkArgs {
 };
 
 // The join of one (token, head) row's pieces by a wave, lane l holding HD / 64 dims: the output, and the row's lse into its
-// column.
+// column.  Bound by the partials' round trips, eight pieces' loads together (34 MB of 4096 rows 8.4 us).
 template <int HD>
 __global__ __launch_bounds__(256) void weigh_join_kernel(ChunkArgs a) {
     constexpr int D = HD / 64;
@@ -241,7 +247,8 @@ constexpr int kWaves = 8;  // of a workgroup
 
 // Few columns: all of them in LDS, and every wave takes tiles of keys of its own, the next one's codes on their way.
 // No barrier but the one behind the columns.  Grid: kv head first, so that the workgroups that read one head's
-// columns share an XCD where the heads divide the XCDs.
+// columns share an XCD where the heads divide the XCDs.  Bound by its chain: the columns and the first codes from L2
+// and HBM, then tile by tile the two passes' products without a neighbour (150 KB of columns leave one workgroup a CU).
 template <int HD, bool SOFTCAP>
 __global__ __launch_bounds__(64 * kWaves, 2) void weigh_window_kernel(ChunkArgs a) {
     using Tile = KeyTile<HD>;
