@@ -197,6 +197,33 @@ def test_weigh_evict_and_go_on(hd):
     assert alone.shape == (2, heads, hd) and bool(torch.isfinite(alone).all())
 
 
+def test_some_sequences_in_place():
+    """Two sequences of four cut, three times over; the others' rows, weights, lengths and bases as they were."""
+    lens, L, n_kv, hd, keep, cap = [90, 300, 131, 64], 2, 2, 128, 120, 300
+    kv = cache(lens, L, n_kv, hd, cap, seed=31)
+    w = rand((L, 4, n_kv, cap), 32).abs()
+    for s, m in enumerate(lens):
+        w[:, s, :, m:] = 0
+    dev = w.cuda()
+    for keep in (120, 119, 65):
+        before, old, now = rows_of(kv, lens), dev.cpu(), [lens[0], min(lens[1], keep), min(lens[2], keep), lens[3]]
+        slots = picked(lens[1:3], L, n_kv, keep, keep)
+        kv.keep_slots(slots.cuda(), dev, seq=1, src_seq=1, n_seq=2)
+        assert kv.seq_lens() == now and [kv.get_window_base(s) for s in range(4)] == [0, 300 - now[1], 131 - now[2], 0]
+        after = rows_of(kv, now)
+        for i in range(L):
+            for s in (0, 3):
+                assert all(torch.equal(x, y) for x, y in zip(after[i][s], before[i][s]))
+                assert torch.equal(dev[i, s].cpu(), old[i, s])
+            for s in (1, 2):
+                for h in range(n_kv):
+                    want = torch.zeros(cap)
+                    want[:now[s]] = old[i, s, h, slots[i, s - 1, h, :now[s]].long()]
+                    assert torch.equal(dev[i, s, h].cpu(), want)
+        check_rows([layer[1:3] for layer in after], [layer[1:3] for layer in before], slots, lens[1:3], keep)
+        lens = now
+
+
 def test_more_rows_than_one_launch_takes():
     """12.6 million rows in six slices: 4.8e9 work-items, where a launch takes 2^32, 21 layers of them."""
     n_layers, n_seq, heads, hd = 24, 32768, 16, 8

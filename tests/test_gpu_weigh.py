@@ -84,6 +84,25 @@ def test_against_64_bits(lens, n_tok, heads, n_kv, hd):
     assert b.kv.seq_lens() == b.lens
 
 
+@pytest.mark.parametrize("n_tok,heads,n_kv", [(1, 8, 2), (1, 40, 2), (3, 8, 2), (200, 16, 2)])
+@pytest.mark.parametrize("m", [5, 63, 333, 1021])
+def test_up_to_the_last_slot(m, n_tok, heads, n_kv):
+    """The new tokens fill the cache of the longest sequence."""
+    b = Batch([m, 1], n_tok, heads, n_kv, 128, slack=0, seed=m)
+    b.append()
+    b.check(b.kv.attn_weigh(b.layer, b.q.cuda(), b.rope, b.w, fresh=True), b.w)
+
+
+@pytest.mark.parametrize("n_tok", [1, 2])
+def test_the_most_query_heads(n_tok):
+    """4096 query heads on one kv head; one more head per kv head is refused."""
+    b = Batch([70], n_tok, 4096, 1, 16, seed=1)
+    b.append()
+    b.check(b.kv.attn_weigh(b.layer, b.q.cuda(), b.rope, b.w, fresh=True), b.w)
+    with pytest.raises(TsError):
+        b.kv.attn_weigh_workspace(4097, n_tok)
+
+
 @pytest.mark.parametrize("n_tok", [1, 5, 140])
 @pytest.mark.parametrize("hd", [64, 96, 128, 256])
 def test_softcap_norm_and_window_base(n_tok, hd):
