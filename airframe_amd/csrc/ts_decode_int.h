@@ -363,11 +363,11 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void decode_split4_kernel(DecodeAr
     // split 1, so the splits that wait for a free CU are the last ones of the longest
     // sequences (config 4: 1.42 vs 1.45 ms per step against the split-fastest order)
     const int split = blockIdx.z, h = blockIdx.x, s = blockIdx.y;
-    const int qpos = a.hlen >= 0 ? a.hlen : a.len[s];
+    int qpos, qrot;  // the query's slot and rotation position
+    token_pos(a, s, qpos, qrot);
     // a captured launch replayed past the cache's capacity (the host checks lengths only when a
     // call is made): no work, nothing written
     if (qpos >= L.P) return;
-    const int qrot = rot_of(a.L, s, qpos);  // rotation position of the query
     const int n_ctx = qpos + 1;
     const int start = split * a.chunk;
     if (start >= n_ctx) return;
@@ -509,7 +509,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void decode_split4_kernel(DecodeAr
         // loads go out with q's.  kd, vd and xnew are read after the barrier that opens the
         // merge.
         if (appender) {
-            append_load<HD, NORM>(a, s, h, qpos, lane, ain, hdr);
+            append_load<HD, NORM>(a, s, h, qpos, qrot, lane, ain, hdr);
             load_q_pairs<HD, 4 * GH * HG>(a, s, h * G, G, lane, qp, hdr);
         }
         __builtin_amdgcn_sched_barrier(0);

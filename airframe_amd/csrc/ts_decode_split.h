@@ -47,6 +47,20 @@ struct DecodeArgs {
     bool fresh;
 };
 
+// The new token's slot of sequence s and its rotation position.  Window base, sinks and length go out
+// together: the former asked for behind the latter cost a captured step a round trip (one sequence of
+// 512 slots 8.7 us a layer, 8.4 so).
+__device__ __forceinline__ void token_pos(const DecodeArgs &a, int s, int &qpos, int &qrot) {
+    const KvLayerView &L = a.L;
+    if (L.rot) {
+        const int len = a.len[s], rot = L.rot[s], sink = L.rot[L.S + s];
+        qpos = a.hlen >= 0 ? a.hlen : len;
+        qrot = min(rot_pos(qpos, rot, sink), L.rot_last);
+    } else {
+        qrot = qpos = a.hlen >= 0 ? a.hlen : a.len[s];
+    }
+}
+
 // Every workgroup of the launch's last kernel calls this once, after its last read of the
 // lengths: the workgroup that arrives last (all others have read them by then) advances every
 // length by one and clears the counter for the next launch.  Call from all threads of the
@@ -305,7 +319,7 @@ __device__ __forceinline__ void process_window(const Window<HD> &w, WaveState<HD
 // row ((code - 8) * scale, the values the cache now holds) in kd / vd.
 //
 // Two phases, so a caller can issue every load of the append together (one memory round trip)
-// before anything else: append_load, then append_store.
+// before anything else: append_load (pr: the position's rotation position), then append_store.
 template <int HD>
 struct AppendIn {
     static constexpr int PPL = HD > 128 ? 2 : 1;
@@ -316,12 +330,11 @@ struct AppendIn {
 };
 
 template <int HD, bool NORM>
-__device__ __forceinline__ void append_load(const DecodeArgs &a, int s, int h, int p, int lane, AppendIn<HD> &in,
+__device__ __forceinline__ void append_load(const DecodeArgs &a, int s, int h, int p, int pr, int lane, AppendIn<HD> &in,
                                             int hdr) {
     constexpr int PPL = AppendIn<HD>::PPL;
     const KvLayerView &L = a.L;
     const size_t row = (size_t)s * L.H + h;
-    const int pr = rot_of(L, s, p);
     const int q = p & 31, gq = (q & 15) >> 2;
     const uint32_t *vb = reinterpret_cast<const uint32_t *>(L.vp + (row * (L.P / 32) + (p >> 5)) * (HD * 16));
 #pragma unroll

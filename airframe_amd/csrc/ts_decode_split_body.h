@@ -54,7 +54,8 @@
     for (int t = 0; t < WPG; t++) q_read8(qrow, k16_word<HD>(g, t), nullptr, 1.0f, qraw[t], hdr);
     asm volatile("" ::: "memory");
 
-    const int qpos = a.hlen >= 0 ? a.hlen : a.len[s];
+    int qpos, qrot;  // the query's slot and rotation position
+    token_pos(a, s, qpos, qrot);
     // a captured launch replayed past the cache's capacity (the host checks lengths only when a
     // call is made): no work, nothing written (the lengths still advance, as the combine
     // kernel's do)
@@ -62,7 +63,6 @@
         if (a.n_split == 1) arrive_and_advance(a);
         return;
     }
-    const int qrot = rot_of(a.L, s, qpos);  // rotation position of the query
     const int n_ctx = qpos + 1;
     if (start >= n_ctx) return;  // (only with a split: its combine kernel advances the lengths)
     const int n_split_s = min((n_ctx + a.chunk - 1) / a.chunk, a.n_split);
@@ -122,7 +122,7 @@
     if (fused && wave == NW - 1) {
         AppendIn<HD> ain;
         float2 qp[8][AppendIn<HD>::PPL];
-        append_load<HD, NORM>(a, s, h, qpos, lane, ain, hdr);
+        append_load<HD, NORM>(a, s, h, qpos, qrot, lane, ain, hdr);
         load_q_pairs<HD, 8>(a, s, hb, G, lane, qp, hdr);
         append_store<HD, NORM>(a, s, h, qpos, lane, ain, kd, vd, hdr, gi == 0);
         new_token_scores<HD, SOFTCAP, NORM, 8>(a, s, hb, G, lane, qp, ain.cs, kd, xnew, hdr);

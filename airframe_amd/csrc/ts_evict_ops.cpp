@@ -65,7 +65,7 @@ int ts_attn_weigh(ts_kv *kv, int32_t layer, const float *d_k, const float *d_v, 
             if (shares(arg[i].p, arg[i].n, arg[j].p, arg[j].n)) return TS_ERR_INVALID;
 
     WeighCall c;
-    c.L = kv->layer(layer);
+    c.L = rotating_layer(kv, layer, rope, stream);
     c.d_len = kv->d_len;
     for (int s = 0; s < kv->d.n_seq; s++) kv->h_ctx[s] = kv->h_len[s] + n_tok;
     c.n_ctx = kv->h_ctx.data();

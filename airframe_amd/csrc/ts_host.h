@@ -17,6 +17,13 @@ inline void note_len_change(ts_kv *kv, void *stream) {
     if (capturing(stream)) kv->len_captured = true;
 }
 
+// The layer as a call on the stream takes it that rotates rows with the table `rope` (or null: none).
+inline KvLayerView rotating_layer(const ts_kv *kv, int layer, const ts_rope *rope, void *stream) {
+    KvLayerView v = kv->layer(layer, kv->len_captured || capturing(stream));
+    if (rope) v.rot_last = rope->n_pos - 1;
+    return v;
+}
+
 inline int hip_status(hipError_t e) { return e == hipSuccess ? TS_OK : TS_ERR_HIP; }
 
 // The kernels move rows in 16-byte pieces.

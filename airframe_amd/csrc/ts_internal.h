@@ -57,11 +57,10 @@ struct KvLayerView {
     uint8_t *vp;  // V packed
     float *ks;    // K scales
     float *vs;    // V scales
-    // Per sequence: window base (the shift total of all compactions) and sink count, or null
-    // while no sequence has been compacted.  The K of slot p is stored rotated at rot_pos(p):
-    // p for the sinks, p + window base otherwise.
+    // Per sequence: window bases [S] (the shift total of all compactions) and behind them sink
+    // counts [S], or null while no sequence has been compacted.  The K of slot p is stored rotated
+    // at rot_pos(p): p for the sinks, p + window base otherwise.
     const int32_t *rot;
-    const int32_t *sink;
     // QK norm of this layer (Qwen3): per-dim weights for q and K, or null (no norm), and eps
     const float *qn, *kn;
     float norm_eps;
@@ -69,14 +68,15 @@ struct KvLayerView {
     // dim (a multiple of 8, at most hd), the row length of q, K, V and outputs.  Stored dims
     // from hdr on hold code 8 (value 0).
     int S, H, P, hd, hdr;
+    int rot_last;  // the last row of the call's RoPE table (a graph may be replayed past it)
 };
 
 __device__ __host__ inline int rot_pos(int p, int rot, int sink) { return p < sink ? p : p + rot; }
 
-// Rotation position of slot p of sequence s (rot/sink are null while no sequence of the cache
-// has been compacted, which saves the kernels two loads).
+// Rotation position of slot p of sequence s (rot is null in an eager call while no sequence of the
+// cache has been compacted, which saves the kernels two loads).
 __device__ inline int rot_of(const KvLayerView &L, int s, int p) {
-    return L.rot ? rot_pos(p, L.rot[s], L.sink[s]) : p;
+    return L.rot ? min(rot_pos(p, L.rot[s], L.rot[L.S + s]), L.rot_last) : p;
 }
 
 }  // namespace ts
@@ -97,13 +97,16 @@ struct ts_kv {
     std::vector<int32_t> h_ctx;  // scratch for the decode plan: len + 1 per sequence
     // Set once a call that changes the device lengths was captured into a graph: replays of it
     // advance the device lengths without the host knowing, so decode launches read the device
-    // lengths from then on instead of taking the host's as arguments.
+    // lengths from then on instead of taking the host's as arguments (and every call the device's
+    // window bases, which such a call may change too).
     bool len_captured = false;
     int device;
     int n_cu;                    // compute units of the device (the decode plan's target)
     int hdp;                     // stored head dim (KvLayerView::hd)
 
-    ts::KvLayerView layer(int l) const {
+    // on_device: whether the call's kernels look up window bases and sinks on the device although the
+    // host knows of none: replays of a captured call see those of their time.
+    ts::KvLayerView layer(int l, bool on_device = false) const {
         ts::KvLayerView v;
         uint64_t nrow = (uint64_t)d.n_seq * d.n_head_kv * P;
         uint8_t *b = base + (uint64_t)l * layer_bytes;
@@ -111,9 +114,9 @@ struct ts_kv {
         v.vp = b + nrow * (hdp / 2);
         v.ks = (float *)(b + nrow * hdp);
         v.vs = v.ks + nrow;
-        const bool compacted = std::any_of(h_rot.begin(), h_rot.end(), [](int32_t r) { return r != 0; });
+        const bool compacted = on_device || std::any_of(h_rot.begin(), h_rot.end(), [](int32_t r) { return r != 0; });
         v.rot = compacted ? d_rot : nullptr;
-        v.sink = compacted ? d_sink : nullptr;
+        v.rot_last = INT32_MAX;
         v.qn = q_norm[l];
         v.kn = k_norm[l];
         v.norm_eps = norm_eps[l];

@@ -382,7 +382,7 @@ int ts_append_quant(ts_kv *kv, int32_t layer, const float *d_k, const float *d_v
     if (n_tok == 0) return TS_OK;
     // Blocks of 32 positions touched by [len, len+n_tok): at most n_tok/32 + 2.
     int32_t max_blocks = n_tok / 32 + 2;
-    return hip_status(ts::launch_quantize_rows(kv->layer(layer), d_k, d_v, kv->d_len, 0, n_tok,
+    return hip_status(ts::launch_quantize_rows(rotating_layer(kv, layer, rope, stream), d_k, d_v, kv->d_len, 0, n_tok,
                                                n_tok, rope->d_table, rope->rope_dim / 2,
                                                max_blocks, as_stream(stream)));
 }
@@ -402,7 +402,7 @@ int ts_requant_all(ts_kv *kv, int32_t layer, const float *d_k_cache, const float
     int32_t blocks = (seq_len + 31) / 32;
     // K is taken as given: the reference normalizes its f32 cache before requantizing, so the
     // layer's QK norm is not applied again
-    ts::KvLayerView L = kv->layer(layer);
+    ts::KvLayerView L = rotating_layer(kv, layer, rope, stream);
     L.qn = L.kn = nullptr;
     return hip_status(ts::launch_quantize_rows(L, d_k_cache, d_v_cache, nullptr, 0,
                                                seq_len, ld_pos, rope ? rope->d_table : nullptr,
@@ -471,7 +471,7 @@ static int attn_decode(const ts_kv *kv, int32_t layer, const float *d_q, int32_t
     const bool cap = capturing(stream);
     if (cap && advance) mkv->len_captured = true;
     const int32_t *h_len = cap || kv->len_captured ? nullptr : kv->h_len.data();
-    const int rc2 = hip_status(ts::launch_decode(kv->layer(layer), kv->d_len, h_len, d_q, n_head, rope->d_table,
+    const int rc2 = hip_status(ts::launch_decode(rotating_layer(kv, layer, rope, stream), kv->d_len, h_len, d_q, n_head, rope->d_table,
                                                  rope->rope_dim / 2, softcap, d_out, (float *)d_workspace,
                                                  plan, k_new, v_new, advance ? kv->d_adv : nullptr,
                                                  as_stream(stream)));
@@ -556,7 +556,7 @@ int ts_attn_prefill(const ts_kv *kv, int32_t layer, const float *d_q, int32_t n_
     int rc = check_rope(rope, kv->d.head_dim, rot_end(kv, n_tok));
     if (rc) return rc;
     if (n_tok == 0) return TS_OK;
-    return hip_status(ts::launch_prefill(kv->layer(layer), kv->d_len, d_q, n_head, n_tok,
+    return hip_status(ts::launch_prefill(rotating_layer(kv, layer, rope, stream), kv->d_len, d_q, n_head, n_tok,
                                          rope->d_table, rope->rope_dim / 2, softcap, d_out,
                                          kv->n_cu, as_stream(stream)));
 }
@@ -642,7 +642,7 @@ static int qkv_append_planes(ts_kv *kv, int32_t layer, const float *d_x, int32_t
         if (e == hipSuccess) e = ts::launch_proj(d_x, M, dim, d_wk, H * hd, kb, nullptr, g.pk, part, planes, st);
         if (e == hipSuccess) e = ts::launch_proj(d_x, M, dim, d_wv, H * hd, vb, nullptr, g.pk, part, planes, st);
         if (e == hipSuccess)
-            e = ts::launch_quantize_rows(kv->layer(layer), kb, vb, kv->d_len, 0, n_tok, n_tok, rope->d_table,
+            e = ts::launch_quantize_rows(rotating_layer(kv, layer, rope, stream), kb, vb, kv->d_len, 0, n_tok, n_tok, rope->d_table,
                                          rope->rope_dim / 2, n_tok / 32 + 2, st);
         return hip_status(e);
     }
@@ -650,7 +650,7 @@ static int qkv_append_planes(ts_kv *kv, int32_t layer, const float *d_x, int32_t
     plan.in_place = qkv_in_place(kv, d_x, dim, n_tok, n_head, d_q, d_k, d_v);
     if (plan.part_bytes > 0 && (!d_workspace || workspace_bytes < plan.part_bytes || !aligned16(d_workspace)))
         return TS_ERR_WORKSPACE;
-    return hip_status(ts::launch_qkv(kv->layer(layer), kv->d_len, d_x, dim, n_tok, d_wq, d_wk, d_wv,
+    return hip_status(ts::launch_qkv(rotating_layer(kv, layer, rope, stream), kv->d_len, d_x, dim, n_tok, d_wq, d_wk, d_wv,
                                      n_head, d_q, d_k, d_v, rope->d_table, rope->rope_dim / 2, plan,
                                      static_cast<float *>(d_workspace), planes, as_stream(stream)));
 }
@@ -742,7 +742,7 @@ int ts_qkv_append_gguf(ts_kv *kv, int32_t layer, const float *d_x, int32_t dim, 
         if (e == hipSuccess) e = ts::launch_proj_kq(d_x, M, dim, ggml_type, d_wk, H * hd, kb, nullptr, g.pk, part, st);
         if (e == hipSuccess) e = ts::launch_proj_kq(d_x, M, dim, ggml_type, d_wv, H * hd, vb, nullptr, g.pk, part, st);
         if (e == hipSuccess)
-            e = ts::launch_quantize_rows(kv->layer(layer), kb, vb, kv->d_len, 0, n_tok, n_tok, rope->d_table,
+            e = ts::launch_quantize_rows(rotating_layer(kv, layer, rope, stream), kb, vb, kv->d_len, 0, n_tok, n_tok, rope->d_table,
                                          rope->rope_dim / 2, n_tok / 32 + 2, st);
         return hip_status(e);
     }
@@ -750,7 +750,7 @@ int ts_qkv_append_gguf(ts_kv *kv, int32_t layer, const float *d_x, int32_t dim, 
                                              qkv_in_place(kv, d_x, dim, n_tok, n_head, d_q, d_k, d_v));
     if (plan.part_bytes > 0 && (!d_workspace || workspace_bytes < plan.part_bytes || !aligned16(d_workspace)))
         return TS_ERR_WORKSPACE;
-    return hip_status(ts::launch_qkv_kq(kv->layer(layer), kv->d_len, d_x, dim, n_tok, ggml_type, d_wq, d_wk, d_wv,
+    return hip_status(ts::launch_qkv_kq(rotating_layer(kv, layer, rope, stream), kv->d_len, d_x, dim, n_tok, ggml_type, d_wq, d_wk, d_wv,
                                         n_head, d_q, d_k, d_v, rope->d_table, rope->rope_dim / 2, plan,
                                         static_cast<float *>(d_workspace), st));
 }

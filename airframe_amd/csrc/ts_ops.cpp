@@ -110,7 +110,7 @@ int ts_append_packed(ts_kv *kv, int32_t layer, int32_t dtype, const void *d_k, i
         const int rc = check_rope(rope, kv->d.head_dim, rot_last);
         if (rc) return rc;
     }
-    KvLayerView L = kv->layer(layer);
+    KvLayerView L = rotating_layer(kv, layer, rope, stream);
     if (!rope) L.qn = L.kn = nullptr;  // (K as it is stored: normalized and rotated by the caller)
     return hip_status(launch_append_packed(L, kv->d_len, dtype, d_k, k_stride, d_v, v_stride, tok_off,
                                            rope ? rope->d_table : nullptr, rope ? rope->rope_dim / 2 : 0,
@@ -272,7 +272,7 @@ int ts_attn_shared(ts_kv *kv, const ts_kv *prefix, int32_t prefix_seq, int32_t l
         return TS_ERR_INVALID;
 
     SharedCall c;
-    c.own = kv->layer(layer);
+    c.own = rotating_layer(kv, layer, rope, stream);
     c.pre = prefix->layer(layer);
     c.prefix_seq = prefix_seq;
     c.prefix_len = P;

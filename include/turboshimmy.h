@@ -148,7 +148,10 @@ int ts_kv_set_qk_norm(ts_kv *kv, int32_t layer, const float *d_q_norm, const flo
  * compaction rotate K there and queries are rotated at (position + window base): window keys
  * then see the compacted distance and the sinks the logical one, as in
  * sh_layer_v1_int4.wgsl:1062-1080.  Call advance after ts_kv_shift of every layer, then
- * ts_kv_set_seq_len(len - shift_amt), as the reference's caller does. */
+ * ts_kv_set_seq_len(len - shift_amt), as the reference's caller does.
+ * A captured call reads window bases and sinks at its replays, like the lengths: a step captured before a cut
+ * (this one or ts_kv_keep) goes on after it.  Its table has to cover the positions that its replays reach; past
+ * the last row they take that row. */
 int ts_kv_window_base(const ts_kv *kv, int32_t seq, int32_t *base);
 int ts_kv_advance_window_base(ts_kv *kv, int32_t seq, int32_t shift_amt, void *stream);
 
