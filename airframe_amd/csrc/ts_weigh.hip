@@ -202,9 +202,10 @@ __device__ __forceinline__ void add_probs(floatx16 (&sc)[KeyTile<HD>::NT], float
             const floatx4 s4 = *reinterpret_cast<const floatx4 *>(sk + 32 * i + 8 * q + 4 * hf);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                float x = sc[i][4 * q + r] * s4[r];
-                if constexpr (SOFTCAP) x = cap<true>(x * back, softcap, inv_softcap) - lse;
-                else x = __builtin_fmaf(x, back, -lse);
+                // (back first, as the walk: a code sum times a large key's scale passes f32 where q is small)
+                float x = sc[i][4 * q + r] * back;
+                if constexpr (SOFTCAP) x = cap<true>(x * s4[r], softcap, inv_softcap) - lse;
+                else x = __builtin_fmaf(x, s4[r], -lse);
                 sc[i][4 * q + r] = __builtin_amdgcn_exp2f(x);
             }
         }
