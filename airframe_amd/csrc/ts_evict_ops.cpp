@@ -4,6 +4,8 @@
 #include <math.h>
 
 #include <cmath>
+#include <memory>
+#include <new>
 
 #include "ts_host.h"
 
@@ -139,10 +141,24 @@ int ts_kv_keep(ts_kv *dst, int32_t dst_seq, const ts_kv *src, int32_t src_seq, i
     if (!(dst == src && d_weights == d_src_weights) && shares(d_src_weights, sb, d_weights, db)) return TS_ERR_INVALID;
     if (shares(d_slots, slot_bytes, d_weights, db)) return TS_ERR_INVALID;
     if (capturing(stream)) return TS_ERR_INVALID;  // (the host's lengths change with the call)
+    // Lengths, bases and sinks as the device has them: replays of a captured call move them past the host's.
+    const int32_t *h_len = src->h_len.data(), *h_rot = src->h_rot.data(), *h_sink = src->h_sink.data();
+    std::unique_ptr<int32_t[]> now;
+    if (src->len_captured) {
+        const size_t ints = 3 * (size_t)src->d.n_seq;
+        now.reset(new (std::nothrow) int32_t[ints]);
+        if (!now) return TS_ERR_NOMEM;
+        if (hipMemcpyAsync(now.get(), src->d_len, ints * sizeof(int32_t), hipMemcpyDeviceToHost, as_stream(stream)) != hipSuccess ||
+            hipStreamSynchronize(as_stream(stream)) != hipSuccess)
+            return TS_ERR_HIP;
+        h_len = now.get();
+        h_rot = h_len + src->d.n_seq;
+        h_sink = h_rot + src->d.n_seq;
+    }
     for (int i = 0; i < n_seq; i++) {
-        const int s = src_seq + i, n = std::min(src->h_len[s], keep);
-        if (src->h_sink[s] != 0) return TS_ERR_INVALID;  // (sinks are rotated at their own slot, the others past the window base)
-        if (n > dst->d.max_seq || (int64_t)src->h_rot[s] + src->h_len[s] - n > INT32_MAX / 2) return TS_ERR_OVERFLOW;
+        const int s = src_seq + i, len = std::min(h_len[s], src->d.max_seq), n = std::min(len, keep);
+        if (h_sink[s] != 0) return TS_ERR_INVALID;  // (sinks are rotated at their own slot, the others past the window base)
+        if (n > dst->d.max_seq || (int64_t)h_rot[s] + len - n > INT32_MAX / 2) return TS_ERR_OVERFLOW;
     }
     KeepCall c;
     c.src = src->layer(0);
@@ -169,8 +185,8 @@ int ts_kv_keep(ts_kv *dst, int32_t dst_seq, const ts_kv *src, int32_t src_seq, i
     c.dst_w = d_weights;
     if (launch_keep(c, as_stream(stream)) != hipSuccess) return TS_ERR_HIP;
     for (int i = 0; i < n_seq; i++) {
-        const int s = src_seq + i, d = dst_seq + i, len = src->h_len[s], n = std::min(len, keep);
-        dst->h_rot[d] = src->h_rot[s] + len - n;
+        const int s = src_seq + i, d = dst_seq + i, len = std::min(h_len[s], src->d.max_seq), n = std::min(len, keep);
+        dst->h_rot[d] = h_rot[s] + len - n;
         dst->h_len[d] = n;
         dst->h_sink[d] = 0;
     }

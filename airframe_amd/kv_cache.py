@@ -421,7 +421,8 @@ class KVCache:
         (ts_kv_keep): in place, or sequences src_seq .. of the cache src into sequences seq .. of this one.
         n_seq: how many (all of src's).  Lengths become what was kept, new tokens go on at the positions
         they would have had.  weights, src_weights: this cache's and src's weights, to move along (in place:
-        weights alone)."""
+        weights alone).  After a captured step of src the call waits for the stream and takes the lengths that
+        the replays left; seq_lens() is theirs again then."""
         src = self if src is None else src
         n = src.n_seq if n_seq is None else n_seq
         if slots.dim() != 4 or tuple(slots.shape[:3]) != (src.n_layers, n, src.n_head_kv):
@@ -439,7 +440,7 @@ class KVCache:
 
     def evict(self, weights: torch.Tensor, keep: int, n_sink: int = 0, n_recent: int = 0, stream=None) -> torch.Tensor:
         """Every sequence cut to the `keep` slots of each layer and kv head that select_slots names, in
-        place, weights with them.  Returns the slots."""
+        place, weights with them.  Behind replays of a captured step as keep_slots.  Returns the slots."""
         slots = self.select_slots(weights, keep, n_sink, n_recent, stream=stream)
         self.keep_slots(slots, weights, stream=stream)
         return slots

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from airframe_amd import TsError
 from airframe_amd.kv_cache import KVCache, RopeTable
 from tests.evict_util import cached, weigh
 from tests.packed_util import offsets, rand
@@ -132,3 +133,47 @@ def test_replays_past_the_table(kind, n_tok):
         rows = cached(st.kv, 0, [LENS[0] + 30 + (i + 1) * n_tok] * 2)
         assert all(bool(torch.isfinite(x).all()) for r in rows for x in r)
         assert bool(torch.isfinite(st.out).all())
+
+
+@pytest.mark.parametrize("elsewhere", [False, True])
+def test_a_cut_behind_replays_alone(elsewhere):
+    """Replays move the lengths past those that the host knows; a cut without set_seq_len takes the device's, for its bases and
+    for the host, twice over."""
+    st = Steps("weigh", 128, 1)
+    st.inputs(0)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        st.run()
+    for s, m in enumerate(LENS):
+        st.kv.set_seq_len(m, s)
+    lens, bases, small = list(LENS), [0, 0], KVCache.new_int4(1, N_KV, 128, 70, 2)
+    for round_ in range(2):
+        for i in range(3):
+            st.inputs(10 * round_ + i)
+            g.replay()
+        lens = [m + 3 for m in lens]
+        if elsewhere:
+            with pytest.raises(TsError) as e:  # (as many slots as the device has, not as the host knows)
+                KVCache.new_int4(1, N_KV, 128, lens[1] - 1, 2).keep_slots(st.kv.select_slots(st.w, 100), src=st.kv)
+            assert e.value.code == -2
+        before = cached(st.kv, 0, lens)
+        slots = st.kv.select_slots(st.w, KEEP, 2, 10)
+        to = small if elsewhere else st.kv
+        to.keep_slots(slots, src=st.kv) if elsewhere else to.keep_slots(slots, st.w)
+        now = [min(m, KEEP) for m in lens]
+        cut_bases = [b + m - n for b, m, n in zip(bases, lens, now)]
+        assert to.seq_lens() == now and [to.get_window_base(s) for s in range(2)] == cut_bases
+        after, at = cached(to, 0, now), slots.cpu().long()
+        for s in range(2):
+            for h in range(N_KV):
+                for x, y in zip(after[s], before[s]):
+                    assert torch.equal(x[:, h], y[at[0, s, h, :now[s]], h])
+        # an eager token on it
+        k, v, q = (rand((2, 1, n, 128), 200 + j, scale=2.0) for j, n in enumerate((N_KV, N_KV, HEADS)))
+        w = to.new_weights()
+        out = to.attn_weigh(0, q.cuda(), st.rope, w[0], k=k.cuda(), v=v.cuda())
+        want, far, _ = weigh(cached(to, 0, [n + 1 for n in now]), q, now, cut_bases, 128, 128, BASE)
+        assert bool(((out.cpu().double() - want).abs() <= far).all())
+        if not elsewhere:
+            lens, bases = now, cut_bases
