@@ -135,8 +135,9 @@ int ts_kv_keep(ts_kv *dst, int32_t dst_seq, const ts_kv *src, int32_t src_seq, i
     const bool in_place = dst == src && dst_seq == src_seq;
     if (dst == src && !in_place && dst_seq < src_seq + n_seq && src_seq < dst_seq + n_seq) return TS_ERR_INVALID;
     const uint64_t rows = (uint64_t)src->d.n_layers * n_seq * src->d.n_head_kv, slot_bytes = rows * keep * sizeof(int32_t);
-    // (a layer's work-items are a 32-bit number: 64 of each of up to 9 slices of 64 slots)
-    if (rows / src->d.n_layers * (((uint64_t)keep + 63) / 64) > UINT32_MAX / (9 * 64)) return TS_ERR_INVALID;
+    // (a layer's work-items are a 32-bit number: 64 of each of up to 9 slices of a row, elsewhere of its windows of 64 slots)
+    const uint64_t windows = in_place ? 1 : ((uint64_t)std::min(keep, dst->d.max_seq) + 63) / 64;
+    if (rows / src->d.n_layers * windows > UINT32_MAX / (9 * 64)) return TS_ERR_INVALID;
     const uint64_t sb = weight_bytes(src) * src->d.n_layers, db = weight_bytes(dst) * dst->d.n_layers;
     if (!(dst == src && d_weights == d_src_weights) && shares(d_src_weights, sb, d_weights, db)) return TS_ERR_INVALID;
     if (shares(d_slots, slot_bytes, d_weights, db)) return TS_ERR_INVALID;

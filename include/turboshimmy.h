@@ -546,7 +546,8 @@ int ts_kv_select(const ts_kv *kv, const float *d_weights, int32_t keep, int32_t 
  * d_src_weights, d_weights: NULL, or the weights of src and dst, which move along, 0 behind the last (in place: the
  * same array, or one apart).  Once a call that changes src's lengths was captured, this call waits for the
  * stream and takes the lengths that the replays left, also for the host.  TS_ERR_INVALID: src sequences with sinks (ts_kv_shift); a stream being
- * captured; n_seq * n_head_kv * keep past 4.7e8.  TS_ERR_OVERFLOW: n slots do not fit dst. */
+ * captured; more than 7456540 rows (n_seq * n_head_kv), in another place windows of 64 kept slots (rows times
+ * ceil(min(keep, dst's max_seq) / 64)).  TS_ERR_OVERFLOW: n slots do not fit dst. */
 int ts_kv_keep(ts_kv *dst, int32_t dst_seq, const ts_kv *src, int32_t src_seq, int32_t n_seq, const int32_t *d_slots,
                int32_t keep, const float *d_src_weights, float *d_weights, void *stream);
 
