@@ -8,7 +8,7 @@ namespace ts {
 constexpr int kColBlk = 32;  // columns of one block
 
 // One block: rotated q's high halves [k-step][lane], its low terms [group of 4 k-steps][term][3][lane][8 bytes], then
-// each column's scale back of q and the log2 sum of its softmax.  Columns past the last hold zeros.
+// each column's scale back of q (over kSkUnit) and the log2 sum of its softmax.  Columns past the last hold zeros.
 template <int HD>
 struct ColBlock {
     half8 hi[HD / 16][64];

@@ -209,6 +209,7 @@ __global__ __launch_bounds__(64 * kPrefillNW, HD > 128 ? 1 : 2) void shared_kern
     }
     float q_s, q_back;
     q_scale(half_max(mc) * qmul, q_s, q_back);
+    if constexpr (COLS) q_back *= 1.0f / kSkUnit;
     sm_back[32 * wave + j] = q_back;
     // the split of this lane's column
     half8 qh[NKS];
@@ -256,7 +257,7 @@ __global__ __launch_bounds__(64 * kPrefillNW, HD > 128 ? 1 : 2) void shared_kern
     bool first = true;
 
     stage_codes<HD, NW>(sm, 0, pd, tid, wave, dk);
-    stage_scales<HD, NW, true>(sm, 0, pd, tid, 1.0f);
+    stage_scales<HD, NW, true>(sm, 0, pd, tid, COLS ? kSkUnit : 1.0f);
     if (1 < n_win) fetch(1);
     __syncthreads();
 
@@ -296,7 +297,7 @@ __global__ __launch_bounds__(64 * kPrefillNW, HD > 128 ? 1 : 2) void shared_kern
         }
         if constexpr (NPART == 0) stage_codes<HD, NW>(sm, buf ^ 1, pd, tid, wave, dk);
         __builtin_amdgcn_s_setprio(0);
-        if (w + 1 < n_win) stage_scales<HD, NW, true>(sm, buf ^ 1, pd, tid, 1.0f);
+        if (w + 1 < n_win) stage_scales<HD, NW, true>(sm, buf ^ 1, pd, tid, COLS ? kSkUnit : 1.0f);
         if (w + 2 < n_win) fetch(w + 2);
         // Keys are numbered within their stream: a column sees the prefix up to k_end, its own keys up to
         // its slot.
@@ -308,11 +309,16 @@ __global__ __launch_bounds__(64 * kPrefillNW, HD > 128 ? 1 : 2) void shared_kern
         const int qmax_w = pre ? k_end - 1 : len_w + (min(c_wave + kColsPerWave, n_cols) - 1) / G;
         if (c_wave < n_cols && base <= qmax_w) {
             const float q_back = sm_back[32 * wave + j];
-            sc[0] *= q_back;
-            sc[1] *= q_back;
             const bool mask = base + kWin - 1 > qmin_w;
-            window_scores<NDB, SOFTCAP, COLS>(sc, sm.sk[buf], sm.svlog[buf], a.softcap, mask, first, base, hf, qpos, m_run,
-                                              l_run, o, a.inv_softcap);
+            if constexpr (COLS) {
+                window_scores_again<NDB, SOFTCAP>(sc, sm.sk[buf], q_back, sm.svlog[buf], a.softcap, mask, first, base, hf,
+                                                  qpos, m_run, l_run, o, a.inv_softcap);
+            } else {
+                sc[0] *= q_back;
+                sc[1] *= q_back;
+                window_scores<NDB, SOFTCAP>(sc, sm.sk[buf], sm.svlog[buf], a.softcap, mask, first, base, hf, qpos, m_run,
+                                            l_run, o);
+            }
             first = false;
 #pragma unroll
             for (int st = 0; st < 4; st++) {

@@ -149,7 +149,8 @@ __device__ __forceinline__ void set_keys(const typename KeyTile<HD>::Raw &r, typ
     }
 }
 
-// Scores of one column block: lane (j, hf) holds column j and keys 32 i + 8 (e / 4) + 4 hf + e % 4.
+// Scores of one column block: lane (j, hf) holds column j and keys 32 i + 8 (e / 4) + 4 hf + e % 4.  Products are summed in
+// the walk's order, so that a score has the same bits in both passes.
 template <int HD>
 __device__ __forceinline__ void tile_scores(const typename KeyTile<HD>::F16 &ka, const typename KeyTile<HD>::F6 &k6,
                                             const ColBlock<HD> &b, int lane, floatx16 (&sc)[KeyTile<HD>::NT]) {
@@ -157,13 +158,13 @@ __device__ __forceinline__ void tile_scores(const typename KeyTile<HD>::F16 &ka,
 #pragma unroll
     for (int i = 0; i < T::NT; i++) sc[i] = (floatx16)0.0f;
 #pragma unroll
-    for (int t = 0; t < T::NKS; t++) {
-        const half8 q = b.hi[t][lane];
+    for (int g = 0; g < T::NG; g++) {
 #pragma unroll
-        for (int i = 0; i < T::NT; i++) sc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[i][t], q, sc[i], 0, 0, 0);
-    }
+        for (int u = 0; u < 4; u++) {
+            const half8 q = b.hi[4 * g + u][lane];
 #pragma unroll
-    for (int g = 0; g < T::NG; g++)
+            for (int i = 0; i < T::NT; i++) sc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[i][4 * g + u], q, sc[i], 0, 0, 0);
+        }
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             int6v q;
@@ -176,18 +177,20 @@ __device__ __forceinline__ void tile_scores(const typename KeyTile<HD>::F16 &ka,
 #pragma unroll
             for (int i = 0; i < T::NT; i++) sc[i] = mfma_lo6(k6[i][g], q, sc[i], u ? kQlo2E8 : kQlo1E8);
         }
-    // the columns' reads run four ahead of the matrix instructions that take them
-    constexpr int READS = T::NKS + 3 * T::NG, MFMAS = T::NT * (T::NKS + 2 * T::NG);
+    }
+    // the columns' reads (one for an f16 step, three for a low term) run at least three ahead of the matrix instructions
+    // that take them: four, then two behind each f16 step and one behind each low term
     __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
-    for (int k = 0; k < READS - 4; k++) {
+    for (int k = 0; k < 6 * T::NG; k++) {
         __builtin_amdgcn_sched_group_barrier(0x8, T::NT, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        if (k >= 6 * T::NG - 3) continue;  // (all are out)
+        if (k % 6 < 4) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        else __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x8, MFMAS, 0);
 }
 
-// Probabilities of one column block added to acc.  sk: the tile's K scales in LDS; cb: the block, of n_cols columns in
+// Probabilities of one column block added to acc.  sk: the tile's K scales times kSkUnit, in LDS; cb: the block, of n_cols columns in
 // all; base: the tile's first key.
 template <int HD, bool SOFTCAP>
 __device__ __forceinline__ void add_probs(floatx16 (&sc)[KeyTile<HD>::NT], float (&acc)[KeyTile<HD>::NT][16], const ColBlock<HD> &b,
@@ -202,10 +205,11 @@ __device__ __forceinline__ void add_probs(floatx16 (&sc)[KeyTile<HD>::NT], float
             const floatx4 s4 = *reinterpret_cast<const floatx4 *>(sk + 32 * i + 8 * q + 4 * hf);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                // (back first, as the walk: a code sum times a large key's scale passes f32 where q is small)
-                float x = sc[i][4 * q + r] * back;
-                if constexpr (SOFTCAP) x = cap<true>(x * s4[r], softcap, inv_softcap) - lse;
-                else x = __builtin_fmaf(x, s4[r], -lse);
+                // (the walk's bits: window_scores_again)
+                const float t = sc[i][4 * q + r] * s4[r];
+                float x;
+                if constexpr (SOFTCAP) x = cap<true>(t * back, softcap, inv_softcap) - lse;
+                else x = __builtin_fmaf(t, back, -lse);
                 sc[i][4 * q + r] = __builtin_amdgcn_exp2f(x);
             }
         }
@@ -273,7 +277,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_window_kernel(ChunkArgs 
     float scale = 0.0f;
     auto fetch = [&](int tile) __attribute__((always_inline)) {
         fetch_keys<HD>(raw, kw, a.L.P, tile * KEYS, j);
-        scale = ks[min(tile * KEYS + (lane & (KEYS - 1)), a.L.P - 1)];
+        scale = ks[min(tile * KEYS + (lane & (KEYS - 1)), a.L.P - 1)] * kSkUnit;
     };
     if (first * KEYS < n) {
         fetch(min(first + wave, (n - 1) / KEYS));
@@ -371,7 +375,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_cols_kernel(ChunkArgs a)
         const DeqConstV dk;
         typename Tile::Raw raw;
         fetch_keys<HD>(raw, reinterpret_cast<const uint32_t *>(a.L.kp + st * a.L.P * (HD / 2)), a.L.P, base, j);
-        if (tid < KEYS) sks[tid] = a.L.ks[st * a.L.P + min(key0 + tid, a.L.P - 1)];
+        if (tid < KEYS) sks[tid] = a.L.ks[st * a.L.P + min(key0 + tid, a.L.P - 1)] * kSkUnit;
         set_keys<HD>(raw, ka, k6, hf, dk);
     }
     float acc[NT][16];

@@ -318,11 +318,10 @@ __device__ inline float half_sum(float v) {
 // online-softmax state update.  The reference is raised only when the window breaks
 // p <= 2^8 or p*s_v <= 2^15 (f16 range), and the scores move down with it; the first window
 // (first, uniform; m_run = 0 and nothing accumulated yet) sets it from its own max.
-// FAST: the softcap by cap() with inv_softcap = 1 / softcap, at most the largest float.
-template <int NDB, bool SOFTCAP, bool FAST = false>
+template <int NDB, bool SOFTCAP>
 __device__ inline void window_scores(floatx16 (&sc)[2], const float *sk, float svl, float softcap,
                                      bool mask, bool first, int base, int h, int qpos, float &m_run,
-                                     float &l_run, floatx16 (&o)[NDB], float inv_softcap = 0.0f) {
+                                     float &l_run, floatx16 (&o)[NDB]) {
 #pragma unroll
     for (int kb = 0; kb < 2; kb++) {
 #pragma unroll
@@ -333,8 +332,7 @@ __device__ inline void window_scores(floatx16 (&sc)[2], const float *sk, float s
                 float x;
                 if constexpr (SOFTCAP) {
                     x = sc[kb][4 * q + r] * sk4[r];
-                    if constexpr (FAST) x = cap<true>(x, softcap, inv_softcap) - m_run;
-                    else x = tanhf(x / softcap) * softcap * kLog2e - m_run;
+                    x = tanhf(x / softcap) * softcap * kLog2e - m_run;
                 } else {
                     x = __builtin_fmaf(sc[kb][4 * q + r], sk4[r], -m_run);
                 }
@@ -374,6 +372,62 @@ __device__ inline void window_scores(floatx16 (&sc)[2], const float *sk, float s
 #pragma unroll
             for (int i = 0; i < 16; i++) sc[kb][i] = sc[kb][i] - delta;
     }
+}
+
+// The same for scores that are made a second time, by whoever needs the final reference: t = (sum of codes) s_k
+// is rounded by itself and the score, t times the column's power of two `back`, is exact, so that it has the same
+// bits in both passes; and m_run is the largest score but for svl's part.  2^(score - reference) is then at most 1 in
+// the second pass too, whatever the scores' size.  (Rounded inside the FMA that takes m_run off, scores
+// from 2^24 on are whole steps away from it.)  sk comes times kSkUnit and `back` over it: a sum of codes (below 2^25) times
+// the largest s_k stays below 2^128 also where small queries make a small score of it.  The softcap by cap(),
+// inv_softcap = 1 / softcap, at most the largest float.
+constexpr float kSkUnit = 0x1p-24f;
+template <int NDB, bool SOFTCAP>
+__device__ inline void window_scores_again(floatx16 (&sc)[2], const float *sk, float back, float svl, float softcap,
+                                           bool mask, bool first, int base, int h, int qpos, float &m_run, float &l_run,
+                                           floatx16 (&o)[NDB], float inv_softcap) {
+#pragma unroll
+    for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const floatx4 sk4 = *reinterpret_cast<const floatx4 *>(sk + 32 * kb + 16 * (q >> 1) + 8 * h + 4 * (q & 1));
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float t = sc[kb][4 * q + r] * sk4[r];
+                sc[kb][4 * q + r] = SOFTCAP ? cap<true>(t * back, softcap, inv_softcap) : t;
+            }
+        }
+    if (mask) {
+        asm volatile("");  // (a branch, as above)
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (base + 32 * kb + 16 * (q >> 1) + 8 * h + 4 * (q & 1) + r > qpos) sc[kb][4 * q + r] = -INFINITY;
+    }
+    float mloc = -INFINITY;
+#pragma unroll
+    for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) mloc = fmaxf(mloc, sc[kb][i]);
+    mloc = fmaxf(half_max(mloc) * (SOFTCAP ? 1.0f : back), kMinit);
+    const float need = mloc - m_run + fmaxf(-8.0f, svl - 15.0f);
+    if (__builtin_amdgcn_ballot_w64(first || need > 0.0f) != 0) {
+        const float m_new = (first || need > 0.0f) ? mloc + fmaxf(0.0f, svl - 15.0f) : m_run;
+        if (!first) {
+            const float alpha = exp2f(m_run - m_new);
+            l_run *= alpha;
+#pragma unroll
+            for (int db = 0; db < NDB; db++) o[db] *= alpha;
+        }
+        m_run = m_new;
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) sc[kb][i] = SOFTCAP ? sc[kb][i] - m_run : __builtin_fmaf(sc[kb][i], back, -m_run);
 }
 
 // Probabilities of 16-key step st (keys 16st + 8h + 0..7 of the window) times s_v, split

@@ -1,11 +1,13 @@
 """attn_weigh in the forms that long and wide batches take: the integer decode kernel with its scores, with and without
 splits, and chunks of more tiles of keys than the waves hold at once."""
+import math
+
 import pytest
 import torch
 
 from airframe_amd.kv_cache import KVCache, RopeTable, decode_plan
 from tests.evict_util import weigh
-from tests.packed_util import offsets, rand
+from tests.packed_util import offsets, rand, rope_angles, rotate
 
 pytestmark = pytest.mark.gpu
 BASE = 10000.0
@@ -121,3 +123,55 @@ def test_large_keys_and_small_queries(n_tok, softcap):
     w = torch.zeros((2, n_kv, 520), device="cuda")
     out = kv.attn_weigh(0, q.cuda(), rope, w, fresh=True, softcap=softcap)
     check(kv, hd, q, lens, [0, 1], out, w, softcap=softcap)
+
+
+def columns(rows, q, m, hd):
+    """The scores of one sequence's columns in 64 bits, [kv heads, columns, slots], -inf where a slot is not seen, and the
+    sizes of their sums."""
+    (k, _), (n_tok, heads) = rows, q.shape[:2]
+    n, H = k.shape[:2]
+    angles = rope_angles(m + n_tok, hd, BASE)[m:]
+    x = rotate(q.double(), angles.cos(), angles.sin(), "interleaved").view(n_tok, H, heads // H, hd)
+    kd = k.double().permute(1, 2, 0)
+    sc = torch.stack([(x[:, h].reshape(-1, hd) @ kd[h]) / hd ** 0.5 for h in range(H)])
+    size = torch.stack([(x[:, h].abs().reshape(-1, hd) @ kd[h].abs()) / hd ** 0.5 for h in range(H)])
+    seen = torch.arange(n) <= m + torch.arange(n_tok).repeat_interleave(heads // H)[:, None]
+    return sc.masked_fill(~seen, -torch.inf), size
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 14, 2.0 ** 26, 2.0 ** 60])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("n_tok", [1, 5, 200])
+def test_scores_past_a_steps_size(n_tok, hd, scale):
+    """Scores whose f32 steps reach whole numbers: a column's probabilities stay at most 1 and, with one slot far above the
+    others, are one 1, whatever window it is in."""
+    n_kv, heads, lens = 2, 8, [90, 700]
+    kv, rope, k, v, q = batch(lens, n_tok, heads, n_kv, hd, 11)
+    q = q * scale
+    kv.append_quant(0, k, v, rope)
+    w = torch.zeros((2, n_kv, kv.max_seq_len), device="cuda")
+    kv.attn_weigh(0, q.cuda(), rope, w, fresh=True)
+    ends = [m + n_tok for m in lens]
+    for s, rows in enumerate(some_of(kv, 0, ends, [0, 1])):
+        sc, size = columns(rows, q[s], lens[s], hd)
+        top = sc.topk(2, -1)
+        # a score is within 24 roundings of the size of its sum (evict_util.weigh), and behind 2^-40 of the
+        # largest a slot's part is below a rounding of what it is added to
+        far = 2 * 24 * 2.0 ** -24 * size.amax(-1) + 40 * math.log(2)
+        clear = top.values[..., 0] - top.values[..., 1] > far
+        want = torch.zeros(n_kv, ends[s], dtype=torch.float64)
+        for h in range(n_kv):
+            want[h].index_add_(0, top.indices[h, :, 0][clear[h]], torch.ones(int(clear[h].sum()), dtype=torch.float64))
+        got = w[s, :, :ends[s]].cpu().double()
+        unclear = (~clear).sum(-1)
+        if scale > 2.0 ** 20:
+            assert int(unclear.max()) <= 2
+        # the exponent's error: the roundings of the score, the reference and the log sum (half a step each) at the largest
+        # score; probabilities of 1 lose 24 roundings more in sums
+        step = 2.0 ** -24 * (3 * 1.45 * float(sc.amax()) + 24)
+        most = torch.exp2(torch.tensor(step if step < 1 else 0.0, dtype=torch.float64)) - 1 + 2.0 ** -20
+        # a clear column leaves every other slot up to 2^-40, an unclear one any slot up to 1
+        other = sc.shape[1] * 2.0 ** -40 + (1 + most) * unclear[:, None]
+        off = got - want
+        low, high = bool((off >= -most * want).all()), bool((off <= most * want + other).all())
+        assert low and high, (float(off.min()), float(off.max()))
