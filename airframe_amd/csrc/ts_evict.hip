@@ -221,9 +221,9 @@ __global__ __launch_bounds__(NT, NT == 256 ? 7 : 8) void select_kernel(const flo
 // memory.  In place a slice is one wave's from its first slot to its last; into another cache the slots
 // are divided among waves too.
 //   Elsewhere it is bound by HBM, whose lines a gather reads for the slots between too: 2048 of 2048-8192 slots of 4
-// layers, 8 sequences, 8 heads of 128 dims 56 us, 143 MB of kept rows read and written, 236 MB with the slots
-// between (4.2 TB/s).  In place a wave's
-// instructions over its windows bound a lone layer (4096 of 4352 slots: 105 us), HBM many (36 layers of 8 sequences: 814
+// layers, 8 sequences, 8 heads of 128 dims 56 us, 143 MB of kept rows read and written, 262 MB with the slots
+// between (counted, 4.7 TB/s).  In place a wave's
+// instructions over its windows bound a lone layer (4096 of 4352 slots: 104 us), HBM many (36 layers of 8 sequences: 823
 // us, 3.2 TB/s); with eight windows of K and five of V on their way instead of four and three 101 and 990 us.
 
 template <int HD>

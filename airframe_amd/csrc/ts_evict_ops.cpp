@@ -93,10 +93,10 @@ int ts_attn_weigh(ts_kv *kv, int32_t layer, const float *d_k, const float *d_v, 
     c.hlen = kv->d.n_seq == 1 && !c.captured ? kv->h_len[0] : -1;
     DecodePlan plan = decode_plan(kv->h_ctx.data(), kv->d.n_seq, kv->d.n_head_kv, n_head / kv->d.n_head_kv, kv->n_cu,
                                   kv->hdp, d_k != nullptr);
-    // The integer kernel runs a workgroup per CU, those past a short sequence's end too: of a ragged batch, longer
-    // splits that fit the CUs in one round, if no longer than 5/2 of the plan's.  4 sequences of 700-6001 slots of
-    // 256-dim heads 28.5 us, 19.6 so; 8 of 1001-16003 with 128 dims 30.7 and 26.2, with 8 query heads per kv head 42.6
-    // and 34.7.
+    // The integer kernel runs a workgroup per CU, those past a short sequence's end too, and the grid is a rectangle of
+    // sequences by the longest one's splits: of a ragged batch, longer splits whose rectangle fits the CUs in one round, if no longer
+    // than 5/2 of the plan's.  4 sequences of 700-6001 slots of 256-dim heads 28.5 us, 19.6 so; 8 of 1001-16003 with 128
+    // dims 30.7 and 26.2, with 8 query heads per kv head 42.6 and 34.7.  (Of the first two's 256 workgroups 120 have keys.)
     const int round = kv->n_cu / (kv->d.n_seq * kv->d.n_head_kv);
     if (plan.g4 && round > 1 && plan.n_split > round) {
         const int chunk = ((c.own_max + round - 1) / round + 63) / 64 * 64;

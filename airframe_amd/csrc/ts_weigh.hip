@@ -9,10 +9,12 @@
 // the join's.  Then the scores are computed a second time with the keys held in registers and the columns streaming
 // past, so that a slot's sum stays in its lane: w[p] += sum over the columns of 2^(x - lse).  The products are the walk's
 // (q in f16 and two fp6 terms, the codes exact in f16), so P here is what the output was made of but for its rounding.
-//   4 sequences of 1024-1536 slots, 512 tokens, 32 heads over 8 of 128 dims: walk 129 us, sums 68 (26 GFLOP of
-// scores, 0.38 PFLOP/s; the low terms double the products).  Of its 159K cycles a SIMD 40K go to the matrix cores and 50K to
-// the exponentials and their sums, the rest to the waits between them: two waves a SIMD is what the keys' registers allow.
-//   32 tokens of 4 sequences of 1003-8003 slots: walk 35 us, join 8.4, sums 18.6; 64 tokens behind 32704 slots 75, 8.2 and 33.
+//   4 sequences of 1024-1536 slots, 512 tokens, 32 heads over 8 of 128 dims: walk 127 us, sums 67 (26 GFLOP of
+// scores, 0.39 PFLOP/s; the low terms double the products; under the profiler, the call itself takes 175). Of its 159K cycles a
+// SIMD 40K go to the matrix cores and 50K to the exponentials and their sums, the rest to the waits between them: two waves a
+// SIMD is what the keys' registers allow.
+//   32 tokens of 4 sequences of 1003-8003 slots: walk 35 us, join 8.5, sums 17 (the call 55); 64 tokens behind 32704 slots 72,
+// 8.2 and 31 (103).
 // (The sums' launch joining the pieces itself: 43 us and 41.5 before or behind its tiles, the two launches 41.4.)
 #include <cfloat>
 

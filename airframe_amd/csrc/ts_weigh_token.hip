@@ -9,7 +9,7 @@
 //   lse = M + log2(sum over the splits of 2^(m - M) l).
 // In the kernel where no sequence is split: 32 sequences of 4096-8192 slots, 32 heads over 8 of 128 dims 56 us (61 with a
 // launch for the sums; 210 MB, 3.8 TB/s), one of 511 slots of 64 dims 9.5 us (12.4; a chain of round trips).  8 of
-// 1001-16003: 21.6 us the splits, 6.0 the join and sums; 4 of 700-6001 with 256 dims 16.0 and 4.0.
+// 1001-16003: 21.4 us the splits, 6.1 the join and sums; 4 of 700-6001 with 256 dims 15.6 and 4.0.
 #include <cfloat>
 
 #include "ts_decode_int.h"
