@@ -150,7 +150,7 @@ def test_scores_past_a_steps_size(n_tok, hd, scale):
     q = q * scale
     kv.append_quant(0, k, v, rope)
     w = torch.zeros((2, n_kv, kv.max_seq_len), device="cuda")
-    kv.attn_weigh(0, q.cuda(), rope, w, fresh=True)
+    out = kv.attn_weigh(0, q.cuda(), rope, w, fresh=True).cpu().double()
     ends = [m + n_tok for m in lens]
     for s, rows in enumerate(some_of(kv, 0, ends, [0, 1])):
         sc, size = columns(rows, q[s], lens[s], hd)
@@ -175,3 +175,8 @@ def test_scores_past_a_steps_size(n_tok, hd, scale):
         off = got - want
         low, high = bool((off >= -most * want).all()), bool((off <= most * want + other).all())
         assert low and high, (float(off.min()), float(off.max()))
+        # the output of a clear column is its slot's value row: kept in two f16 terms (2^-20), a sum's 24 roundings more
+        v = rows[1].double()
+        for h in range(n_kv):
+            o = out[s, :, h * heads // n_kv:(h + 1) * heads // n_kv].reshape(-1, hd)[clear[h]]
+            assert bool(((o - v[top.indices[h, :, 0][clear[h]], h]).abs() <= 2.0 ** -18 * v[:, h].abs().max()).all())
