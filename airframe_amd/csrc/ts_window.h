@@ -379,8 +379,9 @@ __device__ inline void window_scores(floatx16 (&sc)[2], const float *sk, float s
 // bits in both passes; and m_run is the largest score but for svl's part.  2^(score - reference) is then at most 1 in
 // the second pass too, whatever the scores' size.  (Rounded inside the FMA that takes m_run off, scores
 // from 2^24 on are whole steps away from it.)  sk comes times kSkUnit and `back` over it: a sum of codes (below 2^25) times
-// the largest s_k stays below 2^128 also where small queries make a small score of it.  The softcap by cap(),
-// inv_softcap = 1 / softcap, at most the largest float.
+// the largest s_k stays below 2^128 also where small queries make a small score of it.  (An s_k below 2^-102 leaves bits there:
+// 2^-18 of an exponent at most, with queries near 2^100.)  The softcap by cap(), inv_softcap = 1 / softcap, at most the
+// largest float.
 constexpr float kSkUnit = 0x1p-24f;
 template <int NDB, bool SOFTCAP>
 __device__ inline void window_scores_again(floatx16 (&sc)[2], const float *sk, float back, float svl, float softcap,
